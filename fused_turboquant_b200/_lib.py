@@ -62,6 +62,14 @@ SIGNATURES = {
     "ftq_tq_decode_layers_ws": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _i64, _i64, _i64, _i, _vp, _i, _vp,
                                      _vp, _i, _i, _i, _i, _i, _fp, _c.c_float, _i, _vp, _vp, _i, _vp,
                                      _vp, _i, _vp, _i, _i64, _i64, _vp, _sz, _vp]),
+    "ftq_pages_extend": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _i, _vp, _vp, _vp, _vp]),
+    "ftq_pages_trim": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp]),
+    "ftq_tree_masks": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp]),
+    "ftq_tree_commit": (_i, [_vp, _i64, _i64, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp,
+                             _vp, _vp, _vp, _vp]),
+    "ftq_logits_workspace_bytes": (_sz, [_i64, _i]),
+    "ftq_logits_process": (_i, [_vp, _i, _i64, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp,
+                                _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 
 _lib = None

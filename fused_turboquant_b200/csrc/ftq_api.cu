@@ -17,6 +17,7 @@
 #include "../../include/ftq_b200.h"
 #include "ftq_dense.cuh"
 #include "ftq_launch.h"
+#include "ftq_serve_launch.h"
 #include "ftq_tq_v1_launch.h"
 
 namespace {
@@ -1560,4 +1561,147 @@ extern "C" int ftq_tq_decode_layers_ws(const void* q, int q_dtype, int B, int Hq
     if (e != cudaSuccess) return cuda_fail(e, "tq_decode stage 1 launch");
     e = merge();
     return e == cudaSuccess ? FTQ_OK : cuda_fail(e, "tq_decode merge launch");
+}
+
+// ------------------------------------------------------------------ speculative serving
+
+static_assert(FTQ_TREE_MAX_NODES == ftq::kTreeMaxNodes && FTQ_PAGES_MAX_REQUESTS == ftq::kPagesMaxRequests,
+              "header and kernels agree on the limits");
+
+namespace {
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + nb && y < x + na;
+}
+
+int check_pages(const ftq::PagesParams& p, const char* what) {
+    if (p.R < 0 || p.R > ftq::kPagesMaxRequests)
+        return fail(FTQ_ERR_UNSUPPORTED, "%s: %d requests (0 to %d)", what, p.R, ftq::kPagesMaxRequests);
+    if (p.max_blocks <= 0 || p.max_blocks > (1 << 26) || p.num_blocks < 0)
+        return fail(FTQ_ERR_INVALID, "%s: bad shape max_blocks=%d num_blocks=%d", what, p.max_blocks, p.num_blocks);
+    if (p.R > 0 && (!p.table || !p.lens || !p.n_free || !p.arg || (p.num_blocks > 0 && !p.free_blocks)))
+        return fail(FTQ_ERR_INVALID, "%s: NULL pointer", what);
+    return FTQ_OK;
+}
+}  // namespace
+
+extern "C" int ftq_pages_extend(int32_t* block_table, int32_t* seq_lens, int32_t* free_blocks, int32_t* n_free,
+                                int n_requests, int max_blocks, int num_blocks, const int32_t* new_lens,
+                                int width, int packed, int64_t* slots, int32_t* granted, int32_t* starts,
+                                void* stream) {
+    ftq::PagesParams p{block_table, seq_lens, free_blocks, n_free, new_lens, n_requests, max_blocks, num_blocks,
+                       slots, granted, starts, width, packed != 0};
+    const int rc = check_pages(p, "ftq_pages_extend");
+    if (rc) return rc;
+    if (width < 0 || (!packed && static_cast<int64_t>(width) * n_requests > INT32_MAX))
+        return fail(FTQ_ERR_INVALID, "ftq_pages_extend: width %d", width);
+    if (n_requests == 0) return FTQ_OK;
+    if (!granted || !starts || (width > 0 && !slots)) return fail(FTQ_ERR_INVALID, "ftq_pages_extend: NULL pointer");
+    const cudaError_t e = ftq::launch_pages_extend(p, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FTQ_OK : cuda_fail(e, "ftq_pages_extend launch");
+}
+
+extern "C" int ftq_pages_trim(int32_t* block_table, int32_t* seq_lens, int32_t* free_blocks, int32_t* n_free,
+                              int n_requests, int max_blocks, int num_blocks, const int32_t* keep_lens, void* stream) {
+    const ftq::PagesParams p{block_table, seq_lens, free_blocks, n_free, keep_lens, n_requests, max_blocks, num_blocks,
+                             nullptr, nullptr, nullptr, 0, false};
+    const int rc = check_pages(p, "ftq_pages_trim");
+    if (rc) return rc;
+    if (n_requests == 0) return FTQ_OK;
+    const cudaError_t e = ftq::launch_pages_trim(p, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FTQ_OK : cuda_fail(e, "ftq_pages_trim launch");
+}
+
+extern "C" int ftq_tree_masks(const int32_t* parents, const int32_t* tree_lens, const int32_t* context_lens, int B,
+                              int n_nodes, int32_t* masks, int32_t* positions, void* stream) {
+    if (n_nodes <= 0 || n_nodes > ftq::kTreeMaxNodes)
+        return fail(FTQ_ERR_UNSUPPORTED, "a tree has 1 to %d nodes, got %d", ftq::kTreeMaxNodes, n_nodes);
+    if (B < 0) return fail(FTQ_ERR_INVALID, "ftq_tree_masks: B=%d", B);
+    if (B == 0) return FTQ_OK;
+    if (!parents || !masks || !positions) return fail(FTQ_ERR_INVALID, "ftq_tree_masks: NULL pointer");
+    const cudaError_t e = ftq::launch_tree_masks({parents, tree_lens, context_lens, masks, positions, B, n_nodes},
+                                                 static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FTQ_OK : cuda_fail(e, "ftq_tree_masks launch");
+}
+
+extern "C" int ftq_tree_commit(uint8_t* pool, int64_t num_blocks, int64_t pool_layer_stride, int n_layers,
+                               const int32_t* block_table, int max_blocks, const int32_t* seq_lens,
+                               const int32_t* tree_lens, const int32_t* tokens, const int32_t* parents,
+                               const int32_t* next_tokens, int B, int n_nodes, int Hkv, int head_dim, int bits_k,
+                               int bits_v, int32_t* path, int32_t* n_accepted, int32_t* out_tokens,
+                               int32_t* new_lens, void* stream) {
+    if (!dim_ok(head_dim)) return fail(FTQ_ERR_UNSUPPORTED, "head_dim %d (need 64/128/256)", head_dim);
+    if (!bits_ok(bits_k) || !bits_ok(bits_v))
+        return fail(FTQ_ERR_INVALID, "bits must be 2, 3, or 4, got K=%d V=%d", bits_k, bits_v);
+    if (n_nodes <= 0 || n_nodes > ftq::kTreeMaxNodes)
+        return fail(FTQ_ERR_UNSUPPORTED, "a tree has 1 to %d nodes, got %d", ftq::kTreeMaxNodes, n_nodes);
+    if (B < 0 || B > 65535 || Hkv <= 0 || n_layers <= 0 || static_cast<int64_t>(n_layers) * Hkv > (1 << 24) || max_blocks <= 0 || num_blocks < 0)
+        return fail(FTQ_ERR_INVALID, "ftq_tree_commit: bad shape B=%d Hkv=%d layers=%d max_blocks=%d", B, Hkv, n_layers, max_blocks);
+    if (B == 0) return FTQ_OK;
+    if (!pool || !block_table || !seq_lens || !tokens || !parents || !next_tokens || !path || !n_accepted || !out_tokens || !new_lens)
+        return fail(FTQ_ERR_INVALID, "ftq_tree_commit: NULL pointer");
+    if (!aligned(pool, 16) || pool_layer_stride % 16) return fail(FTQ_ERR_INVALID, "pool must be 16-byte aligned");
+    const size_t row = static_cast<size_t>(B) * 4;
+    if (overlap(new_lens, row, seq_lens, row) || (tree_lens && (overlap(new_lens, row, tree_lens, row) || overlap(n_accepted, row, tree_lens, row))) ||
+        overlap(n_accepted, row, seq_lens, row))
+        return fail(FTQ_ERR_INVALID, "ftq_tree_commit: the new lengths need memory of their own");
+    ftq::CommitParams p{};
+    p.block_table = block_table; p.seq_lens = seq_lens; p.tree_lens = tree_lens;
+    p.tokens = tokens; p.parents = parents; p.next = next_tokens;
+    p.path = path; p.n_accepted = n_accepted; p.out_tokens = out_tokens; p.new_lens = new_lens;
+    p.pool = pool; p.layer_stride = pool_layer_stride; p.num_blocks = num_blocks;
+    p.B = B; p.T = n_nodes; p.max_blocks = max_blocks; p.Hkv = Hkv; p.n_layers = n_layers;
+    p.pdk = ftq::packed_dim(head_dim, bits_k); p.pdv = ftq::packed_dim(head_dim, bits_v);
+    p.page_bytes = static_cast<int>(ftq_page_bytes(head_dim, bits_k, bits_v));
+    const cudaError_t e = ftq::launch_tree_commit(p, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FTQ_OK : cuda_fail(e, "ftq_tree_commit launch");
+}
+
+extern "C" size_t ftq_logits_workspace_bytes(int64_t n_rows, int vocab) {
+    if (n_rows <= 0 || vocab <= 0) return 0;
+    return static_cast<size_t>(n_rows) * ((vocab - 1) / ftq::kLogitSegment + 1) * 8;
+}
+
+extern "C" int ftq_logits_process(const void* logits, int dtype, int64_t row_stride, int n_requests, int rows_per_request,
+                                  int vocab, const int32_t* history, int history_stride, const int32_t* history_lens,
+                                  const int32_t* prompt_lens, const float* repetition, const float* frequency,
+                                  const float* presence, const int32_t* bias_ids, const float* bias, int n_bias,
+                                  const int32_t* allowed, int64_t allowed_stride, const int32_t* tree_tokens,
+                                  const int32_t* tree_masks, float* out, int32_t* best, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+    if (dtype != FTQ_F32 && dtype != FTQ_F16 && dtype != FTQ_BF16) return fail(FTQ_ERR_INVALID, "dtype %d", dtype);
+    if (n_requests < 0 || rows_per_request < 0 || vocab <= 0 || row_stride < vocab || history_stride < 0 || n_bias < 0)
+        return fail(FTQ_ERR_INVALID, "ftq_logits_process: bad shape requests=%d rows=%d vocab=%d row_stride=%lld", n_requests,
+                    rows_per_request, vocab, static_cast<long long>(row_stride));
+    if (n_requests > 65535 || rows_per_request > 65535)
+        return fail(FTQ_ERR_UNSUPPORTED, "at most 65535 requests and 65535 rows of each");
+    if (n_requests == 0 || rows_per_request == 0) return FTQ_OK;
+    if (!logits || (!out && !best)) return fail(FTQ_ERR_INVALID, "ftq_logits_process: NULL logits, or nothing to write");
+    if (history && !history_lens) return fail(FTQ_ERR_INVALID, "history needs history_lens");
+    if (n_bias > 0 && (!bias_ids || !bias)) return fail(FTQ_ERR_INVALID, "biases need ids and values");
+    if ((tree_tokens == nullptr) != (tree_masks == nullptr)) return fail(FTQ_ERR_INVALID, "a tree needs its tokens and masks");
+    if (tree_masks && rows_per_request > ftq::kTreeMaxNodes)
+        return fail(FTQ_ERR_UNSUPPORTED, "a tree has 1 to %d nodes, got %d", ftq::kTreeMaxNodes, rows_per_request);
+    if (allowed && (allowed_stride < (vocab + 31) / 32)) return fail(FTQ_ERR_INVALID, "a mask's row has %lld words for %d tokens",
+                                                                   static_cast<long long>(allowed_stride), vocab);
+    const int64_t rows = static_cast<int64_t>(n_requests) * rows_per_request;
+    const size_t es = dtype_size(dtype), out_bytes = static_cast<size_t>(rows) * vocab * 4;
+    if (out && overlap(out, out_bytes, logits, (static_cast<size_t>(rows - 1) * row_stride + vocab) * es) &&
+        !(static_cast<const void*>(out) == logits && dtype == FTQ_F32 && row_stride == vocab))
+        return fail(FTQ_ERR_INVALID, "out overlaps logits: only dense fp32 logits may be processed in place");
+    if (best && (!workspace || workspace_bytes < ftq_logits_workspace_bytes(rows, vocab)))
+        return fail(FTQ_ERR_WORKSPACE, "workspace needs %zu bytes, got %zu", ftq_logits_workspace_bytes(rows, vocab), workspace_bytes);
+    if (best && !aligned(workspace, 8)) return fail(FTQ_ERR_WORKSPACE, "workspace must be 8-byte aligned");
+    ftq::LogitParams p{};
+    p.logits = logits; p.row_stride = row_stride;
+    p.history = history; p.history_lens = history_lens; p.prompt_lens = prompt_lens; p.H = history_stride;
+    p.repetition = repetition; p.frequency = frequency; p.presence = presence;
+    p.bias_ids = bias_ids; p.bias = bias; p.K = n_bias;
+    p.allowed = reinterpret_cast<const uint8_t*>(allowed); p.allowed_stride = allowed_stride * 4;
+    p.tree_tokens = tree_tokens; p.tree_masks = tree_masks;
+    p.out = out; p.keys = best ? static_cast<unsigned long long*>(workspace) : nullptr;
+    p.R = n_requests; p.T = rows_per_request; p.V = vocab;
+    p.segments = (vocab - 1) / ftq::kLogitSegment + 1;
+    const cudaError_t e = ftq::launch_logits(dtype, p, best, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FTQ_OK : cuda_fail(e, "ftq_logits_process launch");
 }

@@ -33,7 +33,9 @@ namespace {
 #define FTQ_BOUND(X)                                                                       \
     X(ftq_encode) X(ftq_decode_dense) X(ftq_rht) X(ftq_decode_workspace_bytes)             \
     X(ftq_flash_decode) X(ftq_paged_store) X(ftq_paged_decode_attn) X(ftq_tq_store_layers) \
-    X(ftq_tq_decode_layers_ws) X(ftq_tq_decode_layers_workspace_bytes) X(ftq_paged_chunk_workspace_bytes) X(ftq_paged_chunk_attn)
+    X(ftq_tq_decode_layers_ws) X(ftq_tq_decode_layers_workspace_bytes) X(ftq_paged_chunk_workspace_bytes) X(ftq_paged_chunk_attn) \
+    X(ftq_pages_extend) X(ftq_pages_trim) X(ftq_tree_masks) X(ftq_tree_commit)             \
+    X(ftq_logits_workspace_bytes) X(ftq_logits_process)
 struct Api {
 #define X(name) decltype(&::name) name = nullptr;
     FTQ_BOUND(X)
@@ -679,6 +681,212 @@ PyObject* tq_decode(PyObject* const* a) {
     return THPVariable_Wrap(out);
 }
 
+// ------------------------------------------------------------------ speculative serving
+// State that a call changes: no copy of it will do.
+at::Tensor state_i32(PyObject* o, const char* name) {
+    const at::Tensor& t = cuda_tensor(o, name);
+    if (t.scalar_type() != at::kInt || !t.is_contiguous())
+        raise(PyExc_ValueError, std::string(name) + " must be a contiguous int32 tensor");
+    return t;
+}
+at::Tensor maybe_i32(PyObject* o, const char* name, const at::Device& dev) {
+    return o == Py_None ? at::Tensor() : as_i32(o, name, dev);
+}
+at::Tensor maybe_f32(PyObject* o, const char* name, const at::Device& dev) {
+    if (o == Py_None) return at::Tensor();
+    const at::Tensor& t = tensor(o, name);
+    if (t.scalar_type() == at::kFloat && t.device() == dev && t.is_contiguous()) return t;
+    return t.to(dev, at::kFloat).contiguous();
+}
+template <class T>
+const T* ptr_or_null(const at::Tensor& t) { return t.defined() ? ptr<T>(t) : nullptr; }
+void want_shape(const at::Tensor& t, at::IntArrayRef shape, const char* name) {
+    if (t.defined() && t.sizes() != shape) {
+        std::string s = std::string(name) + " must be [";
+        for (size_t i = 0; i < shape.size(); i++) s += (i ? ", " : "") + std::to_string(shape[i]);
+        raise(PyExc_ValueError, s + "]");
+    }
+}
+
+struct Pages {   // what a PageTable holds
+    at::Tensor table, lens, free_blocks, n_free;
+    explicit Pages(PyObject* const* a)
+        : table(state_i32(a[0], "block_table")), lens(state_i32(a[1], "seq_lens")),
+          free_blocks(state_i32(a[2], "free_blocks")), n_free(state_i32(a[3], "n_free")) {
+        if (table.dim() != 2 || lens.dim() != 1 || lens.size(0) != table.size(0) || free_blocks.dim() != 1 || n_free.numel() != 1)
+            raise(PyExc_ValueError, "a page table is block_table [R, max_blocks], seq_lens [R], free_blocks [num_blocks], n_free [1]");
+        for (const at::Tensor* t : {&lens, &free_blocks, &n_free})
+            if (t->device() != table.device()) raise(PyExc_ValueError, "a page table lies on one device");
+    }
+};
+
+// pages_extend(block_table, seq_lens, free_blocks, n_free, new_lens, width, packed) -> (slots, granted, starts)
+PyObject* pages_extend(PyObject* const* a) {
+    const Pages p(a);
+    const at::Device dev = p.table.device();
+    const at::Tensor m = as_i32(a[4], "new_lens", dev);
+    const long long width = as_int(a[5]), R = p.table.size(0);
+    const bool packed = as_bool(a[6]);
+    want_shape(m, {R}, "new_lens");
+    if (width < 0 || width > INT32_MAX) raise(PyExc_ValueError, "width must be 0 to 2^31 - 1, got " + std::to_string(width));
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor slots = packed ? empty({width}, at::kLong, dev) : empty({R, width}, at::kLong, dev);
+    const at::Tensor granted = empty({R}, at::kInt, dev), starts = empty({R + 1}, at::kInt, dev);
+    if (R == 0) {
+        slots.fill_(-1);
+        starts.zero_();
+    }
+    void* st = stream_of(dev);
+    int rc;
+    {
+        NoGil nogil;
+        rc = api.ftq_pages_extend(mptr<int32_t>(p.table), mptr<int32_t>(p.lens), mptr<int32_t>(p.free_blocks), mptr<int32_t>(p.n_free),
+                                  R, p.table.size(1), p.free_blocks.size(0), ptr<int32_t>(m), width, packed, mptr<int64_t>(slots),
+                                  mptr<int32_t>(granted), mptr<int32_t>(starts), st);
+    }
+    check(rc, "ftq_pages_extend");
+    Ref r0(THPVariable_Wrap(slots)), r1(THPVariable_Wrap(granted)), r2(THPVariable_Wrap(starts));
+    return PyTuple_Pack(3, r0.o, r1.o, r2.o);
+}
+
+// pages_trim(block_table, seq_lens, free_blocks, n_free, keep_lens)
+PyObject* pages_trim(PyObject* const* a) {
+    const Pages p(a);
+    const at::Device dev = p.table.device();
+    const at::Tensor keep = as_i32(a[4], "keep_lens", dev);
+    want_shape(keep, {p.table.size(0)}, "keep_lens");
+    const c10::cuda::CUDAGuard guard(dev);
+    void* st = stream_of(dev);
+    int rc;
+    {
+        NoGil nogil;
+        rc = api.ftq_pages_trim(mptr<int32_t>(p.table), mptr<int32_t>(p.lens), mptr<int32_t>(p.free_blocks), mptr<int32_t>(p.n_free),
+                                p.table.size(0), p.table.size(1), p.free_blocks.size(0), ptr<int32_t>(keep), st);
+    }
+    check(rc, "ftq_pages_trim");
+    Py_RETURN_NONE;
+}
+
+// tree_masks(parents, tree_lens, context_lens) -> (masks, positions)
+PyObject* tree_masks(PyObject* const* a) {
+    const at::Device dev = cuda_tensor(a[0], "parents").device();
+    const at::Tensor parents = as_i32(a[0], "parents", dev), lens = maybe_i32(a[1], "tree_lens", dev), ctx = maybe_i32(a[2], "context_lens", dev);
+    if (parents.dim() != 2) raise(PyExc_ValueError, "parents must be [B, n_nodes]");
+    const int64_t B = parents.size(0), T = parents.size(1);
+    want_shape(lens, {B}, "tree_lens");
+    want_shape(ctx, {B}, "context_lens");
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor masks = empty({B, T, (T + 31) / 32}, at::kInt, dev), pos = empty({B, T}, at::kInt, dev);
+    void* st = stream_of(dev);
+    int rc;
+    {
+        NoGil nogil;
+        rc = api.ftq_tree_masks(ptr<int32_t>(parents), ptr_or_null<int32_t>(lens), ptr_or_null<int32_t>(ctx), B,
+                                T > INT32_MAX ? INT32_MAX : T, mptr<int32_t>(masks), mptr<int32_t>(pos), st);
+    }
+    check(rc, "ftq_tree_masks");
+    Ref r0(THPVariable_Wrap(masks)), r1(THPVariable_Wrap(pos));
+    return PyTuple_Pack(2, r0.o, r1.o);
+}
+
+// tree_commit(pool, block_table, seq_lens, tokens, parents, next_tokens, tree_lens) -> (path, n_accepted, tokens, new_lens)
+PyObject* tree_commit(PyObject* const* a) {
+    const Pool p(a[0]);
+    const at::Device dev = p.pool.device();
+    const at::Tensor bt = as_i32(a[1], "block_table", dev), sl = as_i32(a[2], "seq_lens", dev), tok = as_i32(a[3], "tokens", dev),
+                     par = as_i32(a[4], "parents", dev), nxt = as_i32(a[5], "next_tokens", dev), tl = maybe_i32(a[6], "tree_lens", dev);
+    if (tok.dim() != 2) raise(PyExc_ValueError, "tokens must be [B, n_nodes]");
+    const int64_t B = tok.size(0), T = tok.size(1);
+    if (bt.dim() != 2 || bt.size(0) != B) raise(PyExc_ValueError, "block_table must be [B, max_blocks]");
+    want_shape(sl, {B}, "seq_lens");
+    want_shape(par, {B, T}, "parents");
+    want_shape(nxt, {B, T}, "next_tokens");
+    want_shape(tl, {B}, "tree_lens");
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor path = empty({B, T}, at::kInt, dev), n = empty({B}, at::kInt, dev), said = empty({B, T}, at::kInt, dev),
+                     lens = empty({B}, at::kInt, dev);
+    void* st = stream_of(dev);
+    int rc;
+    {
+        NoGil nogil;
+        rc = api.ftq_tree_commit(mptr(p.pool), p.num_blocks, p.layer_stride, p.n_layers, ptr<int32_t>(bt), bt.size(1), ptr<int32_t>(sl),
+                                 ptr_or_null<int32_t>(tl), ptr<int32_t>(tok), ptr<int32_t>(par), ptr<int32_t>(nxt), B,
+                                 T > INT32_MAX ? INT32_MAX : T, p.hkv, p.d, p.kb, p.vb, mptr<int32_t>(path), mptr<int32_t>(n),
+                                 mptr<int32_t>(said), mptr<int32_t>(lens), st);
+    }
+    check(rc, "ftq_tree_commit");
+    Ref r0(THPVariable_Wrap(path)), r1(THPVariable_Wrap(n)), r2(THPVariable_Wrap(said)), r3(THPVariable_Wrap(lens));
+    return PyTuple_Pack(4, r0.o, r1.o, r2.o, r3.o);
+}
+
+// logits_process(logits, history, history_lens, prompt_lens, repetition, frequency, presence, bias_ids, bias, allowed,
+//                tree_tokens, tree_masks, out, want_out, want_best) -> (out or None, best or None)
+PyObject* logits_process(PyObject* const* a) {
+    at::Tensor x = cuda_tensor(a[0], "logits");
+    if (x.dim() != 2 && x.dim() != 3) raise(PyExc_ValueError, "logits must be [requests, vocab] or [requests, rows, vocab]");
+    if (dtype_code(x.scalar_type()) < 0) raise(PyExc_ValueError, "logits must be fp32, fp16 or bf16");
+    const at::Device dev = x.device();
+    const int64_t R = x.size(0), T = x.dim() == 3 ? x.size(1) : 1, V = x.size(-1);
+    // rows may lie any distance apart, if it is the same between all of them
+    int64_t row_stride = T > 1 ? x.stride(1) : R > 1 ? x.stride(0) : V;
+    if (x.is_contiguous()) {
+        row_stride = V;
+    } else if (V <= 1 || x.stride(-1) != 1 || row_stride < V || (R > 1 && x.stride(0) != T * row_stride)) {
+        x = x.contiguous();
+        row_stride = V;
+    }
+    const at::Tensor hist = maybe_i32(a[1], "history", dev), hl = maybe_i32(a[2], "history_lens", dev), pl = maybe_i32(a[3], "prompt_lens", dev),
+                     rep = maybe_f32(a[4], "repetition", dev), freq = maybe_f32(a[5], "frequency", dev), pres = maybe_f32(a[6], "presence", dev),
+                     ids = maybe_i32(a[7], "bias_ids", dev), bias = maybe_f32(a[8], "bias", dev), tt = maybe_i32(a[10], "tree_tokens", dev),
+                     tm = maybe_i32(a[11], "tree_masks", dev);
+    at::Tensor ok = maybe_i32(a[9], "allowed", dev);
+    if (hist.defined() && (hist.dim() != 2 || hist.size(0) != R)) raise(PyExc_ValueError, "history must be [requests, tokens]");
+    if (hist.defined() != hl.defined()) raise(PyExc_ValueError, "history and history_lens go together");
+    for (const auto& [t, name] : {std::pair(&hl, "history_lens"), std::pair(&pl, "prompt_lens"), std::pair(&rep, "repetition"),
+                                  std::pair(&freq, "frequency"), std::pair(&pres, "presence")})
+        want_shape(*t, {R}, name);
+    if (ids.defined() != bias.defined()) raise(PyExc_ValueError, "bias_ids and bias go together");
+    if (ids.defined()) {
+        if (ids.dim() != 2 || ids.size(0) != R) raise(PyExc_ValueError, "bias_ids must be [requests, entries]");
+        want_shape(bias, ids.sizes(), "bias");
+    }
+    if (ok.defined() && (ok.numel() == 0 ? R * T != 0 : ok.numel() / ok.size(-1) != R * T || ok.size(-1) < (V + 31) / 32))
+        raise(PyExc_ValueError, "allowed must be [requests, rows, ceil(vocab / 32)]");
+    if (tt.defined() != tm.defined()) raise(PyExc_ValueError, "tree_tokens and tree_masks go together");
+    want_shape(tt, {R, T}, "tree_tokens");
+    want_shape(tm, {R, T, (T + 31) / 32}, "tree_masks");
+    const c10::cuda::CUDAGuard guard(dev);
+    const bool want_out = as_bool(a[13]), want_best = as_bool(a[14]);
+    at::Tensor out, best;
+    if (a[12] != Py_None) {
+        out = cuda_tensor(a[12], "out");
+        if (out.scalar_type() != at::kFloat || !out.is_contiguous() || out.device() != dev) raise(PyExc_ValueError, "out must be a contiguous fp32 tensor on the logits' device");
+        want_shape(out, x.sizes(), "out");
+    } else if (want_out) {
+        out = empty(x.sizes(), at::kFloat, dev);
+    }
+    if (want_best) best = empty(x.sizes().slice(0, x.dim() - 1), at::kInt, dev);
+    void* st = stream_of(dev);
+    const size_t need = want_best ? api.ftq_logits_workspace_bytes(R * T, V) : 0;
+    at::Tensor ws;
+    if (need) ws = workspace(Py_None, dev, st, need);
+    int rc;
+    {
+        NoGil nogil;
+        rc = api.ftq_logits_process(ptr<void>(x), dtype_code(x.scalar_type()), row_stride, R, T, V, ptr_or_null<int32_t>(hist),
+                                    hist.defined() ? hist.size(1) : 0, ptr_or_null<int32_t>(hl), ptr_or_null<int32_t>(pl),
+                                    ptr_or_null<float>(rep), ptr_or_null<float>(freq), ptr_or_null<float>(pres), ptr_or_null<int32_t>(ids),
+                                    ptr_or_null<float>(bias), ids.defined() ? ids.size(1) : 0, ptr_or_null<int32_t>(ok),
+                                    ok.defined() ? ok.size(-1) : 0, ptr_or_null<int32_t>(tt), ptr_or_null<int32_t>(tm),
+                                    out.defined() ? mptr<float>(out) : nullptr, best.defined() ? mptr<int32_t>(best) : nullptr,
+                                    ws.defined() ? mptr<void>(ws) : nullptr, ws.defined() ? ws.numel() : 0, st);
+    }
+    check(rc, "ftq_logits_process");
+    Ref r0(out.defined() ? a[12] != Py_None ? Py_NewRef(a[12]) : THPVariable_Wrap(out) : Py_NewRef(Py_None));
+    Ref r1(best.defined() ? THPVariable_Wrap(best) : Py_NewRef(Py_None));
+    return PyTuple_Pack(2, r0.o, r1.o);
+}
+
 // bind({name: address}, check, get_workspace, workspaces, host_table)
 PyObject* bind(PyObject* const* a) {
 #define X(name)                                                                     \
@@ -721,6 +929,11 @@ PyMethodDef methods[] = {
     FTQ_ENTRY(flash_decode, 15),
     FTQ_ENTRY(tq_store, 9),
     FTQ_ENTRY(tq_decode, 21),
+    FTQ_ENTRY(pages_extend, 7),
+    FTQ_ENTRY(pages_trim, 5),
+    FTQ_ENTRY(tree_masks, 3),
+    FTQ_ENTRY(tree_commit, 7),
+    FTQ_ENTRY(logits_process, 15),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", "Tensor-level host path over libftq_b200.so.",
                           -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -15,6 +15,7 @@ import ctypes
 import torch
 
 from . import _lib, _trace, codebook, kernels
+from .tree import Accepted
 from .kernels import _DT, _host_table, _ptr, _require_cuda, _stream
 
 logger = _trace.get_logger(__name__)
@@ -194,6 +195,18 @@ class PagedKVPool:
         out = self.decode_attention(q.reshape(B * q_len, Hq, D), synth_bt, synth_sl, max_seq_len,
                                     scale, layer=layer)
         return out.view(B, q_len, Hq, D)
+
+    def tree_commit(self, block_table: torch.Tensor, seq_lens: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor,
+                    next_tokens: torch.Tensor, tree_lens: torch.Tensor | None = None) -> Accepted:
+        """Accept a path of every sequence's drafted tree and move its keys and values behind the context, in all layers.
+
+        tokens, parents, next_tokens: [B, n_nodes] (the tree as in ``tree``, and the target model's choice after each
+        node); seq_lens [B] count the tree's ``tree_lens[b]`` (all of them without it) nodes, which are stored behind the context in
+        their order.  Node 0 is accepted; after a node its lowest child whose token is the target's choice.  The
+        lengths it returns are those to keep (``PageTable.trim``); ``seq_lens`` itself is not changed.
+        """
+        _require_cuda(self.pool, "pool")
+        return Accepted(*_lib.native().tree_commit(self, block_table, seq_lens, tokens, parents, next_tokens, tree_lens))
 
 
 def synthetic_decode_batch(block_table: torch.Tensor, seq_lens: torch.Tensor, q_len: int):

@@ -445,6 +445,100 @@ int ftq_tq_decode_layers_ws(const void *q, int q_dtype, int B, int Hq, int Hkv, 
                             int n_layers, int64_t cache_layer_stride, int64_t num_blocks,
                             void *workspace, size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------------- speculative serving */
+
+/*
+ * No counterpart in the reference (its engine keeps pages on the host and verifies drafts as
+ * chains).  A serving step that drafts a tree of tokens for every request: pages for the tree
+ * (ftq_pages_extend), its keys and values stored (ftq_paged_store), every node attends the
+ * context and its own ancestors (ftq_tree_masks, ftq_tree_attn), logits of all nodes
+ * (ftq_logits_process), the accepted path moved behind the context (ftq_tree_commit), the
+ * other pages given back (ftq_pages_trim).
+ */
+
+/* Nodes of a tree, and requests of a page table, at most. */
+#define FTQ_TREE_MAX_NODES 256
+#define FTQ_PAGES_MAX_REQUESTS 8192
+
+/*
+ * Pages of requests, kept on the device: block_table [R, max_blocks], seq_lens [R], a stack
+ * free_blocks [num_blocks] of which the first *n_free entries are free (the last of them is
+ * taken first).  All four are read and changed in place.
+ *
+ * ftq_pages_extend: request r, of n tokens, gets new_lens[r] = m more.  It needs
+ * ceil((n + m) / 16) - ceil(n / 16) further blocks and is granted all of its tokens or none:
+ * none if m < 0, if the tokens do not fit its row of the table or the slot map, or if
+ * the needs of the requests up to and including this one (those that fit) exceed the free blocks and it
+ * needs any.  Written: granted [R]; starts [R + 1]; slots (block * 16 + offset, -1 where
+ * there is no token): [R, width], starts[r] = r * width, or, packed, [width] with the
+ * requests' tokens back to back (starts: the running sum of new_lens, negative ones as 0).
+ *
+ * ftq_pages_trim: request r keeps its first keep_lens[r] tokens (at most what it has; 0 ends
+ * it); blocks without a token go back to the stack and their table entries become -1.
+ * Trimming what the last ftq_pages_extend granted restores the stack.
+ */
+int ftq_pages_extend(int32_t *block_table, int32_t *seq_lens, int32_t *free_blocks, int32_t *n_free,
+                     int n_requests, int max_blocks, int num_blocks, const int32_t *new_lens,
+                     int width, int packed, int64_t *slots, int32_t *granted, int32_t *starts,
+                     void *stream);
+int ftq_pages_trim(int32_t *block_table, int32_t *seq_lens, int32_t *free_blocks, int32_t *n_free,
+                   int n_requests, int max_blocks, int num_blocks, const int32_t *keep_lens,
+                   void *stream);
+
+/*
+ * Ancestor masks of drafted trees.  parents [B, n_nodes]: the index of a node's parent, below
+ * its own; anything else is a root.  tree_lens [B] (NULL: n_nodes): nodes that exist.
+ * masks [B, n_nodes, ceil(n_nodes / 32)]: bit j % 32 of word j / 32 is set where j is the node
+ * or one of its ancestors (none for nodes that do not exist).  positions [B, n_nodes]:
+ * context_lens[b] (NULL: 0) + the node's depth.
+ */
+int ftq_tree_masks(const int32_t *parents, const int32_t *tree_lens, const int32_t *context_lens,
+                   int B, int n_nodes, int32_t *masks, int32_t *positions, void *stream);
+
+/*
+ * Greedy acceptance of drafted trees, and their cache.  seq_lens [B] count the tree's
+ * tree_lens[b] (NULL: n_nodes) tokens, which lie behind the context in the order of the nodes.  Node 0
+ * is accepted (it is the token that the last step ended with); after node c follows the lowest
+ * child of c whose token equals next_tokens[c], the target model's choice there.  Written: path
+ * [B, n_nodes] (accepted nodes, then -1), n_accepted [B], out_tokens [B, n_nodes] (next_tokens
+ * along the path, then -1: the step's new tokens), new_lens [B] = context + n_accepted.  The
+ * compressed keys and values of path[k] move to position context + k in all layers of the pool;
+ * what lies behind new_lens is unspecified.  A block id out of range is not followed.  new_lens
+ * and n_accepted may not lie on seq_lens or tree_lens.
+ */
+int ftq_tree_commit(uint8_t *pool, int64_t num_blocks, int64_t pool_layer_stride, int n_layers,
+                    const int32_t *block_table, int max_blocks, const int32_t *seq_lens,
+                    const int32_t *tree_lens, const int32_t *tokens, const int32_t *parents,
+                    const int32_t *next_tokens, int B, int n_nodes, int Hkv, int head_dim,
+                    int bits_k, int bits_v, int32_t *path, int32_t *n_accepted,
+                    int32_t *out_tokens, int32_t *new_lens, void *stream);
+
+/*
+ * Logits of a step: penalties for repeated tokens, biases, masks, the best token.  logits:
+ * rows_per_request rows of each request, `vocab` values of `dtype` each, row_stride elements apart.
+ *   history [R, history_stride], history_lens [R]: a request's tokens, of which the first
+ *     prompt_lens[r] (NULL: none) are its prompt and the others its answer (history NULL: none);
+ *   tree_tokens [R, rows], tree_masks [R, rows, ceil(rows / 32)] (both or neither): a row is a
+ *     node of a drafted tree, and the tokens of the nodes in its mask count as answer too.
+ *   x > 0 ? x / repetition[r] : x * repetition[r] for tokens of the prompt or the answer; then
+ *   - frequency[r] * (times in the answer) - presence[r] for tokens of the answer (NULL: no such
+ *   penalty); + bias [R, n_bias] at bias_ids (negative or >= vocab: unused; of equal ids the
+ *   last); -inf where bit v % 32 of word v / 32 of a row of allowed is clear (rows
+ *   allowed_stride words apart; NULL: all are allowed).  Each operation rounds once in fp32.
+ * out: fp32 [R * rows, vocab], NULL: not written; dense fp32 logits may be processed in place.
+ * best [R * rows] (NULL: not wanted): the lowest index of the largest value, NaN above all; needs
+ * a workspace of ftq_logits_workspace_bytes(R * rows, vocab) bytes.
+ */
+size_t ftq_logits_workspace_bytes(int64_t n_rows, int vocab);
+int ftq_logits_process(const void *logits, int dtype, int64_t row_stride, int n_requests,
+                       int rows_per_request, int vocab, const int32_t *history, int history_stride,
+                       const int32_t *history_lens, const int32_t *prompt_lens,
+                       const float *repetition, const float *frequency, const float *presence,
+                       const int32_t *bias_ids, const float *bias, int n_bias,
+                       const int32_t *allowed, int64_t allowed_stride, const int32_t *tree_tokens,
+                       const int32_t *tree_masks, float *out, int32_t *best, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
