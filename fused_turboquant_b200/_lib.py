@@ -65,6 +65,9 @@ SIGNATURES = {
     "ftq_pages_extend": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _i, _vp, _vp, _vp, _vp]),
     "ftq_pages_trim": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp]),
     "ftq_tree_masks": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp]),
+    "ftq_tree_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "ftq_tree_attn": (_i, [_vp, _i, _vp, _i, _vp, _i64, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _fp,
+                           _fp, _fp, _f, _vp, _sz, _vp]),
     "ftq_tree_commit": (_i, [_vp, _i64, _i64, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp,
                              _vp, _vp, _vp, _vp]),
     "ftq_logits_workspace_bytes": (_sz, [_i64, _i]),

@@ -22,7 +22,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 OBJ_DIR = os.path.join(PKG_DIR, "build")
 LIB_PATH = os.path.join(PKG_DIR, "libftq_b200.so")
 # A second library for ONE test (tests/test_gpu_wait_expiry.py): the same objects, except that the
-# head_dim-128 decode, chunk attention and slot-format decode units are compiled with FTQ_TEST_WAIT_EXPIRY (one page copy of
+# head_dim-128 decode, chunk attention, tree attention (4-bit) and slot-format decode units are compiled with FTQ_TEST_WAIT_EXPIRY (one page copy of
 # one warp is never issued, one tile of one warp never reported, and the poll limits are small), so that
 # a bounded wait runs out and the give-up path (NaN rows, status word, the context stays usable)
 # executes.  Never loaded by the package.
@@ -32,7 +32,8 @@ TEST_LIB_PATH = os.path.join(PKG_DIR, "libftq_b200_waittest.so")
 NATIVE_PATH = os.path.join(PKG_DIR, "_native.so")
 TEST_UNITS = [(src, f"{tag}_waittest", [*part, "-DFTQ_D=128", "-DFTQ_ONLY_BITS=4", "-DFTQ_TEST_WAIT_EXPIRY"])
               for src, tag, part in (("ftq_attn_inst.cu", "attn_d128", ()), ("ftq_attn_chunk_inst.cu", "attn_chunk_d128", ()),
-                                     ("ftq_tq_v1_inst.cu", "tq_v1_flow_d128", ("-DFTQ_TQ_PART=2",)))]
+                                     ("ftq_tq_v1_inst.cu", "tq_v1_flow_d128", ("-DFTQ_TQ_PART=2",)),
+                                     ("ftq_tree_attn_inst.cu", "tree_attn_d128_k4", ("-DFTQ_BK=4",)))]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -47,6 +48,10 @@ for _d in (256, 128, 64):
     UNITS.append(("ftq_tq_v1_inst.cu", f"tq_v1_decode_d{_d}", [f"-DFTQ_D={_d}", "-DFTQ_TQ_PART=1"]))
     if _d != 256:   # (not for that size)
         UNITS.append(("ftq_tq_v1_inst.cu", f"tq_v1_flow_d{_d}", [f"-DFTQ_D={_d}", "-DFTQ_TQ_PART=2"]))
+for _d in (256, 128, 64):
+    for _b in (4, 3, 2):
+        UNITS.append(("ftq_tree_attn_inst.cu", f"tree_attn_d{_d}_k{_b}", [f"-DFTQ_D={_d}", f"-DFTQ_BK={_b}"]))
+UNITS.append(("ftq_tree_attn_inst.cu", "tree_merge", ["-DFTQ_D=0"]))
 for _d in (256, 128, 64):
     UNITS.append(("ftq_attn_inst.cu", f"attn_d{_d}", [f"-DFTQ_D={_d}"]))
     UNITS.append(("ftq_attn_chunk_inst.cu", f"attn_chunk_d{_d}", [f"-DFTQ_D={_d}"]))

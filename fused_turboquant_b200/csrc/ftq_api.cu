@@ -18,6 +18,7 @@
 #include "ftq_dense.cuh"
 #include "ftq_launch.h"
 #include "ftq_serve_launch.h"
+#include "ftq_tree_launch.h"
 #include "ftq_tq_v1_launch.h"
 
 namespace {
@@ -1704,4 +1705,110 @@ extern "C" int ftq_logits_process(const void* logits, int dtype, int64_t row_str
     p.segments = (vocab - 1) / ftq::kLogitSegment + 1;
     const cudaError_t e = ftq::launch_logits(dtype, p, best, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? FTQ_OK : cuda_fail(e, "ftq_logits_process launch");
+}
+
+// ------------------------------------------------------------------ attention of drafted trees
+
+namespace {
+struct TreeLayout {   // of the workspace, behind a decode workspace of one sequence (whose status word it uses)
+    int n, row_tiles;                        // rows of a product, row tiles of a KV head
+    size_t plan, whole, cut, end;
+};
+TreeLayout tree_layout(int B, int n_nodes, int Hq, int Hkv, int d, size_t head) {
+    const int rows = n_nodes * (Hq / Hkv), n = ftq::tree_rows(d, rows), tiles = (rows + n - 1) / n;
+    const int seqs = std::min(B, ftq::kTreeMaxSeqs);
+    const size_t row = static_cast<size_t>(n) * (d + 4) * sizeof(float);
+    TreeLayout l{n, tiles, (head + 255) / 256 * 256, 0, 0, 0};
+    l.whole = l.plan + (static_cast<size_t>(seqs + 2) * sizeof(int) + 255) / 256 * 256;
+    l.cut = l.whole + static_cast<size_t>(seqs) * Hkv * tiles * row;
+    l.end = l.cut + 2 * static_cast<size_t>(ftq::sm_count()) * row;
+    return l;
+}
+}  // namespace
+
+extern "C" size_t ftq_tree_workspace_bytes(int B, int n_nodes, int Hq, int Hkv, int head_dim, int max_seq_len) {
+    if (B <= 0 || n_nodes <= 0 || n_nodes > ftq::kTreeMaxNodes) return 0;
+    const size_t head = ftq_decode_workspace_bytes(1, Hq, Hkv, head_dim, max_seq_len, 1);
+    return head == 0 ? 0 : tree_layout(B, n_nodes, Hq, Hkv, head_dim, head).end;
+}
+
+extern "C" int ftq_tree_attn(const void* q, int q_dtype, void* out, int out_dtype, const uint8_t* pool, int64_t num_blocks,
+                             const int32_t* block_table, int max_blocks, const int32_t* seq_lens, int max_seq_len,
+                             const int32_t* tree_lens, const int32_t* masks, int B, int n_nodes, int Hq, int Hkv,
+                             int head_dim, int bits_k, int bits_v, const float* levels_k_host,
+                             const float* levels_v_host, const float* signs_host, float scale, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+    int rc = check_attn_common(B, Hq, Hkv, head_dim, bits_k, bits_v, q_dtype, out_dtype);
+    if (rc) return rc;
+    if (q_dtype == FTQ_F32) return fail(FTQ_ERR_UNSUPPORTED, "tree attention takes 16-bit queries");
+    if (n_nodes <= 0 || n_nodes > ftq::kTreeMaxNodes)
+        return fail(FTQ_ERR_UNSUPPORTED, "a tree has 1 to %d nodes, got %d", ftq::kTreeMaxNodes, n_nodes);
+    if (max_blocks <= 0 || max_seq_len < 0 || num_blocks < 0)
+        return fail(FTQ_ERR_INVALID, "bad shape max_blocks=%d max_seq_len=%d", max_blocks, max_seq_len);
+    if (B == 0) return FTQ_OK;
+    if (!q || !out || !pool || !block_table || !seq_lens || !masks) return fail(FTQ_ERR_INVALID, "NULL tensor pointer");
+    if (static_cast<int64_t>(max_blocks) * FTQ_PAGE_TOKENS < max_seq_len)
+        return fail(FTQ_ERR_INVALID, "block_table too narrow: %d blocks < max_seq_len %d", max_blocks, max_seq_len);
+    if (!aligned(q, 16) || !aligned(out, 4) || !aligned(pool, 16))
+        return fail(FTQ_ERR_INVALID, "q and pool must be 16-byte aligned");
+    const size_t need = ftq_tree_workspace_bytes(B, n_nodes, Hq, Hkv, head_dim, max_seq_len);
+    if (!workspace || workspace_bytes < need)
+        return fail(FTQ_ERR_WORKSPACE, "workspace needs %zu bytes, got %zu", need, workspace_bytes);
+    if (!aligned(workspace, 16)) return fail(FTQ_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+    const size_t head = ftq_decode_workspace_bytes(1, Hq, Hkv, head_dim, max_seq_len, 1);
+    const TreeLayout l = tree_layout(B, n_nodes, Hq, Hkv, head_dim, head);
+    const int seqs = std::min(B, ftq::kTreeMaxSeqs), group = Hq / Hkv;
+    const int64_t places = (static_cast<int64_t>(max_seq_len) / ftq::kTreeTile + 1 + ftq::kTreePiece) * Hkv * l.row_tiles;
+    if (places * seqs > INT32_MAX / 2) return fail(FTQ_ERR_UNSUPPORTED, "too many tokens, heads and nodes for one call");
+    ftq::TreeAttnParams p{};
+    rc = pack_levels(levels_k_host, bits_k, &p.lk);
+    if (rc == FTQ_OK) rc = pack_levels(levels_v_host, bits_v, &p.lv);
+    if (rc == FTQ_OK) rc = pack_signs(signs_host, head_dim, &p.signs);
+    if (rc) return rc;
+    const float ks = choose_k_scale(levels_k_host, bits_k, head_dim);
+    for (int i = 0; i < (1 << bits_k); i++) p.lk.v[i] = levels_k_host[i] * ks;
+    const float vs = choose_v_scale(levels_v_host, bits_v, head_dim);
+    for (int i = 0; i < (1 << bits_v); i++) p.lv.v[i] = levels_v_host[i] * vs;
+    p.inv_v_scale = 1.0f / vs;
+    p.q_scale = rsqrt_dim(head_dim) * (scale / ks * ftq::kLog2e);
+    p.pool = pool; p.num_blocks = num_blocks; p.max_blocks = max_blocks;
+    p.max_seq = max_seq_len; p.T = n_nodes; p.W = (n_nodes + 31) / 32; p.Hq = Hq; p.Hkv = Hkv; p.q_dtype = q_dtype;
+    p.row_tiles = l.row_tiles; p.group = ftq::make_fastdiv(group);
+    uint8_t* const ws = static_cast<uint8_t*>(workspace);
+    p.plan = reinterpret_cast<int*>(ws + l.plan);
+    p.whole = reinterpret_cast<float*>(ws + l.whole);
+    p.cut = reinterpret_cast<float*>(ws + l.cut);
+    int* const counters = reinterpret_cast<int*>(ws + head - counter_bytes(1, Hkv, 1));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    for (int b0 = 0; b0 < B; b0 += seqs) {
+        const size_t vec = static_cast<size_t>(b0) * n_nodes * Hq * head_dim;
+        p.B = std::min(seqs, B - b0);
+        p.q = static_cast<const uint8_t*>(q) + vec * dtype_size(q_dtype);
+        p.block_table = block_table + static_cast<int64_t>(b0) * max_blocks;
+        p.seq_lens = seq_lens + b0;
+        p.tree_lens = tree_lens ? tree_lens + b0 : nullptr;
+        p.masks = masks + static_cast<int64_t>(b0) * n_nodes * p.W;
+        const ftq::MergeStatus status{counters + ftq::kStatusWord, reinterpret_cast<unsigned long long*>(counters + 8), next_epoch()};
+        p.errors = status.errors;
+        p.epoch = status.epoch;
+        const int grid = ftq::sm_count();
+        cudaError_t e = cudaErrorInvalidValue;
+        switch (head_dim * 10 + bits_k) {
+#define FTQ_TREE_CASE(DD, KB) case DD * 10 + KB: e = ftq::launch_tree_attn_d##DD##_k##KB(bits_v, l.n, p, grid, st); break;
+            FTQ_TREE_CASE(64, 2) FTQ_TREE_CASE(64, 3) FTQ_TREE_CASE(64, 4)
+            FTQ_TREE_CASE(128, 2) FTQ_TREE_CASE(128, 3) FTQ_TREE_CASE(128, 4)
+            FTQ_TREE_CASE(256, 2) FTQ_TREE_CASE(256, 3) FTQ_TREE_CASE(256, 4)
+#undef FTQ_TREE_CASE
+        }
+        if (e != cudaSuccess) return cuda_fail(e, "ftq_tree_attn launch");
+        ftq::TreeMergeParams m{};
+        m.plan = p.plan; m.whole = p.whole; m.cut = p.cut;
+        m.tree_lens = p.tree_lens; m.seq_lens = p.seq_lens;
+        m.out = static_cast<uint8_t*>(out) + vec * dtype_size(out_dtype);
+        m.B = p.B; m.T = n_nodes; m.Hq = Hq; m.Hkv = Hkv; m.N = l.n; m.row_tiles = l.row_tiles; m.max_seq = max_seq_len;
+        m.group = p.group; m.rsqrt_d = rsqrt_dim(head_dim); m.signs = p.signs; m.status = status; m.more = b0 > 0;
+        e = ftq::launch_tree_merge(head_dim, out_dtype, m, st);
+        if (e != cudaSuccess) return cuda_fail(e, "ftq_tree_attn merge launch");
+    }
+    return FTQ_OK;
 }

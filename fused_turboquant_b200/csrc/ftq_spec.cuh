@@ -55,6 +55,7 @@ __device__ __forceinline__ int pages_of(int tokens) { return (tokens + kPageToke
 
 __device__ __forceinline__ void cluster_barrier(int ctas) {
     if (ctas > 1) {
+        __syncwarp();
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
     } else {
         __syncthreads();

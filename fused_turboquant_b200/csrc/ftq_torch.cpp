@@ -35,6 +35,7 @@ namespace {
     X(ftq_flash_decode) X(ftq_paged_store) X(ftq_paged_decode_attn) X(ftq_tq_store_layers) \
     X(ftq_tq_decode_layers_ws) X(ftq_tq_decode_layers_workspace_bytes) X(ftq_paged_chunk_workspace_bytes) X(ftq_paged_chunk_attn) \
     X(ftq_pages_extend) X(ftq_pages_trim) X(ftq_tree_masks) X(ftq_tree_commit)             \
+    X(ftq_tree_workspace_bytes) X(ftq_tree_attn)                                           \
     X(ftq_logits_workspace_bytes) X(ftq_logits_process)
 struct Api {
 #define X(name) decltype(&::name) name = nullptr;
@@ -789,6 +790,58 @@ PyObject* tree_masks(PyObject* const* a) {
     return PyTuple_Pack(2, r0.o, r1.o);
 }
 
+// paged_tree(self, q, block_table, seq_lens, max_seq_len, masks, tree_lens, scale, layer, out, workspace)
+PyObject* paged_tree(PyObject* const* a) {
+    PyObject* self = a[0];
+    at::Tensor q = cuda_tensor(a[1], "q");
+    if (!q.is_contiguous()) q = q.contiguous();
+    const Pool p(self);
+    if (q.dim() != 4 || q.size(3) != p.d) raise(PyExc_ValueError, "q must be [B, n_nodes, Hq, " + std::to_string(p.d) + "]");
+    if (dtype_code(q.scalar_type()) < 0) raise(PyExc_ValueError, "q must be fp16 or bf16");
+    const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), D = q.size(3);
+    const double scale = a[7] == Py_None ? std::pow(static_cast<double>(D), -0.5) : as_double(a[7]);
+    const at::Device dev = q.device();
+    const at::Tensor bt = as_i32(a[2], "block_table", dev), sl = as_i32(a[3], "seq_lens", dev), tm = as_i32(a[5], "masks", dev),
+                     tl = maybe_i32(a[6], "tree_lens", dev);
+    const long long max_seq = as_int(a[4]);
+    if (bt.dim() != 2 || bt.size(0) != B) raise(PyExc_ValueError, "block_table must be [B, max_blocks]");
+    if (max_seq < 0 || max_seq > INT32_MAX) raise(PyExc_ValueError, "max_seq_len must be 0 to 2^31 - 1, got " + std::to_string(max_seq));
+    want_shape(sl, {B}, "seq_lens");
+    want_shape(tm, {B, T, (T + 31) / 32}, "masks");
+    want_shape(tl, {B}, "tree_lens");
+    const c10::cuda::CUDAGuard guard(dev);
+    at::Tensor out;
+    if (a[9] == Py_None) {
+        out = empty(q.sizes(), q.scalar_type(), dev);
+    } else {
+        out = cuda_tensor(a[9], "out");
+        if (!out.is_contiguous() || out.device() != dev) raise(PyExc_ValueError, "out must be contiguous and on q's device");
+        want_shape(out, q.sizes(), "out");
+    }
+    const int oc = out_dtype_code(out);
+    void* st = stream_of(dev);
+    const int nodes = T > INT32_MAX ? INT32_MAX : static_cast<int>(T);
+    const at::Tensor ws = workspace(a[10], dev, st, api.ftq_tree_workspace_bytes(B, nodes, Hq, p.hkv, p.d, max_seq));
+    uint8_t* base = p.base(a[8]);
+    Ref so(PyObject_GetAttr(self, names.signs)), ko(PyObject_GetAttr(self, names.levels_k)),
+        vo(PyObject_GetAttr(self, names.levels_v));
+    const Table signs(so.o), lk(ko.o), lv(vo.o);
+    int rc;
+    {
+        NoGil nogil;
+        rc = api.ftq_tree_attn(ptr<void>(q), dtype_code(q.scalar_type()), mptr<void>(out), oc, base, p.num_blocks, ptr<int32_t>(bt),
+                               bt.size(1), ptr<int32_t>(sl), max_seq, ptr_or_null<int32_t>(tl), ptr<int32_t>(tm), B, nodes, Hq, p.hkv, D,
+                               p.kb, p.vb, lk.p, lv.p, signs.p, static_cast<float>(scale), mptr<void>(ws), ws.nbytes(), st);
+    }
+    check(rc, "ftq_tree_attn");
+    // (the status word lies where a decode call of one sequence has it)
+    Ref w(THPVariable_Wrap(ws)), d(THPDevice_New(dev));
+    Ref last(Py_BuildValue("(OLLLLO)", w.o, 1ll, static_cast<long long>(Hq), max_seq, 1ll, d.o));
+    if (PyObject_SetAttr(self, names._last_decode, last.o) < 0) throw PyError{};
+    if (a[9] != Py_None) return Py_NewRef(a[9]);
+    return THPVariable_Wrap(out);
+}
+
 // tree_commit(pool, block_table, seq_lens, tokens, parents, next_tokens, tree_lens) -> (path, n_accepted, tokens, new_lens)
 PyObject* tree_commit(PyObject* const* a) {
     const Pool p(a[0]);
@@ -932,6 +985,7 @@ PyMethodDef methods[] = {
     FTQ_ENTRY(pages_extend, 7),
     FTQ_ENTRY(pages_trim, 5),
     FTQ_ENTRY(tree_masks, 3),
+    FTQ_ENTRY(paged_tree, 11),
     FTQ_ENTRY(tree_commit, 7),
     FTQ_ENTRY(logits_process, 15),
     {nullptr, nullptr, 0, nullptr}};

@@ -196,6 +196,26 @@ class PagedKVPool:
                                     scale, layer=layer)
         return out.view(B, q_len, Hq, D)
 
+    def tree_workspace_bytes(self, batch: int, n_nodes: int, num_q_heads: int, max_seq_len: int) -> int:
+        return int(_lib.load().ftq_tree_workspace_bytes(batch, n_nodes, num_q_heads, self.num_kv_heads, self.head_dim, max_seq_len))
+
+    def tree_attention(self, q: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, max_seq_len: int,
+                       masks: torch.Tensor, tree_lens: torch.Tensor | None = None, scale: float | None = None,
+                       layer: int = 0, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of a drafted tree per sequence, its keys and values stored behind the context in the order of its nodes.
+
+        q: [B, n_nodes, Hq, D], fp16 or bf16, not rotated; seq_lens [B] count the tree's ``tree_lens[b]`` (all of them
+        without it) nodes.  Node i attends the context and the nodes whose bits are set in ``masks[b, i]`` (int32 words as
+        ``tree.ancestor_masks`` makes them; any masks will do).  Rows that attend nothing and nodes that do not exist are zero.
+        No host synchronisation; graph-capturable when out / workspace are passed in.  ``decode_status`` covers this call too.
+        """
+        _require_cuda(q, "q")
+        if _trace.ENABLED:
+            with _trace.nvtx("ftq.decode"):
+                return _lib.native().paged_tree(self, q, block_table, seq_lens, max_seq_len, masks, tree_lens, scale, layer, out,
+                                                workspace)
+        return _lib.native().paged_tree(self, q, block_table, seq_lens, max_seq_len, masks, tree_lens, scale, layer, out, workspace)
+
     def tree_commit(self, block_table: torch.Tensor, seq_lens: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor,
                     next_tokens: torch.Tensor, tree_lens: torch.Tensor | None = None) -> Accepted:
         """Accept a path of every sequence's drafted tree and move its keys and values behind the context, in all layers.

@@ -496,6 +496,26 @@ int ftq_tree_masks(const int32_t *parents, const int32_t *tree_lens, const int32
                    int B, int n_nodes, int32_t *masks, int32_t *positions, void *stream);
 
 /*
+ * Attention of drafted trees over one layer of the pool, the trees' keys and values stored.
+ * q / out: [B, n_nodes, Hq, head_dim], 16-bit queries; seq_lens [B] count the tree's tree_lens[b]
+ * (NULL: n_nodes; at most n_nodes and seq_lens[b]) tokens, which lie behind the context in the order of the
+ * nodes.  Node i attends every token of the context and the nodes j (of those that exist) whose bit
+ * j % 32 is set in word j / 32 of masks[b][i] (ftq_tree_masks makes them; any others will do, a node's own
+ * bit included or not).  Rows that attend nothing, and nodes that do not exist, are zero.  The
+ * other arguments are those of ftq_paged_decode_attn.  The workspace holds at least
+ * ftq_tree_workspace_bytes(...) bytes, 16-byte aligned; the call's status is read with
+ * ftq_paged_decode_status(workspace, 1, Hq, Hkv, head_dim, max_seq_len, 1, ...).
+ */
+size_t ftq_tree_workspace_bytes(int B, int n_nodes, int Hq, int Hkv, int head_dim, int max_seq_len);
+int ftq_tree_attn(const void *q, int q_dtype, void *out, int out_dtype, const uint8_t *pool,
+                  int64_t num_blocks, const int32_t *block_table, int max_blocks,
+                  const int32_t *seq_lens, int max_seq_len, const int32_t *tree_lens,
+                  const int32_t *masks, int B, int n_nodes, int Hq, int Hkv, int head_dim, int bits_k,
+                  int bits_v, const float *levels_k_host, const float *levels_v_host,
+                  const float *signs_host, float scale, void *workspace, size_t workspace_bytes,
+                  void *stream);
+
+/*
  * Greedy acceptance of drafted trees, and their cache.  seq_lens [B] count the tree's
  * tree_lens[b] (NULL: n_nodes) tokens, which lie behind the context in the order of the nodes.  Node 0
  * is accepted (it is the token that the last step ended with); after node c follows the lowest
