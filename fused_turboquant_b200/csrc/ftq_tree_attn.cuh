@@ -15,10 +15,12 @@
 // that a quad of lanes reads a token's codes as they lie (16 bytes a lane, whole half pages a warp) and no value is
 // moved between lanes: a 16x256b store to TMEM puts lane 4g + t's codes into row g, columns 8j + 2t.
 //
-// Lazy maxima: a row's weights refer to the largest score of an earlier tile (m); while no score is above m + 3 (base 2) a
+// Lazy maxima: a row's weights refer to the largest score of an earlier tile (m); while no score is above m + 13 (base 2) a
 // tile costs one vote per 32 rows.  Otherwise the warpgroup finds the new maxima and rescales O and the sums.
-// Weights are fp16: p * |v| scaled by a power of two that keeps it between 2^-14 and 2^15 whatever the norms are; queries
-// are scaled to 2^13 the same way.  Scores, sums and O are fp32.
+// (With a slack of 3, as in the decode kernels, half of the tiles did: of 32 rows there is always one that has found a
+// larger score.)  Weights are fp16: |v| is scaled by a power of two, so that the largest so far is 1 to 2, and again when
+// one of 4 or more comes; p * |v| is then at most 2^15, and a weight of 2^-14 of the largest still has all its bits.
+// Queries are scaled the same way.  Scores, sums and O are fp32.
 //
 // Work: units (sequence, KV head, row tile) in a line of places, a place per tile of 128 tokens and kTreePiece more per
 // unit, cut into equal shares, one per CTA (one CTA per SM).  Every piece leaves its rows (O, m, l) in the
@@ -36,6 +38,7 @@ namespace ftq {
 constexpr int kTreeTile = 128;         // tokens of a tile
 constexpr int kTreePiece = 3;          // places that a unit costs besides its tiles
 constexpr int kTreeMaxSeqs = 1024;     // sequences of a launch
+constexpr float kTreeSlack = 13.f, kTreeGrowth = 4.f;
 
 struct TreeAttnParams {
     const void* q;              // [B, T, Hq, D]
@@ -66,9 +69,9 @@ struct TreeCfg {
     static constexpr int WG = N > 32 ? 2 : 1;              // softmax warpgroups
     static constexpr int CW = N / WG;                      // rows of one
     static constexpr int CH = CW < 32 ? CW : 32, NCH = CW / CH;
-    // warps: softmax; keys; values; the products; queries and masks
-    static constexpr int SM_WARPS = 4 * WG, W_K = SM_WARPS, W_V = W_K + 4, W_MMA = W_K + 8, W_Q = W_MMA + 1;
-    static constexpr int Q_WARPS = 3, WARPS = W_Q + Q_WARPS, THREADS = 32 * WARPS;
+    // warps: softmax; keys; values; the products; addresses and norms; queries and masks
+    static constexpr int SM_WARPS = 4 * WG, W_K = SM_WARPS, W_V = W_K + 4, W_MMA = W_K + 8, W_FEED = W_MMA + 1, W_Q = W_MMA + 2;
+    static constexpr int Q_WARPS = 2, WARPS = W_Q + Q_WARPS, THREADS = 32 * WARPS;
     // Registers: 16 warps have 128 each; of the 96 that 20 start with, the softmax warps get some of the others'
     // (the sum stays what the block was launched with)
     static constexpr bool SPLIT = WARPS == 20;
@@ -99,8 +102,12 @@ struct TreeCfg {
     static constexpr int A_RED = A_CORR + N * 4;           // [SM_WARPS][32], [SM_WARPS]
     static constexpr int A_FIRST = A_RED + SM_WARPS * 33 * 4;   // [kTreeMaxSeqs + 1]
     static constexpr int A_MISC = (A_FIRST + (kTreeMaxSeqs + 1) * 4 + 15) / 16 * 16;
-    static constexpr int A_BAR = A_MISC + 256;
-    static constexpr int END_LOW = A_BAR + 256;
+    // rings: pieces (struct TreePiece); block ids of a tile's pages; where they lie (64 bits each); the norms of a tile's
+    // keys and of its values
+    static constexpr int PIECES = 8, PAGES = 8, NORMS = D == 256 ? 4 : 8;
+    static constexpr int A_PIECE = A_MISC + 256, A_ID = A_PIECE + PIECES * 48, A_PAGE = A_ID + PAGES * 32, A_NORM = A_PAGE + PAGES * 64;
+    static constexpr int A_BAR = A_NORM + NORMS * 4 * kTreeTile;
+    static constexpr int END_LOW = A_BAR + 592;
     static constexpr int SMEM_BYTES = A_V + VS * V_SLOT + (P_HIGH ? PST * P_BUF : 0);
     static_assert(END_LOW <= WINDOW && SMEM_BYTES <= 227 * 1024 && THREADS <= 1024, "");
     // TMEM columns
@@ -120,25 +127,75 @@ __device__ __forceinline__ void tc_st_16x256b_x4(uint32_t addr, const uint32_t (
             "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+// The products are issued by one elected lane inside a branch: 32 cycles a product of 64 columns, what the tensor core
+// takes.  (The form of the chunk kernel, a whole warp with a predicate on each instruction, takes 66, whatever the width.)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ void one_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .b64 da, db;\nmov.b64 da, {%1, %3};\nmov.b64 db, {%2, %3};\nsetp.ne.b32 p, %5, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void one_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .b64 db;\nmov.b64 db, {%2, %3};\nsetp.ne.b32 p, %5, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(acc) : "memory");
+}
+// 32 lanes x NC columns, one row per lane, complete
+template <int NC>
+__device__ __forceinline__ void tc_load(uint32_t addr, uint32_t (&r)[NC]) {
+    if constexpr (NC == 32) {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
+            "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\ntcgen05.wait::ld.sync.aligned;\n"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+              "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+              "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+              "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+            : "r"(addr) : "memory");
+    } else {
+        tc_ld16(addr, r);
+        tc_wait_ld(r);
+    }
+}
 __device__ __forceinline__ uint32_t f2h2(float lo, float hi) {
     uint32_t h;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(h) : "f"(hi), "f"(lo));
     return h;
 }
-// barrier of a softmax warpgroup; true if any of its threads says so
+// barrier of some warps; true if any of their threads says so
+template <int THREADS = 128>
 __device__ __forceinline__ bool group_any(int id, bool mine) {
     uint32_t r;
     __syncwarp();
-    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbarrier.cta.red.or.pred q, %2, 128, p;\nselp.u32 %0, 1, 0, q;\n}\n"
-                 : "=r"(r) : "r"(static_cast<uint32_t>(mine)), "r"(id) : "memory");
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbarrier.cta.red.or.pred q, %2, %3, p;\nselp.u32 %0, 1, 0, q;\n}\n"
+                 : "=r"(r) : "r"(static_cast<uint32_t>(mine)), "r"(id), "n"(THREADS) : "memory");
     return r != 0;
 }
 
-// A lane's codes of a tile (its runs in two rows of two pages), and the pages of the tile that comes next.
+// A piece of a CTA's share: some tiles of one unit.
+struct TreePiece {
+    int b, hkv, row0, rows;     // sequence, KV head, first row and rows of the row tile
+    int tile0, n_tiles;         // (n_tiles = 0: there is none any more)
+    int seq, ctx;               // tokens, tokens before the tree
+    float* out;                 // [rows][D + 4]
+    int64_t spare;
+};
+static_assert(sizeof(TreePiece) == 48, "");
+
+// Asynchronous copies of a few bytes to shared memory (coherent: through L1, like an ordinary load).
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+
+// A lane's codes of a tile: its runs in two rows of two pages.
 template <int XW>
 struct TreeCodes {
     uint32_t w[2][2][XW];
-    int id[2], head;
 };
 // SB bytes into words, on the widest loads that their alignment allows (a run starts at a multiple of its size).
 template <int SB, int XW>
@@ -175,12 +232,14 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
     const uint32_t raw = static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw));
     auto at = [&](uint32_t a) { return smem_raw + (a - raw); };
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    uint32_t* const misc = reinterpret_cast<uint32_t*>(at(C::A_MISC));   // 0: TMEM, 1: a wait ran out, 2, 3: largest |q|, 8..: scan
+    uint32_t* const misc = reinterpret_cast<uint32_t*>(at(C::A_MISC));   // 0: TMEM, 1: a wait ran out, 2, 3: largest |q|, 8..: scan, 40..: heads
     volatile uint32_t* const gave_up = misc + 1;
     constexpr uint32_t BAR = C::A_BAR;
     constexpr uint32_t k_full = BAR, k_empty = BAR + 16, s_full = BAR + 32, s_free = BAR + 48, p_full = BAR + 64, o_done = BAR + 80,
                        v_full = BAR + 96, v_empty = BAR + 128, drained = BAR + 160;
-    constexpr uint32_t q_full = BAR + 168, q_empty = BAR + 184, o_free = BAR + 200;
+    constexpr uint32_t q_full = BAR + 168, q_empty = BAR + 184, o_free = BAR + 200, page_full = BAR + 208, page_empty = BAR + 272,
+                       norm_full = BAR + 336, norm_empty = BAR + 400,
+                       piece_full = BAR + 464, piece_empty = BAR + 528;
     constexpr int W_V = C::W_V, W_MMA = C::W_MMA;
 
     // ---- look-up window (struct Window): 256 rows of 256 bytes, keys in the first half of a row, values in the second
@@ -228,6 +287,18 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 mbar_init(q_full + 8 * i, C::Q_WARPS);
                 mbar_init(q_empty + 8 * i, 1 + C::SM_WARPS);
             }
+            for (int i = 0; i < C::PAGES; i++) {
+                mbar_init(page_full + 8 * i, 1);
+                mbar_init(page_empty + 8 * i, 8);
+            }
+            for (int i = 0; i < C::NORMS; i++) {
+                mbar_init(norm_full + 8 * i, 1);
+                mbar_init(norm_empty + 8 * i, C::SM_WARPS);
+            }
+            for (int i = 0; i < C::PIECES; i++) {
+                mbar_init(piece_full + 8 * i, 1);
+                mbar_init(piece_empty + 8 * i, C::SM_WARPS + 1 + C::Q_WARPS);
+            }
             mbar_init(o_free, C::SM_WARPS);
             mbar_init(drained, 1);
             mbar_fence_init();
@@ -274,36 +345,9 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
         for (int b = tid; b <= p.B; b += C::THREADS) p.plan[b] = first[b];
         if (tid == 0) p.plan[p.B + 1] = share;
     }
-    struct Piece {
-        int b, u, tile0, n_tiles, next, seq;
-        float* rows;
-    };
-    // the first piece with tiles from a place on (none: n_tiles = 0)
-    auto piece_from = [&](int pos) {
-        Piece pc{0, 0, 0, 0, end, 0, nullptr};
-        while (pos < end) {
-            int lo = 0, hi = p.B;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (first[mid] <= pos) lo = mid; else hi = mid;
-            }
-            const int len = (first[lo + 1] - first[lo]) / U, rel = pos - first[lo], u = rel / len, off = rel - u * len;
-            const int off_end = min(len, off + end - pos);
-            const int t0 = tree_tile_of(off), t1 = tree_tile_of(off_end);
-            pos += off_end - off;
-            if (t1 > t0) {
-                pc.b = lo; pc.u = u; pc.tile0 = t0; pc.n_tiles = t1 - t0; pc.next = pos;
-                pc.seq = max(0, min(p.seq_lens[lo], p.max_seq));
-                pc.rows = off == 0 && off_end == len ? p.whole + (static_cast<int64_t>(lo) * U + u) * N * ROW
-                                                     : p.cut + (2 * static_cast<int64_t>(cta) + (off == 0 ? 1 : 0)) * N * ROW;
-                return pc;
-            }
-        }
-        return pc;
-    };
-
     // bounded wait; once one has run out nobody waits any more
     auto wait = [&](uint32_t bar, uint32_t parity) {
+#pragma unroll 1
         for (int i = 0; i < kChunkSpinLimit; i++) {
             if (mbar_try_wait(bar, parity & 1u)) return;
             if ((i & 63) == 63 && *gave_up) return;
@@ -311,14 +355,136 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
         *gave_up = 1;
     };
 
-    const Piece start = piece_from(cta * share < end ? cta * share : end);
-    // nodes of a piece's tree, tokens before it
-    auto nodes_of = [&](const Piece& pc) { return min(p.tree_lens ? max(p.tree_lens[pc.b], 0) : p.T, min(p.T, pc.seq)); };
+    // the first piece with tiles from a place on; moves on to the place behind it
+    auto next_piece = [&](int& pos) {
+        TreePiece pc{};
+#pragma unroll 1
+        while (pos < end && pc.n_tiles == 0) {
+            int lo = 0, hi = p.B;
+#pragma unroll 1
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (first[mid] <= pos) lo = mid; else hi = mid;
+            }
+            const int len = (first[lo + 1] - first[lo]) / U, rel = pos - first[lo], u = rel / len, off = rel - u * len;
+            const int off_end = min(len, off + end - pos), t0 = tree_tile_of(off), t1 = tree_tile_of(off_end);
+            pos += off_end - off;
+            if (t1 <= t0) continue;
+            pc.b = lo;
+            pc.hkv = u / p.row_tiles;
+            pc.row0 = (u - pc.hkv * p.row_tiles) * N;
+            pc.rows = min(N, p.T * static_cast<int>(p.group.d) - pc.row0);
+            pc.tile0 = t0;
+            pc.n_tiles = t1 - t0;
+            pc.seq = max(0, min(p.seq_lens[lo], p.max_seq));
+            pc.ctx = pc.seq - min(p.tree_lens ? max(p.tree_lens[lo], 0) : p.T, min(p.T, pc.seq));
+            pc.out = off == 0 && off_end == len ? p.whole + (static_cast<int64_t>(lo) * U + u) * N * ROW
+                                                : p.cut + (2 * static_cast<int64_t>(cta) + (off == 0 ? 1 : 0)) * N * ROW;
+        }
+        return pc;
+    };
+    // piece n, and its slot back
+    auto piece_at = [&](int n) {
+        wait(piece_full + 8 * (n % C::PIECES), n / C::PIECES);
+        __syncwarp();
+        TreePiece pc = *reinterpret_cast<const TreePiece*>(at(C::A_PIECE + n % C::PIECES * 48));
+        if (__any_sync(0xffffffffu, *gave_up != 0)) pc.n_tiles = 0;   // (what stands there may be no piece)
+        if (lane == 0) mbar_arrive(piece_empty + 8 * (n % C::PIECES));
+        return pc;
+    };
     // the power of two that brings every query of a piece below 2^15: |rotated| <= D * largest |q|
     auto query_exponent = [&](int qb) {
         const float top = __uint_as_float(misc[2 + qb]) * (fabsf(p.q_scale) * D);
         return top > 0.f ? max(-120, min(120, 14 - ilogbf(top))) : 0;
     };
+
+    // A piece's queries (rotated, scaled, fp16, K-major with 128-byte swizzle) and masks, by NW warps (thread `me` of them); the
+    // first piece's by all warps, before they part.
+    auto prepare_piece = [&](const TreePiece& pc, int qb, auto warps, int me) {
+        constexpr int NW = decltype(warps)::value, OCTETS = 4 * NW;
+        const int t8 = lane & 7, octet = me >> 3, group = static_cast<int>(p.group.d), rows = pc.rows, row0 = pc.row0;
+        auto meet = [&] { group_any<32 * NW>(NW == C::WARPS ? 0 : 3, false); };
+        auto query = [&](int r) {   // row r's 16-byte pieces: eight coordinates each
+            const int i = fast_div(row0 + r, p.group), h = row0 + r - i * group;
+            return static_cast<const uint4*>(p.q) + (((static_cast<int64_t>(pc.b) * p.T + i) * p.Hq + pc.hkv * group + h) * D) / 8;
+        };
+        auto widen = [&](const uint4& x, float (&o)[8]) {
+            if (p.q_dtype == kBF16) load8<__nv_bfloat16>(reinterpret_cast<const __nv_bfloat16*>(&x), o);
+            else load8<__half>(reinterpret_cast<const __half*>(&x), o);
+        };
+        // the largest query, for their common scale
+        float top = 0.f;
+#pragma unroll 4
+        for (int k = me; k < rows * (D / 8); k += 32 * NW) {
+            float v[8];
+            widen(query(k / (D / 8))[k % (D / 8)], v);
+#pragma unroll
+            for (int c = 0; c < 8; c++) top = fabsf(v[c]) <= FLT_MAX ? fmaxf(top, fabsf(v[c])) : top;
+        }
+        __syncwarp();
+        top = warp_max(top);
+        if (me == 0) misc[2 + qb] = 0;
+        meet();
+        if (lane == 0) atomicMax(misc + 2 + qb, __float_as_uint(top));
+        meet();
+        const float up = p.q_scale * ldexpf(1.f, query_exponent(qb));
+        uint4 x[D / 64];
+        auto load = [&](int r) {
+#pragma unroll
+            for (int k = 0; k < D / 64; k++) x[k] = r < rows ? query(r)[t8 + 8 * k] : make_uint4(0, 0, 0, 0);
+        };
+        load(octet);
+#pragma unroll 1
+        for (int r = octet; r - octet < N; r += OCTETS) {
+            float a[E];
+#pragma unroll
+            for (int k = 0; k < D / 64; k++) {
+                float v[8];
+                widen(x[k], v);
+#pragma unroll
+                for (int c = 0; c < 8; c++)
+                    a[8 * k + c] = __uint_as_float(__float_as_uint(v[c] * up) ^ sign_mask(p.signs, load_coord(t8, 8 * k + c)));
+            }
+            load(r + OCTETS);
+            octet_fwht<E>(a, lane);
+            // Coordinate c = t8 + 8 k is code 4 jj + (c & 3) of lane t's run: place 16 jj + 4 t + (c & 3).  Two lanes have two
+            // neighbours: of two k's the even lane stores the first, the odd lane the second.
+            uint8_t* dst = at(C::A_Q + qb * C::Q_BYTES) + r * 128;
+#pragma unroll
+            for (int k = 0; k < E; k += 2) {
+                const float other = __shfl_xor_sync(0xffffffffu, (t8 & 1) ? a[k] : a[k + 1], 1);
+                const int c = (t8 & 6) + 8 * (k + (t8 & 1)), t = c / (D / 4), jj = (c % (D / 4)) / 4, place = 16 * jj + 4 * t + (c & 3);
+                const uint32_t h = (t8 & 1) ? f2h2(other, a[k + 1]) : f2h2(a[k], other);
+                if (r < N) *reinterpret_cast<uint32_t*>(dst + (place >> 6) * (N * 128) + ((((place & 63) >> 3) ^ (r & 7)) << 4) + (place & 7) * 2) = h;
+            }
+        }
+        // which rows attend a node: bit r of its words
+        if ((pc.tile0 + pc.n_tiles) * kTreeTile > pc.ctx) {
+            uint32_t* const cm = reinterpret_cast<uint32_t*>(at(C::A_MASK)) + qb * (C::MASK_BYTES / 4);
+            for (int k = me; k < (pc.seq - pc.ctx) * C::MW; k += 32 * NW) {
+                const int node = k / C::MW, w = k % C::MW;
+                uint32_t bits = 0;
+                // (a node's heads are neighbours: a run of bits)
+                const int r1 = min(rows, 32 * w + 32);
+#pragma unroll 1
+                for (int r = 32 * w; r < r1;) {
+                    const int i = fast_div(row0 + r, p.group), stop = min(r1, (i + 1) * group - row0);
+                    if ((static_cast<uint32_t>(p.masks[(static_cast<int64_t>(pc.b) * p.T + i) * p.W + (node >> 5)]) >> (node & 31)) & 1u)
+                        bits |= (0xffffffffu >> (32 - (stop - r))) << (r & 31);
+                    r = stop;
+                }
+                cm[k] = bits;
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    };
+    const int begin = static_cast<int>(min(static_cast<int64_t>(cta) * share, static_cast<int64_t>(end)));
+    if (begin < end) {
+        int pos = begin;
+        const TreePiece pc = next_piece(pos);
+        if (pc.n_tiles > 0) prepare_piece(pc, 0, std::integral_constant<int, C::WARPS>{}, tid);
+    }
+    __syncthreads();
 
     // (a warpgroup runs one and the same instruction)
     if constexpr (C::SPLIT && C::R_Q < C::REGS) {
@@ -327,11 +493,10 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
     if (warp < C::SM_WARPS) {
         if constexpr (C::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(C::R_SM));
         // ================= softmax: a thread per token of the tile
-        Piece pc = start;
-        for (int n = 0, g0 = 0; pc.n_tiles > 0; n++) {
-            const int hkv = pc.u / p.row_tiles, row0 = (pc.u - hkv * p.row_tiles) * N, qb = n % C::QB;
-            const int rows = min(N, p.T * static_cast<int>(p.group.d) - row0);
-            const int seq = pc.seq, ctx = seq - nodes_of(pc), n_tiles = pc.n_tiles;
+        for (int n = 0, g0 = 0;; n++) {
+            const TreePiece pc = piece_at(n);
+            if (group_any(1 + (warp >> 2), pc.n_tiles == 0)) break;      // (all warps of the group, or none)
+            const int qb = n % C::QB, rows = pc.rows, seq = pc.seq, ctx = pc.ctx, n_tiles = pc.n_tiles;
             const int wg = warp >> 2, quarter = warp & 3, my_tok = quarter * 32 + lane, bar_id = 1 + wg;
             const uint32_t tl = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
             const float* const s_nm = reinterpret_cast<const float*>(at(C::A_NM)) + wg * C::CW;
@@ -347,27 +512,6 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
 #pragma unroll
                 for (int c = 0; c < CH; c++) l[ch][c] = 0.f;
             }
-            const uint8_t* const head = p.pool + static_cast<int64_t>(hkv) * C::PAGE_BYTES;
-            const int32_t* const btab = p.block_table + static_cast<int64_t>(pc.b) * p.max_blocks;
-            auto page_id = [&](int it) {
-                const int pos = (pc.tile0 + it) * kTreeTile + my_tok;
-                return it < n_tiles && pos < seq ? btab[pos / kPageTokens] : -2;   // -2: no token
-            };
-            struct Norms { float k, v; };
-            auto norms_of = [&](int id) {
-                Norms n{0.f, 0.f};
-                if (static_cast<uint64_t>(static_cast<int64_t>(id)) < static_cast<uint64_t>(p.num_blocks)) {
-                    const uint8_t* page = head + static_cast<int64_t>(id) * p.Hkv * C::PAGE_BYTES;
-                    n.k = __half2float(reinterpret_cast<const __half*>(page + C::OFF_KN)[my_tok & (kPageTokens - 1)]);
-                    n.v = __half2float(reinterpret_cast<const __half*>(page + C::OFF_VN)[my_tok & (kPageTokens - 1)]);
-                } else if (id != -2) {
-                    n.k = __int_as_float(0x7fc00000);
-                    __stcg(p.errors + 1, p.epoch);
-                }
-                return n;
-            };
-            Norms n0 = norms_of(page_id(0)), n1 = norms_of(page_id(1));
-            int id2 = page_id(2);
             if (quarter == 0 && lane < 32) {
 #pragma unroll
                 for (int c = 0; c < C::CW; c += 32)
@@ -378,12 +522,13 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
             __syncwarp();
             const float q_down = ldexpf(1.f, -query_exponent(qb));
             const uint32_t* const cm = reinterpret_cast<const uint32_t*>(at(C::A_MASK)) + qb * (C::MASK_BYTES / 4);
+#pragma unroll 1
             for (int it = 0; it < n_tiles; it++) {
                 const int g = g0 + it, sb = g & 1, pb = g % C::PST;
-                const float kn = n0.k * q_down, vn = n0.v;
-                n0 = n1;
-                n1 = norms_of(id2);
-                id2 = page_id(it + 3);
+                wait(norm_full + 8 * (g % C::NORMS), g / C::NORMS);
+                __syncwarp();
+                const __half* const norms = reinterpret_cast<const __half*>(at(C::A_NORM + (g % C::NORMS) * 4 * kTreeTile));
+                const float kn = __half2float(norms[my_tok]) * q_down, vn = __half2float(norms[kTreeTile + my_tok]);
                 const int pos = (pc.tile0 + it) * kTreeTile + my_tok, node = pos - ctx;
                 const bool boundary = (pc.tile0 + it + 1) * kTreeTile > ctx;     // (uniform: the tile reaches the tree or the end)
                 wait(s_full + 8 * sb, g >> 1);
@@ -400,10 +545,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                     // x = score - maximum (base 2), -inf where the row does not attend the token
                     auto scores = [&](bool masked) {
                         uint32_t s[CH];
-#pragma unroll
-                        for (int c = 0; c < CH; c += 16) tc_ld16(s_at + c, s + c);
-#pragma unroll
-                        for (int c = 0; c < CH; c += 16) tc_wait_ld(s + c);
+                        tc_load(s_at, s);
                         const u64 kn2 = pk2(kn, kn);
 #pragma unroll
                         for (int c = 0; c < CH; c += 4) {
@@ -422,8 +564,8 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                     for (int c = 1; c + 1 < CH; c += 2) top = fmaxf(fmaxf(top, x[c]), x[c + 1]);
                     top = fmaxf(top, x[CH - 1]);
                     const float av = fabsf(vn);
-                    const bool grow = av <= FLT_MAX && (vs[ch] == 0.f ? av > 0.f : av * vs[ch] > 4096.f);
-                    if (group_any(bar_id, top > kLazyMaxSlack || grow)) {
+                    const bool grow = av <= FLT_MAX && (vs[ch] == 0.f ? av > 0.f : av * vs[ch] > kTreeGrowth);
+                    if (group_any(bar_id, top > kTreeSlack || grow)) {
                         // ---- new maxima of these rows
                         float mine = -INFINITY;
 #pragma unroll 1
@@ -449,8 +591,8 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                         }
                         const float lc = m_run[ch] == -INFINITY ? 0.f : fast_exp2(m_run[ch] - m_new);
                         float v_ratio = 1.f;
-                        if (v_top > 0.f && (vs[ch] == 0.f || v_top * vs[ch] > 4096.f)) {   // the largest |v| becomes 2^5 to 2^6
-                            const float to = ldexpf(1.f, 5 - ilogbf(v_top));
+                        if (v_top > 0.f && (vs[ch] == 0.f || v_top * vs[ch] > kTreeGrowth)) {   // the largest |v| becomes 1 to 2
+                            const float to = ldexpf(1.f, -ilogbf(v_top));
                             v_ratio = vs[ch] == 0.f ? 1.f : to / vs[ch];
                             vs[ch] = to;
                         }
@@ -485,7 +627,10 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                     if (ch == NCH - 1) {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(s_free + 8 * sb);
+                        if (lane == 0) {
+                            mbar_arrive(s_free + 8 * sb);
+                            mbar_arrive(norm_empty + 8 * (g % C::NORMS));
+                        }
                     }
                     if (!p_free) {
                         if (g >= C::PST) wait(o_done + 8 * pb, g / C::PST - 1);
@@ -526,7 +671,6 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 __syncwarp();
                 tc_fence_after();
             }
-            const bool lost = *gave_up != 0;
 #pragma unroll
             for (int ch = 0; ch < NCH; ch++) {
                 const int col = wg * C::CW + ch * CH;
@@ -550,8 +694,8 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 group_any(bar_id, false);
                 sum = red[(4 * wg) * 32 + lane] + red[(4 * wg + 1) * 32 + lane] + red[(4 * wg + 2) * 32 + lane] + red[(4 * wg + 3) * 32 + lane];
                 if (quarter == 0 && lane < CH && col + lane < rows) {
-                    float* dst = pc.rows + static_cast<int64_t>(col + lane) * ROW + D;
-                    dst[0] = lost ? __int_as_float(0x7fc00000) : m_run[ch];
+                    float* dst = pc.out + (col + lane) * ROW + D;
+                    dst[0] = m_run[ch];
                     dst[1] = sum;
                 }
                 const float scale = p.inv_v_scale / (vs[ch] == 0.f ? 1.f : vs[ch]);
@@ -567,7 +711,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                     if (D == 64 && m >= 64) continue;
 #pragma unroll
                     for (int j = 0; j < 16; j++)
-                        if (col + c + j < rows) pc.rows[static_cast<int64_t>(col + c + j) * ROW + coord] = __uint_as_float(o[j]) * scale;
+                        if (col + c + j < rows) pc.out[(col + c + j) * ROW + coord] = __uint_as_float(o[j]) * scale;
                 }
             }
             tc_fence_before();
@@ -576,60 +720,48 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 mbar_arrive(o_free);
                 mbar_arrive(q_empty + 8 * qb);
             }
-            if (lost && tid == 0) __stcg(p.errors, p.epoch);
             g0 += n_tiles;
-            pc = piece_from(pc.next);
         }
     } else if (warp < W_MMA) {
         if constexpr (C::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(C::R_DQ));
         // ================= dequantisation: one stream of tiles, whatever pieces they belong to; the codes of AHEAD tiles are
-        // under way in registers, and the block ids of as many more
+        // under way in registers
         constexpr int KSB = C::PDK / 4, VSB = C::PDV / 4;                  // bytes of a lane's run of D / 4 codes
         constexpr int KW = (KSB + 3) / 4, VW = (VSB + 3) / 4, XW = KW > VW ? KW : VW;
         const int g8 = lane >> 2, t4 = lane & 3, dq = warp & 3;
         const bool is_k = warp < W_V;
-        int n_tiles = 0;
-        for (Piece pc = start; pc.n_tiles > 0; pc = piece_from(pc.next)) n_tiles += pc.n_tiles;
         TreeCodes<XW> f[C::AHEAD];
-        Piece lead = start;
-        int lead_it = 0;
-        auto fetch_ids = [&](TreeCodes<XW>& f) {    // of the stream's next tile
-            const int n_pages = (lead.seq + kPageTokens - 1) / kPageTokens;
-            f.head = lead.u / p.row_tiles;
+        int n_tiles = INT_MAX;     // (known when the stream's end has been seen: places of -2)
+        auto fetch = [&](int g, TreeCodes<XW>& f) {    // the codes of the stream's tile g
+            if (g >= n_tiles) return;
+            const int slot = g % C::PAGES;
+            wait(page_full + 8 * slot, g / C::PAGES);
+            __syncwarp();
+            const int64_t* const where = reinterpret_cast<const int64_t*>(at(C::A_PAGE + slot * 64));
+            const int64_t page[2] = {where[is_k ? 2 * dq : dq], where[is_k ? 2 * dq + 1 : 4 + dq]};
+            __syncwarp();
+            if (lane == 0) mbar_arrive(page_empty + 8 * slot);
+            if (page[0] == -2 || __any_sync(0xffffffffu, *gave_up != 0)) {   // (then what stands there may be no place)
+                n_tiles = g;
+                return;
+            }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int pg = (lead.tile0 + lead_it) * (kTreeTile / kPageTokens) + (is_k ? 2 * dq + i : 4 * i + dq);
-                f.id[i] = lead.n_tiles > 0 && pg < n_pages ? p.block_table[static_cast<int64_t>(lead.b) * p.max_blocks + pg] : -1;
-            }
-            if (lead.n_tiles > 0 && ++lead_it == lead.n_tiles) {
-                lead = piece_from(lead.next);
-                lead_it = 0;
-            }
-        };
-        auto fetch_codes = [&](TreeCodes<XW>& f) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const bool ok = static_cast<uint64_t>(static_cast<int64_t>(f.id[i])) < static_cast<uint64_t>(p.num_blocks);
-                const uint8_t* page = p.pool + ((ok ? static_cast<int64_t>(f.id[i]) : 0) * p.Hkv + f.head) * C::PAGE_BYTES;
+                const uint8_t* src = p.pool + page[i];
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
 #pragma unroll
                     for (int j = 0; j < XW; j++) f.w[i][r][j] = 0;
-                    if (!ok) continue;
+                    if (page[i] < 0) continue;
                     const int tok = g8 + 8 * r;
                     // (a V row has its halves exchanged where bit 1 of its token's place is set)
-                    if (is_k) tree_fetch<KSB>(page + tok * C::PDK + t4 * KSB, f.w[i][r]);
-                    else tree_fetch<VSB>(page + C::OFF_VC + tok * C::PDV + (t4 ^ (tok & 2)) * VSB, f.w[i][r]);
+                    if (is_k) tree_fetch<KSB>(src + tok * C::PDK + t4 * KSB, f.w[i][r]);
+                    else tree_fetch<VSB>(src + C::OFF_VC + tok * C::PDV + (t4 ^ (tok & 2)) * VSB, f.w[i][r]);
                 }
             }
         };
 #pragma unroll
-        for (int i = 0; i < C::AHEAD; i++) fetch_ids(f[i]);
-#pragma unroll
-        for (int i = 0; i < C::AHEAD; i++) {
-            fetch_codes(f[i]);
-            fetch_ids(f[i]);
-        }
+        for (int i = 0; i < C::AHEAD; i++) fetch(i, f[i]);
         if (is_k) {
             // ================= keys: codes -> TMEM, rows of lanes = tokens
             const uint32_t base = C::WINDOW + (BK == 2 ? (lane & 15) * 8 : lane * 4);
@@ -660,8 +792,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                         tc_st_16x256b_x4(rows_at + (static_cast<uint32_t>(16 * i) << 16) + st * (D / 2) + 32 * q, x);
                     }
                 }
-                fetch_codes(f);
-                fetch_ids(f);
+                fetch(g + C::AHEAD, f);
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -670,6 +801,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
 #endif
                 if (lane == 0) mbar_arrive(k_full + 8 * st);
             };
+#pragma unroll 1
             for (int g = 0; g < n_tiles; g += C::AHEAD) {
 #pragma unroll
                 for (int i = 0; i < C::AHEAD; i++)
@@ -706,9 +838,9 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(v_full + 8 * slot);
                 }
-                fetch_codes(f);
-                fetch_ids(f);
+                fetch(g + C::AHEAD, f);
             };
+#pragma unroll 1
             for (int g = 0; g < n_tiles; g += C::AHEAD) {
 #pragma unroll
                 for (int i = 0; i < C::AHEAD; i++)
@@ -717,10 +849,9 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
         }
     } else if (warp == W_MMA) {
         // ================= the products
-        Piece pc = start;
-        for (int np = 0, g0 = 0; pc.n_tiles > 0; np++) {
-            const int qb = np % C::QB, n_tiles = pc.n_tiles;
-            const bool one = lane == 0;
+        for (int np = 0, g0 = 0;; np++) {
+            const int qb = np % C::QB, n_tiles = piece_at(np).n_tiles;
+            if (n_tiles == 0) break;
             constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(N / 8) << 17) | (8u << 24);
             constexpr uint32_t kIdescO = kIdescS | (1u << 15) | (1u << 16);
             constexpr uint32_t kHi = (1024u >> 4) | (1u << 14) | (2u << 29);
@@ -739,30 +870,32 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                     __syncwarp();
                     tc_fence_after();
                     const uint32_t v = kV + slot * (C::V_SLOT >> 4), q = kP + pb * (C::P_BUF >> 4) + h * (8192 >> 4);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int mb = 0; mb < C::MB; mb++)
+                        for (int mb = 0; mb < C::MB; mb++)
 #pragma unroll
-                        for (int ks = 0; ks < 4; ks++)
-                            tc_mma_ss(one, tmem + C::COL_O + mb * N, v + mb * (16384 >> 4) + ks * (2048 >> 4), q + ks * (2048 >> 4), kHi,
-                                      kIdescO, it > 0 || h > 0 || ks > 0);
-                    if (one) tc_commit(v_empty + 8 * slot);
+                            for (int ks = 0; ks < 4; ks++)
+                                one_mma_ss(tmem + C::COL_O + mb * N, v + mb * (16384 >> 4) + ks * (2048 >> 4), q + ks * (2048 >> 4), kHi, kIdescO,
+                                           h > 0 || ks > 0 ? 1u : static_cast<uint32_t>(it));
+                        tc_commit(v_empty + 8 * slot);
+                        if (h == 1) tc_commit(o_done + 8 * pb);
+                    }
                     __syncwarp();
                 }
-                if (one) tc_commit(o_done + 8 * pb);
-                __syncwarp();
             };
             wait(q_full + 8 * qb, np / C::QB);
+#pragma unroll 1
             for (int it = 0; it < n_tiles; it++) {
                 const int g = g0 + it, st = g & 1;
                 wait(k_full + 8 * st, g >> 1);
                 if (g >= 2) wait(s_free + 8 * st, (g >> 1) - 1);
                 __syncwarp();
                 tc_fence_after();
+                if (elect_one()) {
 #pragma unroll
-                for (int kb = 0; kb < D / 16; kb++)
-                    tc_mma_ts(one, tmem + C::COL_S + st * N, tmem + C::COL_K + st * (D / 2) + 8 * kb,
-                              kQ + qb * (C::Q_BYTES >> 4) + ((kb >> 2) * (N * 128) + (kb & 3) * 32) / 16, kHi, kIdescS, kb > 0);
-                if (one) {
+                    for (int kb = 0; kb < D / 16; kb++)
+                        one_mma_ts(tmem + C::COL_S + st * N, tmem + C::COL_K + st * (D / 2) + 8 * kb,
+                                   kQ + qb * (C::Q_BYTES >> 4) + ((kb >> 2) * (N * 128) + (kb & 3) * 32) / 16, kHi, kIdescS, kb > 0);
                     tc_commit(s_full + 8 * st);
                     tc_commit(k_empty + 8 * st);
                     if (it == n_tiles - 1) tc_commit(q_empty + 8 * qb);
@@ -772,95 +905,108 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
             }
             pv(n_tiles - 1);
             g0 += n_tiles;
-            pc = piece_from(pc.next);
+        }
+    } else if (warp == C::W_FEED) {
+        // ================= the pieces; where the pages of their tiles lie; the norms of the tokens.  In step s the block ids of
+        // tile s are requested, the norms of tile s - 2, and those of tile s - 4 are handed over.  Lane l has page l / 4 of a
+        // tile and four of its tokens.  No token: norms of zero; a block id outside the pool: keys that are not numbers.
+        int pos = begin;                                           // next place
+        int n_pieces = 0, n_tiles = 0, head = 0;
+        int tile = 0, tiles_left = 0, seq = 0;                     // of the piece that the ids are requested for
+        const int32_t* btab = nullptr;
+        bool more = true;
+        const int page_of_lane = lane >> 2, part = lane & 3;
+#pragma unroll 1
+        for (int s = 0; more || s - 4 < n_tiles; s++) {
+            if (more && tiles_left == 0) {
+                const TreePiece pc = next_piece(pos);
+                const int slot = n_pieces % C::PIECES;
+                if (n_pieces >= C::PIECES) wait(piece_empty + 8 * slot, n_pieces / C::PIECES - 1);
+                __syncwarp();
+                if (lane == 0) *reinterpret_cast<TreePiece*>(at(C::A_PIECE + slot * 48)) = pc;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(piece_full + 8 * slot);
+                n_pieces++;
+                more = pc.n_tiles > 0;
+                tile = pc.tile0; tiles_left = pc.n_tiles; seq = pc.seq;
+                btab = p.block_table + static_cast<int64_t>(pc.b) * p.max_blocks;
+                head = pc.hkv;
+            }
+            if (more) {
+                const int pg = tile * (kTreeTile / kPageTokens) + page_of_lane;
+                const uint32_t dst = C::A_ID + s % C::PAGES * 32 + page_of_lane * 4;
+                if (part == 0) {
+                    if (pg * kPageTokens < seq) copy_async<4>(dst, btab + pg);
+                    else *reinterpret_cast<int*>(at(dst)) = -2;
+                }
+                // (the KV head of the tile, for the step after next)
+                if (lane == 0) misc[40 + s % C::PAGES] = head;
+                n_tiles++;
+                tile++;
+                tiles_left--;
+            }
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+            const int t = s - 2;
+            if (t >= 0 && t <= n_tiles) {
+                // (four younger groups: two of step s - 1, one each of steps s - 2 and s)
+                asm volatile("cp.async.wait_group 4;\n" ::: "memory");
+                __syncwarp();
+                const int slot = t % C::PAGES, ns = t % C::NORMS;
+                if (t >= C::PAGES) wait(page_empty + 8 * slot, t / C::PAGES - 1);
+                __syncwarp();
+                const bool last = t == n_tiles;        // (the end of the stream)
+                const int id = *reinterpret_cast<const int*>(at(C::A_ID + slot * 32 + page_of_lane * 4));
+                const bool ok = !last && static_cast<uint64_t>(static_cast<int64_t>(id)) < static_cast<uint64_t>(p.num_blocks), bad = !last && !ok && id != -2;
+                const int64_t page = last ? -2 : ok ? (static_cast<int64_t>(id) * p.Hkv + static_cast<int>(misc[40 + slot])) * C::PAGE_BYTES : -1;
+                if (bad) __stcg(p.errors + 1, p.epoch);
+                if (part == 0) *reinterpret_cast<int64_t*>(at(C::A_PAGE + slot * 64 + page_of_lane * 8)) = page;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(page_full + 8 * slot);
+                if (!last) {
+                    if (t >= C::NORMS) wait(norm_empty + 8 * ns, t / C::NORMS - 1);
+                    __syncwarp();
+                    const uint32_t dst = C::A_NORM + ns * 4 * kTreeTile + lane * 8;
+                    if (ok) {
+                        copy_async<8>(dst, p.pool + page + C::OFF_KN + 8 * part);
+                        copy_async<8>(dst + 2 * kTreeTile, p.pool + page + C::OFF_VN + 8 * part);
+                    } else {
+                        *reinterpret_cast<uint2*>(at(dst)) = bad ? make_uint2(0x7e007e00u, 0x7e007e00u) : make_uint2(0u, 0u);
+                        *reinterpret_cast<uint2*>(at(dst + 2 * kTreeTile)) = make_uint2(0u, 0u);
+                    }
+                }
+            }
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+            if (s >= 4 && s - 4 < n_tiles) {
+                // (younger than the norms' group of step s - 2: the two of step s - 1, the two of step s)
+                asm volatile("cp.async.wait_group 4;\n" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(norm_full + 8 * ((s - 4) % C::NORMS));
+            }
         }
     } else {
-        // ================= queries (rotated, scaled, fp16) and masks of the pieces, one ahead where there is room
-        const int me = tid - 32 * C::W_Q, t8 = lane & 7, octet = me >> 3, group = static_cast<int>(p.group.d);
-        constexpr int OCTETS = 4 * C::Q_WARPS;
-        Piece pc = start;
-        for (int n = 0; pc.n_tiles > 0; n++) {
-            const int qb = n % C::QB, hkv = pc.u / p.row_tiles, row0 = (pc.u - hkv * p.row_tiles) * N;
-            const int rows = min(N, p.T * group - row0), nodes = nodes_of(pc), ctx = pc.seq - nodes;
-            auto query = [&](int r) {   // row r's 16-byte pieces: eight coordinates each
-                const int i = fast_div(row0 + r, p.group), h = row0 + r - i * group;
-                return static_cast<const uint4*>(p.q) + (((static_cast<int64_t>(pc.b) * p.T + i) * p.Hq + hkv * group + h) * D) / 8;
-            };
-            auto widen = [&](const uint4& x, float (&o)[8]) {
-                if (p.q_dtype == kBF16) load8<__nv_bfloat16>(reinterpret_cast<const __nv_bfloat16*>(&x), o);
-                else load8<__half>(reinterpret_cast<const __half*>(&x), o);
-            };
+        // ================= queries and masks of the other pieces, one ahead where there is room
+        if (lane == 0) mbar_arrive(q_full);     // (the first piece's)
+        bool more = !group_any<32 * C::Q_WARPS>(3, piece_at(0).n_tiles == 0);
+        for (int n = 1; more; n++) {
+            const TreePiece pc = piece_at(n);
+            more = !group_any<32 * C::Q_WARPS>(3, pc.n_tiles == 0);
+            if (!more) break;
+            const int qb = n % C::QB;
             if (n >= C::QB) wait(q_empty + 8 * qb, n / C::QB - 1);
             __syncwarp();
-            float top = 0.f;
-#pragma unroll 4
-            for (int k = me; k < rows * (D / 8); k += 32 * C::Q_WARPS) {
-                float x[8];
-                widen(query(k / (D / 8))[k % (D / 8)], x);
-#pragma unroll
-                for (int c = 0; c < 8; c++) top = fabsf(x[c]) <= FLT_MAX ? fmaxf(top, fabsf(x[c])) : top;
-            }
-            __syncwarp();
-            top = warp_max(top);
-            if (n >= C::QB) asm volatile("barrier.cta.sync 3, %0;\n" ::"n"(32 * C::Q_WARPS) : "memory");
-            if (me == 0) misc[2 + qb] = 0;
-            __syncwarp();
-            asm volatile("barrier.cta.sync 3, %0;\n" ::"n"(32 * C::Q_WARPS) : "memory");
-            if (lane == 0) atomicMax(misc + 2 + qb, __float_as_uint(top));
-            __syncwarp();
-            asm volatile("barrier.cta.sync 3, %0;\n" ::"n"(32 * C::Q_WARPS) : "memory");
-            const float up = p.q_scale * ldexpf(1.f, query_exponent(qb));
-#pragma unroll 2
-            for (int r0 = 0; r0 < N; r0 += OCTETS) {
-                const int r = r0 + octet;
-                float a[E];
-#pragma unroll
-                for (int k = 0; k < E / 8; k++) {
-                    float tmp[8];
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (r < rows) x = query(r)[t8 + 8 * k];
-                    widen(x, tmp);
-#pragma unroll
-                    for (int c = 0; c < 8; c++)
-                        a[8 * k + c] = __uint_as_float(__float_as_uint(tmp[c] * up) ^ sign_mask(p.signs, load_coord(t8, 8 * k + c)));
-                }
-                octet_fwht<E>(a, lane);
-                uint8_t* dst = at(C::A_Q + qb * C::Q_BYTES) + r * 128;
-                if (r < N) {
-#pragma unroll
-                    for (int k = 0; k < E; k++) {
-                        // coordinate c = t8 + 8 k is code 4 jj + uh of lane t's run: place 16 jj + 4 t + uh
-                        const int c = t8 + 8 * k, t = c / (D / 4), jj = (c % (D / 4)) / 4, place = 16 * jj + 4 * t + (c & 3);
-                        *reinterpret_cast<__half*>(dst + (place >> 6) * (N * 128) + ((((place & 63) >> 3) ^ (r & 7)) << 4) + (place & 7) * 2) =
-                            __float2half_rn(a[k]);
-                    }
-                }
-            }
-            // which rows attend a node: bit r of its words
-            if ((pc.tile0 + pc.n_tiles) * kTreeTile > ctx) {
-                uint32_t* const cm = reinterpret_cast<uint32_t*>(at(C::A_MASK)) + qb * (C::MASK_BYTES / 4);
-                for (int k = me; k < nodes * C::MW; k += 32 * C::Q_WARPS) {
-                    const int node = k / C::MW, w = k % C::MW;
-                    uint32_t bits = 0;
-#pragma unroll 8
-                    for (int j = 0; j < 32; j++) {
-                        const int r = 32 * w + j;
-                        if (r < rows) {
-                            const int i = fast_div(row0 + r, p.group);
-                            bits |= ((static_cast<uint32_t>(p.masks[(static_cast<int64_t>(pc.b) * p.T + i) * p.W + (node >> 5)]) >> (node & 31)) & 1u) << j;
-                        }
-                    }
-                    cm[k] = bits;
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            prepare_piece(pc, qb, std::integral_constant<int, C::Q_WARPS>{}, tid - 32 * C::W_Q);
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full + 8 * qb);
-            pc = piece_from(pc.next);
         }
     }
     __syncwarp();
     __syncthreads();
+    if (*gave_up) {   // all that this CTA has
+        int pos = begin;
+        for (TreePiece pc = next_piece(pos); pc.n_tiles > 0; pc = next_piece(pos))
+            for (int r = tid; r < pc.rows; r += C::THREADS) pc.out[r * ROW + D] = __int_as_float(0x7fc00000);
+        if (tid == 0) __stcg(p.errors, p.epoch);
+    }
     if (warp == W_MMA) {   // nothing may be in flight when TMEM is given back
         if (lane == 0) tc_commit(drained);
         __syncwarp();
