@@ -1717,11 +1717,11 @@ struct TreeLayout {   // of the workspace, behind a decode workspace of one sequ
 TreeLayout tree_layout(int B, int n_nodes, int Hq, int Hkv, int d, size_t head) {
     const int rows = n_nodes * (Hq / Hkv), n = ftq::tree_rows(d, rows), tiles = (rows + n - 1) / n;
     const int seqs = std::min(B, ftq::kTreeMaxSeqs);
-    const size_t row = static_cast<size_t>(n) * (d + 4) * sizeof(float);
+    const size_t row = static_cast<size_t>(n) * (d + 4) * sizeof(float);   // of a piece
     TreeLayout l{n, tiles, (head + 255) / 256 * 256, 0, 0, 0};
     l.whole = l.plan + (static_cast<size_t>(seqs + 2) * sizeof(int) + 255) / 256 * 256;
     l.cut = l.whole + static_cast<size_t>(seqs) * Hkv * tiles * row;
-    l.end = l.cut + 2 * static_cast<size_t>(ftq::sm_count()) * row;
+    l.end = l.cut + 2 * static_cast<size_t>(ftq::sm_count()) * ftq::tree_halves(d, n) * row;
     return l;
 }
 }  // namespace

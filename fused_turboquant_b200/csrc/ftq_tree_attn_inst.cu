@@ -14,15 +14,7 @@ template <int BV, int N>
 static cudaError_t run_tree(const TreeAttnParams& p, int grid, cudaStream_t stream) {
     using C = TreeCfg<FTQ_D, FTQ_BK, BV, N>;
     constexpr auto kern = tree_attn_kernel<FTQ_D, FTQ_BK, BV, N>;
-    cudaError_t e = allow_smem<kern>(C::SMEM_BYTES);
-    if constexpr (C::SPLIT) {
-        // (the warps' shares of registers are those of a block launched with exactly this many: with fewer they would wait for good)
-        static const int regs = [] {
-            cudaFuncAttributes a{};
-            return cudaFuncGetAttributes(&a, kern) == cudaSuccess ? a.numRegs : -1;
-        }();
-        if (e == cudaSuccess && regs != C::REGS) e = cudaErrorInvalidKernelImage;
-    }
+    const cudaError_t e = allow_smem<kern>(C::SMEM_BYTES);
     return e != cudaSuccess ? e : launch_dependent(kern, dim3(grid), C::THREADS, C::SMEM_BYTES, stream, p);
 }
 

@@ -12,6 +12,9 @@ inline int tree_rows(int head_dim, int rows) {
     return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || head_dim == 256 ? 64 : 128;
 }
 
+// (TreeCfg::HALVES)
+inline int tree_halves(int head_dim, int n) { return head_dim == 256 || n == 128 ? 1 : 2; }
+
 #define FTQ_DECLARE_TREE(DD, KB) \
     cudaError_t launch_tree_attn_d##DD##_k##KB(int bits_v, int n, const TreeAttnParams& p, int grid, cudaStream_t stream);
 FTQ_DECLARE_TREE(64, 2) FTQ_DECLARE_TREE(64, 3) FTQ_DECLARE_TREE(64, 4)
