@@ -69,8 +69,8 @@ __host__ __device__ __forceinline__ int tree_tile_of(int off) { return off > kTr
 
 template <int D, int BK, int BV, int N>
 struct TreeCfg {
-    static constexpr int HALVES = D == 256 || N == 128 ? 1 : 2, WARPS = 16, THREADS = 512;
-    static constexpr int WH = WARPS / HALVES, HT = 32 * WH;        // warps and threads of a half
+    static constexpr int HALVES = D == 256 || N == 128 ? 1 : 2, WARPS = 16, THREADS = 512 + 64 * HALVES;
+    static constexpr int WH = WARPS / HALVES, HT = 32 * WH;        // warps and threads of a half, without its two helpers
     // softmax: column groups of four warps (a warp reaches the 32 tokens of its quarter), rows of a group
     static constexpr int CG = WH / 4 < N / 8 ? WH / 4 : N / 8, CW = N / CG;
     static constexpr int PDK = packed_dim(D, BK), PDV = packed_dim(D, BV);
@@ -82,14 +82,19 @@ struct TreeCfg {
     // Shared memory of a half: V (one buffer, two where there is room), P, queries, masks.  The look-up window takes 64 KB at 64 KB;
     // the dynamic part (the only one) starts in the first 4 KB.  (At head_dim 64 a product reads an atom beyond V, P's: unused rows.)
     static constexpr int VB = HALVES == 1 && D <= 128 ? 2 : 1, V_ATOM = kTreeTile * 128, V_BUF = V_ATOM * (D / 64);
+    static constexpr bool LATE_V = HALVES == 2;     // a tile's values are looked up after its weights
     static constexpr int P_ATOM = kTreeTile * 128, P_BUF = P_ATOM * ((N + 63) / 64);
     static constexpr int Q_BYTES = N * D * 2, MW = (N + 31) / 32, MASK_BYTES = kTreeMaxNodes * MW * 4;
     static constexpr int WINDOW = 65536, LOW = 4096, A_V = 131072, A_P = A_V + HALVES * VB * V_BUF;
-    static constexpr int SMEM_BYTES = A_P + HALVES * P_BUF;
     static constexpr int A_Q = LOW, A_MASK = A_Q + HALVES * Q_BYTES;
     static constexpr int A_ROW = A_MASK + HALVES * MASK_BYTES, ROW_BYTES = 7 * N * 4 + 64;   // - maximum, factors of l and O, red[4][N], red_v
-    static constexpr int A_FIRST = A_ROW + HALVES * ROW_BYTES;     // [kTreeMaxSeqs + 1]
-    static constexpr int A_MISC = (A_FIRST + (kTreeMaxSeqs + 1) * 4 + 15) / 16 * 16, A_BAR = A_MISC + 128, END_LOW = A_BAR + 64;
+    // codes on their way: the page of a warp (at head_dim 256 the value warps' lie behind P)
+    static constexpr int STAGE = 16 * (PDK > PDV ? PDK : PDV), LOW_STAGES = D == 256 ? 8 : 16;
+    static constexpr int A_STAGE = (A_ROW + HALVES * ROW_BYTES + 127) / 128 * 128, A_STAGE_HI = A_P + HALVES * P_BUF;
+    static constexpr int A_FIRST = A_STAGE + LOW_STAGES * STAGE, END_LOW = A_FIRST + (kTreeMaxSeqs + 1) * 4;     // [kTreeMaxSeqs + 1]
+    static constexpr int A_NORM = A_STAGE_HI + (WARPS - LOW_STAGES) * STAGE;       // a half's norms: keys [128], values [128]
+    static constexpr int A_MISC = A_NORM + HALVES * 512, A_BAR = A_MISC + 128, BARS = 9, A_PIECE = A_BAR + HALVES * BARS * 8;
+    static constexpr int SMEM_BYTES = A_PIECE + 128;
     static_assert(END_LOW <= WINDOW && SMEM_BYTES <= 227 * 1024 && Q_BYTES % 1024 == 0, "");
     // TMEM columns of a half: two key buffers, S, O
     static constexpr int COLS = 512 / HALVES, COL_S = D, COL_O = D + N;
@@ -155,12 +160,6 @@ __device__ __forceinline__ int load_id_if(bool ok, const int32_t* p, int otherwi
                  : "=&r"(v) : "r"(static_cast<uint32_t>(ok)), "l"(p), "r"(otherwise) : "memory");
     return v;
 }
-__device__ __forceinline__ uint16_t load_half_if(bool ok, const uint8_t* p) {
-    uint16_t v;
-    asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %1, 0;\nmov.b16 %0, 0;\n@q ld.global.b16 %0, [%2];\n}\n"
-                 : "=&h"(v) : "r"(static_cast<uint32_t>(ok)), "l"(p) : "memory");
-    return v;
-}
 // 32 lanes x NC columns, one row per lane, complete
 template <int NC>
 __device__ __forceinline__ void tc_load(uint32_t addr, uint32_t (&r)[NC]) {
@@ -187,35 +186,36 @@ __device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t* r) {
                  "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 
-// A lane's codes of a tile: its runs in two rows of a page.
-template <int XW>
-struct TreeCodes {
-    uint32_t w[2][XW];
-};
-// SB bytes into words, on the widest loads that their alignment allows (a run starts at a multiple of its size).
-template <int SB, int XW>
-__device__ __forceinline__ void tree_fetch(const uint8_t* src, uint32_t (&w)[XW]) {
+// SB bytes of codes into words (zeros if not ok), on the widest loads that their alignment allows: a run starts at a multiple
+// of its size.  Loads into the very registers that the values stay in: what is loaded to one and moved to another is
+// Run number `t` (SB bytes) of a row of codes in shared memory, codes from bit 0 on (rows start on 4 bytes).
+template <int SB, class Run>
+__device__ __forceinline__ void tree_run(uint32_t row, int t, Run& run) {
+    const uint32_t a = row + t * SB;
     if constexpr (SB % 16 == 0) {
 #pragma unroll
-        for (int i = 0; i < SB / 16; i++) {
-            const uint4 x = reinterpret_cast<const uint4*>(src)[i];
-            w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
-        }
+        for (int i = 0; i < SB / 16; i++)
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(run.w[4 * i]), "=r"(run.w[4 * i + 1]), "=r"(run.w[4 * i + 2]), "=r"(run.w[4 * i + 3])
+                         : "r"(a + 16 * i) : "memory");
     } else if constexpr (SB % 8 == 0) {
 #pragma unroll
-        for (int i = 0; i < SB / 8; i++) {
-            const uint2 x = reinterpret_cast<const uint2*>(src)[i];
-            w[2 * i] = x.x; w[2 * i + 1] = x.y;
-        }
+        for (int i = 0; i < SB / 8; i++)
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(run.w[2 * i]), "=r"(run.w[2 * i + 1]) : "r"(a + 8 * i) : "memory");
     } else if constexpr (SB % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < SB / 4; i++) w[i] = reinterpret_cast<const uint32_t*>(src)[i];
-    } else {   // six bytes on a two-byte boundary
+        for (int i = 0; i < SB / 4; i++) asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(run.w[i]) : "r"(a + 4 * i) : "memory");
+    } else {        // (six bytes on a two-byte boundary, in two words)
         static_assert(SB == 6, "");
-        const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
-        w[0] = h[0] | static_cast<uint32_t>(h[1]) << 16;
-        w[1] = h[2];
+        uint32_t lo, hi;
+        asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(lo) : "r"(a & ~3u) : "memory");
+        asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(hi) : "r"((a & ~3u) + 4) : "memory");
+        const int sh = (t & 1) * 16;
+        run.w[0] = __funnelshift_r(lo, hi, sh);
+        run.w[1] = hi >> sh;
     }
+}
+__device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
 template <int D, int BK, int BV, int N>
@@ -229,18 +229,21 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
     const uint32_t raw = static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw));
     auto at = [&](uint32_t a) { return smem_raw + (a - raw); };
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    const int half = warp / C::WH, hw = warp % C::WH, me = tid - half * C::HT;    // half, warp and thread in it
+    // half, warp and thread in it; of the last warps every half has two, one that issues its products and one that fetches its pages
+    const bool helper = warp >= C::WARPS;
+    const int half = helper ? (warp - C::WARPS) >> 1 : warp / C::WH, hw = warp % C::WH, me = helper ? C::HT + lane : tid - half * C::HT;
     uint32_t* const misc = reinterpret_cast<uint32_t*>(at(C::A_MISC));   // 0: TMEM, 1, 2: a half's wait ran out, 3, 4: its largest |q|, 8..: scan
     volatile uint32_t* const gave_up = misc + 1 + half;
-    const uint32_t s_done = C::A_BAR + 16 * half, o_done = s_done + 8, drained = C::A_BAR + 32 + 16 * half;
-    constexpr int kSums = C::HALVES == 2 ? 1 : 9;      // the warp of a half that issues P.V
+    // a half's barriers: products; codes and norms that are there, and that were looked at (one phase each per tile)
+    const uint32_t s_done = C::A_BAR + 8 * C::BARS * half, o_done = s_done + 8, drained = s_done + 16;
+    const uint32_t k_full = s_done + 24, v_full = s_done + 32, n_full = s_done + 40, k_free = s_done + 48, v_free = s_done + 56, n_free = s_done + 64;
 
     // ---- look-up window (struct Window): 256 rows of 256 bytes, keys in the first half of a row, values in the second
     {
         auto build = [&](int off, auto bits, const Codebook& cb) {
             constexpr int NB = decltype(bits)::value;
             const float lev = cb.v[lane & 15];
-            for (int e = warp; e < 256; e += C::WARPS) {
+            for (int e = warp; e < 256; e += C::THREADS / 32) {
                 auto pair = [&](int lo, int hi) {
                     const __half2 h = __floats2half2_rn(__shfl_sync(0xffffffffu, lev, lo), __shfl_sync(0xffffffffu, lev, hi));
                     return *reinterpret_cast<const uint32_t*>(&h);
@@ -264,7 +267,10 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(static_cast<uint32_t>(C::A_MISC)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
         if (lane == 0) {
-            for (int i = 0; i < 8; i++) mbar_init(C::A_BAR + 8 * i, 1);
+            for (int h = 0; h < C::HALVES; h++) {
+                const uint32_t bars = C::A_BAR + 8 * C::BARS * h;
+                for (int i = 0; i < C::BARS; i++) mbar_init(bars + 8 * i, i < 3 ? 1 : i == 5 ? 16 : i == 8 ? C::WH : 8);
+            }
             mbar_fence_init();
         }
         tc_fence_before();
@@ -291,7 +297,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
             if (lane == 31) misc[8 + warp] = x;
             __syncthreads();
             int sum = 0, before = 0;
-            for (int w = 0; w < C::WARPS; w++) {
+            for (int w = 0; w < C::THREADS / 32; w++) {
                 before += w < warp ? static_cast<int>(misc[8 + w]) : 0;
                 sum += misc[8 + w];
             }
@@ -306,7 +312,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
     const int total = first[p.B], share = (total + workers - 1) / workers;
     const int end = static_cast<int>(min(static_cast<int64_t>(total), static_cast<int64_t>(worker + 1) * share));
     const int begin = static_cast<int>(min(static_cast<int64_t>(worker) * share, static_cast<int64_t>(end)));
-    if (worker == 0) {
+    if (worker == 0 && !helper) {
         for (int b = me; b <= p.B; b += C::HT) p.plan[b] = first[b];
         if (me == 0) p.plan[p.B + 1] = share;
     }
@@ -321,8 +327,25 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
         __syncwarp();
         tc_fence_after();
     };
-    // the half's barrier; true if any thread says so
-    auto meet = [&](bool mine) { return group_any<C::HT>(1 + half, mine); };
+    // The same for copies, which are waited for whatever has happened to the products (none may be in flight when the CTA ends).
+    bool stalled = false;
+    auto copied = [&](uint32_t bar, uint32_t parity) {
+        if (stalled) return;
+        bool there = false;
+#pragma unroll 1
+        for (int i = 0; i < kDrainSpinLimit && !there; i++) there = mbar_try_wait(bar, parity & 1u);
+        stalled = !__all_sync(0xffffffffu, there);
+        if (stalled) *gave_up = 1;
+    };
+    // the warp has looked at what came
+    auto taken = [&](uint32_t bar) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+    };
+    // barriers of a half: its workers'; theirs and the issuer's (true if any thread says so); theirs and the feeder's
+    auto meet = [&](bool) { group_any<C::HT>(3 + half, false); };
+    auto meet_issuer = [&](bool mine) { return group_any<C::HT + 32>(1 + half, mine); };
+    auto meet_feeder = [&]() { group_any<C::HT + 32>(5 + half, false); };
     // the first piece with tiles from a place on; moves on to the place behind it
     auto next_piece = [&](int& pos) {
         TreePiece pc{};
@@ -366,101 +389,17 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
     float *const s_lc = s_nm + N, *const s_corr = s_lc + N, *const red = s_corr + N, *const red_v = red + 4 * N;
     uint32_t* const cm = reinterpret_cast<uint32_t*>(at(C::A_MASK + half * C::MASK_BYTES));
     const uint32_t k_base = C::WINDOW + (BK == 2 ? (lane & 15) * 8 : lane * 4), v_base = C::WINDOW + 128 + (BV == 2 ? (lane & 15) * 8 : lane * 4);
-    int s_waits = 0, o_waits = 0;      // phases of the half's two barriers
+    const uint32_t a_norm = C::A_NORM + 512 * half;
+    auto stage_of = [&](int w) { return w < C::LOW_STAGES ? C::A_STAGE + w * C::STAGE : C::A_STAGE_HI + (w - C::LOW_STAGES) * C::STAGE; };
+    int done = 0;       // tiles of earlier pieces: barriers have a phase for each tile
 
-    int pos = begin;
-#pragma unroll 1
-    for (TreePiece pc = next_piece(pos); pc.n_tiles > 0; pc = next_piece(pos)) {
-        const int n_tiles = pc.n_tiles, group = static_cast<int>(p.group.d);
-        // ---- block ids: lane l has those of tile base + l and of base + 32 + l, for the two pages of the warp's quarter
-        const int32_t* const btab = p.block_table + static_cast<int64_t>(pc.b) * p.max_blocks;
-        auto load_ids = [&](int tile, int which) {
-            const int pg = (pc.tile0 + tile + lane) * (kTreeTile / kPageTokens) + 2 * quarter + which;
-            return load_id_if(tile + lane < n_tiles && pg * kPageTokens < pc.seq, btab + pg, -2);     // -2: no tokens
-        };
-        int base = 0, ida[2] = {load_ids(0, 0), load_ids(0, 1)}, idb[2] = {load_ids(32, 0), load_ids(32, 1)};
-        auto id_of = [&](int tile, int which) {
-            const int src = tile - base, ids = src < 32 ? (which ? ida[1] : ida[0]) : (which ? idb[1] : idb[0]);
-            return __shfl_sync(0xffffffffu, ids, src & 31);
-        };
-        auto page_at = [&](int id) { return p.pool + (static_cast<int64_t>(id) * p.Hkv + pc.hkv) * C::PAGE_BYTES; };
-        auto in_pool = [&](int id) { return static_cast<uint64_t>(static_cast<int64_t>(id)) < static_cast<uint64_t>(p.num_blocks); };
-        uint32_t fk[2][KW], fv[2][VW];
-        auto fetch_k = [&](int tile) {
-            const int id = tile < n_tiles ? id_of(tile, odd) : -2;
-            if (!in_pool(id)) {
-#pragma unroll
-                for (int j = 0; j < KW; j++) fk[0][j] = fk[1][j] = 0;
-                return;
-            }
-#pragma unroll
-            for (int r = 0; r < 2; r++) tree_fetch<KSB>(page_at(id) + (g8 + 8 * r) * C::PDK + t4 * KSB, fk[r]);
-        };
-        auto fetch_v = [&](int tile) {
-            const int id = tile < n_tiles ? id_of(tile, odd) : -2;
-            if (!in_pool(id)) {
-#pragma unroll
-                for (int j = 0; j < VW; j++) fv[0][j] = fv[1][j] = 0;
-                return;
-            }
-            // (a V row has its halves exchanged where bit 1 of its token's place is set)
-#pragma unroll
-            for (int r = 0; r < 2; r++) tree_fetch<VSB>(page_at(id) + C::OFF_VC + (g8 + 8 * r) * C::PDV + (t4 ^ (g8 & 2)) * VSB, fv[r]);
-        };
-        uint16_t nk = 0, nv = 0;       // norms of the thread's token in the next tile
-        bool bad = false;
-        auto fetch_norms = [&](int tile) {
-            const int a = id_of(tile, 0), b = id_of(tile, 1), id = lane < 16 ? a : b;
-            const bool ok = in_pool(id);
-            const uint8_t* page = page_at(id) + 2 * (lane & 15);
-            nk = load_half_if(ok, page + C::OFF_KN);
-            nv = load_half_if(ok, page + C::OFF_VN);
-            bad = !ok && id != -2;
-        };
-        // keys: codes -> TMEM, rows = tokens
-        auto put_k = [&](int tile) {
-            typename Window<BK, false>::template Run<KW> r0, r1;
-#pragma unroll
-            for (int j = 0; j < KW; j++) {
-                r0.w[j] = fk[0][j];
-                r1.w[j] = fk[1][j];
-            }
-            Window<BK, false>::shift(r0);
-            Window<BK, false>::shift(r1);
-            const uint32_t dst = tmem + (static_cast<uint32_t>(16 * my_page) << 16) + (tile & 1) * (D / 2);
-#pragma unroll
-            for (int q = 0; q < D / 64; q++) {
-                uint32_t x[16];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    Window<BK, false>::pairs(r0, 4 * q + j, k_base, x[4 * j], x[4 * j + 1]);
-                    Window<BK, false>::pairs(r1, 4 * q + j, k_base, x[4 * j + 2], x[4 * j + 3]);
-                }
-                tc_st_16x256b_x4(dst + 32 * q, x);
-            }
-        };
-        // values: codes -> fp16 tile, MN-major with 128-byte swizzle
-        auto put_v = [&](int tile) {
-#pragma unroll
-            for (int r = 0; r < 2; r++) {
-                typename Window<BV, false>::template Run<VW> run;
-#pragma unroll
-                for (int j = 0; j < VW; j++) run.w[j] = fv[r][j];
-                Window<BV, false>::shift(run);
-                const int row = 16 * my_page + g8 + 8 * r;
-                const uint32_t dst = a_v + (tile % C::VB) * C::V_BUF + row * 128;
-#pragma unroll
-                for (int jj = 0; jj < D / 32; jj++) {
-                    uint32_t x[4];
-                    Window<BV, false>::pairs(run, 2 * jj, v_base, x[0], x[1]);
-                    Window<BV, false>::pairs(run, 2 * jj + 1, v_base, x[2], x[3]);
-                    // (eight lanes that store together have two rows and four chunks apart by two: no two on the same banks)
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(dst + (jj >> 1) * C::V_ATOM + (((2 * t4 + (jj & 1)) ^ (row & 7)) << 4)),
-                                 "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
-                }
-            }
-        };
-        // ---- the products, by one lane
+    // (In shared memory: what is needed once a piece would take the registers that the tiles need.  One thread finds a piece and
+    // keeps the place behind it; the barrier at the end of a piece is behind every look at it.)
+    static_assert(sizeof(TreePiece) <= 56, "");
+    volatile TreePiece& pc = *reinterpret_cast<volatile TreePiece*>(at(C::A_PIECE + 64 * half));
+    volatile int& pos = *reinterpret_cast<volatile int*>(at(C::A_PIECE + 64 * half + 56));
+    if (helper && (warp & 1) == 0) {
+        // ---- the products of a half: one lane of its first helper
         constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(N / 8) << 17) | (8u << 24);
         constexpr uint32_t kIdescO = kIdescS | (1u << 15) | (1u << 16);
         constexpr uint32_t kHi = (1024u >> 4) | (1u << 14) | (2u << 29);
@@ -491,10 +430,239 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
             }
             __syncwarp();
         };
-        // ---- the first keys and values on their way, then the queries: rotated, scaled, fp16, K-major with 128-byte swizzle
-        fetch_norms(0);
-        if (has_k) fetch_k(0);
-        if (has_v) fetch_v(0);
+#pragma unroll 1
+        while (true) {
+            meet_issuer(false);
+            tc_fence_after();
+            const int n_tiles = pc.n_tiles;
+            if (n_tiles == 0) break;
+            scores(0);
+#pragma unroll 1
+            for (int it = 0; it < n_tiles; it++) {
+                if (meet_issuer(false)) meet_issuer(false);     // (new maxima: the tile's weights come again)
+                tc_fence_after();
+                if (it + 1 < n_tiles) scores(it + 1);
+                sums(it);
+            }
+        }
+        // nothing may be in flight when TMEM is given back
+        if (elect_one()) tc_commit(drained);
+        __syncwarp();
+#pragma unroll 1
+        for (int i = 0; i < kDrainSpinLimit && !mbar_try_wait(drained, 0); i++) {}
+    }
+    // ---- the pages of a half: its second helper.  Codes and norms come by bulk copies, a page of codes a warp, as soon as what lay
+    // in their place was looked at.  (Registers would be the wrong place for them: loads that share one of the few scoreboards
+    // complete together, so that a look at anything waits for the newest; and a copy takes its issuer 400 cycles.)
+    if (helper && (warp & 1) == 1) {
+        int k_sent = 0, v_sent = 0, n_sent = 0;
+#pragma unroll 1
+        while (true) {
+            meet_feeder();
+            const int n_tiles = pc.n_tiles;
+            if (n_tiles == 0) break;
+            const int tile0 = pc.tile0, seq = pc.seq;
+            const int32_t* const btab = p.block_table + static_cast<int64_t>(pc.b) * p.max_blocks;
+            const uint8_t* const pool = p.pool + static_cast<int64_t>(pc.hkv) * C::PAGE_BYTES;
+            // block ids of four tiles' pages (idb: of the next four); -2: no tokens
+            auto load_ids = [&](int tile) {
+                const int t = tile + (lane >> 3), pg = (tile0 + t) * (kTreeTile / kPageTokens) + (lane & 7);
+                return load_id_if(t < n_tiles && pg * kPageTokens < seq, btab + pg, -2);
+            };
+            int ida = load_ids(0), idb = load_ids(4);
+            // of lane's page of a tile, while `now` is the tile that ida begins with or one of the three behind it
+            auto id_of = [&](int tile, int now) { return __shfl_sync(0xffffffffu, (tile ^ now) < 4 ? ida : idb, (tile & 3) * 8 + (lane & 7)); };
+            auto in_pool = [&](int id) { return static_cast<uint64_t>(static_cast<int64_t>(id)) < static_cast<uint64_t>(p.num_blocks); };
+            auto page_of = [&](int id) { return pool + static_cast<int64_t>(id) * p.Hkv * C::PAGE_BYTES; };
+            // page g of a tile is warp 4 (g & 1) + g / 2's; values: of the warps behind, if there are any
+            const int owner = half * C::WH + 4 * (lane & 1) + ((lane & 7) >> 1);
+            const uint32_t k_stage = stage_of(owner), v_stage = C::LATE_V ? a_v + 2048 * (lane & 7) : stage_of(owner + 8);
+            // (what lies in the place of a page that is not there is as good: its weights are zero, or no numbers)
+            auto fetch = [&](uint32_t bar, uint32_t dst, int id, int off, uint32_t bytes, int& sent) {
+                if (stalled) return;
+                sent++;
+                if (lane < 8) {
+                    if (in_pool(id)) {
+                        mbar_expect_tx(bar, bytes);
+                        bulk_g2s(dst, page_of(id) + off, bytes, bar);
+                    } else {
+                        mbar_arrive(bar);
+                    }
+                }
+                __syncwarp();
+            };
+            constexpr uint32_t kKeys = kPageTokens * C::PDK, kValues = kPageTokens * C::PDV;
+            auto fetch_k = [&](int tile, int now) { fetch(k_full, k_stage, id_of(tile, now), 0, kKeys, k_sent); };
+            auto fetch_v = [&](int tile, int now) { fetch(v_full, v_stage, id_of(tile, now), C::OFF_VC, kValues, v_sent); };
+            // norms of a tile; a key of a page that is not in the pool has one that is no number
+            auto fetch_norms = [&](int tile, int now) {
+                const int id = id_of(tile, now);
+                if (stalled) return;
+                n_sent++;
+                if (lane < 16) {
+                    const bool value = lane & 8;
+                    const uint32_t to = a_norm + 32 * lane;
+                    if (in_pool(id)) {
+                        mbar_expect_tx(n_full, 32);
+                        bulk_g2s(to, page_of(id) + (value ? C::OFF_VN : C::OFF_KN), 32, n_full);
+                    } else {
+                        if (id != -2) {
+                            if (!value) {
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(to), "r"(0x7e007e00u) : "memory");
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(to + 16), "r"(0x7e007e00u) : "memory");
+                            }
+                            __stcg(p.errors + 1, p.epoch);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                        mbar_arrive(n_full);
+                    }
+                }
+                __syncwarp();
+            };
+            if (C::LATE_V) {
+                // The first two tiles' keys at once and in one phase; the second's to where the warp's first values will be.  (Values
+                // wait in the place that they are written to as fp16: a page's 2 KB there have room for two pages' codes.)
+                const int id0 = id_of(0, 0), id1 = id_of(1, 0);
+                if (!stalled) {
+                    k_sent++;
+                    if (lane < 8) {
+                        const bool has0 = in_pool(id0), has1 = n_tiles > 1 && in_pool(id1);
+                        mbar_expect_tx(k_full, (has0 ? kKeys : 0) + (has1 ? kKeys : 0));
+                        if (has0) bulk_g2s(k_stage, page_of(id0), kKeys, k_full);
+                        if (has1) bulk_g2s(v_stage + 1024, page_of(id1), kKeys, k_full);
+                    }
+                    __syncwarp();
+                }
+                fetch_norms(0, 0);
+                fetch_v(0, 0);
+                if (n_tiles > 1) {
+                    copied(k_free, done);
+                    if (!stalled) {
+                        k_sent++;
+                        if (lane < 8) mbar_arrive(k_full);
+                        __syncwarp();
+                    }
+                    if (n_tiles > 2) fetch_k(2, 0);
+                    copied(k_free, done + 1);
+                }
+            } else {
+                fetch_k(0, 0);
+                fetch_v(0, 0);
+                fetch_norms(0, 0);
+                if (n_tiles > 1) {
+                    copied(k_free, done);
+                    fetch_k(1, 0);
+                    copied(v_free, done);
+                    fetch_v(1, 0);
+                }
+                if (n_tiles > 2) {
+                    copied(k_free, done + 1);
+                    fetch_k(2, 0);
+                }
+            }
+#pragma unroll 1
+            for (int it = 0; it + 1 < n_tiles; it++) {
+                copied(n_free, done + it);
+                fetch_norms(it + 1, it + 1);
+                if (it + 3 < n_tiles) {
+                    copied(k_free, done + it + 2);
+                    fetch_k(it + 3, it + 1);
+                }
+                if (C::LATE_V) {
+                    wait(o_done, done + it);
+                    fetch_v(it + 1, it + 1);
+                } else if (it + 2 < n_tiles) {
+                    copied(v_free, done + it + 1);
+                    fetch_v(it + 2, it + 1);
+                }
+                if (((it + 2) & 3) == 0) {      // (ida has the ids of the next round's tile it + 1)
+                    ida = idb;
+                    idb = load_ids(it + 6);
+                }
+            }
+            done += n_tiles;
+        }
+        auto drain = [&](uint32_t bar, int sent) {
+#pragma unroll 1
+            for (int i = 0; i < kDrainSpinLimit && sent > 0 && !mbar_try_wait(bar, (sent - 1) & 1); i++) {}
+        };
+        drain(k_full, k_sent);
+        drain(v_full, v_sent);
+        drain(n_full, n_sent);
+    }
+    if (me == 0) pos = begin;
+    const uint32_t stage = stage_of(warp);
+#pragma unroll 1
+    while (!helper) {
+        if (me == 0) {
+            int from = pos;
+            const TreePiece x = next_piece(from);
+            pc.b = x.b;
+            pc.hkv = x.hkv;
+            pc.row0 = x.row0;
+            pc.rows = x.rows;
+            pc.tile0 = x.tile0;
+            pc.n_tiles = x.n_tiles;
+            pc.seq = x.seq;
+            pc.ctx = x.ctx;
+            pc.out = x.out;
+            pos = from;
+        }
+        meet_feeder();
+        const int n_tiles = pc.n_tiles, group = static_cast<int>(p.group.d);
+        if (n_tiles == 0) {
+            meet_issuer(false);
+            break;
+        }
+        const int first_masked = pc.ctx / kTreeTile - pc.tile0;       // (from here on tiles reach the tree or the sequence's end)
+        // keys: codes -> TMEM, rows = tokens
+        auto put_k = [&](int tile, uint32_t from) {
+            copied(k_full, done + tile);
+            typename Window<BK, false>::template Run<KW> r0, r1;
+            tree_run<KSB>(from + g8 * C::PDK, t4, r0);
+            tree_run<KSB>(from + (g8 + 8) * C::PDK, t4, r1);
+            taken(k_free);
+            Window<BK, false>::shift(r0);
+            Window<BK, false>::shift(r1);
+            const uint32_t dst = tmem + (static_cast<uint32_t>(16 * my_page) << 16) + (tile & 1) * (D / 2);
+#pragma unroll
+            for (int q = 0; q < D / 64; q++) {
+                uint32_t x[16];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    Window<BK, false>::pairs(r0, 4 * q + j, k_base, x[4 * j], x[4 * j + 1]);
+                    Window<BK, false>::pairs(r1, 4 * q + j, k_base, x[4 * j + 2], x[4 * j + 3]);
+                }
+                tc_st_16x256b_x4(dst + 32 * q, x);
+            }
+        };
+        // values: codes -> fp16 tile, MN-major with 128-byte swizzle
+        // (a V row has its halves exchanged where bit 1 of its token's place is set)
+        auto put_v = [&](int tile) {
+            copied(v_full, done + tile);
+            const uint32_t from = (C::LATE_V ? a_v + 2048 * my_page : stage) + g8 * C::PDV;
+            typename Window<BV, false>::template Run<VW> run[2];
+#pragma unroll
+            for (int r = 0; r < 2; r++) tree_run<VSB>(from + 8 * r * C::PDV, t4 ^ (g8 & 2), run[r]);
+            if (C::LATE_V) __syncwarp();
+            else taken(v_free);
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                Window<BV, false>::shift(run[r]);
+                const int row = 16 * my_page + g8 + 8 * r;
+                const uint32_t dst = a_v + (tile % C::VB) * C::V_BUF + row * 128;
+#pragma unroll
+                for (int jj = 0; jj < D / 32; jj++) {
+                    uint32_t x[4];
+                    Window<BV, false>::pairs(run[r], 2 * jj, v_base, x[0], x[1]);
+                    Window<BV, false>::pairs(run[r], 2 * jj + 1, v_base, x[2], x[3]);
+                    // (eight lanes that store together have two rows and four chunks apart by two: no two on the same banks)
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(dst + (jj >> 1) * C::V_ATOM + (((2 * t4 + (jj & 1)) ^ (row & 7)) << 4)),
+                                 "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+                }
+            }
+        };
+        // ---- the queries: rotated, scaled, fp16, K-major with 128-byte swizzle
         float q_down;
         {
             constexpr int OCTETS = C::HT / 8;
@@ -507,33 +675,54 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 if (p.q_dtype == kBF16) load8<__nv_bfloat16>(reinterpret_cast<const __nv_bfloat16*>(&x), o);
                 else load8<__half>(reinterpret_cast<const __half*>(&x), o);
             };
+            // (read once: two rows an octet at most)
+            constexpr int NR = (N + OCTETS - 1) / OCTETS;
+            uint4 raw[NR][D / 64];
+#pragma unroll
+            for (int k = 0; k < NR; k++)
+#pragma unroll
+                for (int j = 0; j < D / 64; j++) {
+                    const int r = octet + k * OCTETS;
+                    raw[k][j] = r < pc.rows ? query(r)[t8 + 8 * j] : make_uint4(0, 0, 0, 0);
+                }
+            // the mask words of the rows' nodes (to where weights will be)
+            const bool trees = (pc.tile0 + n_tiles) * kTreeTile > pc.ctx;
+            const int i0 = fast_div(pc.row0, p.group), words = (p.T + 31) / 32;
+            uint32_t* const mask_words = reinterpret_cast<uint32_t*>(at(a_p));
+            static_assert(N * (kTreeMaxNodes / 32) * 4 <= C::P_BUF, "");
+            if (trees)
+                for (int k = me; k < (fast_div(pc.row0 + pc.rows - 1, p.group) - i0 + 1) * words; k += C::HT)
+                    mask_words[k] = p.masks[(static_cast<int64_t>(pc.b) * p.T + i0 + k / words) * p.W + k % words];
             // the largest, for a common scale: |rotated| <= D * largest |q|, and that shall be below 2^15
             float top = 0.f;
-#pragma unroll 4
-            for (int k = me; k < pc.rows * (D / 8); k += C::HT) {
-                float v[8];
-                widen(query(k / (D / 8))[k % (D / 8)], v);
 #pragma unroll
-                for (int c = 0; c < 8; c++) top = fabsf(v[c]) <= FLT_MAX ? fmaxf(top, fabsf(v[c])) : top;
-            }
+            for (int k = 0; k < NR; k++)
+#pragma unroll
+                for (int j = 0; j < D / 64; j++) {
+                    float v[8];
+                    widen(raw[k][j], v);
+#pragma unroll
+                    for (int c = 0; c < 8; c++) top = fabsf(v[c]) <= FLT_MAX ? fmaxf(top, fabsf(v[c])) : top;
+                }
             __syncwarp();
             top = warp_max(top);
-            if (me == 0) misc[3 + half] = 0;
+            if (lane == 0) red[hw] = top;
             if (me < N) s_nm[me] = INFINITY;
             meet(false);
-            if (lane == 0) atomicMax(misc + 3 + half, __float_as_uint(top));
-            meet(false);
-            const float all = __uint_as_float(misc[3 + half]) * (fabsf(p.q_scale) * D);
+#pragma unroll
+            for (int w = 0; w < C::WH; w++) top = fmaxf(top, red[w]);
+            const float all = top * (fabsf(p.q_scale) * D);
             const int e = all > 0.f ? max(-120, min(120, 14 - ilogbf(all))) : 0;
             const float up = p.q_scale * ldexpf(1.f, e);
             q_down = ldexpf(1.f, -e);
-#pragma unroll 1
-            for (int r = octet; r - octet < N; r += OCTETS) {
+#pragma unroll
+            for (int k2 = 0; k2 < NR; k2++) {
+                const int r = octet + k2 * OCTETS;
                 float a[E];
 #pragma unroll
                 for (int k = 0; k < D / 64; k++) {
                     float v[8];
-                    widen(r < pc.rows ? query(r)[t8 + 8 * k] : make_uint4(0, 0, 0, 0), v);
+                    widen(raw[k2][k], v);
 #pragma unroll
                     for (int c = 0; c < 8; c++)
                         a[8 * k + c] = __uint_as_float(__float_as_uint(v[c] * up) ^ sign_mask(p.signs, load_coord(t8, 8 * k + c)));
@@ -551,7 +740,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 }
             }
             // which rows attend a node: bit r of its words
-            if ((pc.tile0 + n_tiles) * kTreeTile > pc.ctx) {
+            if (trees) {
                 for (int k = me; k < (pc.seq - pc.ctx) * C::MW; k += C::HT) {
                     const int node = k / C::MW, w = k % C::MW;
                     uint32_t bits = 0;
@@ -560,7 +749,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
 #pragma unroll 1
                     for (int r = 32 * w; r < r1;) {
                         const int i = fast_div(pc.row0 + r, p.group), stop = min(r1, (i + 1) * group - pc.row0);
-                        if ((static_cast<uint32_t>(p.masks[(static_cast<int64_t>(pc.b) * p.T + i) * p.W + (node >> 5)]) >> (node & 31)) & 1u)
+                        if ((mask_words[(i - i0) * words + (node >> 5)] >> (node & 31)) & 1u)
                             bits |= (0xffffffffu >> (32 - (stop - r))) << (r & 31);
                         r = stop;
                     }
@@ -568,37 +757,32 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 }
             }
         }
-        if (has_k) {
-            put_k(0);
-            fetch_k(1);
-        }
-        if (has_v) {
-            put_v(0);
-            fetch_v(1);
-        }
+        if (has_k) put_k(0, stage);
+        if (has_v && !C::LATE_V) put_v(0);
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
         tc_wait_st();
         tc_fence_before();
-        meet(false);
-        tc_fence_after();
-        if (hw == 0) scores(0);
-        if (has_k && n_tiles > 1) {
-            put_k(1);
-            fetch_k(2);
-        }
-        float l[CW], m_run = -INFINITY, vs = 0.f;      // sums of the thread's tokens; lane c: maximum of the group's row c; scale of |v|
+        meet_issuer(false);
+        if (has_k && n_tiles > 1) put_k(1, C::LATE_V ? a_v + 2048 * my_page + 1024 : stage);
+        float l[CW], vs = 0.f;      // sums of the thread's tokens; scale of |v|
 #pragma unroll
         for (int c = 0; c < CW; c++) l[c] = 0.f;
 
 #pragma unroll 1
         for (int it = 0; it < n_tiles; it++) {
-            const int node = (pc.tile0 + it) * kTreeTile + my_tok - pc.ctx;
-            const bool masked = (pc.tile0 + it + 1) * kTreeTile > pc.ctx;     // (the tile reaches the tree or the sequence's end)
-            const float kn = bad ? __int_as_float(0x7fc00000) : half_bits_to_float(nk) * q_down, vn = half_bits_to_float(nv);
-            if (bad) __stcg(p.errors + 1, p.epoch);
+            const bool masked = it >= first_masked;
+            uint32_t nk, nv;
+            copied(n_full, done + it);
+            asm volatile("ld.shared.u16 %0, [%1];\n" : "=r"(nk) : "r"(a_norm + 2 * my_tok) : "memory");
+            asm volatile("ld.shared.u16 %0, [%1];\n" : "=r"(nv) : "r"(a_norm + 256 + 2 * my_tok) : "memory");
+            taken(n_free);
+            const float kn = half_bits_to_float(nk) * q_down, vn = half_bits_to_float(nv);
             // which of the group's rows attend the token; |v| where one does and it is finite
             uint32_t bits = 0xffffffffu;
-            if (masked && node >= 0) bits = node >= pc.seq - pc.ctx ? 0u : cm[node * C::MW + col0 / 32] >> (col0 & 31);
+            if (masked) {
+                const int node = (pc.tile0 + it) * kTreeTile + my_tok - pc.ctx;
+                if (node >= 0) bits = node >= pc.seq - pc.ctx ? 0u : cm[node * C::MW + col0 / 32] >> (col0 & 31);
+            }
             if (CW < 32) bits &= (1u << (CW & 31)) - 1u;
             const float av = bits != 0 && fabsf(vn) <= FLT_MAX ? fabsf(vn) : 0.f;
             const uint32_t s_at = tl + C::COL_S + col0;
@@ -639,38 +823,47 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 }
             };
             auto apply_masks = [&](float* x) {
+                asm volatile("" ::: "memory");      // (a branch: selects in every tile would be a tenth of its instructions)
 #pragma unroll
                 for (int c = 0; c < CW; c++) x[c] = (bits >> c) & 1u ? x[c] : -INFINITY;
             };
-            wait(s_done, s_waits++);
-            if (C::VB == 2 && it > 0) wait(o_done, o_waits++);       // (P.V of the tile before has read the weights)
+            wait(s_done, done + it);
+            if (!C::LATE_V && C::VB == 2 && it > 0) wait(o_done, done + it - 1);       // (P.V of the tile before has read the weights)
             bool above = false;
+            float x[CW];
             if (soft) {
-                float x[CW];
                 exponents(x);
                 if (masked) apply_masks(x);
                 float top = fmaxf(x[0], x[1]);
 #pragma unroll
                 for (int c = 2; c < CW; c += 2) top = fmaxf(fmaxf(top, x[c]), x[c + 1]);
                 above = __any_sync(0xffffffffu, top > kTreeSlack || (vs == 0.f ? av > 0.f : av * vs > kTreeGrowth));
-                if (!above) {
-                    if (masked) weights(x, std::true_type{}, true);
-                    else weights(x, std::false_type{}, true);
-                }
+            }
+            if (C::LATE_V && it > 0) wait(o_done, done + it - 1);
+            if (soft && !above) {
+                if (masked) weights(x, std::true_type{}, true);
+                else weights(x, std::false_type{}, true);
+            }
+            if (C::LATE_V) {
+                put_v(it);
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             tc_wait_st();
             tc_fence_before();
-            if (meet(above)) {
+            if (meet_issuer(above)) {
                 // ---- new maxima; O, the sums and the tile's weights refer to them
+                const float m_run = soft && lane < CW ? -s_nm[col0 + lane] : 0.f;
                 if (soft) {
-                    uint32_t s[CW];
-                    tc_load(s_at, s);
                     float mine = -INFINITY;
+#pragma unroll 1
+                    for (int c0 = 0; c0 < CW; c0 += 8) {
+                        uint32_t s[8];
+                        tc_load(s_at + c0, s);
 #pragma unroll
-                    for (int c = 0; c < CW; c++) {
-                        const float r = warp_max((bits >> c) & 1u ? __uint_as_float(s[c]) * kn : -INFINITY);
-                        if (lane == c) mine = r;
+                        for (int c = 0; c < 8; c++) {
+                            const float r = warp_max((bits >> (c0 + c)) & 1u ? __uint_as_float(s[c]) * kn : -INFINITY);
+                            if (lane == c0 + c) mine = r;
+                        }
                     }
                     const float wv = warp_max(av);
                     if (lane < CW) red[quarter * N + col0 + lane] = mine;
@@ -692,7 +885,6 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
 #pragma unroll
                         for (int w = 0; w < 4; w++) m_new = fmaxf(m_new, red[w * N + col0 + lane]);
                         const float lc = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
-                        m_run = m_new;
                         if (quarter == 0) {
                             s_nm[col0 + lane] = -m_new;
                             s_lc[col0 + lane] = lc;
@@ -707,16 +899,17 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                     if (it > 0) {       // (P.V of the tile before is complete)
 #pragma unroll
                         for (int mb = 0; mb < C::MB; mb++) {
-                            uint32_t o[CW];
-                            const uint32_t o_at = tl + C::COL_O + mb * N + col0;
-                            tc_load(o_at, o);
+#pragma unroll 1
+                            for (int c = 0; c < CW; c += 8) {       // (few registers: what this path spills the others pay for)
+                                uint32_t o[8];
+                                const uint32_t o_at = tl + C::COL_O + mb * N + col0 + c;
+                                tc_load(o_at, o);
 #pragma unroll
-                            for (int c = 0; c < CW; c++) o[c] = __float_as_uint(__uint_as_float(o[c]) * s_corr[col0 + c]);
-#pragma unroll
-                            for (int c = 0; c < CW; c += 8) tc_st8(o_at + c, o + c);
+                                for (int k = 0; k < 8; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * s_corr[col0 + c + k]);
+                                tc_st8(o_at, o);
+                            }
                         }
                     }
-                    float x[CW];
                     exponents(x);
                     apply_masks(x);
                     weights(x, std::true_type{}, above);
@@ -724,34 +917,20 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 tc_wait_st();
                 tc_fence_before();
-                meet(false);
+                meet_issuer(false);
             }
             tc_fence_after();
-            // ---- the products: this tile's P.V, the next one's scores
-            if (hw == 0 && it + 1 < n_tiles) scores(it + 1);
-            if (hw == kSums) sums(it);
             if (it + 1 == n_tiles) break;
             // ---- the tiles to come
-            if (it + 1 - base == 32) {        // (norms are the last to need a tile's ids)
-                ida[0] = idb[0];
-                ida[1] = idb[1];
-                base += 32;
-                idb[0] = load_ids(base + 32, 0);
-                idb[1] = load_ids(base + 32, 1);
-            }
-            fetch_norms(it + 1);
-            if (has_k && it + 2 < n_tiles) {
-                put_k(it + 2);
-                fetch_k(it + 3);
-            }
-            if (C::VB == 1) wait(o_done, o_waits++);
-            if (has_v) {
-                put_v(it + 1);
-                fetch_v(it + 2);
+            if (has_k && it + 2 < n_tiles) put_k(it + 2, stage);
+            if (!C::LATE_V) {
+                if (C::VB == 1) wait(o_done, done + it);
+                if (has_v) put_v(it + 1);
             }
         }
         // ---- the piece's rows
-        wait(o_done, o_waits++);
+        wait(o_done, done + n_tiles - 1);
+        done += n_tiles;
         if (soft) {
             // sums over the lanes, then over the warps: lane c gets row c's
             float sum[CW];
@@ -777,7 +956,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
             if (quarter == 0 && lane < CW && col0 + lane < pc.rows) {
                 float* dst = pc.out + (col0 + lane) * ROW + D;
                 const float* r = red + col0 + lane;
-                dst[0] = m_run;
+                dst[0] = -s_nm[col0 + lane];
                 dst[1] = r[0] + r[N] + r[2 * N] + r[3 * N];
             }
             const float scale = p.inv_v_scale / (vs == 0.f ? 1.f : vs);
@@ -800,19 +979,11 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
     }
     __syncwarp();
     __syncthreads();
-    if (*gave_up) {   // all that this half has
+    if (*gave_up && !helper) {   // all that this half has
         int at_pos = begin;
         for (TreePiece pc = next_piece(at_pos); pc.n_tiles > 0; pc = next_piece(at_pos))
             for (int r = me; r < N; r += C::HT) pc.out[r * ROW + D] = __int_as_float(0x7fc00000);
         if (me == 0) __stcg(p.errors, p.epoch);
-    }
-    // nothing may be in flight when TMEM is given back: the two warps of a half that issue products wait for theirs
-    if (hw == 0 || hw == kSums) {
-        const uint32_t bar = drained + (hw == 0 ? 0 : 8);
-        if (elect_one()) tc_commit(bar);
-        __syncwarp();
-#pragma unroll 1
-        for (int i = 0; i < kDrainSpinLimit && !mbar_try_wait(bar, 0); i++) {}
     }
     __syncthreads();
     if (warp == 0) {
