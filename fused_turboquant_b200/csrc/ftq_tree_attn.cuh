@@ -243,6 +243,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
         auto build = [&](int off, auto bits, const Codebook& cb) {
             constexpr int NB = decltype(bits)::value;
             const float lev = cb.v[lane & 15];
+#pragma unroll 4
             for (int e = warp; e < 256; e += C::THREADS / 32) {
                 auto pair = [&](int lo, int hi) {
                     const __half2 h = __floats2half2_rn(__shfl_sync(0xffffffffu, lev, lo), __shfl_sync(0xffffffffu, lev, hi));
@@ -665,11 +666,12 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
         // ---- the queries: rotated, scaled, fp16, K-major with 128-byte swizzle
         float q_down;
         {
+            const int b = pc.b, hkv = pc.hkv, row0 = pc.row0, rows = pc.rows, ctx = pc.ctx;
             constexpr int OCTETS = C::HT / 8;
             const int t8 = lane & 7, octet = me >> 3;
             auto query = [&](int r) {   // row r's 16-byte pieces: eight coordinates each
-                const int i = fast_div(pc.row0 + r, p.group), h = pc.row0 + r - i * group;
-                return static_cast<const uint4*>(p.q) + (((static_cast<int64_t>(pc.b) * p.T + i) * p.Hq + pc.hkv * group + h) * D) / 8;
+                const int i = fast_div(row0 + r, p.group), h = row0 + r - i * group;
+                return static_cast<const uint4*>(p.q) + (((static_cast<int64_t>(b) * p.T + i) * p.Hq + hkv * group + h) * D) / 8;
             };
             auto widen = [&](const uint4& x, float (&o)[8]) {
                 if (p.q_dtype == kBF16) load8<__nv_bfloat16>(reinterpret_cast<const __nv_bfloat16*>(&x), o);
@@ -683,16 +685,16 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
 #pragma unroll
                 for (int j = 0; j < D / 64; j++) {
                     const int r = octet + k * OCTETS;
-                    raw[k][j] = r < pc.rows ? query(r)[t8 + 8 * j] : make_uint4(0, 0, 0, 0);
+                    raw[k][j] = r < rows ? query(r)[t8 + 8 * j] : make_uint4(0, 0, 0, 0);
                 }
             // the mask words of the rows' nodes (to where weights will be)
-            const bool trees = (pc.tile0 + n_tiles) * kTreeTile > pc.ctx;
-            const int i0 = fast_div(pc.row0, p.group), words = (p.T + 31) / 32;
+            const bool trees = (pc.tile0 + n_tiles) * kTreeTile > ctx;
+            const int i0 = fast_div(row0, p.group), words = (p.T + 31) / 32;
             uint32_t* const mask_words = reinterpret_cast<uint32_t*>(at(a_p));
             static_assert(N * (kTreeMaxNodes / 32) * 4 <= C::P_BUF, "");
             if (trees)
-                for (int k = me; k < (fast_div(pc.row0 + pc.rows - 1, p.group) - i0 + 1) * words; k += C::HT)
-                    mask_words[k] = p.masks[(static_cast<int64_t>(pc.b) * p.T + i0 + k / words) * p.W + k % words];
+                for (int k = me; k < (fast_div(row0 + rows - 1, p.group) - i0 + 1) * words; k += C::HT)
+                    mask_words[k] = p.masks[(static_cast<int64_t>(b) * p.T + i0 + k / words) * p.W + k % words];
             // the largest, for a common scale: |rotated| <= D * largest |q|, and that shall be below 2^15
             float top = 0.f;
 #pragma unroll
@@ -741,14 +743,15 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
             }
             // which rows attend a node: bit r of its words
             if (trees) {
-                for (int k = me; k < (pc.seq - pc.ctx) * C::MW; k += C::HT) {
+                const int nodes = pc.seq - ctx;
+                for (int k = me; k < nodes * C::MW; k += C::HT) {
                     const int node = k / C::MW, w = k % C::MW;
                     uint32_t bits = 0;
                     // (a node's heads are neighbours: a run of bits)
-                    const int r1 = min(pc.rows, 32 * w + 32);
+                    const int r1 = min(rows, 32 * w + 32);
 #pragma unroll 1
                     for (int r = 32 * w; r < r1;) {
-                        const int i = fast_div(pc.row0 + r, p.group), stop = min(r1, (i + 1) * group - pc.row0);
+                        const int i = fast_div(row0 + r, p.group), stop = min(r1, (i + 1) * group - row0);
                         if ((mask_words[(i - i0) * words + (node >> 5)] >> (node & 31)) & 1u)
                             bits |= (0xffffffffu >> (32 - (stop - r))) << (r & 31);
                         r = stop;
@@ -931,6 +934,8 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
         // ---- the piece's rows
         wait(o_done, done + n_tiles - 1);
         done += n_tiles;
+        const int rows = pc.rows;
+        float* const to = pc.out;
         if (soft) {
             // sums over the lanes, then over the warps: lane c gets row c's
             float sum[CW];
@@ -953,8 +958,8 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
         }
         meet(false);
         if (soft) {
-            if (quarter == 0 && lane < CW && col0 + lane < pc.rows) {
-                float* dst = pc.out + (col0 + lane) * ROW + D;
+            if (quarter == 0 && lane < CW && col0 + lane < rows) {
+                float* dst = to + (col0 + lane) * ROW + D;
                 const float* r = red + col0 + lane;
                 dst[0] = -s_nm[col0 + lane];
                 dst[1] = r[0] + r[N] + r[2 * N] + r[3 * N];
@@ -970,7 +975,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 if (D == 64 && m >= 64) continue;
 #pragma unroll
                 for (int c = 0; c < CW; c++)
-                    if (col0 + c < pc.rows) pc.out[(col0 + c) * ROW + coord] = __uint_as_float(o[c]) * scale;
+                    if (col0 + c < rows) to[(col0 + c) * ROW + coord] = __uint_as_float(o[c]) * scale;
             }
         }
         tc_fence_before();
