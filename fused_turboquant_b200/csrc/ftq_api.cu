@@ -1758,7 +1758,7 @@ extern "C" int ftq_tree_attn(const void* q, int q_dtype, void* out, int out_dtyp
     const size_t head = ftq_decode_workspace_bytes(1, Hq, Hkv, head_dim, max_seq_len, 1);
     const TreeLayout l = tree_layout(B, n_nodes, Hq, Hkv, head_dim, head);
     const int seqs = std::min(B, ftq::kTreeMaxSeqs), group = Hq / Hkv;
-    const int64_t places = (static_cast<int64_t>(max_seq_len) / ftq::kTreeTile + 1 + ftq::kTreePiece) * Hkv * l.row_tiles;
+    const int64_t places = (static_cast<int64_t>(max_seq_len) / ftq::kTreeTile + 1 + ftq::tree_piece(head_dim)) * Hkv * l.row_tiles;
     if (places * seqs > INT32_MAX / 2) return fail(FTQ_ERR_UNSUPPORTED, "too many tokens, heads and nodes for one call");
     ftq::TreeAttnParams p{};
     rc = pack_levels(levels_k_host, bits_k, &p.lk);
@@ -1806,6 +1806,7 @@ extern "C" int ftq_tree_attn(const void* q, int q_dtype, void* out, int out_dtyp
         m.tree_lens = p.tree_lens; m.seq_lens = p.seq_lens;
         m.out = static_cast<uint8_t*>(out) + vec * dtype_size(out_dtype);
         m.B = p.B; m.T = n_nodes; m.Hq = Hq; m.Hkv = Hkv; m.N = l.n; m.row_tiles = l.row_tiles; m.max_seq = max_seq_len;
+        m.piece = ftq::tree_piece(head_dim);
         m.group = p.group; m.rsqrt_d = rsqrt_dim(head_dim); m.signs = p.signs; m.status = status; m.more = b0 > 0;
         e = ftq::launch_tree_merge(head_dim, out_dtype, m, st);
         if (e != cudaSuccess) return cuda_fail(e, "ftq_tree_attn merge launch");

@@ -22,7 +22,7 @@
 // two, so that the largest so far is 1 to 2, and again when one of 4 or more comes; p * |v| is then at most 2^15, and a weight of
 // 2^-14 of the largest still has all its bits.  Queries are scaled the same way.  Scores, sums and O are fp32.
 //
-// Work: units (sequence, KV head, row tile) in a line of places, a place per tile of 128 tokens and kTreePiece more per
+// Work: units (sequence, KV head, row tile) in a line of places, a place per tile of 128 tokens and tree_piece more per
 // unit, cut into equal shares, one per half of a CTA (one CTA per SM).  A half's eight warps do all that a tile takes, one thing
 // after the other -- codes to registers, keys to TMEM, values to shared memory, softmax -- and while one half waits for
 // a product or a barrier the other one has the SM.  From 64 rows on, and for heads of 256, one half of sixteen warps has
@@ -39,7 +39,9 @@
 namespace ftq {
 
 constexpr int kTreeTile = 128;         // tokens of a tile
-constexpr int kTreePiece = 3;          // places that a unit costs besides its tiles
+// Places that a unit costs besides its tiles: its queries, its first maxima and its rows take as long as so many tiles.  (24 ragged
+// sequences with heads of 256: 2, 3, 4, 6 places 124, 111, 99, 102 us; 40 with heads of 64: 42, 41, 43, 46 us.)
+__host__ __device__ constexpr int tree_piece(int head_dim) { return head_dim == 256 ? 4 : 3; }
 constexpr int kTreeMaxSeqs = 1024;     // sequences of a launch
 constexpr float kTreeSlack = 13.f, kTreeGrowth = 4.f;
 
@@ -64,12 +66,12 @@ struct TreeAttnParams {
     SignBits signs;
 };
 
-// The part of a unit that a CTA has: places [off, off_end) of its tiles + kTreePiece.
-__host__ __device__ __forceinline__ int tree_tile_of(int off) { return off > kTreePiece ? off - kTreePiece : 0; }
+// The part of a unit that a half has: places [off, off_end) of its tiles + tree_piece.
+__host__ __device__ __forceinline__ int tree_tile_of(int off, int piece) { return off > piece ? off - piece : 0; }
 
 template <int D, int BK, int BV, int N>
 struct TreeCfg {
-    static constexpr int HALVES = D == 256 || N == 128 ? 1 : 2, WARPS = 16, THREADS = 512 + 64 * HALVES;
+    static constexpr int HALVES = D == 256 || N == 128 ? 1 : 2, WARPS = 16, THREADS = 512 + 64 * HALVES, PIECE = tree_piece(D);
     static constexpr int WH = WARPS / HALVES, HT = 32 * WH;        // warps and threads of a half, without its two helpers
     // softmax: column groups of four warps (a warp reaches the 32 tokens of its quarter), rows of a group
     static constexpr int CG = WH / 4 < N / 8 ? WH / 4 : N / 8, CW = N / CG;
@@ -287,7 +289,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
         for (int b0 = 0; b0 < p.B; b0 += C::THREADS) {
             const int b = b0 + tid;
             const int len = b < p.B ? max(0, min(p.seq_lens[b], p.max_seq)) : 0;
-            const int v = b < p.B ? U * ((len + kTreeTile - 1) / kTreeTile + kTreePiece) : 0;
+            const int v = b < p.B ? U * ((len + kTreeTile - 1) / kTreeTile + C::PIECE) : 0;
             int x = v;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -359,7 +361,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 if (first[mid] <= pos) lo = mid; else hi = mid;
             }
             const int len = (first[lo + 1] - first[lo]) / U, rel = pos - first[lo], u = rel / len, off = rel - u * len;
-            const int off_end = min(len, off + end - pos), t0 = tree_tile_of(off), t1 = tree_tile_of(off_end);
+            const int off_end = min(len, off + end - pos), t0 = tree_tile_of(off, C::PIECE), t1 = tree_tile_of(off_end, C::PIECE);
             pos += off_end - off;
             if (t1 <= t0) continue;
             pc.b = lo;
@@ -898,7 +900,13 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 meet(false);
                 if (soft) {
 #pragma unroll
-                    for (int c = 0; c < CW; c++) l[c] *= s_lc[col0 + c];
+                    for (int c = 0; c < CW; c += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(s_lc + col0 + c);
+                        l[c] *= f.x;
+                        l[c + 1] *= f.y;
+                        l[c + 2] *= f.z;
+                        l[c + 3] *= f.w;
+                    }
                     if (it > 0) {       // (P.V of the tile before is complete)
 #pragma unroll
                         for (int mb = 0; mb < C::MB; mb++) {
@@ -906,9 +914,11 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                             for (int c = 0; c < CW; c += 8) {       // (few registers: what this path spills the others pay for)
                                 uint32_t o[8];
                                 const uint32_t o_at = tl + C::COL_O + mb * N + col0 + c;
+                                const float4 f = *reinterpret_cast<const float4*>(s_corr + col0 + c), g = *reinterpret_cast<const float4*>(s_corr + col0 + c + 4);
+                                const float by[8] = {f.x, f.y, f.z, f.w, g.x, g.y, g.z, g.w};
                                 tc_load(o_at, o);
 #pragma unroll
-                                for (int k = 0; k < 8; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * s_corr[col0 + c + k]);
+                                for (int k = 0; k < 8; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * by[k]);
                                 tc_st8(o_at, o);
                             }
                         }
@@ -1004,7 +1014,7 @@ struct TreeMergeParams {
     const float *whole, *cut;
     const int32_t *tree_lens, *seq_lens;
     void* out;
-    int B, T, Hq, Hkv, N, row_tiles, max_seq;
+    int B, T, Hq, Hkv, N, row_tiles, max_seq, piece;
     FastDiv group;
     float rsqrt_d;
     SignBits signs;
@@ -1034,7 +1044,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
     auto row_of = [&](int k) -> const float* {   // part k's row, NULL: it has no tiles
         const int c = c0 + k;
         const int from = max(pos, c * share), to = static_cast<int>(min(static_cast<int64_t>(pos) + len, static_cast<int64_t>(c + 1) * share));
-        if (tree_tile_of(to - pos) <= tree_tile_of(from - pos)) return nullptr;
+        if (tree_tile_of(to - pos, p.piece) <= tree_tile_of(from - pos, p.piece)) return nullptr;
         return c0 == c1 ? p.whole + ((static_cast<int64_t>(b) * U + u) * p.N + n) * ROW
                         : p.cut + ((2 * static_cast<int64_t>(c) + (k == 0 ? 1 : 0)) * p.N + n) * ROW;
     };
