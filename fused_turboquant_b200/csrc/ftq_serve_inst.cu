@@ -33,6 +33,8 @@ cudaError_t run_pages(const PagesParams& p, int64_t writes, int smem, cudaStream
 
 template <typename T>
 cudaError_t run_logits(const LogitParams& p, bool vec, dim3 grid, int smem, cudaStream_t stream) {
+    const cudaError_t e = vec ? allow_smem<logits_kernel<T, true>>(kLogitSegment * 13) : allow_smem<logits_kernel<T, false>>(kLogitSegment * 13);
+    if (e != cudaSuccess) return e;
     return vec ? launch_dependent(logits_kernel<T, true>, grid, kLogitThreads, smem, stream, p)
                : launch_dependent(logits_kernel<T, false>, grid, kLogitThreads, smem, stream, p);
 }
@@ -61,13 +63,14 @@ cudaError_t launch_logits(int dtype, LogitParams p, int32_t* best, cudaStream_t 
     auto aligned16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
     // eight tokens a load where every row begins on 16 bytes and ends with a whole load; else a token a load, coalesced
     const bool vec = p.V % 8 == 0 && aligned16(p.logits) && p.row_stride * es % 16 == 0 && (!p.out || aligned16(p.out));
-    // rows of a request that share a count: as few as fill the device (eight CTAs an SM) once
-    const int64_t ctas = static_cast<int64_t>(p.segments) * p.R, want = 8 * sm_count();
+    // rows of a request that share a count: as few as fill the device (five CTAs an SM) once, and no more than a CTA has room for
+    const int64_t ctas = static_cast<int64_t>(p.segments) * p.R, want = 5 * sm_count();
     int chunks = static_cast<int>(ctas >= want ? 1 : std::min<int64_t>(p.T, (want + ctas - 1) / ctas));
+    chunks = std::max(chunks, (p.T + kTreeMaxNodes - 1) / kTreeMaxNodes);
     p.rows_per_cta = (p.T + chunks - 1) / chunks;
     chunks = (p.T + p.rows_per_cta - 1) / p.rows_per_cta;
     const dim3 grid(p.segments, p.R, chunks);
-    const int smem = kLogitSegment * 4 * (p.K > 0 ? 2 : 1);
+    const int smem = kLogitSegment * (p.K > 0 ? 13 : 9);
     cudaError_t e = dtype == kF32 ? run_logits<float>(p, vec, grid, smem, stream)
                     : dtype == kF16 ? run_logits<__half>(p, vec, grid, smem, stream)
                                     : run_logits<__nv_bfloat16>(p, vec, grid, smem, stream);

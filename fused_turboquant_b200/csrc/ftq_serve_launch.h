@@ -8,7 +8,7 @@ namespace ftq {
 
 constexpr int kTreeMaxNodes = 256;      // nodes of a tree
 constexpr int kPagesMaxRequests = 8192; // requests of a page table
-constexpr int kLogitSegment = 4096;     // tokens of the vocabulary a CTA takes
+constexpr int kLogitSegment = 2048;     // tokens of the vocabulary a CTA takes
 
 struct PagesParams {
     int32_t* table;         // [R, max_blocks]
