@@ -1577,7 +1577,7 @@ bool overlap(const void* a, size_t na, const void* b, size_t nb) {
 
 int check_pages(const ftq::PagesParams& p, const char* what) {
     if (p.R < 0 || p.R > ftq::kPagesMaxRequests)
-        return fail(FTQ_ERR_UNSUPPORTED, "%s: %d requests (0 to %d)", what, p.R, ftq::kPagesMaxRequests);
+        return fail(p.R < 0 ? FTQ_ERR_INVALID : FTQ_ERR_UNSUPPORTED, "%s: %d requests (0 to %d)", what, p.R, ftq::kPagesMaxRequests);
     if (p.max_blocks <= 0 || p.max_blocks > (1 << 26) || p.num_blocks < 0)
         return fail(FTQ_ERR_INVALID, "%s: bad shape max_blocks=%d num_blocks=%d", what, p.max_blocks, p.num_blocks);
     if (p.R > 0 && (!p.table || !p.lens || !p.n_free || !p.arg || (p.num_blocks > 0 && !p.free_blocks)))

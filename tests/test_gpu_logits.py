@@ -162,6 +162,20 @@ def test_values_that_are_not_finite():
     assert call(x, dict())[1].tolist() == [0]
 
 
+@pytest.mark.parametrize("v", [9000, 9001])
+def test_more_rows_of_a_request_than_a_tree_has_nodes(v):
+    """600 rows without a tree: CTAs have at most 256 of them, and a warp keeps the best of 32 at a time."""
+    import torch
+    rng = np.random.default_rng(v)
+    r, t = 2, 600
+    a = make(rng, r, t, v, h=300, k=5)
+    x = (8 * rng.standard_normal((r, t, v))).astype(np.float32)
+    got, best = call(torch.from_numpy(x).cuda(), a)
+    want, _ = plain(x, np.float32, **a)
+    np.testing.assert_array_equal(got.cpu().numpy(), want)
+    np.testing.assert_array_equal(best.view(r, t).cpu().numpy(), lowest_best(want))
+
+
 def test_many_repetitions_and_long_histories():
     import torch
     hist = np.full((1, 200000), 4, np.int32)
