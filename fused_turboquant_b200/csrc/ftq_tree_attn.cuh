@@ -20,14 +20,26 @@
 // and the sums and write the tile's weights again.  (With a slack of 3, as in the decode kernels, half of the tiles
 // did: of 32 rows there is always one that has found a larger score.)  Weights are fp16: |v| is scaled by a power of
 // two, so that the largest so far is 1 to 2, and again when one of 4 or more comes; p * |v| is then at most 2^15, and a weight of
-// 2^-14 of the largest still has all its bits.  Queries are scaled the same way.  Scores, sums and O are fp32.
+// 2^-14 of the largest still has all its bits.  Queries are scaled the same way.  Scores, sums and O are fp32.  Three operands are rounded to fp16, as in
+// the decode kernels, for the tensor cores' sake: rotated queries, centroids and weights; against 64 bits an output is off by 4e-4 of its
+// size, by 2e-4 if only the output were rounded to fp16, and by 1.7e-3 either way if to bf16.
 //
 // Work: units (sequence, KV head, row tile) in a line of places, a place per tile of 128 tokens and tree_piece more per
-// unit, cut into equal shares, one per half of a CTA (one CTA per SM).  A half's eight warps do all that a tile takes, one thing
-// after the other -- codes to registers, keys to TMEM, values to shared memory, softmax -- and while one half waits for
-// a product or a barrier the other one has the SM.  From 64 rows on, and for heads of 256, one half of sixteen warps has
-// the CTA to itself: its rows share what was dequantised.  Every piece leaves its rows (O, m, l) in the workspace;
-// tree_merge_kernel joins the pieces of a unit, rotates back and stores.
+// unit, cut into equal shares, one per half of a CTA (one CTA per SM).  A half's eight warps do all that a tile takes of a
+// thread, one thing after the other: keys to TMEM, softmax, values to shared memory, a barrier.  While one half waits for
+// something the other has the SM.  Two helper warps a half do what would hold the others up: one issues the products (about
+// 700 cycles a tile), one fetches codes and norms by bulk copies (400 cycles to issue one) as their places become free.
+// Beyond 64 rows (products of 128), and for heads of 256, one half of sixteen warps has the
+// CTA to itself: its rows share what was dequantised, and eight warps have the keys, eight the values.  Every piece leaves its rows
+// (O, m, l) in the workspace; tree_merge_kernel joins the pieces of a unit, rotates back and stores.
+//
+// Bound: instruction issue and the latency of the chain of a tile, about 6000 cycles for a half, of which the look-ups (a
+// 16-bit pair of codes a 4-byte load), the softmax and the waits for shared memory in between are most; the tensor cores are
+// busy 15 to 35 % of the time, HBM 3 to 25 %.  Measured (K4V4, bf16): one sequence of 900 tokens, 8 nodes, 32 heads of 128 over
+// 8: 17.2 us; 32 of 8192, 16 nodes: 180 us (floor by HBM 44), where dequantising and a CTA of 128 rows of one sequence after
+// the other took 413, one CTA of specialised warps 261 to 350 (handing tiles over cost more than the work), two halves
+// that fetched and issued for themselves 205; 2 of 131072, 64 nodes, 64 heads: 894 us (615 TFLOP/s, 38 % of the measured
+// bf16 rate); 24 ragged of up to 16384, heads of 256: 99 us; 40 ragged of up to 4096, 25 nodes, 14 heads of 64 over 2: 41 us.
 //
 // Every wait is bounded.  After one has run out nothing waits any more, the half's rows become NaN and the status word says
 // so.  Block ids outside the pool are not followed: the rows that attend a token of such a page are NaN.
