@@ -358,7 +358,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
         if (lane == 0) mbar_arrive(bar);
     };
     // barriers of a half: its workers'; theirs and the issuer's (true if any thread says so); theirs and the feeder's
-    auto meet = [&](bool) { group_any<C::HT>(3 + half, false); };
+    auto meet = [&]() { group_any<C::HT>(3 + half, false); };
     auto meet_issuer = [&](bool mine) { return group_any<C::HT + 32>(1 + half, mine); };
     auto meet_feeder = [&]() { group_any<C::HT + 32>(5 + half, false); };
     // the first piece with tiles from a place on; moves on to the place behind it
@@ -724,7 +724,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
             top = warp_max(top);
             if (lane == 0) red[hw] = top;
             if (me < N) s_nm[me] = INFINITY;
-            meet(false);
+            meet();
 #pragma unroll
             for (int w = 0; w < C::WH; w++) top = fmaxf(top, red[w]);
             const float all = top * (fabsf(p.q_scale) * D);
@@ -886,7 +886,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                     if (lane < CW) red[quarter * N + col0 + lane] = mine;
                     if (lane == 0) red_v[hw] = wv;
                 }
-                meet(false);
+                meet();
                 float v_ratio = 1.f;
                 if (soft) {
                     float v_top = 0.f;
@@ -909,7 +909,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                         }
                     }
                 }
-                meet(false);
+                meet();
                 if (soft) {
 #pragma unroll
                     for (int c = 0; c < CW; c += 4) {
@@ -978,7 +978,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
             }
             if (lane < CW) red[quarter * N + col0 + lane] = sum[0];
         }
-        meet(false);
+        meet();
         if (soft) {
             if (quarter == 0 && lane < CW && col0 + lane < rows) {
                 float* dst = to + (col0 + lane) * ROW + D;
@@ -1001,7 +1001,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
             }
         }
         tc_fence_before();
-        meet(false);      // (the next piece writes to what these reads came from)
+        meet();      // (the next piece writes to what these reads came from)
         tc_fence_after();
     }
     __syncwarp();
