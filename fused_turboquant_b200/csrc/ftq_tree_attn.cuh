@@ -27,7 +27,7 @@
 // Work: units (sequence, KV head, row tile) in a line of places, a place per tile of 128 tokens and tree_piece more per
 // unit, cut into equal shares, one per half of a CTA (one CTA per SM).  A half's eight warps do all that a tile takes of a
 // thread, one thing after the other: keys to TMEM, softmax, values to shared memory, a barrier.  While one half waits for
-// something the other has the SM.  Two helper warps a half do what would hold the others up: one issues the products (about
+// something the other has the SM.  Two helper warps a half (of the last four warps) do what would hold the others up: one issues the products (about
 // 700 cycles a tile), one fetches codes and norms by bulk copies (400 cycles to issue one) as their places become free.
 // Beyond 64 rows (products of 128), and for heads of 256, one half of sixteen warps has the
 // CTA to itself: its rows share what was dequantised, and eight warps have the keys, eight the values.  Every piece leaves its rows
@@ -36,9 +36,9 @@
 // Bound: instruction issue and the latency of the chain of a tile, about 6000 cycles for a half, of which the look-ups (a
 // 16-bit pair of codes a 4-byte load), the softmax and the waits for shared memory in between are most; the tensor cores are
 // busy 15 to 35 % of the time, HBM 3 to 25 %.  Measured (K4V4, bf16): one sequence of 900 tokens, 8 nodes, 32 heads of 128 over
-// 8: 17.2 us; 32 of 8192, 16 nodes: 180 us (floor by HBM 44), where dequantising and a CTA of 128 rows of one sequence after
+// 8: 17.2 us; 32 of 8192, 16 nodes: 173 us (floor by HBM 44), where dequantising and a CTA of 128 rows of one sequence after
 // the other took 413, one CTA of specialised warps 261 to 350 (handing tiles over cost more than the work), two halves
-// that fetched and issued for themselves 205; 2 of 131072, 64 nodes, 64 heads: 894 us (615 TFLOP/s, 38 % of the measured
+// that fetched and issued for themselves 205; 2 of 131072, 64 nodes, 64 heads: 889 us (619 TFLOP/s, 38 % of the measured
 // bf16 rate); 24 ragged of up to 16384, heads of 256: 99 us; 40 ragged of up to 4096, 25 nodes, 14 heads of 64 over 2: 41 us.
 //
 // Every wait is bounded.  After one has run out nothing waits any more, the half's rows become NaN and the status word says
@@ -83,7 +83,7 @@ __host__ __device__ __forceinline__ int tree_tile_of(int off, int piece) { retur
 
 template <int D, int BK, int BV, int N>
 struct TreeCfg {
-    static constexpr int HALVES = D == 256 || N == 128 ? 1 : 2, WARPS = 16, THREADS = 512 + 64 * HALVES, PIECE = tree_piece(D);
+    static constexpr int HALVES = D == 256 || N == 128 ? 1 : 2, WARPS = 16, THREADS = 640, PIECE = tree_piece(D);
     static constexpr int WH = WARPS / HALVES, HT = 32 * WH;        // warps and threads of a half, without its two helpers
     // softmax: column groups of four warps (a warp reaches the 32 tokens of its quarter), rows of a group
     static constexpr int CG = WH / 4 < N / 8 ? WH / 4 : N / 8, CW = N / CG;
@@ -413,596 +413,605 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
     static_assert(sizeof(TreePiece) <= 56, "");
     volatile TreePiece& pc = *reinterpret_cast<volatile TreePiece*>(at(C::A_PIECE + 64 * half));
     volatile int& pos = *reinterpret_cast<volatile int*>(at(C::A_PIECE + 64 * half + 56));
-    if (helper && (warp & 1) == 0) {
-        // ---- the products of a half: one lane of its first helper
-        constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(N / 8) << 17) | (8u << 24);
-        constexpr uint32_t kIdescO = kIdescS | (1u << 15) | (1u << 16);
-        constexpr uint32_t kHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-        auto scores = [&](int tile) {
-            if (elect_one()) {
-                const uint32_t q = (a_q >> 4) | ((16u >> 4) << 16);
+    // Registers: the workers get some of what the last four warps do not need, 512 x 104 + 128 x 64 of the 640 x 96 of the launch.
+    // (Products of 64 rows spilled in every tile: 180 -> 173 us for 32 sequences of 8192 tokens and 16 nodes.)
+    static_assert(C::THREADS == 640 && 512 * 104 + 128 * 64 <= 640 * 96, "");
+    __syncwarp();
+    if (helper) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n");
+        if (half < C::HALVES && (warp & 1) == 0) {
+            // ---- the products of a half: one lane of its first helper
+            constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(N / 8) << 17) | (8u << 24);
+            constexpr uint32_t kIdescO = kIdescS | (1u << 15) | (1u << 16);
+            constexpr uint32_t kHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+            auto scores = [&](int tile) {
+                if (elect_one()) {
+                    const uint32_t q = (a_q >> 4) | ((16u >> 4) << 16);
 #pragma unroll
-                for (int kb = 0; kb < D / 16; kb++)
-                    one_mma_ts(tmem + C::COL_S, tmem + (tile & 1) * (D / 2) + 8 * kb, q + ((kb >> 2) * (N * 128) + (kb & 3) * 32) / 16, kHi, kIdescS, kb > 0);
+                    for (int kb = 0; kb < D / 16; kb++)
+                        one_mma_ts(tmem + C::COL_S, tmem + (tile & 1) * (D / 2) + 8 * kb, q + ((kb >> 2) * (N * 128) + (kb & 3) * 32) / 16, kHi, kIdescS, kb > 0);
 #ifdef FTQ_TEST_WAIT_EXPIRY
-                if (!(tile == 1 && worker == 0))
+                    if (!(tile == 1 && worker == 0))
 #endif
-                tc_commit(s_done);
-            }
-            __syncwarp();
-        };
-        auto sums = [&](int tile) {
-            if (elect_one()) {
-                const uint32_t v = ((a_v + (tile % C::VB) * C::V_BUF) >> 4) | ((static_cast<uint32_t>(C::V_ATOM) >> 4) << 16);
-                const uint32_t w = (a_p >> 4) | ((static_cast<uint32_t>(C::P_ATOM) >> 4) << 16);
+                    tc_commit(s_done);
+                }
+                __syncwarp();
+            };
+            auto sums = [&](int tile) {
+                if (elect_one()) {
+                    const uint32_t v = ((a_v + (tile % C::VB) * C::V_BUF) >> 4) | ((static_cast<uint32_t>(C::V_ATOM) >> 4) << 16);
+                    const uint32_t w = (a_p >> 4) | ((static_cast<uint32_t>(C::P_ATOM) >> 4) << 16);
 #pragma unroll
-                for (int mb = 0; mb < C::MB; mb++)
+                    for (int mb = 0; mb < C::MB; mb++)
 #pragma unroll
-                    for (int ks = 0; ks < kTreeTile / 16; ks++)
-                        one_mma_ss(tmem + C::COL_O + mb * N, v + mb * (2 * C::V_ATOM >> 4) + ks * (2048 >> 4), w + ks * (2048 >> 4), kHi, kIdescO,
-                                   ks > 0 ? 1u : static_cast<uint32_t>(tile));
-                tc_commit(o_done);
-            }
-            __syncwarp();
-        };
+                        for (int ks = 0; ks < kTreeTile / 16; ks++)
+                            one_mma_ss(tmem + C::COL_O + mb * N, v + mb * (2 * C::V_ATOM >> 4) + ks * (2048 >> 4), w + ks * (2048 >> 4), kHi, kIdescO,
+                                       ks > 0 ? 1u : static_cast<uint32_t>(tile));
+                    tc_commit(o_done);
+                }
+                __syncwarp();
+            };
 #pragma unroll 1
-        while (true) {
-            meet_issuer(false);
-            tc_fence_after();
-            const int n_tiles = pc.n_tiles;
-            if (n_tiles == 0) break;
-            scores(0);
-#pragma unroll 1
-            for (int it = 0; it < n_tiles; it++) {
-                if (meet_issuer(false)) meet_issuer(false);     // (new maxima: the tile's weights come again)
+            while (true) {
+                meet_issuer(false);
                 tc_fence_after();
-                if (it + 1 < n_tiles) scores(it + 1);
-                sums(it);
+                const int n_tiles = pc.n_tiles;
+                if (n_tiles == 0) break;
+                scores(0);
+#pragma unroll 1
+                for (int it = 0; it < n_tiles; it++) {
+                    if (meet_issuer(false)) meet_issuer(false);     // (new maxima: the tile's weights come again)
+                    tc_fence_after();
+                    if (it + 1 < n_tiles) scores(it + 1);
+                    sums(it);
+                }
             }
+            // nothing may be in flight when TMEM is given back
+            if (elect_one()) tc_commit(drained);
+            __syncwarp();
+#pragma unroll 1
+            for (int i = 0; i < kDrainSpinLimit && !mbar_try_wait(drained, 0); i++) {}
         }
-        // nothing may be in flight when TMEM is given back
-        if (elect_one()) tc_commit(drained);
-        __syncwarp();
+        // ---- the pages of a half: its second helper.  Codes and norms come by bulk copies, a page of codes a warp, as soon as what lay
+        // in their place was looked at.  (Registers would be the wrong place for them: loads that share one of the few scoreboards
+        // complete together, so that a look at anything waits for the newest; and a copy takes its issuer 400 cycles.)
+        if (half < C::HALVES && (warp & 1) == 1) {
+            int k_sent = 0, v_sent = 0, n_sent = 0;
 #pragma unroll 1
-        for (int i = 0; i < kDrainSpinLimit && !mbar_try_wait(drained, 0); i++) {}
-    }
-    // ---- the pages of a half: its second helper.  Codes and norms come by bulk copies, a page of codes a warp, as soon as what lay
-    // in their place was looked at.  (Registers would be the wrong place for them: loads that share one of the few scoreboards
-    // complete together, so that a look at anything waits for the newest; and a copy takes its issuer 400 cycles.)
-    if (helper && (warp & 1) == 1) {
-        int k_sent = 0, v_sent = 0, n_sent = 0;
-#pragma unroll 1
-        while (true) {
-            meet_feeder();
-            const int n_tiles = pc.n_tiles;
-            if (n_tiles == 0) break;
-            const int tile0 = pc.tile0, seq = pc.seq;
-            const int32_t* const btab = p.block_table + static_cast<int64_t>(pc.b) * p.max_blocks;
-            const uint8_t* const pool = p.pool + static_cast<int64_t>(pc.hkv) * C::PAGE_BYTES;
-            // block ids of four tiles' pages (idb: of the next four); -2: no tokens
-            auto load_ids = [&](int tile) {
-                const int t = tile + (lane >> 3), pg = (tile0 + t) * (kTreeTile / kPageTokens) + (lane & 7);
-                return load_id_if(t < n_tiles && pg * kPageTokens < seq, btab + pg, -2);
-            };
-            int ida = load_ids(0), idb = load_ids(4);
-            // of lane's page of a tile, while `now` is the tile that ida begins with or one of the three behind it
-            auto id_of = [&](int tile, int now) { return __shfl_sync(0xffffffffu, (tile ^ now) < 4 ? ida : idb, (tile & 3) * 8 + (lane & 7)); };
-            auto in_pool = [&](int id) { return static_cast<uint64_t>(static_cast<int64_t>(id)) < static_cast<uint64_t>(p.num_blocks); };
-            auto page_of = [&](int id) { return pool + static_cast<int64_t>(id) * p.Hkv * C::PAGE_BYTES; };
-            // page g of a tile is warp 4 (g & 1) + g / 2's; values: of the warps behind, if there are any
-            const int owner = half * C::WH + 4 * (lane & 1) + ((lane & 7) >> 1);
-            const uint32_t k_stage = stage_of(owner), v_stage = C::LATE_V ? a_v + 2048 * (lane & 7) : stage_of(owner + 8);
-            // (what lies in the place of a page that is not there is as good: its weights are zero, or no numbers)
-            auto fetch = [&](uint32_t bar, uint32_t dst, int id, int off, uint32_t bytes, int& sent) {
-                if (stalled) return;
-                sent++;
-                if (lane < 8) {
-                    if (in_pool(id)) {
-                        mbar_expect_tx(bar, bytes);
-                        bulk_g2s(dst, page_of(id) + off, bytes, bar);
-                    } else {
-                        mbar_arrive(bar);
-                    }
-                }
-                __syncwarp();
-            };
-            constexpr uint32_t kKeys = kPageTokens * C::PDK, kValues = kPageTokens * C::PDV;
-            auto fetch_k = [&](int tile, int now) { fetch(k_full, k_stage, id_of(tile, now), 0, kKeys, k_sent); };
-            auto fetch_v = [&](int tile, int now) { fetch(v_full, v_stage, id_of(tile, now), C::OFF_VC, kValues, v_sent); };
-            // norms of a tile; a key of a page that is not in the pool has one that is no number
-            auto fetch_norms = [&](int tile, int now) {
-                const int id = id_of(tile, now);
-                if (stalled) return;
-                n_sent++;
-                if (lane < 16) {
-                    const bool value = lane & 8;
-                    const uint32_t to = a_norm + 32 * lane;
-                    if (in_pool(id)) {
-                        mbar_expect_tx(n_full, 32);
-                        bulk_g2s(to, page_of(id) + (value ? C::OFF_VN : C::OFF_KN), 32, n_full);
-                    } else {
-                        if (id != -2) {
-                            if (!value) {
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(to), "r"(0x7e007e00u) : "memory");
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(to + 16), "r"(0x7e007e00u) : "memory");
-                            }
-                            __stcg(p.errors + 1, p.epoch);
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                        mbar_arrive(n_full);
-                    }
-                }
-                __syncwarp();
-            };
-            if (C::LATE_V) {
-                // The first two tiles' keys at once and in one phase; the second's to where the warp's first values will be.  (Values
-                // wait in the place that they are written to as fp16: a page's 2 KB there have room for two pages' codes.)
-                const int id0 = id_of(0, 0), id1 = id_of(1, 0);
-                if (!stalled) {
-                    k_sent++;
+            while (true) {
+                meet_feeder();
+                const int n_tiles = pc.n_tiles;
+                if (n_tiles == 0) break;
+                const int tile0 = pc.tile0, seq = pc.seq;
+                const int32_t* const btab = p.block_table + static_cast<int64_t>(pc.b) * p.max_blocks;
+                const uint8_t* const pool = p.pool + static_cast<int64_t>(pc.hkv) * C::PAGE_BYTES;
+                // block ids of four tiles' pages (idb: of the next four); -2: no tokens
+                auto load_ids = [&](int tile) {
+                    const int t = tile + (lane >> 3), pg = (tile0 + t) * (kTreeTile / kPageTokens) + (lane & 7);
+                    return load_id_if(t < n_tiles && pg * kPageTokens < seq, btab + pg, -2);
+                };
+                int ida = load_ids(0), idb = load_ids(4);
+                // of lane's page of a tile, while `now` is the tile that ida begins with or one of the three behind it
+                auto id_of = [&](int tile, int now) { return __shfl_sync(0xffffffffu, (tile ^ now) < 4 ? ida : idb, (tile & 3) * 8 + (lane & 7)); };
+                auto in_pool = [&](int id) { return static_cast<uint64_t>(static_cast<int64_t>(id)) < static_cast<uint64_t>(p.num_blocks); };
+                auto page_of = [&](int id) { return pool + static_cast<int64_t>(id) * p.Hkv * C::PAGE_BYTES; };
+                // page g of a tile is warp 4 (g & 1) + g / 2's; values: of the warps behind, if there are any
+                const int owner = half * C::WH + 4 * (lane & 1) + ((lane & 7) >> 1);
+                const uint32_t k_stage = stage_of(owner), v_stage = C::LATE_V ? a_v + 2048 * (lane & 7) : stage_of(owner + 8);
+                // (what lies in the place of a page that is not there is as good: its weights are zero, or no numbers)
+                auto fetch = [&](uint32_t bar, uint32_t dst, int id, int off, uint32_t bytes, int& sent) {
+                    if (stalled) return;
+                    sent++;
                     if (lane < 8) {
-                        const bool has0 = in_pool(id0), has1 = n_tiles > 1 && in_pool(id1);
-                        mbar_expect_tx(k_full, (has0 ? kKeys : 0) + (has1 ? kKeys : 0));
-                        if (has0) bulk_g2s(k_stage, page_of(id0), kKeys, k_full);
-                        if (has1) bulk_g2s(v_stage + 1024, page_of(id1), kKeys, k_full);
+                        if (in_pool(id)) {
+                            mbar_expect_tx(bar, bytes);
+                            bulk_g2s(dst, page_of(id) + off, bytes, bar);
+                        } else {
+                            mbar_arrive(bar);
+                        }
                     }
                     __syncwarp();
-                }
-                fetch_norms(0, 0);
-                fetch_v(0, 0);
-                if (n_tiles > 1) {
-                    copied(k_free, done);
+                };
+                constexpr uint32_t kKeys = kPageTokens * C::PDK, kValues = kPageTokens * C::PDV;
+                auto fetch_k = [&](int tile, int now) { fetch(k_full, k_stage, id_of(tile, now), 0, kKeys, k_sent); };
+                auto fetch_v = [&](int tile, int now) { fetch(v_full, v_stage, id_of(tile, now), C::OFF_VC, kValues, v_sent); };
+                // norms of a tile; a key of a page that is not in the pool has one that is no number
+                auto fetch_norms = [&](int tile, int now) {
+                    const int id = id_of(tile, now);
+                    if (stalled) return;
+                    n_sent++;
+                    if (lane < 16) {
+                        const bool value = lane & 8;
+                        const uint32_t to = a_norm + 32 * lane;
+                        if (in_pool(id)) {
+                            mbar_expect_tx(n_full, 32);
+                            bulk_g2s(to, page_of(id) + (value ? C::OFF_VN : C::OFF_KN), 32, n_full);
+                        } else {
+                            if (id != -2) {
+                                if (!value) {
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(to), "r"(0x7e007e00u) : "memory");
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(to + 16), "r"(0x7e007e00u) : "memory");
+                                }
+                                __stcg(p.errors + 1, p.epoch);
+                            }
+                            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                            mbar_arrive(n_full);
+                        }
+                    }
+                    __syncwarp();
+                };
+                if (C::LATE_V) {
+                    // The first two tiles' keys at once and in one phase; the second's to where the warp's first values will be.  (Values
+                    // wait in the place that they are written to as fp16: a page's 2 KB there have room for two pages' codes.)
+                    const int id0 = id_of(0, 0), id1 = id_of(1, 0);
                     if (!stalled) {
                         k_sent++;
-                        if (lane < 8) mbar_arrive(k_full);
+                        if (lane < 8) {
+                            const bool has0 = in_pool(id0), has1 = n_tiles > 1 && in_pool(id1);
+                            mbar_expect_tx(k_full, (has0 ? kKeys : 0) + (has1 ? kKeys : 0));
+                            if (has0) bulk_g2s(k_stage, page_of(id0), kKeys, k_full);
+                            if (has1) bulk_g2s(v_stage + 1024, page_of(id1), kKeys, k_full);
+                        }
                         __syncwarp();
                     }
-                    if (n_tiles > 2) fetch_k(2, 0);
-                    copied(k_free, done + 1);
-                }
-            } else {
-                fetch_k(0, 0);
-                fetch_v(0, 0);
-                fetch_norms(0, 0);
-                if (n_tiles > 1) {
-                    copied(k_free, done);
-                    fetch_k(1, 0);
-                    copied(v_free, done);
-                    fetch_v(1, 0);
-                }
-                if (n_tiles > 2) {
-                    copied(k_free, done + 1);
-                    fetch_k(2, 0);
-                }
-            }
-#pragma unroll 1
-            for (int it = 0; it + 1 < n_tiles; it++) {
-                copied(n_free, done + it);
-                fetch_norms(it + 1, it + 1);
-                if (it + 3 < n_tiles) {
-                    copied(k_free, done + it + 2);
-                    fetch_k(it + 3, it + 1);
-                }
-                if (C::LATE_V) {
-                    wait(o_done, done + it);
-                    fetch_v(it + 1, it + 1);
-                } else if (it + 2 < n_tiles) {
-                    copied(v_free, done + it + 1);
-                    fetch_v(it + 2, it + 1);
-                }
-                if (((it + 2) & 3) == 0) {      // (ida has the ids of the next round's tile it + 1)
-                    ida = idb;
-                    idb = load_ids(it + 6);
-                }
-            }
-            done += n_tiles;
-        }
-        auto drain = [&](uint32_t bar, int sent) {
-#pragma unroll 1
-            for (int i = 0; i < kDrainSpinLimit && sent > 0 && !mbar_try_wait(bar, (sent - 1) & 1); i++) {}
-        };
-        drain(k_full, k_sent);
-        drain(v_full, v_sent);
-        drain(n_full, n_sent);
-    }
-    if (me == 0) pos = begin;
-    const uint32_t stage = stage_of(warp);
-#pragma unroll 1
-    while (!helper) {
-        if (me == 0) {
-            int from = pos;
-            const TreePiece x = next_piece(from);
-            pc.b = x.b;
-            pc.hkv = x.hkv;
-            pc.row0 = x.row0;
-            pc.rows = x.rows;
-            pc.tile0 = x.tile0;
-            pc.n_tiles = x.n_tiles;
-            pc.seq = x.seq;
-            pc.ctx = x.ctx;
-            pc.out = x.out;
-            pos = from;
-        }
-        meet_feeder();
-        const int n_tiles = pc.n_tiles, group = static_cast<int>(p.group.d);
-        if (n_tiles == 0) {
-            meet_issuer(false);
-            break;
-        }
-        const int first_masked = pc.ctx / kTreeTile - pc.tile0;       // (from here on tiles reach the tree or the sequence's end)
-        // keys: codes -> TMEM, rows = tokens
-        auto put_k = [&](int tile, uint32_t from) {
-            copied(k_full, done + tile);
-            typename Window<BK, false>::template Run<KW> r0, r1;
-            tree_run<KSB>(from + g8 * C::PDK, t4, r0);
-            tree_run<KSB>(from + (g8 + 8) * C::PDK, t4, r1);
-            taken(k_free);
-            Window<BK, false>::shift(r0);
-            Window<BK, false>::shift(r1);
-            const uint32_t dst = tmem + (static_cast<uint32_t>(16 * my_page) << 16) + (tile & 1) * (D / 2);
-#pragma unroll
-            for (int q = 0; q < D / 64; q++) {
-                uint32_t x[16];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    Window<BK, false>::pairs(r0, 4 * q + j, k_base, x[4 * j], x[4 * j + 1]);
-                    Window<BK, false>::pairs(r1, 4 * q + j, k_base, x[4 * j + 2], x[4 * j + 3]);
-                }
-                tc_st_16x256b_x4(dst + 32 * q, x);
-            }
-        };
-        // values: codes -> fp16 tile, MN-major with 128-byte swizzle
-        // (a V row has its halves exchanged where bit 1 of its token's place is set)
-        auto put_v = [&](int tile) {
-            copied(v_full, done + tile);
-            const uint32_t from = (C::LATE_V ? a_v + 2048 * my_page : stage) + g8 * C::PDV;
-            typename Window<BV, false>::template Run<VW> run[2];
-#pragma unroll
-            for (int r = 0; r < 2; r++) tree_run<VSB>(from + 8 * r * C::PDV, t4 ^ (g8 & 2), run[r]);
-            if (C::LATE_V) __syncwarp();
-            else taken(v_free);
-#pragma unroll
-            for (int r = 0; r < 2; r++) {
-                Window<BV, false>::shift(run[r]);
-                const int row = 16 * my_page + g8 + 8 * r;
-                const uint32_t dst = a_v + (tile % C::VB) * C::V_BUF + row * 128;
-#pragma unroll
-                for (int jj = 0; jj < D / 32; jj++) {
-                    uint32_t x[4];
-                    Window<BV, false>::pairs(run[r], 2 * jj, v_base, x[0], x[1]);
-                    Window<BV, false>::pairs(run[r], 2 * jj + 1, v_base, x[2], x[3]);
-                    // (eight lanes that store together have two rows and four chunks apart by two: no two on the same banks)
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(dst + (jj >> 1) * C::V_ATOM + (((2 * t4 + (jj & 1)) ^ (row & 7)) << 4)),
-                                 "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
-                }
-            }
-        };
-        // ---- the queries: rotated, scaled, fp16, K-major with 128-byte swizzle
-        float q_down;
-        {
-            const int b = pc.b, hkv = pc.hkv, row0 = pc.row0, rows = pc.rows, ctx = pc.ctx;
-            constexpr int OCTETS = C::HT / 8;
-            const int t8 = lane & 7, octet = me >> 3;
-            auto query = [&](int r) {   // row r's 16-byte pieces: eight coordinates each
-                const int i = fast_div(row0 + r, p.group), h = row0 + r - i * group;
-                return static_cast<const uint4*>(p.q) + (((static_cast<int64_t>(b) * p.T + i) * p.Hq + hkv * group + h) * D) / 8;
-            };
-            auto widen = [&](const uint4& x, float (&o)[8]) {
-                if (p.q_dtype == kBF16) load8<__nv_bfloat16>(reinterpret_cast<const __nv_bfloat16*>(&x), o);
-                else load8<__half>(reinterpret_cast<const __half*>(&x), o);
-            };
-            // (read once: two rows an octet at most)
-            constexpr int NR = (N + OCTETS - 1) / OCTETS;
-            uint4 raw[NR][D / 64];
-#pragma unroll
-            for (int k = 0; k < NR; k++)
-#pragma unroll
-                for (int j = 0; j < D / 64; j++) {
-                    const int r = octet + k * OCTETS;
-                    raw[k][j] = r < rows ? query(r)[t8 + 8 * j] : make_uint4(0, 0, 0, 0);
-                }
-            // the mask words of the rows' nodes (to where weights will be)
-            const bool trees = (pc.tile0 + n_tiles) * kTreeTile > ctx;
-            const int i0 = fast_div(row0, p.group), words = (p.T + 31) / 32;
-            uint32_t* const mask_words = reinterpret_cast<uint32_t*>(at(a_p));
-            static_assert(N * (kTreeMaxNodes / 32) * 4 <= C::P_BUF, "");
-            if (trees)
-                for (int k = me; k < (fast_div(row0 + rows - 1, p.group) - i0 + 1) * words; k += C::HT)
-                    mask_words[k] = p.masks[(static_cast<int64_t>(b) * p.T + i0 + k / words) * p.W + k % words];
-            // the largest, for a common scale: |rotated| <= D * largest |q|, and that shall be below 2^15
-            float top = 0.f;
-#pragma unroll
-            for (int k = 0; k < NR; k++)
-#pragma unroll
-                for (int j = 0; j < D / 64; j++) {
-                    float v[8];
-                    widen(raw[k][j], v);
-#pragma unroll
-                    for (int c = 0; c < 8; c++) top = fabsf(v[c]) <= FLT_MAX ? fmaxf(top, fabsf(v[c])) : top;
-                }
-            __syncwarp();
-            top = warp_max(top);
-            if (lane == 0) red[hw] = top;
-            if (me < N) s_nm[me] = INFINITY;
-            meet();
-#pragma unroll
-            for (int w = 0; w < C::WH; w++) top = fmaxf(top, red[w]);
-            const float all = top * (fabsf(p.q_scale) * D);
-            const int e = all > 0.f ? max(-120, min(120, 14 - ilogbf(all))) : 0;
-            const float up = p.q_scale * ldexpf(1.f, e);
-            q_down = ldexpf(1.f, -e);
-#pragma unroll
-            for (int k2 = 0; k2 < NR; k2++) {
-                const int r = octet + k2 * OCTETS;
-                float a[E];
-#pragma unroll
-                for (int k = 0; k < D / 64; k++) {
-                    float v[8];
-                    widen(raw[k2][k], v);
-#pragma unroll
-                    for (int c = 0; c < 8; c++)
-                        a[8 * k + c] = __uint_as_float(__float_as_uint(v[c] * up) ^ sign_mask(p.signs, load_coord(t8, 8 * k + c)));
-                }
-                octet_fwht<E>(a, lane);
-                // Coordinate c = t8 + 8 k is code 4 jj + (c & 3) of lane t's run: place 16 jj + 4 t + (c & 3).  Two lanes have two
-                // neighbours: of two k's the even lane stores the first, the odd lane the second.
-                uint8_t* dst = at(a_q) + r * 128;
-#pragma unroll
-                for (int k = 0; k < E; k += 2) {
-                    const float other = __shfl_xor_sync(0xffffffffu, (t8 & 1) ? a[k] : a[k + 1], 1);
-                    const int c = (t8 & 6) + 8 * (k + (t8 & 1)), t = c / (D / 4), jj = (c % (D / 4)) / 4, place = 16 * jj + 4 * t + (c & 3);
-                    const uint32_t h = (t8 & 1) ? f2h2(other, a[k + 1]) : f2h2(a[k], other);
-                    if (r < N) *reinterpret_cast<uint32_t*>(dst + (place >> 6) * (N * 128) + ((((place & 63) >> 3) ^ (r & 7)) << 4) + (place & 7) * 2) = h;
-                }
-            }
-            // which rows attend a node: bit r of its words
-            if (trees) {
-                const int nodes = pc.seq - ctx;
-                for (int k = me; k < nodes * C::MW; k += C::HT) {
-                    const int node = k / C::MW, w = k % C::MW;
-                    uint32_t bits = 0;
-                    // (a node's heads are neighbours: a run of bits)
-                    const int r1 = min(rows, 32 * w + 32);
-#pragma unroll 1
-                    for (int r = 32 * w; r < r1;) {
-                        const int i = fast_div(row0 + r, p.group), stop = min(r1, (i + 1) * group - row0);
-                        if ((mask_words[(i - i0) * words + (node >> 5)] >> (node & 31)) & 1u)
-                            bits |= (0xffffffffu >> (32 - (stop - r))) << (r & 31);
-                        r = stop;
+                    fetch_norms(0, 0);
+                    fetch_v(0, 0);
+                    if (n_tiles > 1) {
+                        copied(k_free, done);
+                        if (!stalled) {
+                            k_sent++;
+                            if (lane < 8) mbar_arrive(k_full);
+                            __syncwarp();
+                        }
+                        if (n_tiles > 2) fetch_k(2, 0);
+                        copied(k_free, done + 1);
                     }
-                    cm[k] = bits;
+                } else {
+                    fetch_k(0, 0);
+                    fetch_v(0, 0);
+                    fetch_norms(0, 0);
+                    if (n_tiles > 1) {
+                        copied(k_free, done);
+                        fetch_k(1, 0);
+                        copied(v_free, done);
+                        fetch_v(1, 0);
+                    }
+                    if (n_tiles > 2) {
+                        copied(k_free, done + 1);
+                        fetch_k(2, 0);
+                    }
                 }
-            }
-        }
-        if (has_k) put_k(0, stage);
-        if (has_v && !C::LATE_V) put_v(0);
-        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-        tc_wait_st();
-        tc_fence_before();
-        meet_issuer(false);
-        if (has_k && n_tiles > 1) put_k(1, C::LATE_V ? a_v + 2048 * my_page + 1024 : stage);
-        float l[CW], vs = 0.f;      // sums of the thread's tokens; scale of |v|
-#pragma unroll
-        for (int c = 0; c < CW; c++) l[c] = 0.f;
-
 #pragma unroll 1
-        for (int it = 0; it < n_tiles; it++) {
-            const bool masked = it >= first_masked;
-            uint32_t nk, nv;
-            copied(n_full, done + it);
-            asm volatile("ld.shared.u16 %0, [%1];\n" : "=r"(nk) : "r"(a_norm + 2 * my_tok) : "memory");
-            asm volatile("ld.shared.u16 %0, [%1];\n" : "=r"(nv) : "r"(a_norm + 256 + 2 * my_tok) : "memory");
-            taken(n_free);
-            const float kn = half_bits_to_float(nk) * q_down, vn = half_bits_to_float(nv);
-            // which of the group's rows attend the token; |v| where one does and it is finite
-            uint32_t bits = 0xffffffffu;
-            if (masked) {
-                const int node = (pc.tile0 + it) * kTreeTile + my_tok - pc.ctx;
-                if (node >= 0) bits = node >= pc.seq - pc.ctx ? 0u : cm[node * C::MW + col0 / 32] >> (col0 & 31);
-            }
-            if (CW < 32) bits &= (1u << (CW & 31)) - 1u;
-            const float av = bits != 0 && fabsf(vn) <= FLT_MAX ? fabsf(vn) : 0.f;
-            const uint32_t s_at = tl + C::COL_S + col0;
-            // scores - maxima (base 2)
-            auto exponents = [&](float* x) {
-                uint32_t s[CW];
-                tc_load(s_at, s);
-                const u64 kn2 = pk2(kn, kn);
-#pragma unroll
-                for (int c = 0; c < CW; c += 4) {
-                    const float4 nm = *reinterpret_cast<const float4*>(s_nm + col0 + c);
-                    upk2(fma2(pk2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), kn2, pk2(nm.x, nm.y)), x[c], x[c + 1]);
-                    upk2(fma2(pk2(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])), kn2, pk2(nm.z, nm.w)), x[c + 2], x[c + 3]);
+                for (int it = 0; it + 1 < n_tiles; it++) {
+                    copied(n_free, done + it);
+                    fetch_norms(it + 1, it + 1);
+                    if (it + 3 < n_tiles) {
+                        copied(k_free, done + it + 2);
+                        fetch_k(it + 3, it + 1);
+                    }
+                    if (C::LATE_V) {
+                        wait(o_done, done + it);
+                        fetch_v(it + 1, it + 1);
+                    } else if (it + 2 < n_tiles) {
+                        copied(v_free, done + it + 1);
+                        fetch_v(it + 2, it + 1);
+                    }
+                    if (((it + 2) & 3) == 0) {      // (ida has the ids of the next round's tile it + 1)
+                        ida = idb;
+                        idb = load_ids(it + 6);
+                    }
                 }
+                done += n_tiles;
+            }
+            auto drain = [&](uint32_t bar, int sent) {
+#pragma unroll 1
+                for (int i = 0; i < kDrainSpinLimit && sent > 0 && !mbar_try_wait(bar, (sent - 1) & 1); i++) {}
             };
-            // weights to shared memory and into the sums
-            auto weights = [&](const float* x, auto with_masks, bool add) {
-                const float vw = vn * vs;
-                const u64 vw2 = pk2(vw, vw);
+            drain(k_full, k_sent);
+            drain(v_full, v_sent);
+            drain(n_full, n_sent);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n");
+        if (me == 0) pos = begin;
+        const uint32_t stage = stage_of(warp);
+#pragma unroll 1
+        while (true) {
+            if (me == 0) {
+                int from = pos;
+                const TreePiece x = next_piece(from);
+                pc.b = x.b;
+                pc.hkv = x.hkv;
+                pc.row0 = x.row0;
+                pc.rows = x.rows;
+                pc.tile0 = x.tile0;
+                pc.n_tiles = x.n_tiles;
+                pc.seq = x.seq;
+                pc.ctx = x.ctx;
+                pc.out = x.out;
+                pos = from;
+            }
+            meet_feeder();
+            const int n_tiles = pc.n_tiles, group = static_cast<int>(p.group.d);
+            if (n_tiles == 0) {
+                meet_issuer(false);
+                break;
+            }
+            const int first_masked = pc.ctx / kTreeTile - pc.tile0;       // (from here on tiles reach the tree or the sequence's end)
+            // keys: codes -> TMEM, rows = tokens
+            auto put_k = [&](int tile, uint32_t from) {
+                copied(k_full, done + tile);
+                typename Window<BK, false>::template Run<KW> r0, r1;
+                tree_run<KSB>(from + g8 * C::PDK, t4, r0);
+                tree_run<KSB>(from + (g8 + 8) * C::PDK, t4, r1);
+                taken(k_free);
+                Window<BK, false>::shift(r0);
+                Window<BK, false>::shift(r1);
+                const uint32_t dst = tmem + (static_cast<uint32_t>(16 * my_page) << 16) + (tile & 1) * (D / 2);
 #pragma unroll
-                for (int c = 0; c < CW; c += 8) {
-                    uint32_t h[4];
+                for (int q = 0; q < D / 64; q++) {
+                    uint32_t x[16];
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const int k = c + 2 * j;
-                        const float e0 = fast_exp2(x[k]), e1 = fast_exp2(x[k + 1]);
-                        if (!decltype(with_masks)::value || add) upk2(add2(pk2(l[k], l[k + 1]), pk2(e0, e1)), l[k], l[k + 1]);
-                        float w0, w1;
-                        upk2(mul2(pk2(e0, e1), vw2), w0, w1);
-                        if constexpr (decltype(with_masks)::value) {    // (what a row does not attend may have a norm that is not a number)
-                            w0 = (bits >> k) & 1u ? w0 : 0.f;
-                            w1 = (bits >> (k + 1)) & 1u ? w1 : 0.f;
-                        }
-                        h[j] = f2h2(w0, w1);
+                        Window<BK, false>::pairs(r0, 4 * q + j, k_base, x[4 * j], x[4 * j + 1]);
+                        Window<BK, false>::pairs(r1, 4 * q + j, k_base, x[4 * j + 2], x[4 * j + 3]);
                     }
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(p_row + (((((col0 & 63) + c) >> 3) ^ (my_tok & 7)) << 4)),
-                                 "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                    tc_st_16x256b_x4(dst + 32 * q, x);
                 }
             };
-            auto apply_masks = [&](float* x) {
-                asm volatile("" ::: "memory");      // (a branch: selects in every tile would be a tenth of its instructions)
+            // values: codes -> fp16 tile, MN-major with 128-byte swizzle
+            // (a V row has its halves exchanged where bit 1 of its token's place is set)
+            auto put_v = [&](int tile) {
+                copied(v_full, done + tile);
+                const uint32_t from = (C::LATE_V ? a_v + 2048 * my_page : stage) + g8 * C::PDV;
+                typename Window<BV, false>::template Run<VW> run[2];
 #pragma unroll
-                for (int c = 0; c < CW; c++) x[c] = (bits >> c) & 1u ? x[c] : -INFINITY;
+                for (int r = 0; r < 2; r++) tree_run<VSB>(from + 8 * r * C::PDV, t4 ^ (g8 & 2), run[r]);
+                if (C::LATE_V) __syncwarp();
+                else taken(v_free);
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    Window<BV, false>::shift(run[r]);
+                    const int row = 16 * my_page + g8 + 8 * r;
+                    const uint32_t dst = a_v + (tile % C::VB) * C::V_BUF + row * 128;
+#pragma unroll
+                    for (int jj = 0; jj < D / 32; jj++) {
+                        uint32_t x[4];
+                        Window<BV, false>::pairs(run[r], 2 * jj, v_base, x[0], x[1]);
+                        Window<BV, false>::pairs(run[r], 2 * jj + 1, v_base, x[2], x[3]);
+                        // (eight lanes that store together have two rows and four chunks apart by two: no two on the same banks)
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(dst + (jj >> 1) * C::V_ATOM + (((2 * t4 + (jj & 1)) ^ (row & 7)) << 4)),
+                                     "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+                    }
+                }
             };
-            wait(s_done, done + it);
-            if (!C::LATE_V && C::VB == 2 && it > 0) wait(o_done, done + it - 1);       // (P.V of the tile before has read the weights)
-            bool above = false;
-            float x[CW];
-            if (soft) {
-                exponents(x);
-                if (masked) apply_masks(x);
-                float top = fmaxf(x[0], x[1]);
+            // ---- the queries: rotated, scaled, fp16, K-major with 128-byte swizzle
+            float q_down;
+            {
+                const int b = pc.b, hkv = pc.hkv, row0 = pc.row0, rows = pc.rows, ctx = pc.ctx;
+                constexpr int OCTETS = C::HT / 8;
+                const int t8 = lane & 7, octet = me >> 3;
+                auto query = [&](int r) {   // row r's 16-byte pieces: eight coordinates each
+                    const int i = fast_div(row0 + r, p.group), h = row0 + r - i * group;
+                    return static_cast<const uint4*>(p.q) + (((static_cast<int64_t>(b) * p.T + i) * p.Hq + hkv * group + h) * D) / 8;
+                };
+                auto widen = [&](const uint4& x, float (&o)[8]) {
+                    if (p.q_dtype == kBF16) load8<__nv_bfloat16>(reinterpret_cast<const __nv_bfloat16*>(&x), o);
+                    else load8<__half>(reinterpret_cast<const __half*>(&x), o);
+                };
+                // (read once: two rows an octet at most)
+                constexpr int NR = (N + OCTETS - 1) / OCTETS;
+                uint4 raw[NR][D / 64];
 #pragma unroll
-                for (int c = 2; c < CW; c += 2) top = fmaxf(fmaxf(top, x[c]), x[c + 1]);
-                above = __any_sync(0xffffffffu, top > kTreeSlack || (vs == 0.f ? av > 0.f : av * vs > kTreeGrowth));
+                for (int k = 0; k < NR; k++)
+#pragma unroll
+                    for (int j = 0; j < D / 64; j++) {
+                        const int r = octet + k * OCTETS;
+                        raw[k][j] = r < rows ? query(r)[t8 + 8 * j] : make_uint4(0, 0, 0, 0);
+                    }
+                // the mask words of the rows' nodes (to where weights will be)
+                const bool trees = (pc.tile0 + n_tiles) * kTreeTile > ctx;
+                const int i0 = fast_div(row0, p.group), words = (p.T + 31) / 32;
+                uint32_t* const mask_words = reinterpret_cast<uint32_t*>(at(a_p));
+                static_assert(N * (kTreeMaxNodes / 32) * 4 <= C::P_BUF, "");
+                if (trees)
+                    for (int k = me; k < (fast_div(row0 + rows - 1, p.group) - i0 + 1) * words; k += C::HT)
+                        mask_words[k] = p.masks[(static_cast<int64_t>(b) * p.T + i0 + k / words) * p.W + k % words];
+                // the largest, for a common scale: |rotated| <= D * largest |q|, and that shall be below 2^15
+                float top = 0.f;
+#pragma unroll
+                for (int k = 0; k < NR; k++)
+#pragma unroll
+                    for (int j = 0; j < D / 64; j++) {
+                        float v[8];
+                        widen(raw[k][j], v);
+#pragma unroll
+                        for (int c = 0; c < 8; c++) top = fabsf(v[c]) <= FLT_MAX ? fmaxf(top, fabsf(v[c])) : top;
+                    }
+                __syncwarp();
+                top = warp_max(top);
+                if (lane == 0) red[hw] = top;
+                if (me < N) s_nm[me] = INFINITY;
+                meet();
+#pragma unroll
+                for (int w = 0; w < C::WH; w++) top = fmaxf(top, red[w]);
+                const float all = top * (fabsf(p.q_scale) * D);
+                const int e = all > 0.f ? max(-120, min(120, 14 - ilogbf(all))) : 0;
+                const float up = p.q_scale * ldexpf(1.f, e);
+                q_down = ldexpf(1.f, -e);
+#pragma unroll
+                for (int k2 = 0; k2 < NR; k2++) {
+                    const int r = octet + k2 * OCTETS;
+                    float a[E];
+#pragma unroll
+                    for (int k = 0; k < D / 64; k++) {
+                        float v[8];
+                        widen(raw[k2][k], v);
+#pragma unroll
+                        for (int c = 0; c < 8; c++)
+                            a[8 * k + c] = __uint_as_float(__float_as_uint(v[c] * up) ^ sign_mask(p.signs, load_coord(t8, 8 * k + c)));
+                    }
+                    octet_fwht<E>(a, lane);
+                    // Coordinate c = t8 + 8 k is code 4 jj + (c & 3) of lane t's run: place 16 jj + 4 t + (c & 3).  Two lanes have two
+                    // neighbours: of two k's the even lane stores the first, the odd lane the second.
+                    uint8_t* dst = at(a_q) + r * 128;
+#pragma unroll
+                    for (int k = 0; k < E; k += 2) {
+                        const float other = __shfl_xor_sync(0xffffffffu, (t8 & 1) ? a[k] : a[k + 1], 1);
+                        const int c = (t8 & 6) + 8 * (k + (t8 & 1)), t = c / (D / 4), jj = (c % (D / 4)) / 4, place = 16 * jj + 4 * t + (c & 3);
+                        const uint32_t h = (t8 & 1) ? f2h2(other, a[k + 1]) : f2h2(a[k], other);
+                        if (r < N) *reinterpret_cast<uint32_t*>(dst + (place >> 6) * (N * 128) + ((((place & 63) >> 3) ^ (r & 7)) << 4) + (place & 7) * 2) = h;
+                    }
+                }
+                // which rows attend a node: bit r of its words
+                if (trees) {
+                    const int nodes = pc.seq - ctx;
+                    for (int k = me; k < nodes * C::MW; k += C::HT) {
+                        const int node = k / C::MW, w = k % C::MW;
+                        uint32_t bits = 0;
+                        // (a node's heads are neighbours: a run of bits)
+                        const int r1 = min(rows, 32 * w + 32);
+#pragma unroll 1
+                        for (int r = 32 * w; r < r1;) {
+                            const int i = fast_div(row0 + r, p.group), stop = min(r1, (i + 1) * group - row0);
+                            if ((mask_words[(i - i0) * words + (node >> 5)] >> (node & 31)) & 1u)
+                                bits |= (0xffffffffu >> (32 - (stop - r))) << (r & 31);
+                            r = stop;
+                        }
+                        cm[k] = bits;
+                    }
+                }
             }
-            if (C::LATE_V && it > 0) wait(o_done, done + it - 1);
-            if (soft && !above) {
-                if (masked) weights(x, std::true_type{}, true);
-                else weights(x, std::false_type{}, true);
-            }
-            if (C::LATE_V) {
-                put_v(it);
-            }
+            if (has_k) put_k(0, stage);
+            if (has_v && !C::LATE_V) put_v(0);
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             tc_wait_st();
             tc_fence_before();
-            if (meet_issuer(above)) {
-                // ---- new maxima; O, the sums and the tile's weights refer to them
-                const float m_run = soft && lane < CW ? -s_nm[col0 + lane] : 0.f;
-                if (soft) {
-                    float mine = -INFINITY;
+            meet_issuer(false);
+            if (has_k && n_tiles > 1) put_k(1, C::LATE_V ? a_v + 2048 * my_page + 1024 : stage);
+            float l[CW], vs = 0.f;      // sums of the thread's tokens; scale of |v|
+#pragma unroll
+            for (int c = 0; c < CW; c++) l[c] = 0.f;
+
 #pragma unroll 1
-                    for (int c0 = 0; c0 < CW; c0 += 8) {
-                        uint32_t s[8];
-                        tc_load(s_at + c0, s);
-#pragma unroll
-                        for (int c = 0; c < 8; c++) {
-                            const float r = warp_max((bits >> (c0 + c)) & 1u ? __uint_as_float(s[c]) * kn : -INFINITY);
-                            if (lane == c0 + c) mine = r;
-                        }
-                    }
-                    const float wv = warp_max(av);
-                    if (lane < CW) red[quarter * N + col0 + lane] = mine;
-                    if (lane == 0) red_v[hw] = wv;
+            for (int it = 0; it < n_tiles; it++) {
+                const bool masked = it >= first_masked;
+                uint32_t nk, nv;
+                copied(n_full, done + it);
+                asm volatile("ld.shared.u16 %0, [%1];\n" : "=r"(nk) : "r"(a_norm + 2 * my_tok) : "memory");
+                asm volatile("ld.shared.u16 %0, [%1];\n" : "=r"(nv) : "r"(a_norm + 256 + 2 * my_tok) : "memory");
+                taken(n_free);
+                const float kn = half_bits_to_float(nk) * q_down, vn = half_bits_to_float(nv);
+                // which of the group's rows attend the token; |v| where one does and it is finite
+                uint32_t bits = 0xffffffffu;
+                if (masked) {
+                    const int node = (pc.tile0 + it) * kTreeTile + my_tok - pc.ctx;
+                    if (node >= 0) bits = node >= pc.seq - pc.ctx ? 0u : cm[node * C::MW + col0 / 32] >> (col0 & 31);
                 }
-                meet();
-                float v_ratio = 1.f;
-                if (soft) {
-                    float v_top = 0.f;
-#pragma unroll
-                    for (int w = 0; w < 4; w++) v_top = fmaxf(v_top, red_v[4 * cg + w]);
-                    if (v_top > 0.f && (vs == 0.f || v_top * vs > kTreeGrowth)) {   // the largest |v| becomes 1 to 2
-                        const float to = ldexpf(1.f, -ilogbf(v_top));
-                        v_ratio = vs == 0.f ? 1.f : to / vs;
-                        vs = to;
-                    }
-                    if (lane < CW) {
-                        float m_new = m_run;
-#pragma unroll
-                        for (int w = 0; w < 4; w++) m_new = fmaxf(m_new, red[w * N + col0 + lane]);
-                        const float lc = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
-                        if (quarter == 0) {
-                            s_nm[col0 + lane] = -m_new;
-                            s_lc[col0 + lane] = lc;
-                            s_corr[col0 + lane] = lc * v_ratio;
-                        }
-                    }
-                }
-                meet();
-                if (soft) {
+                if (CW < 32) bits &= (1u << (CW & 31)) - 1u;
+                const float av = bits != 0 && fabsf(vn) <= FLT_MAX ? fabsf(vn) : 0.f;
+                const uint32_t s_at = tl + C::COL_S + col0;
+                // scores - maxima (base 2)
+                auto exponents = [&](float* x) {
+                    uint32_t s[CW];
+                    tc_load(s_at, s);
+                    const u64 kn2 = pk2(kn, kn);
 #pragma unroll
                     for (int c = 0; c < CW; c += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(s_lc + col0 + c);
-                        l[c] *= f.x;
-                        l[c + 1] *= f.y;
-                        l[c + 2] *= f.z;
-                        l[c + 3] *= f.w;
+                        const float4 nm = *reinterpret_cast<const float4*>(s_nm + col0 + c);
+                        upk2(fma2(pk2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), kn2, pk2(nm.x, nm.y)), x[c], x[c + 1]);
+                        upk2(fma2(pk2(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])), kn2, pk2(nm.z, nm.w)), x[c + 2], x[c + 3]);
                     }
-                    if (it > 0) {       // (P.V of the tile before is complete)
+                };
+                // weights to shared memory and into the sums
+                auto weights = [&](const float* x, auto with_masks, bool add) {
+                    const float vw = vn * vs;
+                    const u64 vw2 = pk2(vw, vw);
 #pragma unroll
-                        for (int mb = 0; mb < C::MB; mb++) {
-#pragma unroll 1
-                            for (int c = 0; c < CW; c += 8) {       // (few registers: what this path spills the others pay for)
-                                uint32_t o[8];
-                                const uint32_t o_at = tl + C::COL_O + mb * N + col0 + c;
-                                const float4 f = *reinterpret_cast<const float4*>(s_corr + col0 + c), g = *reinterpret_cast<const float4*>(s_corr + col0 + c + 4);
-                                const float by[8] = {f.x, f.y, f.z, f.w, g.x, g.y, g.z, g.w};
-                                tc_load(o_at, o);
+                    for (int c = 0; c < CW; c += 8) {
+                        uint32_t h[4];
 #pragma unroll
-                                for (int k = 0; k < 8; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * by[k]);
-                                tc_st8(o_at, o);
+                        for (int j = 0; j < 4; j++) {
+                            const int k = c + 2 * j;
+                            const float e0 = fast_exp2(x[k]), e1 = fast_exp2(x[k + 1]);
+                            if (!decltype(with_masks)::value || add) upk2(add2(pk2(l[k], l[k + 1]), pk2(e0, e1)), l[k], l[k + 1]);
+                            float w0, w1;
+                            upk2(mul2(pk2(e0, e1), vw2), w0, w1);
+                            if constexpr (decltype(with_masks)::value) {    // (what a row does not attend may have a norm that is not a number)
+                                w0 = (bits >> k) & 1u ? w0 : 0.f;
+                                w1 = (bits >> (k + 1)) & 1u ? w1 : 0.f;
                             }
+                            h[j] = f2h2(w0, w1);
                         }
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(p_row + (((((col0 & 63) + c) >> 3) ^ (my_tok & 7)) << 4)),
+                                     "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
                     }
+                };
+                auto apply_masks = [&](float* x) {
+                    asm volatile("" ::: "memory");      // (a branch: selects in every tile would be a tenth of its instructions)
+#pragma unroll
+                    for (int c = 0; c < CW; c++) x[c] = (bits >> c) & 1u ? x[c] : -INFINITY;
+                };
+                wait(s_done, done + it);
+                if (!C::LATE_V && C::VB == 2 && it > 0) wait(o_done, done + it - 1);       // (P.V of the tile before has read the weights)
+                bool above = false;
+                float x[CW];
+                if (soft) {
                     exponents(x);
-                    apply_masks(x);
-                    weights(x, std::true_type{}, above);
+                    if (masked) apply_masks(x);
+                    float top = fmaxf(x[0], x[1]);
+#pragma unroll
+                    for (int c = 2; c < CW; c += 2) top = fmaxf(fmaxf(top, x[c]), x[c + 1]);
+                    above = __any_sync(0xffffffffu, top > kTreeSlack || (vs == 0.f ? av > 0.f : av * vs > kTreeGrowth));
+                }
+                if (C::LATE_V && it > 0) wait(o_done, done + it - 1);
+                if (soft && !above) {
+                    if (masked) weights(x, std::true_type{}, true);
+                    else weights(x, std::false_type{}, true);
+                }
+                if (C::LATE_V) {
+                    put_v(it);
                 }
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 tc_wait_st();
                 tc_fence_before();
-                meet_issuer(false);
-            }
-            tc_fence_after();
-            if (it + 1 == n_tiles) break;
-            // ---- the tiles to come
-            if (has_k && it + 2 < n_tiles) put_k(it + 2, stage);
-            if (!C::LATE_V) {
-                if (C::VB == 1) wait(o_done, done + it);
-                if (has_v) put_v(it + 1);
-            }
-        }
-        // ---- the piece's rows
-        wait(o_done, done + n_tiles - 1);
-        done += n_tiles;
-        const int rows = pc.rows;
-        float* const to = pc.out;
-        if (soft) {
-            // sums over the lanes, then over the warps: lane c gets row c's
-            float sum[CW];
+                if (meet_issuer(above)) {
+                    // ---- new maxima; O, the sums and the tile's weights refer to them
+                    const float m_run = soft && lane < CW ? -s_nm[col0 + lane] : 0.f;
+                    if (soft) {
+                        float mine = -INFINITY;
+#pragma unroll 1
+                        for (int c0 = 0; c0 < CW; c0 += 8) {
+                            uint32_t s[8];
+                            tc_load(s_at + c0, s);
 #pragma unroll
-            for (int c = 0; c < CW; c++) {
-                sum[c] = l[c];
+                            for (int c = 0; c < 8; c++) {
+                                const float r = warp_max((bits >> (c0 + c)) & 1u ? __uint_as_float(s[c]) * kn : -INFINITY);
+                                if (lane == c0 + c) mine = r;
+                            }
+                        }
+                        const float wv = warp_max(av);
+                        if (lane < CW) red[quarter * N + col0 + lane] = mine;
+                        if (lane == 0) red_v[hw] = wv;
+                    }
+                    meet();
+                    float v_ratio = 1.f;
+                    if (soft) {
+                        float v_top = 0.f;
 #pragma unroll
-                for (int d = CW; d < 32; d <<= 1) sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], d);
-            }
+                        for (int w = 0; w < 4; w++) v_top = fmaxf(v_top, red_v[4 * cg + w]);
+                        if (v_top > 0.f && (vs == 0.f || v_top * vs > kTreeGrowth)) {   // the largest |v| becomes 1 to 2
+                            const float to = ldexpf(1.f, -ilogbf(v_top));
+                            v_ratio = vs == 0.f ? 1.f : to / vs;
+                            vs = to;
+                        }
+                        if (lane < CW) {
+                            float m_new = m_run;
 #pragma unroll
-            for (int d = CW / 2; d > 0; d >>= 1) {
+                            for (int w = 0; w < 4; w++) m_new = fmaxf(m_new, red[w * N + col0 + lane]);
+                            const float lc = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
+                            if (quarter == 0) {
+                                s_nm[col0 + lane] = -m_new;
+                                s_lc[col0 + lane] = lc;
+                                s_corr[col0 + lane] = lc * v_ratio;
+                            }
+                        }
+                    }
+                    meet();
+                    if (soft) {
 #pragma unroll
-                for (int i = 0; i < d; i++) {
-                    const bool hi = (lane & d) != 0;
-                    const float send = hi ? sum[i] : sum[i + d], keep = hi ? sum[i + d] : sum[i];
-                    sum[i] = keep + __shfl_xor_sync(0xffffffffu, send, d);
+                        for (int c = 0; c < CW; c += 4) {
+                            const float4 f = *reinterpret_cast<const float4*>(s_lc + col0 + c);
+                            l[c] *= f.x;
+                            l[c + 1] *= f.y;
+                            l[c + 2] *= f.z;
+                            l[c + 3] *= f.w;
+                        }
+                        if (it > 0) {       // (P.V of the tile before is complete)
+#pragma unroll
+                            for (int mb = 0; mb < C::MB; mb++) {
+#pragma unroll 1
+                                for (int c = 0; c < CW; c += 8) {       // (few registers: what this path spills the others pay for)
+                                    uint32_t o[8];
+                                    const uint32_t o_at = tl + C::COL_O + mb * N + col0 + c;
+                                    const float4 f = *reinterpret_cast<const float4*>(s_corr + col0 + c), g = *reinterpret_cast<const float4*>(s_corr + col0 + c + 4);
+                                    const float by[8] = {f.x, f.y, f.z, f.w, g.x, g.y, g.z, g.w};
+                                    tc_load(o_at, o);
+#pragma unroll
+                                    for (int k = 0; k < 8; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * by[k]);
+                                    tc_st8(o_at, o);
+                                }
+                            }
+                        }
+                        exponents(x);
+                        apply_masks(x);
+                        weights(x, std::true_type{}, above);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    tc_wait_st();
+                    tc_fence_before();
+                    meet_issuer(false);
+                }
+                tc_fence_after();
+                if (it + 1 == n_tiles) break;
+                // ---- the tiles to come
+                if (has_k && it + 2 < n_tiles) put_k(it + 2, stage);
+                if (!C::LATE_V) {
+                    if (C::VB == 1) wait(o_done, done + it);
+                    if (has_v) put_v(it + 1);
                 }
             }
-            if (lane < CW) red[quarter * N + col0 + lane] = sum[0];
-        }
-        meet();
-        if (soft) {
-            if (quarter == 0 && lane < CW && col0 + lane < rows) {
-                float* dst = to + (col0 + lane) * ROW + D;
-                const float* r = red + col0 + lane;
-                dst[0] = -s_nm[col0 + lane];
-                dst[1] = r[0] + r[N] + r[2 * N] + r[3 * N];
-            }
-            const float scale = p.inv_v_scale / (vs == 0.f ? 1.f : vs);
+            // ---- the piece's rows
+            wait(o_done, done + n_tiles - 1);
+            done += n_tiles;
+            const int rows = pc.rows;
+            float* const to = pc.out;
+            if (soft) {
+                // sums over the lanes, then over the warps: lane c gets row c's
+                float sum[CW];
 #pragma unroll
-            for (int mb = 0; mb < C::MB; mb++) {
-                uint32_t o[CW];
-                tc_load(tl + C::COL_O + mb * N + col0, o);
-                // TMEM row m: atom m / 64, 16-byte chunk (m % 64) / 8 = 2 t + (jj & 1): coordinate 8 jj + m % 8 of run t
-                const int m = my_tok + 128 * mb, chunk = (m & 63) >> 3, jj = 2 * (m >> 6) + (chunk & 1);
-                const int coord = (chunk >> 1) * (D / 4) + 8 * jj + (m & 7);
-                if (D == 64 && m >= 64) continue;
+                for (int c = 0; c < CW; c++) {
+                    sum[c] = l[c];
 #pragma unroll
-                for (int c = 0; c < CW; c++)
-                    if (col0 + c < rows) to[(col0 + c) * ROW + coord] = __uint_as_float(o[c]) * scale;
+                    for (int d = CW; d < 32; d <<= 1) sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], d);
+                }
+#pragma unroll
+                for (int d = CW / 2; d > 0; d >>= 1) {
+#pragma unroll
+                    for (int i = 0; i < d; i++) {
+                        const bool hi = (lane & d) != 0;
+                        const float send = hi ? sum[i] : sum[i + d], keep = hi ? sum[i + d] : sum[i];
+                        sum[i] = keep + __shfl_xor_sync(0xffffffffu, send, d);
+                    }
+                }
+                if (lane < CW) red[quarter * N + col0 + lane] = sum[0];
             }
+            meet();
+            if (soft) {
+                if (quarter == 0 && lane < CW && col0 + lane < rows) {
+                    float* dst = to + (col0 + lane) * ROW + D;
+                    const float* r = red + col0 + lane;
+                    dst[0] = -s_nm[col0 + lane];
+                    dst[1] = r[0] + r[N] + r[2 * N] + r[3 * N];
+                }
+                const float scale = p.inv_v_scale / (vs == 0.f ? 1.f : vs);
+#pragma unroll
+                for (int mb = 0; mb < C::MB; mb++) {
+                    uint32_t o[CW];
+                    tc_load(tl + C::COL_O + mb * N + col0, o);
+                    // TMEM row m: atom m / 64, 16-byte chunk (m % 64) / 8 = 2 t + (jj & 1): coordinate 8 jj + m % 8 of run t
+                    const int m = my_tok + 128 * mb, chunk = (m & 63) >> 3, jj = 2 * (m >> 6) + (chunk & 1);
+                    const int coord = (chunk >> 1) * (D / 4) + 8 * jj + (m & 7);
+                    if (D == 64 && m >= 64) continue;
+#pragma unroll
+                    for (int c = 0; c < CW; c++)
+                        if (col0 + c < rows) to[(col0 + c) * ROW + coord] = __uint_as_float(o[c]) * scale;
+                }
+            }
+            tc_fence_before();
+            meet();      // (the next piece writes to what these reads came from)
+            tc_fence_after();
         }
-        tc_fence_before();
-        meet();      // (the next piece writes to what these reads came from)
-        tc_fence_after();
     }
     __syncwarp();
     __syncthreads();
