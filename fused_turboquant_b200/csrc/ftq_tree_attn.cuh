@@ -38,7 +38,7 @@
 // busy 15 to 35 % of the time, HBM 3 to 25 %.  Measured (K4V4, bf16): one sequence of 900 tokens, 8 nodes, 32 heads of 128 over
 // 8: 17.2 us; 32 of 8192, 16 nodes: 173 us (floor by HBM 44), where dequantising and a CTA of 128 rows of one sequence after
 // the other took 413, one CTA of specialised warps 261 to 350 (handing tiles over cost more than the work), two halves
-// that fetched and issued for themselves 205; 2 of 131072, 64 nodes, 64 heads: 889 us (619 TFLOP/s, 38 % of the measured
+// that fetched and issued for themselves 205; 2 of 131072, 64 nodes, 64 heads: 884 us (622 TFLOP/s, 38 % of the measured
 // bf16 rate); 24 ragged of up to 16384, heads of 256: 99 us; 40 ragged of up to 4096, 25 nodes, 14 heads of 64 over 2: 41 us.
 //
 // Every wait is bounded.  After one has run out nothing waits any more, the half's rows become NaN and the status word says
@@ -848,7 +848,6 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                     }
                 };
                 auto apply_masks = [&](float* x) {
-                    asm volatile("" ::: "memory");      // (a branch: selects in every tile would be a tenth of its instructions)
 #pragma unroll
                     for (int c = 0; c < CW; c++) x[c] = (bits >> c) & 1u ? x[c] : -INFINITY;
                 };
@@ -856,13 +855,20 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 if (!C::LATE_V && C::VB == 2 && it > 0) wait(o_done, done + it - 1);       // (P.V of the tile before has read the weights)
                 bool above = false;
                 float x[CW];
-                if (soft) {
-                    exponents(x);
-                    if (masked) apply_masks(x);
-                    float top = fmaxf(x[0], x[1]);
+                auto too_high = [&](const float* y) {
+                    float top = fmaxf(y[0], y[1]);
 #pragma unroll
-                    for (int c = 2; c < CW; c += 2) top = fmaxf(fmaxf(top, x[c]), x[c + 1]);
-                    above = __any_sync(0xffffffffu, top > kTreeSlack || (vs == 0.f ? av > 0.f : av * vs > kTreeGrowth));
+                    for (int c = 2; c < CW; c += 2) top = fmaxf(fmaxf(top, y[c]), y[c + 1]);
+                    return __any_sync(0xffffffffu, top > kTreeSlack || (vs == 0.f ? av > 0.f : av * vs > kTreeGrowth)) != 0;
+                };
+                // (two paths down to the vote: a branch around the selects alone becomes selects in every tile)
+                if (soft && !masked) {
+                    exponents(x);
+                    above = too_high(x);
+                } else if (soft) {
+                    exponents(x);
+                    apply_masks(x);
+                    above = too_high(x);
                 }
                 if (C::LATE_V && it > 0) wait(o_done, done + it - 1);
                 if (soft && !above) {
