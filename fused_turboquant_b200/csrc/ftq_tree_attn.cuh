@@ -39,7 +39,7 @@
 // 8: 17.2 us; 32 of 8192, 16 nodes: 173 us (floor by HBM 44), where dequantising and a CTA of 128 rows of one sequence after
 // the other took 413, one CTA of specialised warps 261 to 350 (handing tiles over cost more than the work), two halves
 // that fetched and issued for themselves 205; 2 of 131072, 64 nodes, 64 heads: 884 us (622 TFLOP/s, 38 % of the measured
-// bf16 rate); 24 ragged of up to 16384, heads of 256: 99 us; 40 ragged of up to 4096, 25 nodes, 14 heads of 64 over 2: 41 us.
+// bf16 rate); 24 ragged of up to 16384, heads of 256: 99 us; 40 ragged of up to 4096, 25 nodes, 14 heads of 64 over 2: 40 us.
 //
 // Every wait is bounded.  After one has run out nothing waits any more, the half's rows become NaN and the status word says
 // so.  Block ids outside the pool are not followed: the rows that attend a token of such a page are NaN.
