@@ -165,6 +165,7 @@ struct TreePiece {
     int tile0, n_tiles;         // (n_tiles = 0: there is none any more)
     int seq, ctx;               // tokens, tokens before the tree
     float* out;                 // [N][D + 4]
+    int k_phase;                // of k_full and k_free at its first tile
 };
 
 // A load whose value is not looked at before its use: a select on it, or a conversion, would wait for memory here and now.
@@ -407,6 +408,10 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
     const uint32_t a_norm = C::A_NORM + 512 * half;
     auto stage_of = [&](int w) { return w < C::LOW_STAGES ? C::A_STAGE + w * C::STAGE : C::A_STAGE_HI + (w - C::LOW_STAGES) * C::STAGE; };
     int done = 0;       // tiles of earlier pieces: barriers have a phase for each tile
+    // ... those of the keys' codes (LATE_V) but for a piece's second tile, whose codes come with the first's, to a place of their own.
+    // (With phases that the feeder alone completes a slow warp could find two of them over, and wait for the one after.)
+    auto k_phases = [&](int n_tiles) { return C::LATE_V && n_tiles > 1 ? n_tiles - 1 : n_tiles; };
+    auto k_phase_of = [&](int tile) { return C::LATE_V && tile > 1 ? tile - 1 : tile; };      // (not of tile 1)
 
     // (In shared memory: what is needed once a piece would take the registers that the tiles need.  One thread finds a piece and
     // keeps the place behind it; the barrier at the end of a piece is behind every look at it.)
@@ -482,7 +487,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 meet_feeder();
                 const int n_tiles = pc.n_tiles;
                 if (n_tiles == 0) break;
-                const int tile0 = pc.tile0, seq = pc.seq;
+                const int tile0 = pc.tile0, seq = pc.seq, k_phase = pc.k_phase;
                 const int32_t* const btab = p.block_table + static_cast<int64_t>(pc.b) * p.max_blocks;
                 const uint8_t* const pool = p.pool + static_cast<int64_t>(pc.hkv) * C::PAGE_BYTES;
                 // block ids of four tiles' pages (idb: of the next four); -2: no tokens
@@ -541,8 +546,9 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                     __syncwarp();
                 };
                 if (C::LATE_V) {
-                    // The first two tiles' keys at once and in one phase; the second's to where the warp's first values will be.  (Values
-                    // wait in the place that they are written to as fp16: a page's 2 KB there have room for two pages' codes.)
+                    // The first two tiles' keys at once and in one phase; the second's to where the warp will write its first values, after it
+                    // has looked at them.  (Values wait in the place that they are written to as fp16: a page's 2 KB there have room
+                    // for two pages' codes.)
                     const int id0 = id_of(0, 0), id1 = id_of(1, 0);
                     if (!stalled) {
                         k_sent++;
@@ -556,28 +562,22 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                     }
                     fetch_norms(0, 0);
                     fetch_v(0, 0);
-                    if (n_tiles > 1) {
-                        copied(k_free, done);
-                        if (!stalled) {
-                            k_sent++;
-                            if (lane < 8) mbar_arrive(k_full);
-                            __syncwarp();
-                        }
-                        if (n_tiles > 2) fetch_k(2, 0);
-                        copied(k_free, done + 1);
+                    if (n_tiles > 2) {
+                        copied(k_free, k_phase);
+                        fetch_k(2, 0);
                     }
                 } else {
                     fetch_k(0, 0);
                     fetch_v(0, 0);
                     fetch_norms(0, 0);
                     if (n_tiles > 1) {
-                        copied(k_free, done);
+                        copied(k_free, k_phase);
                         fetch_k(1, 0);
                         copied(v_free, done);
                         fetch_v(1, 0);
                     }
                     if (n_tiles > 2) {
-                        copied(k_free, done + 1);
+                        copied(k_free, k_phase + 1);
                         fetch_k(2, 0);
                     }
                 }
@@ -586,7 +586,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                     copied(n_free, done + it);
                     fetch_norms(it + 1, it + 1);
                     if (it + 3 < n_tiles) {
-                        copied(k_free, done + it + 2);
+                        copied(k_free, k_phase + k_phase_of(it + 2));
                         fetch_k(it + 3, it + 1);
                     }
                     if (C::LATE_V) {
@@ -613,13 +613,17 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n");
-        if (me == 0) pos = begin;
+        if (me == 0) {
+            pos = begin;
+            pc.n_tiles = pc.k_phase = 0;
+        }
         const uint32_t stage = stage_of(warp);
 #pragma unroll 1
         while (true) {
             if (me == 0) {
                 int from = pos;
                 const TreePiece x = next_piece(from);
+                pc.k_phase = pc.k_phase + k_phases(pc.n_tiles);
                 pc.b = x.b;
                 pc.hkv = x.hkv;
                 pc.row0 = x.row0;
@@ -640,11 +644,12 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
             const int first_masked = pc.ctx / kTreeTile - pc.tile0;       // (from here on tiles reach the tree or the sequence's end)
             // keys: codes -> TMEM, rows = tokens
             auto put_k = [&](int tile, uint32_t from) {
-                copied(k_full, done + tile);
+                const bool own_phase = !C::LATE_V || tile != 1;
+                if (own_phase) copied(k_full, pc.k_phase + k_phase_of(tile));
                 typename Window<BK, false>::template Run<KW> r0, r1;
                 tree_run<KSB>(from + g8 * C::PDK, t4, r0);
                 tree_run<KSB>(from + (g8 + 8) * C::PDK, t4, r1);
-                taken(k_free);
+                if (own_phase) taken(k_free);
                 Window<BK, false>::shift(r0);
                 Window<BK, false>::shift(r1);
                 const uint32_t dst = tmem + (static_cast<uint32_t>(16 * my_page) << 16) + (tile & 1) * (D / 2);

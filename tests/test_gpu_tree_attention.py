@@ -341,3 +341,26 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="CUDA"):
         run(c.q.cpu(), bt, sl, 26, m)
     assert run(c.q[:0], bt[:0], sl[:0], 26, m[:0]).shape == (0, 6, 4, 64)
+
+
+@pytest.mark.parametrize("d,t", [(64, 8), (128, 8), (128, 40), (256, 8)])
+@pytest.mark.parametrize("tiles", [range(0, 13), range(2, 3), range(1, 2), range(5, 9)])
+def test_whole_tiles_of_ids_outside_the_pool(d, t, tiles):
+    """Shares of many tiles, of which some have no page that is there: their copies are over before they began, and no other
+    sequence sees anything of it."""
+    import torch
+    c = Case(19, d, 4, 4, 8, 2, t, [1600] * 20 + [1000] * 8)
+    good = c.run().clone()
+    assert c.pool.decode_status() == 0
+    c.table = c.table.copy()
+    lost = [3, 4, 11, 19, 27]
+    for b, bad in zip(lost, (-1, 10 ** 6, c.pool.num_blocks, -2 ** 31, 2 ** 31 - 1)):
+        for tile in tiles:
+            c.table[b, 8 * tile:8 * tile + 8] = bad
+    if tiles[0] >= 1000 // 128:
+        lost.remove(27)
+    for _ in range(5):
+        out = c.run()
+        assert c.pool.decode_status() == 1
+        for b in range(28):
+            assert out[b].isnan().all() if b in lost else torch.equal(out[b], good[b])
