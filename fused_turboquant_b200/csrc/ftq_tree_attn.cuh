@@ -490,10 +490,11 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 const int tile0 = pc.tile0, seq = pc.seq, k_phase = pc.k_phase;
                 const int32_t* const btab = p.block_table + static_cast<int64_t>(pc.b) * p.max_blocks;
                 const uint8_t* const pool = p.pool + static_cast<int64_t>(pc.hkv) * C::PAGE_BYTES;
-                // block ids of four tiles' pages (idb: of the next four); -2: no tokens
+                // block ids of four tiles' pages (idb: of the next four); -1: no tokens
+                auto has_tokens = [&](int tile) { return ((tile0 + tile) * (kTreeTile / kPageTokens) + (lane & 7)) * kPageTokens < seq; };
                 auto load_ids = [&](int tile) {
                     const int t = tile + (lane >> 3), pg = (tile0 + t) * (kTreeTile / kPageTokens) + (lane & 7);
-                    return load_id_if(t < n_tiles && pg * kPageTokens < seq, btab + pg, -2);
+                    return load_id_if(t < n_tiles && has_tokens(t), btab + pg, -1);
                 };
                 int ida = load_ids(0), idb = load_ids(4);
                 // of lane's page of a tile, while `now` is the tile that ida begins with or one of the three behind it
@@ -532,7 +533,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                             mbar_expect_tx(n_full, 32);
                             bulk_g2s(to, page_of(id) + (value ? C::OFF_VN : C::OFF_KN), 32, n_full);
                         } else {
-                            if (id != -2) {
+                            if (has_tokens(tile)) {     // (by its place, not by its id: a table may hold any)
                                 if (!value) {
                                     asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(to), "r"(0x7e007e00u) : "memory");
                                     asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(to + 16), "r"(0x7e007e00u) : "memory");

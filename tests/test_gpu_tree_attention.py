@@ -364,3 +364,20 @@ def test_whole_tiles_of_ids_outside_the_pool(d, t, tiles):
         assert c.pool.decode_status() == 1
         for b in range(28):
             assert out[b].isnan().all() if b in lost else torch.equal(out[b], good[b])
+
+
+@pytest.mark.parametrize("d,t", [(64, 8), (128, 8), (128, 40), (256, 8)])
+@pytest.mark.parametrize("bad", [-1, -2, -3, -2 ** 31, 2 ** 31 - 1])
+def test_every_id_outside_the_pool_is_told(d, t, bad):
+    import torch
+    c = Case(20, d, 4, 4, 2, 2, t, [700, 600])
+    good = c.run().clone()
+    c.table = c.table.copy()
+    for page in (0, 21, 37):
+        keep = c.table[1, page]
+        c.table[1, page] = bad
+        out = c.run()
+        assert c.pool.decode_status() == 1
+        assert out[1].isnan().all() and torch.equal(out[0], good[0])
+        c.table[1, page] = keep
+    assert torch.equal(c.run(), good) and c.pool.decode_status() == 0
