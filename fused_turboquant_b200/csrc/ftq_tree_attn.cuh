@@ -603,6 +603,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                     }
                 }
                 done += n_tiles;
+                meet_feeder();      // (after a wait that ran out the workers do not wait for what is fetched: the piece stays until it was read)
             }
             auto drain = [&](uint32_t bar, int sent) {
 #pragma unroll 1
@@ -1021,7 +1022,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 }
             }
             tc_fence_before();
-            meet();      // (the next piece writes to what these reads came from)
+            meet_feeder();      // (the next piece writes to what these reads came from)
             tc_fence_after();
         }
     }
