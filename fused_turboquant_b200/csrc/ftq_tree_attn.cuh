@@ -380,11 +380,13 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
             pc.b = lo;
             pc.hkv = u / p.row_tiles;
             pc.row0 = (u - pc.hkv * p.row_tiles) * N;
-            pc.rows = min(N, p.T * static_cast<int>(p.group.d) - pc.row0);
-            pc.tile0 = t0;
-            pc.n_tiles = t1 - t0;
             pc.seq = max(0, min(p.seq_lens[lo], p.max_seq));
             pc.ctx = pc.seq - min(p.tree_lens ? max(p.tree_lens[lo], 0) : p.T, min(p.T, pc.seq));
+            // (of the nodes that exist: what lies in the others' queries is not looked at, nor is a context that no node attends)
+            pc.rows = min(N, (pc.seq - pc.ctx) * static_cast<int>(p.group.d) - pc.row0);
+            if (pc.rows <= 0) continue;
+            pc.tile0 = t0;
+            pc.n_tiles = t1 - t0;
             pc.out = off == 0 && off_end == len ? p.whole + (static_cast<int64_t>(lo) * U + u) * N * ROW
                                                 : p.cut + (2 * static_cast<int64_t>(worker) + (off == 0 ? 1 : 0)) * N * ROW;
         }

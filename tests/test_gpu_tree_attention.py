@@ -381,3 +381,29 @@ def test_every_id_outside_the_pool_is_told(d, t, bad):
         assert out[1].isnan().all() and torch.equal(out[0], good[0])
         c.table[1, page] = keep
     assert torch.equal(c.run(), good) and c.pool.decode_status() == 0
+
+
+@pytest.mark.parametrize("fill", [0.0, 1e4, 1e30, 3e38, float("inf"), float("nan")])
+@pytest.mark.parametrize("d,hkv,group,t", [(64, 2, 7, 25), (128, 2, 4, 8), (128, 8, 4, 16), (128, 2, 4, 40), (256, 2, 2, 12)])
+def test_queries_of_missing_nodes_may_be_anything(d, hkv, group, t, fill):
+    """Their rows are zero, and the rows of the nodes that exist are what they are without them."""
+    import torch
+    lens = [t, 1, t // 2, 0, t - 1, 3]
+    c = Case(21, d, 4, 4, hkv, group, t, [300, 700, 5, 90, 128, 0], tree_lens=lens)
+    for b, n in enumerate(lens):
+        c.q[b, n:] = 0
+    want = check32(c)
+    for b, n in enumerate(lens):
+        c.q[b, n:] = fill
+    out = torch.full_like(want, 7.0)
+    c.run(out=out)
+    assert c.pool.decode_status() == 0 and torch.equal(out, want)
+
+
+def test_pages_of_a_sequence_without_nodes_are_not_looked_at():
+    import torch
+    c = Case(22, 128, 4, 4, 2, 4, 40, [300, 700, 90], tree_lens=[40, 0, 3])
+    want = c.run().clone()
+    c.table = c.table.copy()
+    c.table[1] = -1
+    assert torch.equal(c.run(), want) and c.pool.decode_status() == 0
