@@ -56,6 +56,7 @@ constexpr int kTreeTile = 128;         // tokens of a tile
 __host__ __device__ constexpr int tree_piece(int head_dim) { return head_dim == 256 ? 4 : 3; }
 constexpr int kTreeMaxSeqs = 1024;     // sequences of a launch
 constexpr float kTreeSlack = 13.f, kTreeGrowth = 4.f;
+constexpr float kTreeRounded = 1 << 20;    // (half a unit in its last place: 2^-4)
 
 struct TreeAttnParams {
     const void* q;              // [B, T, Hq, D]
@@ -108,7 +109,7 @@ struct TreeCfg {
     static constexpr int A_FIRST = A_STAGE + LOW_STAGES * STAGE, END_LOW = A_FIRST + (kTreeMaxSeqs + 1) * 4;     // [kTreeMaxSeqs + 1]
     static constexpr int A_NORM = A_STAGE_HI + (WARPS - LOW_STAGES) * STAGE;       // a half's norms: keys [128], values [128]
     static constexpr int A_MISC = A_NORM + HALVES * 512, A_BAR = A_MISC + 128, BARS = 9, A_PIECE = A_BAR + HALVES * BARS * 8;
-    static constexpr int SMEM_BYTES = A_PIECE + 128;
+    static constexpr int A_SPECIAL = A_PIECE + 128, SMEM_BYTES = A_SPECIAL + 16;        // whether S needs settle(), a word a half
     static_assert(END_LOW <= WINDOW && SMEM_BYTES <= 227 * 1024 && Q_BYTES % 1024 == 0, "");
     // TMEM columns of a half: two key buffers, S, O
     static constexpr int COLS = 512 / HALVES, COL_S = D, COL_O = D + N;
@@ -405,6 +406,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
     const uint32_t p_row = a_p + (col0 / 64) * C::P_ATOM + my_tok * 128;
     float* const s_nm = reinterpret_cast<float*>(at(C::A_ROW + half * C::ROW_BYTES));
     float *const s_lc = s_nm + N, *const s_corr = s_lc + N, *const red = s_corr + N, *const red_v = red + 4 * N;
+    volatile uint32_t* const special = reinterpret_cast<volatile uint32_t*>(at(C::A_SPECIAL)) + half;
     uint32_t* const cm = reinterpret_cast<uint32_t*>(at(C::A_MASK + half * C::MASK_BYTES));
     const uint32_t k_base = C::WINDOW + (BK == 2 ? (lane & 15) * 8 : lane * 4), v_base = C::WINDOW + 128 + (BV == 2 ? (lane & 15) * 8 : lane * 4);
     const uint32_t a_norm = C::A_NORM + 512 * half;
@@ -741,6 +743,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 top = warp_max(top);
                 if (lane == 0) red[hw] = top;
                 if (me < N) s_nm[me] = INFINITY;
+                if (me == 0) *special = 0;
                 meet();
 #pragma unroll
                 for (int w = 0; w < C::WH; w++) top = fmaxf(top, red[w]);
@@ -810,7 +813,9 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 asm volatile("ld.shared.u16 %0, [%1];\n" : "=r"(nk) : "r"(a_norm + 2 * my_tok) : "memory");
                 asm volatile("ld.shared.u16 %0, [%1];\n" : "=r"(nv) : "r"(a_norm + 256 + 2 * my_tok) : "memory");
                 taken(n_free);
-                const float kn = half_bits_to_float(nk) * q_down, vn = half_bits_to_float(nv);
+                const bool settled = *special != 0;
+                float kn = half_bits_to_float(nk) * q_down;
+                const float vn = half_bits_to_float(nv);
                 // which of the group's rows attend the token; |v| where one does and it is finite
                 uint32_t bits = 0xffffffffu;
                 if (masked) {
@@ -820,6 +825,20 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 if (CW < 32) bits &= (1u << (CW & 31)) - 1u;
                 const float av = bits != 0 && fabsf(vn) <= FLT_MAX ? fabsf(vn) : 0.f;
                 const uint32_t s_at = tl + C::COL_S + col0;
+                // Where a maximum is so large that what an fma does not round is far from zero as an exponent: S becomes the scores, rounded
+                // as they were when the maximum was taken.
+                auto settle = [&]() {
+#pragma unroll 1
+                    for (int c0 = 0; c0 < CW; c0 += 8) {
+                        uint32_t s[8];
+                        tc_load(s_at + c0, s);
+#pragma unroll
+                        for (int c = 0; c < 8; c++) s[c] = __float_as_uint(__uint_as_float(s[c]) * kn);
+                        tc_st8(s_at + c0, s);
+                    }
+                    tc_wait_st();
+                    kn = 1.f;
+                };
                 // scores - maxima (base 2)
                 auto exponents = [&](float* x) {
                     uint32_t s[CW];
@@ -861,6 +880,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                     for (int c = 0; c < CW; c++) x[c] = (bits >> c) & 1u ? x[c] : -INFINITY;
                 };
                 wait(s_done, done + it);
+                if (soft && settled) settle();
                 if (!C::LATE_V && C::VB == 2 && it > 0) wait(o_done, done + it - 1);       // (P.V of the tile before has read the weights)
                 bool above = false;
                 float x[CW];
@@ -929,10 +949,12 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                                 s_nm[col0 + lane] = -m_new;
                                 s_lc[col0 + lane] = lc;
                                 s_corr[col0 + lane] = lc * v_ratio;
+                                if (fabsf(m_new) > kTreeRounded && m_new != -INFINITY) *special = 1;
                             }
                         }
                     }
                     meet();
+                    if (soft && !settled && *special) settle();
                     if (soft) {
 #pragma unroll
                         for (int c = 0; c < CW; c += 4) {

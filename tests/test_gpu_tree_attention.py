@@ -407,3 +407,21 @@ def test_pages_of_a_sequence_without_nodes_are_not_looked_at():
     c.table = c.table.copy()
     c.table[1] = -1
     assert torch.equal(c.run(), want) and c.pool.decode_status() == 0
+
+
+@pytest.mark.parametrize("q_scale", [1e5, 1e7, 1e9, 1e15, 1e28])
+@pytest.mark.parametrize("d,t", [(64, 8), (128, 8), (128, 40), (256, 12)])
+def test_scores_of_any_size(d, t, q_scale):
+    """Scores whose unit in the last place is above one: a row is one token's value, or some with ties, and finite."""
+    import torch
+    c = Case(25, d, 4, 4, 2, 4, t, [600, 3, 2000], q_scale=q_scale)
+    c.masks[:, np.arange(t), np.arange(t)] = True
+    out = check32(c)
+    assert torch.isfinite(out).all()
+    # as in fp32 with the same operands: a weight of one for the largest score, so that no row is longer than the longest value
+    for b in range(3):
+        for h in range(2):
+            (v, vn) = c.vectors(b, h, "v")
+            top = (v.norm(dim=-1) * vn).max()
+            assert (out[b, :, 4 * h:4 * h + 4].double().norm(dim=-1) <= 1.01 * top).all()
+            assert (out[b, :, 4 * h:4 * h + 4].norm(dim=-1) > 0).all()
