@@ -20,7 +20,8 @@
 // and the sums and write the tile's weights again.  (With a slack of 3, as in the decode kernels, half of the tiles
 // did: of 32 rows there is always one that has found a larger score.)  Weights are fp16: |v| is scaled by a power of
 // two, so that the largest so far is 1 to 2, and again when one of 4 or more comes; p * |v| is then at most 2^15, and a weight of
-// 2^-14 of the largest still has all its bits.  Queries are scaled the same way.  Scores, sums and O are fp32.  Three operands are rounded to fp16, as in
+// 2^-14 of the largest still has all its bits.  Queries have a common scale, and rows that are much smaller one of their own, so that
+// no row costs another its precision.  Scores, sums and O are fp32.  Three operands are rounded to fp16, as in
 // the decode kernels, for the tensor cores' sake: rotated queries, centroids and weights; against 64 bits an output is off by 4e-4 of its
 // size, by 2e-4 if only the output were rounded to fp16, and by 1.7e-3 either way if to bf16.
 //
@@ -57,6 +58,7 @@ __host__ __device__ constexpr int tree_piece(int head_dim) { return head_dim == 
 constexpr int kTreeMaxSeqs = 1024;     // sequences of a launch
 constexpr float kTreeSlack = 13.f, kTreeGrowth = 4.f;
 constexpr float kTreeRounded = 1 << 20;    // (half a unit in its last place: 2^-4)
+constexpr int kTreeSpread = 12;
 
 struct TreeAttnParams {
     const void* q;              // [B, T, Hq, D]
@@ -109,7 +111,8 @@ struct TreeCfg {
     static constexpr int A_FIRST = A_STAGE + LOW_STAGES * STAGE, END_LOW = A_FIRST + (kTreeMaxSeqs + 1) * 4;     // [kTreeMaxSeqs + 1]
     static constexpr int A_NORM = A_STAGE_HI + (WARPS - LOW_STAGES) * STAGE;       // a half's norms: keys [128], values [128]
     static constexpr int A_MISC = A_NORM + HALVES * 512, A_BAR = A_MISC + 128, BARS = 9, A_PIECE = A_BAR + HALVES * BARS * 8;
-    static constexpr int A_SPECIAL = A_PIECE + 128, SMEM_BYTES = A_SPECIAL + 16;        // whether S needs settle(), a word a half
+    static constexpr int A_DOWN = A_PIECE + 128, DOWN_BYTES = N * 4 + 16;          // a half's scales of S, and whether it needs settle()
+    static constexpr int SMEM_BYTES = A_DOWN + HALVES * DOWN_BYTES;
     static_assert(END_LOW <= WINDOW && SMEM_BYTES <= 227 * 1024 && Q_BYTES % 1024 == 0, "");
     // TMEM columns of a half: two key buffers, S, O
     static constexpr int COLS = 512 / HALVES, COL_S = D, COL_O = D + N;
@@ -406,7 +409,8 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
     const uint32_t p_row = a_p + (col0 / 64) * C::P_ATOM + my_tok * 128;
     float* const s_nm = reinterpret_cast<float*>(at(C::A_ROW + half * C::ROW_BYTES));
     float *const s_lc = s_nm + N, *const s_corr = s_lc + N, *const red = s_corr + N, *const red_v = red + 4 * N;
-    volatile uint32_t* const special = reinterpret_cast<volatile uint32_t*>(at(C::A_SPECIAL)) + half;
+    float* const s_down = reinterpret_cast<float*>(at(C::A_DOWN + half * C::DOWN_BYTES));
+    volatile uint32_t* const special = reinterpret_cast<volatile uint32_t*>(s_down + N);
     uint32_t* const cm = reinterpret_cast<uint32_t*>(at(C::A_MASK + half * C::MASK_BYTES));
     const uint32_t k_base = C::WINDOW + (BK == 2 ? (lane & 15) * 8 : lane * 4), v_base = C::WINDOW + 128 + (BV == 2 ? (lane & 15) * 8 : lane * 4);
     const uint32_t a_norm = C::A_NORM + 512 * half;
@@ -697,7 +701,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 }
             };
             // ---- the queries: rotated, scaled, fp16, K-major with 128-byte swizzle
-            float q_down;
+            float q_down;           // of the common scale
             {
                 const int b = pc.b, hkv = pc.hkv, row0 = pc.row0, rows = pc.rows, ctx = pc.ctx;
                 constexpr int OCTETS = C::HT / 8;
@@ -728,18 +732,22 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 if (trees)
                     for (int k = me; k < (fast_div(row0 + rows - 1, p.group) - i0 + 1) * words; k += C::HT)
                         mask_words[k] = p.masks[(static_cast<int64_t>(b) * p.T + i0 + k / words) * p.W + k % words];
-                // the largest, for a common scale: |rotated| <= D * largest |q|, and that shall be below 2^15
-                float top = 0.f;
+                // the largest of each row and of all, for their scale: |rotated| <= D * largest |q|, and that shall be below 2^15
+                float row_top[NR], top = 0.f;
 #pragma unroll
-                for (int k = 0; k < NR; k++)
+                for (int k = 0; k < NR; k++) {
+                    row_top[k] = 0.f;
 #pragma unroll
                     for (int j = 0; j < D / 64; j++) {
                         float v[8];
                         widen(raw[k][j], v);
 #pragma unroll
-                        for (int c = 0; c < 8; c++) top = fabsf(v[c]) <= FLT_MAX ? fmaxf(top, fabsf(v[c])) : top;
+                        for (int c = 0; c < 8; c++) row_top[k] = fabsf(v[c]) <= FLT_MAX ? fmaxf(row_top[k], fabsf(v[c])) : row_top[k];
                     }
-                __syncwarp();
+#pragma unroll
+                    for (int x = 1; x < 8; x <<= 1) row_top[k] = fmaxf(row_top[k], __shfl_xor_sync(0xffffffffu, row_top[k], x));
+                    top = fmaxf(top, row_top[k]);
+                }
                 top = warp_max(top);
                 if (lane == 0) red[hw] = top;
                 if (me < N) s_nm[me] = INFINITY;
@@ -747,13 +755,23 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 meet();
 #pragma unroll
                 for (int w = 0; w < C::WH; w++) top = fmaxf(top, red[w]);
-                const float all = top * (fabsf(p.q_scale) * D);
-                const int e = all > 0.f ? max(-120, min(120, 14 - ilogbf(all))) : 0;
-                const float up = p.q_scale * ldexpf(1.f, e);
-                q_down = ldexpf(1.f, -e);
+                // powers of two: the exponent of a scale, and the scale
+                auto exponent = [&](float t) {
+                    const int x = (__float_as_int(t * (fabsf(p.q_scale) * D)) >> 23) - 127;      // (128: infinite, that is below 2^134)
+                    return max(-120, min(120, 14 - (x == 128 ? 134 : x)));
+                };
+                auto two_to = [](int e) { return __int_as_float((127 + e) << 23); };
+                // A common scale where it costs nothing: rows of up to 2^kTreeSpread times less than the largest keep all their bits, or
+                // lose some of 2^-15 of their size.  Smaller ones are scaled up, and their scores down again.
+                const int e = top > 0.f ? exponent(top) : 0;
+                q_down = two_to(-e);
 #pragma unroll
                 for (int k2 = 0; k2 < NR; k2++) {
                     const int r = octet + k2 * OCTETS;
+                    const int more = row_top[k2] > 0.f ? min(120, exponent(row_top[k2]) - e) : 0, own = more > kTreeSpread ? more : 0;
+                    const float up = p.q_scale * two_to(e + own);
+                    if (t8 == 0 && r < N) s_down[r] = two_to(-own);
+                    if (own > 0) *special = 1;
                     float a[E];
 #pragma unroll
                     for (int k = 0; k < D / 64; k++) {
@@ -825,15 +843,15 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
                 if (CW < 32) bits &= (1u << (CW & 31)) - 1u;
                 const float av = bits != 0 && fabsf(vn) <= FLT_MAX ? fabsf(vn) : 0.f;
                 const uint32_t s_at = tl + C::COL_S + col0;
-                // Where a maximum is so large that what an fma does not round is far from zero as an exponent: S becomes the scores, rounded
-                // as they were when the maximum was taken.
+                // Where rows have scales of their own, or a maximum is so large that what an fma does not round is far from zero as an
+                // exponent: S becomes the scores, rounded as they were when a maximum was taken.
                 auto settle = [&]() {
 #pragma unroll 1
                     for (int c0 = 0; c0 < CW; c0 += 8) {
                         uint32_t s[8];
                         tc_load(s_at + c0, s);
 #pragma unroll
-                        for (int c = 0; c < 8; c++) s[c] = __float_as_uint(__uint_as_float(s[c]) * kn);
+                        for (int c = 0; c < 8; c++) s[c] = __float_as_uint(__uint_as_float(s[c]) * s_down[col0 + c0 + c] * kn);
                         tc_st8(s_at + c0, s);
                     }
                     tc_wait_st();
