@@ -12,6 +12,9 @@ A step is what a serving engine does with a tree of drafted tokens:
     pool.tree_commit         accept a path, move its keys and values behind the context
     table.trim               give the other nodes' pages back
 
+A request that gets no pages (`granted` 0) has no tree in this step: as `tree_lens`, `granted` says so to the masks, the
+attention and the commit, and the request tries again with the next step.
+
 The model is a small random one, whose next token mostly depends on the last, and the drafts come from what followed a
 token before; with greedy decoding the answers are those of one token a step, in fewer steps.
 """
@@ -55,21 +58,25 @@ class Server:
         self.prompt_lens = torch.zeros(n_requests, **i32)
         self.repetition = torch.full((n_requests,), repetition, device="cuda")
 
-    def step(self, tokens: torch.Tensor, parents: torch.Tensor):
-        """Logits' best token after every node; keys and values of all nodes are in the cache."""
+    def step(self, tokens: torch.Tensor, parents: torch.Tensor, live: torch.Tensor | None = None):
+        """(logits' best token after every node, nodes of every request: all of them, or none where it is not live or no pages
+        are left for it).  Keys and values of the nodes are in the cache."""
         m, (R, T) = self.m, tokens.shape
         context = self.table.seq_lens.clone()
-        more = self.table.extend(torch.full((R,), T, dtype=torch.int32, device="cuda"), width=T)
-        masks, _ = tree.ancestor_masks(parents, context_lens=context)
+        want = torch.full((R,), T, dtype=torch.int32, device="cuda")
+        more = self.table.extend(want if live is None else want * live, width=T)
+        nodes = more.granted
+        masks, _ = tree.ancestor_masks(parents, nodes, context_lens=context)
         x = m.embed[tokens.long()]
         for layer in range(m.n_layers):
             q, k, v = (x @ m.qkv[layer]).view(R, T, -1, m.head_dim).split((m.hq, m.hkv, m.hkv), dim=2)
             self.pool.store(k.reshape(R * T, m.hkv, -1), v.reshape(R * T, m.hkv, -1), more.slots.view(-1), layer=layer)
-            a = self.pool.tree_attention(q.contiguous(), self.table.block_table, self.table.seq_lens, self.max_len, masks, layer=layer)
+            a = self.pool.tree_attention(q.contiguous(), self.table.block_table, self.table.seq_lens, self.max_len, masks, tree_lens=nodes,
+                                         layer=layer)
             x = x + a.reshape(R, T, -1) @ m.o[layer]
         _, best = logits.process(x @ m.head, history=self.history, history_lens=self.history_lens, prompt_lens=self.prompt_lens,
                                  repetition=self.repetition, tree_tokens=tokens, tree_masks=masks, return_logits=False)
-        return best.view(R, T)
+        return best.view(R, T), nodes
 
     def remember(self, tokens: torch.Tensor, count: torch.Tensor) -> None:
         """The first count[r] of each row's tokens go behind the request's history."""
@@ -88,7 +95,9 @@ class Server:
         # (a prompt's tokens count as prompt, not as a path: none of its nodes is in the history yet, and only the last row matters)
         self.remember(prompts, self.prompt_lens)
         lens, self.history_lens = self.history_lens, torch.zeros_like(self.history_lens)
-        best = self.step(prompts, chain)
+        best, nodes = self.step(prompts, chain)
+        if int(nodes.min()) < n:
+            raise RuntimeError("the pool has no pages for all prompts")
         self.history_lens = lens
         return best[:, -1].contiguous()
 
@@ -118,15 +127,15 @@ class Server:
         steps = 0
         while int(self.history_lens.min()) < n + n_new:
             tokens, parents = self.draft(root, depth)
-            best = self.step(tokens, parents)
-            done = self.pool.tree_commit(self.table.block_table, self.table.seq_lens, tokens, parents, best)
-            # a request that has its answer keeps its context as it is
-            live = self.history_lens < n + n_new
-            count = torch.where(live, done.n_accepted, 0)
-            self.table.trim(torch.where(live, done.seq_lens, self.table.seq_lens - tokens.shape[1]))
-            self.remember(torch.cat([root[:, None], done.tokens[:, :-1]], 1), count)
-            fresh = done.tokens.gather(1, (done.n_accepted - 1).long()[:, None])[:, 0]
-            root = torch.where(live, fresh, root)
+            # a request that has its answer, or gets no pages, has no nodes: nothing is accepted
+            best, nodes = self.step(tokens, parents, self.history_lens < n + n_new)
+            if int(nodes.max()) == 0:
+                raise RuntimeError("the pool has no pages for any request that wants one")
+            done = self.pool.tree_commit(self.table.block_table, self.table.seq_lens, tokens, parents, best, tree_lens=nodes)
+            self.remember(torch.cat([root[:, None], done.tokens[:, :-1]], 1), done.n_accepted)
+            self.table.trim(torch.where(self.history_lens < n + n_new, done.seq_lens, 0))     # (an answered request ends)
+            fresh = done.tokens.gather(1, (done.n_accepted - 1).clamp(min=0).long()[:, None])[:, 0]
+            root = torch.where(done.n_accepted > 0, fresh, root)
             steps += 1
         return self.history[:, n:n + n_new].clone(), steps
 

@@ -15,7 +15,7 @@ from . import _lib
 
 class Extension(NamedTuple):
     """What ``PageTable.extend`` gave: ``slots`` int64, ``granted`` int32 [R] (tokens, all of a request's or
-    none), ``starts`` int32 [R + 1] (place of a request's first token in the flat slot map)."""
+    none: of a drafted tree the ``tree_lens`` of the calls that follow), ``starts`` int32 [R + 1] (place of a request's first token in the flat slot map)."""
     slots: torch.Tensor
     granted: torch.Tensor
     starts: torch.Tensor

@@ -453,7 +453,8 @@ int ftq_tq_decode_layers_ws(const void *q, int q_dtype, int B, int Hq, int Hkv, 
  * (ftq_pages_extend), its keys and values stored (ftq_paged_store), every node attends the
  * context and its own ancestors (ftq_tree_masks, ftq_tree_attn), logits of all nodes
  * (ftq_logits_process), the accepted path moved behind the context (ftq_tree_commit), the
- * other pages given back (ftq_pages_trim).
+ * other pages given back (ftq_pages_trim).  A request that ftq_pages_extend refuses has no tree
+ * behind its context: its `granted` goes to the later calls as tree_lens.
  */
 
 /* Nodes of a tree, and requests of a page table, at most. */
