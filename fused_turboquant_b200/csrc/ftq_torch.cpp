@@ -873,7 +873,7 @@ PyObject* tree_commit(PyObject* const* a) {
 }
 
 // logits_process(logits, history, history_lens, prompt_lens, repetition, frequency, presence, bias_ids, bias, allowed,
-//                tree_tokens, tree_masks, out, want_out, want_best) -> (out or None, best or None)
+//                tree_tokens, tree_masks, out, want_out, want_best, workspace) -> (out or None, best or None)
 PyObject* logits_process(PyObject* const* a) {
     at::Tensor x = cuda_tensor(a[0], "logits");
     if (x.dim() != 2 && x.dim() != 3) raise(PyExc_ValueError, "logits must be [requests, vocab] or [requests, rows, vocab]");
@@ -922,7 +922,10 @@ PyObject* logits_process(PyObject* const* a) {
     void* st = stream_of(dev);
     const size_t need = want_best ? api.ftq_logits_workspace_bytes(R * T, V) : 0;
     at::Tensor ws;
-    if (need) ws = workspace(Py_None, dev, st, need);
+    if (need) {
+        ws = workspace(a[15], dev, st, need);
+        if (ws.device() != dev || !ws.is_contiguous()) raise(PyExc_ValueError, "workspace must be contiguous and on the logits' device");
+    }
     int rc;
     {
         NoGil nogil;
@@ -932,7 +935,7 @@ PyObject* logits_process(PyObject* const* a) {
                                     ptr_or_null<float>(bias), ids.defined() ? ids.size(1) : 0, ptr_or_null<int32_t>(ok),
                                     ok.defined() ? ok.size(-1) : 0, ptr_or_null<int32_t>(tt), ptr_or_null<int32_t>(tm),
                                     out.defined() ? mptr<float>(out) : nullptr, best.defined() ? mptr<int32_t>(best) : nullptr,
-                                    ws.defined() ? mptr<void>(ws) : nullptr, ws.defined() ? ws.numel() : 0, st);
+                                    ws.defined() ? mptr<void>(ws) : nullptr, ws.defined() ? ws.nbytes() : 0, st);
     }
     check(rc, "ftq_logits_process");
     Ref r0(out.defined() ? a[12] != Py_None ? Py_NewRef(a[12]) : THPVariable_Wrap(out) : Py_NewRef(Py_None));
@@ -987,7 +990,7 @@ PyMethodDef methods[] = {
     FTQ_ENTRY(tree_masks, 3),
     FTQ_ENTRY(paged_tree, 11),
     FTQ_ENTRY(tree_commit, 7),
-    FTQ_ENTRY(logits_process, 15),
+    FTQ_ENTRY(logits_process, 16),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", "Tensor-level host path over libftq_b200.so.",
                           -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -239,3 +239,53 @@ def _alias(half):
     big = torch.zeros(4, 64, device="cuda")
     half.set_(big.view(-1).view(torch.float16).untyped_storage(), 0, (4, 64))
     return big
+
+
+def test_graphs_with_scratch_of_their_own_run_side_by_side():
+    import torch
+    from fused_turboquant_b200 import logits
+    r, t, v = 4, 32, 50001
+    xs = [torch.randn(r, t, v, device="cuda", generator=torch.Generator("cuda").manual_seed(s)).bfloat16() for s in range(2)]
+    want = [logits.process(x, return_logits=False)[1] for x in xs]
+    assert logits.workspace_bytes(r * t, v) == r * t * -(-v // 2048) * 8
+    assert logits.workspace_bytes(0, v) == logits.workspace_bytes(r * t, 0) == 0
+    graphs, got, scratch = [], [], []
+    side = torch.cuda.Stream()
+    for x in xs:                                                # both captured on the same stream
+        ws = torch.full((logits.workspace_bytes(r * t, v),), 255, dtype=torch.uint8, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got.append(logits.process(x, return_logits=False, workspace=ws)[1])
+        graphs.append(graph)
+        scratch.append(ws)
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(20):
+        for best in got:
+            best.fill_(-1)
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all((ws != 255).any() for ws in scratch)
+
+
+def test_scratch_that_will_not_do():
+    import torch
+    from fused_turboquant_b200 import logits
+    x = torch.randn(4, 5000, device="cuda")
+    want = logits.process(x)
+    need = logits.workspace_bytes(4, 5000)
+    with pytest.raises(RuntimeError, match="workspace needs"):
+        logits.process(x, workspace=torch.empty(need - 1, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(RuntimeError, match="8-byte aligned"):
+        logits.process(x, workspace=torch.empty(need + 8, dtype=torch.uint8, device="cuda")[4:])
+    with pytest.raises(ValueError, match="workspace"):
+        logits.process(x, workspace=torch.empty(need, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="workspace"):
+        logits.process(x, workspace=torch.empty(2 * need, dtype=torch.uint8, device="cuda")[::2])
+    got = logits.process(x, workspace=torch.empty(need // 8, dtype=torch.int64, device="cuda"))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    none = torch.empty(0, dtype=torch.uint8, device="cuda")     # (nothing is needed without the best tokens)
+    assert torch.equal(logits.process(x, return_best=False, workspace=none)[0], want[0])
