@@ -217,7 +217,12 @@ struct Table {
 
 // Scratch of the current (device, stream), shared with the Python callers (kernels.get_workspace).
 at::Tensor workspace(PyObject* given, const at::Device& dev, void* stream, size_t need) {
-    if (given != Py_None) return tensor(given, "workspace");
+    if (given != Py_None) {
+        const at::Tensor& t = tensor(given, "workspace");
+        if (t.device() != dev || !t.is_contiguous())
+            raise(PyExc_ValueError, "workspace must be a contiguous tensor on the call's device");
+        return t;
+    }
     PyObject* key = Py_BuildValue("(iK)", static_cast<int>(dev.index()),
                                   static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(stream)));
     if (!key) throw PyError{};
@@ -922,10 +927,7 @@ PyObject* logits_process(PyObject* const* a) {
     void* st = stream_of(dev);
     const size_t need = want_best ? api.ftq_logits_workspace_bytes(R * T, V) : 0;
     at::Tensor ws;
-    if (need) {
-        ws = workspace(a[15], dev, st, need);
-        if (ws.device() != dev || !ws.is_contiguous()) raise(PyExc_ValueError, "workspace must be contiguous and on the logits' device");
-    }
+    if (need) ws = workspace(a[15], dev, st, need);
     int rc;
     {
         NoGil nogil;

@@ -454,3 +454,16 @@ def test_small_rows_beside_ordinary_ones(tiny):
     c = Case(24, 128, 4, 4, 2, 4, 16, [300, 1000])
     c.q[:, ::2] = (c.q[:, ::2].float() * tiny).to(c.q.dtype)
     check32(c)
+
+
+def test_scratch_in_other_memory_is_refused():
+    """Host memory, and every other byte of a buffer: by the attention over a tree and by the decode attention."""
+    import torch
+    c = Case(26, 64, 4, 4, 2, 2, 6, [20])
+    bt, sl, m = torch.from_numpy(c.table).cuda(), torch.tensor(c.lens, dtype=torch.int32, device="cuda"), c.words()
+    need = max(c.pool.tree_workspace_bytes(1, 6, 4, 26), c.pool.workspace_bytes(1, 4, 26, 1))
+    for ws in (torch.empty(need, dtype=torch.uint8), torch.empty(2 * need, dtype=torch.uint8, device="cuda")[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            c.pool.tree_attention(c.q, bt, sl, 26, m, workspace=ws)
+        with pytest.raises(ValueError, match="workspace"):
+            c.pool.decode_attention(c.q[:, 0].contiguous(), bt, sl, 26, layer=0, workspace=ws)
