@@ -800,6 +800,7 @@ PyObject* paged_tree(PyObject* const* a) {
     PyObject* self = a[0];
     at::Tensor q = cuda_tensor(a[1], "q");
     if (!q.is_contiguous()) q = q.contiguous();
+    else if (reinterpret_cast<uintptr_t>(q.data_ptr()) % 16) q = q.clone();     // (a part of a larger tensor, at an odd place)
     const Pool p(self);
     if (q.dim() != 4 || q.size(3) != p.d) raise(PyExc_ValueError, "q must be [B, n_nodes, Hq, " + std::to_string(p.d) + "]");
     if (dtype_code(q.scalar_type()) < 0) raise(PyExc_ValueError, "q must be fp16 or bf16");

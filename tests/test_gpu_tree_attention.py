@@ -467,3 +467,15 @@ def test_scratch_in_other_memory_is_refused():
             c.pool.tree_attention(c.q, bt, sl, 26, m, workspace=ws)
         with pytest.raises(ValueError, match="workspace"):
             c.pool.decode_attention(c.q[:, 0].contiguous(), bt, sl, 26, layer=0, workspace=ws)
+
+
+@pytest.mark.parametrize("offset", [1, 2, 4, 7])
+def test_queries_at_any_place_of_a_larger_tensor(offset):
+    import torch
+    c = Case(27, 128, 4, 4, 2, 4, 9, [250, 400])
+    want = c.run().clone()
+    big = torch.zeros(c.q.numel() + offset, dtype=c.q.dtype, device="cuda")
+    big[offset:] = c.q.reshape(-1)
+    c.q = big[offset:].view(c.q.shape)
+    assert c.q.is_contiguous() and c.q.data_ptr() % 16 != 0
+    assert torch.equal(c.run(), want)
