@@ -22,20 +22,21 @@ constexpr int kPagesThreads = 512, kPagesCluster = 8;
 
 
 // Exclusive scan over the CTA's threads, and the sum of all.
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, int64_t* warp_sums, T& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x = v;
+    T x = v;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, d);
+        const T y = __shfl_up_sync(0xffffffffu, x, d);
         if (lane >= d) x += y;
     }
     __syncthreads();        // (the sums of the scan before have been read)
     if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
-    int before = 0, all = 0;
+    T before = 0, all = 0;
     for (int w = 0; w < kPagesThreads / 32; w++) {
-        const int s = warp_sums[w];
+        const T s = static_cast<T>(warp_sums[w]);
         before += w < warp ? s : 0;
         all += s;
     }
@@ -66,7 +67,7 @@ __device__ __forceinline__ void cluster_barrier(int ctas) {
 
 __global__ void __launch_bounds__(kPagesThreads) pages_extend_kernel(const PagesParams p) {
     extern __shared__ int s_requests[];
-    __shared__ int warp_sums[kPagesThreads / 32];
+    __shared__ int64_t warp_sums[kPagesThreads / 32];
     __shared__ int s_taken;
     int* const s_off = s_requests;                 // blocks wanted by the requests before
     int* const s_len = s_requests + p.R;           // tokens so far
@@ -78,18 +79,21 @@ __global__ void __launch_bounds__(kPagesThreads) pages_extend_kernel(const Pages
     const int room = kPageTokens * p.max_blocks;
     const int avail = min(max(*p.n_free, 0), p.num_blocks);
     if (tid == 0) s_taken = 0;
-    int base_off = 0, base_start = 0;
+    int base_off = 0;
+    int64_t base_start = 0;     // (of refused requests too, and those may have asked for anything)
     for (int r0 = 0; r0 < p.R; r0 += kPagesThreads) {
         const int r = r0 + tid;
         const bool live = r < p.R;
         const int n = live ? min(max(p.lens[r], 0), room) : 0, m = live ? p.arg[r] : 0;
-        int start = 0, total;
+        int64_t start = 0;
         if (p.packed) {
-            start = base_start + block_scan(max(m, 0), warp_sums, total);
-            base_start += total;
+            int64_t sum;
+            start = base_start + block_scan<int64_t>(max(m, 0), warp_sums, sum);
+            base_start += sum;
         }
         const bool fits = live && m >= 0 && m <= room - n && m <= p.width - start;
         const int want = fits ? pages_of(n + m) - pages_of(n) : 0;
+        int total;
         const int off = base_off + block_scan(want, warp_sums, total);
         base_off += total;
         const bool ok = fits && (want == 0 || off + want <= avail);
@@ -97,7 +101,7 @@ __global__ void __launch_bounds__(kPagesThreads) pages_extend_kernel(const Pages
             s_off[r] = off;
             s_len[r] = n;
             s_get[r] = ok ? m : -1;
-            if (p.packed) s_start[r] = start;
+            if (p.packed) s_start[r] = static_cast<int>(min(start, static_cast<int64_t>(INT32_MAX)));
             if (ok && want > 0) atomicMax(&s_taken, off + want);
         }
     }
@@ -129,7 +133,7 @@ __global__ void __launch_bounds__(kPagesThreads) pages_extend_kernel(const Pages
     if (cta == 0) {
         for (int r = tid; r <= p.R; r += kPagesThreads) {
             if (r < p.R) p.granted[r] = max(s_get[r], 0);
-            p.starts[r] = !p.packed ? r * p.width : r < p.R ? s_start[r] : base_start;
+            p.starts[r] = !p.packed ? r * p.width : r < p.R ? s_start[r] : static_cast<int>(min(base_start, static_cast<int64_t>(INT32_MAX)));
         }
     }
     cluster_barrier(ctas);
@@ -141,7 +145,7 @@ __global__ void __launch_bounds__(kPagesThreads) pages_extend_kernel(const Pages
 
 __global__ void __launch_bounds__(kPagesThreads) pages_trim_kernel(const PagesParams p) {
     extern __shared__ int s_requests[];
-    __shared__ int warp_sums[kPagesThreads / 32];
+    __shared__ int64_t warp_sums[kPagesThreads / 32];
     int* const s_off = s_requests;                 // blocks given back by the requests before
     int* const s_keep = s_requests + p.R;          // tokens that stay
     const int tid = threadIdx.x, cta = blockIdx.x, ctas = gridDim.x;

@@ -163,3 +163,18 @@ def test_refusals():
     with pytest.raises(ValueError, match="int32"):
         table.trim(torch.zeros(2, dtype=torch.int32, device="cuda"))
     assert PageTable(4, 0, 4).extend(torch.zeros(0, device="cuda"), 3).slots.shape == (0, 3)
+
+
+@pytest.mark.parametrize("new,width", [
+    ([2 ** 31 - 1, 2 ** 31 - 1, 5], 64), ([5, 2 ** 31 - 1, 7, 3], 64), ([2 ** 30, 2 ** 30, 2 ** 30, 2 ** 30, 3, 0], 1000),
+    ([2 ** 31 - 1, 1, 1, 2 ** 31 - 2, 0, 9, -2 ** 31, 4], 40), ([3, 2 ** 31 - 1, -5, 2] + [2 ** 29] * 600 + [4, 0, 6], 30)])
+def test_packed_lengths_whose_sum_passes_32_bits(new, width):
+    """Requests behind the end of the slot map get nothing, however far behind it they are."""
+    import torch
+    from fused_turboquant_b200 import PageTable
+    table, plain = PageTable(200, len(new), 4), Plain(200, len(new), 4)
+    got = table.extend(torch.tensor(new, dtype=torch.int32, device="cuda"), width, packed=True)
+    slots, granted, starts = plain.extend(new, width, True)
+    assert got.granted.tolist() == granted and np.array_equal(got.slots.cpu().numpy(), slots)
+    assert got.starts.tolist() == [min(s, 2 ** 31 - 1) for s in starts]
+    same(table, plain)
