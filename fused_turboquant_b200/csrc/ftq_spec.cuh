@@ -130,15 +130,14 @@ __global__ void __launch_bounds__(kPagesThreads) pages_extend_kernel(const Pages
         }
         p.slots[i] = slot;
     }
-    if (cta == 0) {
-        for (int r = tid; r <= p.R; r += kPagesThreads) {
-            if (r < p.R) p.granted[r] = max(s_get[r], 0);
-            p.starts[r] = !p.packed ? r * p.width : r < p.R ? s_start[r] : static_cast<int>(min(base_start, static_cast<int64_t>(INT32_MAX)));
-        }
-    }
     cluster_barrier(ctas);
-    if (cta == 0) {
-        for (int r = tid; r < p.R; r += kPagesThreads) p.lens[r] = s_len[r] + max(s_get[r], 0);
+    if (cta == 0) {     // (granted and starts may lie where the other CTAs found new_lens)
+        for (int r = tid; r <= p.R; r += kPagesThreads) {
+            p.starts[r] = !p.packed ? r * p.width : r < p.R ? s_start[r] : static_cast<int>(min(base_start, static_cast<int64_t>(INT32_MAX)));
+            if (r == p.R) continue;
+            p.granted[r] = max(s_get[r], 0);
+            p.lens[r] = s_len[r] + max(s_get[r], 0);
+        }
         if (tid == 0) *p.n_free = avail - taken;
     }
 }

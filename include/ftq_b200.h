@@ -473,7 +473,7 @@ int ftq_tq_decode_layers_ws(const void *q, int q_dtype, int B, int Hq, int Hkv, 
  * needs any.  Written: granted [R]; starts [R + 1]; slots (block * 16 + offset, -1 where
  * there is no token): [R, width], starts[r] = r * width, or, packed, [width] with the
  * requests' tokens back to back (starts: the running sum of new_lens, negative ones as 0, at
- * most INT32_MAX).
+ * most INT32_MAX).  granted may be new_lens itself.
  *
  * ftq_pages_trim: request r keeps its first keep_lens[r] tokens (at most what it has; 0 ends
  * it); blocks without a token go back to the stack and their table entries become -1.

@@ -178,3 +178,26 @@ def test_packed_lengths_whose_sum_passes_32_bits(new, width):
     assert got.granted.tolist() == granted and np.array_equal(got.slots.cpu().numpy(), slots)
     assert got.starts.tolist() == [min(s, 2 ** 31 - 1) for s in starts]
     same(table, plain)
+
+
+@pytest.mark.parametrize("requests,width,packed", [(8192, 40, False), (8192, 200000, True), (5, 7, False)])
+def test_granted_in_the_place_of_the_new_lengths(requests, width, packed):
+    """C ABI: the numbers granted replace those that were asked for (many CTAs read them)."""
+    import ctypes
+    import torch
+    from fused_turboquant_b200 import PageTable, _lib
+    lib, p = _lib.load(), lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    rng = np.random.default_rng(requests)
+    new = torch.tensor(rng.integers(-2, 45, requests), dtype=torch.int32, device="cuda")
+    for _ in range(10):
+        one, two = PageTable(12000, requests, 3), PageTable(12000, requests, 3)
+        want = one.extend(new, width, packed)
+        both = new.clone()
+        slots = torch.zeros(want.slots.shape, dtype=torch.int64, device="cuda")
+        starts = torch.zeros(requests + 1, dtype=torch.int32, device="cuda")
+        rc = lib.ftq_pages_extend(p(two.block_table), p(two.seq_lens), p(two.free_blocks), p(two.n_free), requests, 3, 12000, p(both), width,
+                                  int(packed), p(slots), p(both), p(starts), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        assert rc == 0
+        assert torch.equal(both, want.granted) and torch.equal(slots, want.slots) and torch.equal(starts, want.starts)
+        for k, v in one.state_dict().items():
+            assert torch.equal(v, two.state_dict()[k]), k
