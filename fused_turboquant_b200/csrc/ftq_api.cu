@@ -10,6 +10,7 @@
 #include <atomic>
 #include <cstdint>
 #include <cstring>
+#include <utility>
 #include <random>
 #include <cstdlib>
 #include <mutex>
@@ -1642,10 +1643,14 @@ extern "C" int ftq_tree_commit(uint8_t* pool, int64_t num_blocks, int64_t pool_l
     if (!pool || !block_table || !seq_lens || !tokens || !parents || !next_tokens || !path || !n_accepted || !out_tokens || !new_lens)
         return fail(FTQ_ERR_INVALID, "ftq_tree_commit: NULL pointer");
     if (!aligned(pool, 16) || pool_layer_stride % 16) return fail(FTQ_ERR_INVALID, "pool must be 16-byte aligned");
-    const size_t row = static_cast<size_t>(B) * 4;
-    if (overlap(new_lens, row, seq_lens, row) || (tree_lens && (overlap(new_lens, row, tree_lens, row) || overlap(n_accepted, row, tree_lens, row))) ||
-        overlap(n_accepted, row, seq_lens, row))
-        return fail(FTQ_ERR_INVALID, "ftq_tree_commit: the new lengths need memory of their own");
+    // (other CTAs read the inputs while one writes)
+    const size_t row = static_cast<size_t>(B) * 4, all = row * n_nodes;
+    const std::pair<const void*, size_t> ins[] = {{seq_lens, row}, {tree_lens, row}, {tokens, all}, {parents, all}, {next_tokens, all}, {block_table, row * max_blocks}},
+                                         outs[] = {{new_lens, row}, {n_accepted, row}, {path, all}, {out_tokens, all}};
+    for (const auto& o : outs)
+        for (const auto& i : ins)
+            if (i.first && overlap(o.first, o.second, i.first, i.second))
+                return fail(FTQ_ERR_INVALID, "ftq_tree_commit: path, tokens, counts and new lengths need memory of their own");
     ftq::CommitParams p{};
     p.block_table = block_table; p.seq_lens = seq_lens; p.tree_lens = tree_lens;
     p.tokens = tokens; p.parents = parents; p.next = next_tokens;

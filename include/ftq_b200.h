@@ -525,8 +525,8 @@ int ftq_tree_attn(const void *q, int q_dtype, void *out, int out_dtype, const ui
  * [B, n_nodes] (accepted nodes, then -1), n_accepted [B], out_tokens [B, n_nodes] (next_tokens
  * along the path, then -1: the step's new tokens), new_lens [B] = context + n_accepted.  The
  * compressed keys and values of path[k] move to position context + k in all layers of the pool;
- * what lies behind new_lens is unspecified.  A block id out of range is not followed.  new_lens
- * and n_accepted may not lie on seq_lens or tree_lens.
+ * what lies behind new_lens is unspecified.  A block id out of range is not followed.  What is
+ * written may not lie on what is read.
  */
 int ftq_tree_commit(uint8_t *pool, int64_t num_blocks, int64_t pool_layer_stride, int n_layers,
                     const int32_t *block_table, int max_blocks, const int32_t *seq_lens,

@@ -121,3 +121,16 @@ def test_workspace_sizes(lib):
     assert lib.ftq_tree_workspace_bytes(2, 8, 8, 3, 128, 64) == 0
     a, b = (lib.ftq_tree_workspace_bytes(n, 8, 32, 8, 128, 4096) for n in (1, 64))
     assert 0 < a < b
+
+
+@pytest.mark.parametrize("out", ["path", "n_accepted", "out_tokens", "new_lens"])
+@pytest.mark.parametrize("read", ["seq_lens", "tree_lens", "tokens", "parents", "next_tokens", "block_table"])
+def test_what_a_commit_writes_lies_apart_from_what_it_reads(lib, out, read):
+    """Every output on every input, from the first byte on and at its last; the rest of the call is sound."""
+    size = dict(seq_lens=8, tree_lens=8, tokens=64, parents=64, next_tokens=64, block_table=32, path=64, n_accepted=8, out_tokens=64, new_lens=8)
+    good = dict(COMMIT, tree_lens=1, **{})
+    for i, name in enumerate(size):
+        good[name] = (A << 4) + 4096 * i
+    for at in (0, size[read] - 4, 4 - size[out]):
+        rc, message = call(lib, "ftq_tree_commit", dict(good, **{out: good[read] + at}))
+        assert rc == INVALID and "memory of their own" in message
