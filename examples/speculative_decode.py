@@ -16,7 +16,8 @@ A request that gets no pages (`granted` 0) has no tree in this step: as `tree_le
 attention and the commit, and the request tries again with the next step.
 
 The model is a small random one, whose next token mostly depends on the last, and the drafts come from what followed a
-token before; with greedy decoding the answers are those of one token a step, in fewer steps.
+token before.  Decoding is greedy, so that the answers are those of one token a step, in fewer steps, but for near ties: products of
+another shape add up in another order, and a token whose logit is within rounding of the best may take its place.
 """
 import argparse
 import time

@@ -113,3 +113,37 @@ def test_the_documented_step_with_a_refused_request():
     assert table.seq_lens.tolist() == [ctx[0] + 5, ctx[1]]
     pages = held[r, :-(-ctx[r] // 16)].long()
     assert torch.equal(table.block_table[r], held[r]) and torch.equal(pool.pool[:, pages], before[:, pages])
+
+
+@pytest.mark.parametrize("requests,prompt,depth", [(1, 5, 3), (3, 40, 1), (6, 129, 7)])
+def test_every_token_of_an_answer_is_the_best_one(example, monkeypatch, requests, prompt, depth):
+    """An answer with trees, fed to the model token by token: each of its tokens has the largest logit there, or one within rounding.
+
+    A rounding to bf16 is off by up to 2^-9 of its size, and where sums come in another order it may fall the other way, by 2^-8.  The
+    queries, values, attention and sums of two layers and the embedding's path make 8 such places; each moves a logit, a sum over
+    independent coordinates, by 2^-8 of the logits' own spread at most, so that together it is sqrt(8) * 2^-8 of it in the mean and
+    never four times that for two logits, sqrt(2) more.  The logits' own rounding adds 2^-8 of the largest on either side.
+    """
+    import torch
+    model, n_new = example.Model(seed=prompt), 60
+    prompts = torch.randint(model.vocab, (requests, prompt), dtype=torch.int32, device="cuda", generator=torch.Generator("cuda").manual_seed(depth))
+    answer, _ = example.Server(model, requests, prompt + n_new).generate(prompts, n_new, depth)
+    process, seen = example.logits.process, []
+
+    def keeping(x, **kw):
+        out, best = process(x, **dict(kw, return_logits=True))
+        seen.append((out[:, -1], x[:, -1].float()))
+        return out, best
+
+    monkeypatch.setattr(example.logits, "process", keeping)
+    server = example.Server(model, requests, prompt + n_new)
+    root = torch.full((requests, 1), -1, dtype=torch.int32, device="cuda")
+    server.prefill(prompts)
+    for k in range(n_new):
+        y, raw = seen[-1]
+        token = answer[:, k:k + 1]
+        short = y.amax(1) - y.gather(1, token.long())[:, 0]
+        limit = 4 * 2 ** 0.5 * 8 ** 0.5 * 2.0 ** -8 * raw.std(1) + 2 * 2.0 ** -8 * raw.abs().amax(1)
+        assert (short <= limit).all(), (k, short.tolist(), limit.tolist())
+        server.step(token.contiguous(), root)
+        server.remember(token, torch.ones(requests, dtype=torch.int32, device="cuda"))
