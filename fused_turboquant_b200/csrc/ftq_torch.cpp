@@ -695,6 +695,11 @@ at::Tensor state_i32(PyObject* o, const char* name) {
         raise(PyExc_ValueError, std::string(name) + " must be a contiguous int32 tensor");
     return t;
 }
+// Numbers of tokens: one that 32 bits do not hold is the largest or smallest that they do (more than there is room for, or none).
+at::Tensor counts_i32(PyObject* o, const char* name, const at::Device& dev) {
+    const at::Tensor& t = tensor(o, name);
+    return t.scalar_type() == at::kLong ? t.to(dev).clamp(INT32_MIN, INT32_MAX).to(at::kInt).contiguous() : as_i32(o, name, dev);
+}
 at::Tensor maybe_i32(PyObject* o, const char* name, const at::Device& dev) {
     return o == Py_None ? at::Tensor() : as_i32(o, name, dev);
 }
@@ -730,7 +735,7 @@ struct Pages {   // what a PageTable holds
 PyObject* pages_extend(PyObject* const* a) {
     const Pages p(a);
     const at::Device dev = p.table.device();
-    const at::Tensor m = as_i32(a[4], "new_lens", dev);
+    const at::Tensor m = counts_i32(a[4], "new_lens", dev);
     const long long width = as_int(a[5]), R = p.table.size(0);
     const bool packed = as_bool(a[6]);
     want_shape(m, {R}, "new_lens");
@@ -759,7 +764,7 @@ PyObject* pages_extend(PyObject* const* a) {
 PyObject* pages_trim(PyObject* const* a) {
     const Pages p(a);
     const at::Device dev = p.table.device();
-    const at::Tensor keep = as_i32(a[4], "keep_lens", dev);
+    const at::Tensor keep = counts_i32(a[4], "keep_lens", dev);
     want_shape(keep, {p.table.size(0)}, "keep_lens");
     const c10::cuda::CUDAGuard guard(dev);
     void* st = stream_of(dev);

@@ -201,3 +201,20 @@ def test_granted_in_the_place_of_the_new_lengths(requests, width, packed):
         assert torch.equal(both, want.granted) and torch.equal(slots, want.slots) and torch.equal(starts, want.starts)
         for k, v in one.state_dict().items():
             assert torch.equal(v, two.state_dict()[k]), k
+
+
+def test_numbers_of_tokens_beyond_32_bits():
+    """int64 numbers: none of them wraps to a small one, or to none."""
+    import torch
+    from fused_turboquant_b200 import PageTable
+    table = PageTable(40, 4, 8)
+    big = torch.tensor([20, 2 ** 32 + 5, 2 ** 62, -2 ** 32 + 7], device="cuda")
+    got = table.extend(big, 30)
+    assert got.granted.tolist() == [20, 0, 0, 0] and table.seq_lens.tolist() == [20, 0, 0, 0]
+    table.extend(torch.tensor([0, 9, 30, 17], device="cuda"), 30)
+    before = {k: v.clone() for k, v in table.state_dict().items()}
+    table.trim(torch.tensor([2 ** 32, 2 ** 62, 2 ** 31, 2 ** 63 - 1], device="cuda"))          # all that they have
+    for k, v in table.state_dict().items():
+        assert torch.equal(v, before[k]), k
+    table.trim(torch.tensor([-2 ** 32 + 3, 4, 0, -2 ** 62], device="cuda"))
+    assert table.seq_lens.tolist() == [0, 4, 0, 0] and int(table.n_free) == 39
