@@ -14,11 +14,13 @@
 // [requests, vocabulary] count exists in memory.
 //
 // A row's 2 bytes in, 4 out and a bit of mask per token are 63 us of HBM for 32 requests of 16 nodes, 131072 tokens, 8192 of
-// history and 100 biases; it takes 126 us (3.25 TB/s): the issue slots of a warp's 256 tokens (masks, maxima, listed tokens) and
-// the starts of the CTAs, in which the history is read.  152 us had the eight tokens of a thread adjusted where they lie (a division
-// for one or two lanes at a time), the index of the largest carried from token to token and two barriers a row.  Segments of
-// 4096 tokens, CTAs of 512: 130 us.  The row on its way and 48 registers (five CTAs an SM) go together: without the one 154 us,
-// with 40 or 32 registers, which spill, 175 and 193; four tokens and four more a lane, for whole sectors in a store, 147.
+// history and 100 biases; it takes 127 us (3.25 TB/s).  68 % of the issue slots are in use (240 instructions for a warp's 256 tokens of a
+// row: masks, maxima, listed tokens); the longest stalls are loads from global memory (one row is on its way), then the barriers between
+// rows, whose counts change, and 2.8 rounds of CTAs begin with the history.  152 us had the eight tokens of a thread adjusted where
+// they lie (a division for one or two lanes at a time), the index of the largest carried from token to token and two barriers a
+// row.  Segments of 4096 tokens, CTAs of 512: 130 us.  The row on its way and 48 registers (five CTAs an SM; fp32 logits spill eight
+// words) go together: without the one 154 us, with 40 or 32 registers, which spill more, 175 and 193; four tokens and four more a
+// lane, for whole sectors in a store, 147.
 #pragma once
 
 #include "ftq_serve_launch.h"

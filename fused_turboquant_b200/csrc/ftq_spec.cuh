@@ -1,8 +1,9 @@
 // Speculative serving around the paged cache: pages of the requests, ancestor masks of drafted token trees, and the
 // move of the accepted tokens' compressed keys and values.  Integers and bytes only.  All of it is bound by latency
 // (launch, dependent loads, the walk down a tree), so every operator is one launch and keeps its state on the device.
-// Measured: giving back, taking and the masks together 15.5 us, for one request of 8 nodes as for 256 of 16 or whole prompts of new
-// ones; accepting and moving 8.6 us for one request of 32 layers, 11.4 us for 32 (0.6 us of HBM).
+// Measured: giving back, taking and the masks together 16.5 us, for one request of 8 nodes as for 256 of 16 or whole prompts of new
+// ones, which is what three calls from Python take: in a graph 5.8, 10.2 and 15.2 us.  Accepting and moving 9.0 us for one request of 32
+// layers (in a graph 4.8), 11.4 us for 32 (0.6 us of HBM).
 #pragma once
 
 #include "ftq_serve_launch.h"

@@ -20,7 +20,8 @@
 // and the sums and write the tile's weights again.  (With a slack of 3, as in the decode kernels, half of the tiles
 // did: of 32 rows there is always one that has found a larger score.)  Weights are fp16: |v| is scaled by a power of
 // two, so that the largest so far is 1 to 2, and again when one of 4 or more comes; p * |v| is then at most 2^15, and a weight of
-// 2^-14 of the largest still has all its bits.  Queries have a common scale, and rows that are much smaller one of their own, so that
+// 2^-14 of the largest still has all its bits (a row that attends none but values 2^14 times shorter than the longest that its column
+// group has met loses some).  Queries have a common scale, and rows that are much smaller one of their own, so that
 // no row costs another its precision.  Scores, sums and O are fp32.  Three operands are rounded to fp16, as in
 // the decode kernels, for the tensor cores' sake: rotated queries, centroids and weights; against 64 bits an output is off by 4e-4 of its
 // size, by 2e-4 if only the output were rounded to fp16, and by 1.7e-3 either way if to bf16.
@@ -34,13 +35,13 @@
 // CTA to itself: its rows share what was dequantised, and eight warps have the keys, eight the values.  Every piece leaves its rows
 // (O, m, l) in the workspace; tree_merge_kernel joins the pieces of a unit, rotates back and stores.
 //
-// Bound: instruction issue and the latency of the chain of a tile, about 6000 cycles for a half, of which the look-ups (a
-// 16-bit pair of codes a 4-byte load), the softmax and the waits for shared memory in between are most; the tensor cores are
-// busy 15 to 35 % of the time, HBM 3 to 25 %.  Measured (K4V4, bf16): one sequence of 900 tokens, 8 nodes, 32 heads of 128 over
-// 8: 17.2 us; 32 of 8192, 16 nodes: 173 us (floor by HBM 44), where dequantising and a CTA of 128 rows of one sequence after
+// Bound: the latency of the chain of a tile, about 6000 cycles for a half: look-ups (a 16-bit pair of codes a 4-byte load), softmax,
+// and the waits for shared memory and at barriers between them.  No unit is full: issue slots 38 (heads of 256) to 50 %, tensor cores
+// 11 to 24 %, HBM 2 to 25 %; barriers and shared memory are the longest stalls.  Measured (K4V4, bf16): one sequence of 900 tokens,
+// 8 nodes, 32 heads of 128 over 8: 17.5 us; 32 of 8192, 16 nodes: 175 us (floor by HBM 44), where dequantising and a CTA of 128 rows of one sequence after
 // the other took 413, one CTA of specialised warps 261 to 350 (handing tiles over cost more than the work), two halves
-// that fetched and issued for themselves 205; 2 of 131072, 64 nodes, 64 heads: 884 us (622 TFLOP/s, 38 % of the measured
-// bf16 rate); 24 ragged of up to 16384, heads of 256: 99 us; 40 ragged of up to 4096, 25 nodes, 14 heads of 64 over 2: 40 us.
+// that fetched and issued for themselves 205; 2 of 131072, 64 nodes, 64 heads: 893 us (616 TFLOP/s, 38 % of the measured
+// bf16 rate); 24 ragged of up to 16384, heads of 256: 99 us; 40 ragged of up to 4096, 25 nodes, 14 heads of 64 over 2: 41 us.
 //
 // Every wait is bounded.  After one has run out nothing waits any more, the half's rows become NaN and the status word says
 // so.  Block ids outside the pool are not followed: the rows that attend a token of such a page are NaN.
@@ -53,11 +54,14 @@ namespace ftq {
 
 constexpr int kTreeTile = 128;         // tokens of a tile
 // Places that a unit costs besides its tiles: its queries, its first maxima and its rows take as long as so many tiles.  (24 ragged
-// sequences with heads of 256: 2, 3, 4, 6 places 124, 111, 99, 102 us; 40 with heads of 64: 42, 41, 43, 46 us.)
+// sequences with heads of 256: 2, 3, 4, 6 places 124, 111, 99, 102 us; 40 with heads of 64: 42, 41, 43, 46 us.  Heads of 128, 2, 3, 4
+// places: 40 ragged of up to 4096 51, 52, 53 us; 8 of 2048 28, 27, 28; 64 ragged of up to 500, 25 nodes, 59, 67, 69; 32 of 8192 all 175.)
 __host__ __device__ constexpr int tree_piece(int head_dim) { return head_dim == 256 ? 4 : 3; }
 constexpr int kTreeMaxSeqs = 1024;     // sequences of a launch
 constexpr float kTreeSlack = 13.f, kTreeGrowth = 4.f;
 constexpr float kTreeRounded = 1 << 20;    // (half a unit in its last place: 2^-4)
+// Rows that differ by less have a common scale.  (Were every row given its own, a tile's scores would all be scaled back: 32 sequences of
+// 8192 tokens, 16 nodes of ordinary queries 191 us instead of 175.)
 constexpr int kTreeSpread = 12;
 
 struct TreeAttnParams {
@@ -205,8 +209,6 @@ __device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t* r) {
                  "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 
-// SB bytes of codes into words (zeros if not ok), on the widest loads that their alignment allows: a run starts at a multiple
-// of its size.  Loads into the very registers that the values stay in: what is loaded to one and moved to another is
 // Run number `t` (SB bytes) of a row of codes in shared memory, codes from bit 0 on (rows start on 4 bytes).
 template <int SB, class Run>
 __device__ __forceinline__ void tree_run(uint32_t row, int t, Run& run) {
@@ -427,7 +429,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnParams p) {
     volatile TreePiece& pc = *reinterpret_cast<volatile TreePiece*>(at(C::A_PIECE + 64 * half));
     volatile int& pos = *reinterpret_cast<volatile int*>(at(C::A_PIECE + 64 * half + 56));
     // Registers: the workers get some of what the last four warps do not need, 512 x 104 + 128 x 64 of the 640 x 96 of the launch.
-    // (Products of 64 rows spilled in every tile: 180 -> 173 us for 32 sequences of 8192 tokens and 16 nodes.)
+    // (Products of 64 rows spilled in every tile: 180 -> 173 us for 32 sequences of 8192 tokens and 16 nodes, before scales of rows.)
     static_assert(C::THREADS == 640 && 512 * 104 + 128 * 64 <= 640 * 96, "");
     __syncwarp();
     if (helper) {

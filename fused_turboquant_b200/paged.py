@@ -207,7 +207,9 @@ class PagedKVPool:
         q: [B, n_nodes, Hq, D], fp16 or bf16, not rotated; seq_lens [B] count the tree's ``tree_lens[b]`` (all of them
         without it) nodes.  Node i attends the context and the nodes whose bits are set in ``masks[b, i]`` (int32 words as
         ``tree.ancestor_masks`` makes them; any masks will do).  Rows that attend nothing and nodes that do not exist are zero;
-        the queries of nodes that do not exist may hold anything.  No host synchronisation; graph-capturable when out / workspace are passed in.  ``decode_status`` covers this call too.
+        the queries of nodes that do not exist may hold anything.  A sequence without a tree (``PageTable.extend`` granted it
+        nothing) has a ``tree_lens`` of 0.  No host synchronisation; graph-capturable when out / workspace are passed in.
+        ``decode_status`` covers this call too.
         """
         _require_cuda(q, "q")
         if _trace.ENABLED:

@@ -504,8 +504,8 @@ int ftq_tree_masks(const int32_t *parents, const int32_t *tree_lens, const int32
  * nodes.  Node i attends every token of the context and the nodes j (of those that exist) whose bit
  * j % 32 is set in word j / 32 of masks[b][i] (ftq_tree_masks makes them; any others will do, a node's own
  * bit included or not).  Rows that attend nothing, and nodes that do not exist, are zero; what lies
- * in the queries of the latter does not matter.  The other arguments are those of ftq_paged_decode_attn.  The workspace holds at least
- * ftq_tree_workspace_bytes(...) bytes, 16-byte aligned; the call's status is read with
+ * in the queries of the latter does not matter.  The other arguments are those of
+ * ftq_paged_decode_attn.  The workspace holds at least ftq_tree_workspace_bytes(...) bytes, 16-byte aligned; the call's status is read with
  * ftq_paged_decode_status(workspace, 1, Hq, Hkv, head_dim, max_seq_len, 1, ...).
  */
 size_t ftq_tree_workspace_bytes(int B, int n_nodes, int Hq, int Hkv, int head_dim, int max_seq_len);
