@@ -12,6 +12,6 @@ from .quantizer import CompressedTensor, TurboQuantMSE  # noqa: F401
 from .paged import PagedKVPool  # noqa: F401
 from .page_table import PageTable  # noqa: F401
 from . import kernels  # noqa: F401
-from . import hf_cache, logits, tq_v1, tree  # noqa: F401
+from . import beam, hf_cache, logits, tq_v1, tree  # noqa: F401
 
 __version__ = "0.1.0"

@@ -73,6 +73,14 @@ SIGNATURES = {
     "ftq_logits_workspace_bytes": (_sz, [_i64, _i]),
     "ftq_logits_process": (_i, [_vp, _i, _i64, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp,
                                 _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ftq_beam_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "ftq_beam_select": (_i, [_vp, _i, _i64, _i, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ftq_pages_fork_workspace_bytes": (_sz, [_i, _i, _i]),
+    "ftq_pages_fork": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ftq_pages_compact_workspace_bytes": (_sz, [_i]),
+    "ftq_pages_compact": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _sz, _vp]),
+    "ftq_pages_shared_lens": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp]),
+    "ftq_copy_pages": (_i, [_vp, _i64, _i64, _i, _i, _i, _i, _i, _vp, _i, _vp]),
 }
 
 _lib = None

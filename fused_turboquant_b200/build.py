@@ -57,6 +57,7 @@ for _d in (256, 128, 64):
     UNITS.append(("ftq_attn_chunk_inst.cu", f"attn_chunk_d{_d}", [f"-DFTQ_D={_d}"]))
     UNITS.append(("ftq_encode_inst.cu", f"encode_d{_d}", [f"-DFTQ_D={_d}"]))
 UNITS.append(("ftq_serve_inst.cu", "serve", []))
+UNITS.append(("ftq_beam_inst.cu", "beam", []))
 UNITS.append(("ftq_api.cu", "api", []))
 
 

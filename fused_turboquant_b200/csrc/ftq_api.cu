@@ -16,6 +16,7 @@
 #include <mutex>
 
 #include "../../include/ftq_b200.h"
+#include "ftq_beam_launch.h"
 #include "ftq_dense.cuh"
 #include "ftq_launch.h"
 #include "ftq_serve_launch.h"
@@ -1817,4 +1818,179 @@ extern "C" int ftq_tree_attn(const void* q, int q_dtype, void* out, int out_dtyp
         if (e != cudaSuccess) return cuda_fail(e, "ftq_tree_attn merge launch");
     }
     return FTQ_OK;
+}
+
+// ------------------------------------------------------------------ beam search and parallel sampling
+
+static_assert(FTQ_BEAM_MAX == ftq::kBeamMax && FTQ_BEAM_MAX_ENDS == ftq::kBeamMaxEnds, "header and kernels agree on the limits");
+
+namespace {
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+int check_workspace(const void* workspace, size_t bytes, size_t need) {
+    if (!workspace || bytes < need) return fail(FTQ_ERR_WORKSPACE, "workspace needs %zu bytes, got %zu", need, bytes);
+    if (!aligned(workspace, 16)) return fail(FTQ_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+    return FTQ_OK;
+}
+
+// whether one of the written ranges lies on one that is read, or on another written one
+int check_apart(const char* what, const std::pair<const void*, size_t>* outs, int n_outs, const std::pair<const void*, size_t>* ins, int n_ins) {
+    for (int o = 0; o < n_outs; o++) {
+        for (int i = 0; i < n_ins; i++)
+            if (ins[i].first && outs[o].first && overlap(outs[o].first, outs[o].second, ins[i].first, ins[i].second))
+                return fail(FTQ_ERR_INVALID, "%s: what is written needs memory of its own", what);
+        for (int k = 0; k < o; k++)
+            if (outs[k].first && outs[o].first && overlap(outs[o].first, outs[o].second, outs[k].first, outs[k].second))
+                return fail(FTQ_ERR_INVALID, "%s: what is written needs memory of its own", what);
+    }
+    return FTQ_OK;
+}
+}  // namespace
+
+extern "C" size_t ftq_pages_fork_workspace_bytes(int n_requests, int max_blocks, int num_blocks) {
+    if (n_requests <= 0 || max_blocks <= 0 || num_blocks < 0) return 0;
+    return round256(static_cast<size_t>(n_requests) * max_blocks * 4) + round256((ftq::kForkWarps + 1) * 4) +
+           round256(static_cast<size_t>(n_requests) * 4) + 2 * round256(static_cast<size_t>(num_blocks) * 4);
+}
+
+extern "C" int ftq_pages_fork(int32_t* block_table, int32_t* seq_lens, int32_t* free_blocks, int32_t* n_free, int32_t* shares,
+                              int n_requests, int max_blocks, int num_blocks, const int32_t* parents, int group,
+                              const int32_t* keep_lens, int32_t* copies, int32_t* done, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+    const ftq::PagesParams pages{block_table, seq_lens, free_blocks, n_free, parents, n_requests, max_blocks, num_blocks,
+                                 nullptr, nullptr, nullptr, 0, false};
+    int rc = check_pages(pages, "ftq_pages_fork");
+    if (rc) return rc;
+    if (group < 0 || (group > 0 && n_requests % group != 0))
+        return fail(FTQ_ERR_INVALID, "ftq_pages_fork: %d requests in groups of %d", n_requests, group);
+    if (static_cast<int64_t>(n_requests) * max_blocks >= INT32_MAX)
+        return fail(FTQ_ERR_UNSUPPORTED, "ftq_pages_fork: a table of %d requests of %d blocks is too large", n_requests, max_blocks);
+    if (n_requests == 0) return FTQ_OK;
+    if (!copies || !done || (num_blocks > 0 && !shares)) return fail(FTQ_ERR_INVALID, "ftq_pages_fork: NULL pointer");
+    const size_t R = n_requests, row = R * 4, all = row * max_blocks, nb = static_cast<size_t>(num_blocks) * 4,
+                 need = ftq_pages_fork_workspace_bytes(n_requests, max_blocks, num_blocks);
+    rc = check_workspace(workspace, workspace_bytes, need);
+    if (rc) return rc;
+    const std::pair<const void*, size_t> outs[] = {{copies, 2 * row}, {done, 4}, {workspace, need}},
+                                         ins[] = {{block_table, all}, {seq_lens, row}, {free_blocks, nb}, {n_free, 4}, {shares, nb}, {parents, row}, {keep_lens, row}};
+    rc = check_apart("ftq_pages_fork", outs, 3, ins, 7);
+    if (rc) return rc;
+    ftq::ForkParams p{};
+    p.table = block_table; p.lens = seq_lens; p.free_blocks = free_blocks; p.n_free = n_free; p.shares = shares;
+    p.parents = parents; p.keep = keep_lens; p.R = n_requests; p.max_blocks = max_blocks; p.num_blocks = num_blocks; p.group = group;
+    p.copies = copies; p.done = done;
+    uint8_t* at = static_cast<uint8_t*>(workspace);
+    auto take = [&](size_t n) { int32_t* x = reinterpret_cast<int32_t*>(at); at += round256(n); return x; };
+    p.next = take(all);
+    p.counts = take((ftq::kForkWarps + 1) * 4);
+    p.ranks = take(row);
+    p.part_count = take(nb);
+    p.part_first = take(nb);
+    const cudaError_t e = ftq::launch_pages_fork(p, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FTQ_OK : cuda_fail(e, "ftq_pages_fork launch");
+}
+
+extern "C" size_t ftq_pages_compact_workspace_bytes(int num_blocks) {
+    return num_blocks <= 0 ? 0 : round256(static_cast<size_t>(num_blocks) * 4) + 256;
+}
+
+extern "C" int ftq_pages_compact(int32_t* block_table, int32_t* seq_lens, int32_t* free_blocks, int32_t* n_free, int32_t* shares,
+                                 int n_requests, int max_blocks, int num_blocks, int32_t* copies, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+    const ftq::PagesParams pages{block_table, seq_lens, free_blocks, n_free, seq_lens, n_requests, max_blocks, num_blocks,
+                                 nullptr, nullptr, nullptr, 0, false};
+    int rc = check_pages(pages, "ftq_pages_compact");
+    if (rc) return rc;
+    if (num_blocks == 0) return FTQ_OK;
+    if (!free_blocks || !n_free || (num_blocks > 1 && !copies)) return fail(FTQ_ERR_INVALID, "ftq_pages_compact: NULL pointer");
+    if (!aligned(copies, 8)) return fail(FTQ_ERR_INVALID, "ftq_pages_compact: copies must be 8-byte aligned");
+    const size_t row = static_cast<size_t>(n_requests) * 4, nb = static_cast<size_t>(num_blocks) * 4, need = ftq_pages_compact_workspace_bytes(num_blocks);
+    rc = check_workspace(workspace, workspace_bytes, need);
+    if (rc) return rc;
+    const std::pair<const void*, size_t> outs[] = {{copies, nb / 8 * 8}, {workspace, need}},
+                                         ins[] = {{block_table, row * max_blocks}, {seq_lens, row}, {free_blocks, nb}, {n_free, 4}, {shares, nb}};
+    rc = check_apart("ftq_pages_compact", outs, 2, ins, 5);
+    if (rc) return rc;
+    ftq::CompactParams p{};
+    p.table = block_table; p.lens = seq_lens; p.free_blocks = free_blocks; p.n_free = n_free; p.shares = shares;
+    p.R = n_requests; p.max_blocks = max_blocks; p.num_blocks = num_blocks; p.copies = copies;
+    p.map = static_cast<int32_t*>(workspace);
+    p.counts = p.map + round256(nb) / 4;
+    const cudaError_t e = ftq::launch_pages_compact(p, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FTQ_OK : cuda_fail(e, "ftq_pages_compact launch");
+}
+
+extern "C" int ftq_pages_shared_lens(const int32_t* block_table, const int32_t* seq_lens, int n_groups, int group, int max_blocks,
+                                     int32_t* shared_lens, void* stream) {
+    if (n_groups < 0 || group <= 0 || max_blocks <= 0 || max_blocks > (1 << 26) || static_cast<int64_t>(n_groups) * group > INT32_MAX)
+        return fail(FTQ_ERR_INVALID, "ftq_pages_shared_lens: bad shape groups=%d group=%d max_blocks=%d", n_groups, group, max_blocks);
+    if (n_groups == 0) return FTQ_OK;
+    if (!block_table || !seq_lens || !shared_lens) return fail(FTQ_ERR_INVALID, "ftq_pages_shared_lens: NULL pointer");
+    const size_t row = static_cast<size_t>(n_groups) * group * 4;
+    const std::pair<const void*, size_t> outs[] = {{shared_lens, static_cast<size_t>(n_groups) * 4}}, ins[] = {{block_table, row * max_blocks}, {seq_lens, row}};
+    const int rc = check_apart("ftq_pages_shared_lens", outs, 1, ins, 2);
+    if (rc) return rc;
+    const cudaError_t e = ftq::launch_shared_lens({block_table, seq_lens, shared_lens, n_groups, group, max_blocks}, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FTQ_OK : cuda_fail(e, "ftq_pages_shared_lens launch");
+}
+
+extern "C" int ftq_copy_pages(uint8_t* pool, int64_t num_blocks, int64_t pool_layer_stride, int n_layers, int Hkv, int head_dim,
+                              int bits_k, int bits_v, const int32_t* copies, int n_copies, void* stream) {
+    if (!dim_ok(head_dim)) return fail(FTQ_ERR_UNSUPPORTED, "head_dim %d (need 64/128/256)", head_dim);
+    if (!bits_ok(bits_k) || !bits_ok(bits_v))
+        return fail(FTQ_ERR_INVALID, "bits must be 2, 3, or 4, got K=%d V=%d", bits_k, bits_v);
+    if (num_blocks < 0 || n_layers < 0 || Hkv <= 0 || Hkv > 65535 || n_copies < 0)
+        return fail(FTQ_ERR_INVALID, "ftq_copy_pages: bad shape Hkv=%d layers=%d copies=%d", Hkv, n_layers, n_copies);
+    if (n_layers > 65535) return fail(FTQ_ERR_UNSUPPORTED, "at most 65535 layers");
+    if (n_copies == 0 || n_layers == 0 || num_blocks == 0) return FTQ_OK;
+    if (!pool || !copies) return fail(FTQ_ERR_INVALID, "ftq_copy_pages: NULL pointer");
+    if (!aligned(pool, 16) || pool_layer_stride % 16) return fail(FTQ_ERR_INVALID, "pool must be 16-byte aligned");
+    const cudaError_t e = ftq::launch_copy_pages({pool, copies, pool_layer_stride, Hkv * ftq_page_bytes(head_dim, bits_k, bits_v), num_blocks,
+                                                  n_copies, n_layers}, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FTQ_OK : cuda_fail(e, "ftq_copy_pages launch");
+}
+
+extern "C" size_t ftq_beam_workspace_bytes(int dtype, int n_requests, int beams, int vocab, int n_best, int n_ends) {
+    if (!dtype_ok(dtype) || n_requests <= 0 || beams <= 0 || beams > FTQ_BEAM_MAX || vocab <= 0 || n_best <= 0 || n_best > FTQ_BEAM_MAX ||
+        n_ends < 0 || n_ends > FTQ_BEAM_MAX_ENDS) return 0;
+    const ftq::SelectPlan plan = ftq::select_plan(dtype, n_requests, beams, vocab, n_best + n_ends);
+    const size_t parts = static_cast<size_t>(n_requests) * beams * plan.chunks;
+    return round256(parts * sizeof(float2)) + parts * (n_best + n_ends) * 8;
+}
+
+extern "C" int ftq_beam_select(const void* logits, int dtype, int64_t row_stride, int n_requests, int beams, int vocab,
+                               const float* scores, const int32_t* end_tokens, int n_ends, int n_best, float* out_scores,
+                               int32_t* parents, int32_t* tokens, float* end_scores, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+    if (!dtype_ok(dtype)) return fail(FTQ_ERR_INVALID, "dtype %d", dtype);
+    if (beams <= 0 || beams > FTQ_BEAM_MAX || n_best <= 0 || n_best > FTQ_BEAM_MAX)
+        return fail(FTQ_ERR_UNSUPPORTED, "1 to %d beams and continuations, got %d and %d", FTQ_BEAM_MAX, beams, n_best);
+    if (n_ends < 0 || n_ends > FTQ_BEAM_MAX_ENDS)
+        return fail(FTQ_ERR_UNSUPPORTED, "up to %d tokens that end an answer, got %d", FTQ_BEAM_MAX_ENDS, n_ends);
+    if (n_requests < 0 || vocab <= 0 || row_stride < vocab)
+        return fail(FTQ_ERR_INVALID, "ftq_beam_select: bad shape requests=%d vocab=%d row_stride=%lld", n_requests, vocab,
+                    static_cast<long long>(row_stride));
+    if (n_requests > 65535) return fail(FTQ_ERR_UNSUPPORTED, "at most 65535 requests");
+    if (n_requests == 0) return FTQ_OK;
+    if (!logits || !scores || !out_scores || !parents || !tokens || (n_ends > 0 && (!end_tokens || !end_scores)))
+        return fail(FTQ_ERR_INVALID, "ftq_beam_select: NULL pointer");
+    const size_t es = dtype_size(dtype), rows = static_cast<size_t>(n_requests) * beams, best = static_cast<size_t>(n_requests) * n_best * 4;
+    if (!aligned(logits, es)) return fail(FTQ_ERR_INVALID, "ftq_beam_select: logits lie between two values' places");
+    const size_t need = ftq_beam_workspace_bytes(dtype, n_requests, beams, vocab, n_best, n_ends);
+    int rc = check_workspace(workspace, workspace_bytes, need);
+    if (rc) return rc;
+    const std::pair<const void*, size_t> outs[] = {{out_scores, best}, {parents, best}, {tokens, best}, {n_ends ? end_scores : nullptr, rows * n_ends * 4}, {workspace, need}},
+                                         ins[] = {{logits, ((rows - 1) * row_stride + vocab) * es}, {scores, rows * 4}, {n_ends ? end_tokens : nullptr, n_ends * size_t{4}}};
+    rc = check_apart("ftq_beam_select", outs, 5, ins, 3);
+    if (rc) return rc;
+    ftq::SelectParams p{};
+    const ftq::SelectPlan plan = ftq::select_plan(dtype, n_requests, beams, vocab, n_best + n_ends);
+    p.logits = logits; p.row_stride = row_stride; p.scores = scores; p.ends = end_tokens;
+    p.out_scores = out_scores; p.parents = parents; p.tokens = tokens; p.end_scores = end_scores;
+    p.sums = static_cast<float2*>(workspace);
+    p.keys = reinterpret_cast<unsigned long long*>(static_cast<uint8_t*>(workspace) + round256(rows * plan.chunks * sizeof(float2)));
+    p.R = n_requests; p.K = beams; p.V = vocab; p.n = n_best; p.n_ends = n_ends; p.keep = n_best + n_ends;
+    p.chunks = plan.chunks; p.chunk = plan.chunk;
+    const cudaError_t e = ftq::launch_select(dtype, p, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FTQ_OK : cuda_fail(e, "ftq_beam_select launch");
 }

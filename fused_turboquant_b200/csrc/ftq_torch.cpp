@@ -36,7 +36,9 @@ namespace {
     X(ftq_tq_decode_layers_ws) X(ftq_tq_decode_layers_workspace_bytes) X(ftq_paged_chunk_workspace_bytes) X(ftq_paged_chunk_attn) \
     X(ftq_pages_extend) X(ftq_pages_trim) X(ftq_tree_masks) X(ftq_tree_commit)             \
     X(ftq_tree_workspace_bytes) X(ftq_tree_attn)                                           \
-    X(ftq_logits_workspace_bytes) X(ftq_logits_process)
+    X(ftq_logits_workspace_bytes) X(ftq_logits_process)                                    \
+    X(ftq_beam_workspace_bytes) X(ftq_beam_select) X(ftq_pages_fork_workspace_bytes) X(ftq_pages_fork) \
+    X(ftq_pages_compact_workspace_bytes) X(ftq_pages_compact) X(ftq_pages_shared_lens) X(ftq_copy_pages)
 struct Api {
 #define X(name) decltype(&::name) name = nullptr;
     FTQ_BOUND(X)
@@ -951,6 +953,154 @@ PyObject* logits_process(PyObject* const* a) {
     return PyTuple_Pack(2, r0.o, r1.o);
 }
 
+// ------------------------------------------------------------------ beam search and parallel sampling
+// Scratch that a call without any is not asked for.
+at::Tensor maybe_workspace(PyObject* given, const at::Device& dev, void* stream, size_t need) {
+    return need || given != Py_None ? workspace(given, dev, stream, need) : at::Tensor();
+}
+void* ws_ptr(const at::Tensor& ws) { return ws.defined() ? mptr<void>(ws) : nullptr; }
+size_t ws_bytes(const at::Tensor& ws) { return ws.defined() ? ws.nbytes() : 0; }
+
+at::Tensor shares_of(PyObject* o, const Pages& p) {
+    const at::Tensor t = state_i32(o, "shares");
+    if (t.device() != p.table.device()) raise(PyExc_ValueError, "a page table lies on one device");
+    want_shape(t, {p.free_blocks.size(0)}, "shares");
+    return t;
+}
+
+// pages_fork(block_table, seq_lens, free_blocks, n_free, shares, parents, keep_lens, workspace) -> (copies, done)
+PyObject* pages_fork(PyObject* const* a) {
+    const Pages p(a);
+    const at::Device dev = p.table.device();
+    const at::Tensor shares = shares_of(a[4], p), par = counts_i32(a[5], "parents", dev);
+    const at::Tensor keep = a[6] == Py_None ? at::Tensor() : counts_i32(a[6], "keep_lens", dev);
+    const int64_t R = p.table.size(0), W = p.table.size(1), nb = p.free_blocks.size(0);
+    if ((par.dim() != 1 && par.dim() != 2) || par.numel() != R)
+        raise(PyExc_ValueError, "parents must be [" + std::to_string(R) + "], or [groups, rows of a group] of as many rows");
+    if (keep.defined() && keep.numel() != R) raise(PyExc_ValueError, "keep_lens must have " + std::to_string(R) + " entries");
+    const int64_t group = par.dim() == 2 && R > 0 ? par.size(1) : 0;
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor copies = empty({R, 2}, at::kInt, dev), done = empty({1}, at::kInt, dev);
+    if (R == 0) done.fill_(1);
+    void* st = stream_of(dev);
+    const at::Tensor ws = maybe_workspace(a[7], dev, st, api.ftq_pages_fork_workspace_bytes(R, W, nb));
+    int rc;
+    {
+        NoGil nogil;
+        rc = api.ftq_pages_fork(mptr<int32_t>(p.table), mptr<int32_t>(p.lens), mptr<int32_t>(p.free_blocks), mptr<int32_t>(p.n_free),
+                                mptr<int32_t>(shares), R, W, nb, ptr<int32_t>(par), group, ptr_or_null<int32_t>(keep),
+                                mptr<int32_t>(copies), mptr<int32_t>(done), ws_ptr(ws), ws_bytes(ws), st);
+    }
+    check(rc, "ftq_pages_fork");
+    Ref r0(THPVariable_Wrap(copies)), r1(THPVariable_Wrap(done));
+    return PyTuple_Pack(2, r0.o, r1.o);
+}
+
+// pages_compact(block_table, seq_lens, free_blocks, n_free, shares or None, workspace) -> copies
+PyObject* pages_compact(PyObject* const* a) {
+    const Pages p(a);
+    const at::Device dev = p.table.device();
+    const at::Tensor shares = a[4] == Py_None ? at::Tensor() : shares_of(a[4], p);
+    const int64_t nb = p.free_blocks.size(0);
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor copies = empty({nb / 2, 2}, at::kInt, dev);
+    void* st = stream_of(dev);
+    const at::Tensor ws = maybe_workspace(a[5], dev, st, api.ftq_pages_compact_workspace_bytes(nb));
+    int rc;
+    {
+        NoGil nogil;
+        rc = api.ftq_pages_compact(mptr<int32_t>(p.table), mptr<int32_t>(p.lens), mptr<int32_t>(p.free_blocks), mptr<int32_t>(p.n_free),
+                                   shares.defined() ? mptr<int32_t>(shares) : nullptr, p.table.size(0), p.table.size(1), nb,
+                                   mptr<int32_t>(copies), ws_ptr(ws), ws_bytes(ws), st);
+    }
+    check(rc, "ftq_pages_compact");
+    return THPVariable_Wrap(copies);
+}
+
+// pages_shared_lens(block_table, seq_lens, group) -> lens
+PyObject* pages_shared_lens(PyObject* const* a) {
+    const at::Device dev = cuda_tensor(a[0], "block_table").device();
+    const at::Tensor bt = as_i32(a[0], "block_table", dev), sl = as_i32(a[1], "seq_lens", dev);
+    const long long group = as_int(a[2]);
+    if (bt.dim() != 2) raise(PyExc_ValueError, "block_table must be [B, max_blocks]");
+    const int64_t B = bt.size(0);
+    want_shape(sl, {B}, "seq_lens");
+    if (group < 1 || B % group != 0) raise(PyExc_ValueError, std::to_string(B) + " rows are no groups of " + std::to_string(group));
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor out = empty({B / group}, at::kInt, dev);
+    void* st = stream_of(dev);
+    int rc;
+    {
+        NoGil nogil;
+        rc = api.ftq_pages_shared_lens(ptr<int32_t>(bt), ptr<int32_t>(sl), B / group, B == 0 ? 1 : group, bt.size(1), mptr<int32_t>(out), st);
+    }
+    check(rc, "ftq_pages_shared_lens");
+    return THPVariable_Wrap(out);
+}
+
+// copy_pages(pool, copies)
+PyObject* copy_pages(PyObject* const* a) {
+    const Pool p(a[0]);
+    const at::Device dev = p.pool.device();
+    const at::Tensor c = as_i32(a[1], "copies", dev);
+    if (c.dim() != 2 || c.size(1) != 2) raise(PyExc_ValueError, "copies must be [n, 2]");
+    if (c.size(0) > INT32_MAX) raise(PyExc_ValueError, "too many copies");
+    const c10::cuda::CUDAGuard guard(dev);
+    void* st = stream_of(dev);
+    int rc;
+    {
+        NoGil nogil;
+        rc = api.ftq_copy_pages(mptr(p.pool), p.num_blocks, p.layer_stride, p.n_layers, p.hkv, p.d, p.kb, p.vb, ptr<int32_t>(c), c.size(0), st);
+    }
+    check(rc, "ftq_copy_pages");
+    Py_RETURN_NONE;
+}
+
+// beam_select(logits, scores, n_best, end_tokens, workspace) -> (scores, parents, tokens, end_scores or None)
+PyObject* beam_select(PyObject* const* a) {
+    at::Tensor x = cuda_tensor(a[0], "logits");
+    if (x.dim() != 3) raise(PyExc_ValueError, "logits must be [requests, beams, vocab]");
+    if (dtype_code(x.scalar_type()) < 0) raise(PyExc_ValueError, "logits must be fp32, fp16 or bf16");
+    const at::Device dev = x.device();
+    const int64_t R = x.size(0), K = x.size(1), V = x.size(2);
+    // rows may lie any distance apart, if it is the same between all of them
+    int64_t row_stride = K > 1 ? x.stride(1) : R > 1 ? x.stride(0) : V;
+    if (x.is_contiguous()) {
+        row_stride = V;
+    } else if (V <= 1 || x.stride(-1) != 1 || row_stride < V || (R > 1 && x.stride(0) != K * row_stride)) {
+        x = x.contiguous();
+        row_stride = V;
+    }
+    const at::Tensor scores = maybe_f32(a[1], "scores", dev), ends = a[3] == Py_None ? at::Tensor() : counts_i32(a[3], "end_tokens", dev);
+    if (!scores.defined()) raise(PyExc_TypeError, "scores must be a tensor");
+    want_shape(scores, {R, K}, "scores");
+    if (ends.defined() && ends.dim() != 1) raise(PyExc_ValueError, "end_tokens must be [n]");
+    const long long n = as_int(a[2]);
+    if (n < 1 || n > FTQ_BEAM_MAX || K < 1 || K > FTQ_BEAM_MAX)
+        raise(PyExc_ValueError, "1 to " + std::to_string(FTQ_BEAM_MAX) + " beams and continuations, got " + std::to_string(K) + " and " + std::to_string(n));
+    if (V < 1 || V > INT32_MAX || R > INT32_MAX) raise(PyExc_ValueError, "logits must be [requests, beams, vocab] with a vocabulary");
+    const int64_t E = ends.defined() ? ends.size(0) : 0;
+    if (E > FTQ_BEAM_MAX_ENDS) raise(PyExc_ValueError, "up to " + std::to_string(FTQ_BEAM_MAX_ENDS) + " end_tokens, got " + std::to_string(E));
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor best = empty({R, n}, at::kFloat, dev), parents = empty({R, n}, at::kInt, dev), tokens = empty({R, n}, at::kInt, dev);
+    at::Tensor end_scores;
+    if (ends.defined()) end_scores = empty({R, K, E}, at::kFloat, dev);
+    void* st = stream_of(dev);
+    const int dt = dtype_code(x.scalar_type());
+    const at::Tensor ws = maybe_workspace(a[4], dev, st, api.ftq_beam_workspace_bytes(dt, R, K, V, n, E));
+    int rc;
+    {
+        NoGil nogil;
+        rc = api.ftq_beam_select(ptr<void>(x), dt, row_stride, R, K, V, ptr<float>(scores), E ? ptr<int32_t>(ends) : nullptr, E, n,
+                                 mptr<float>(best), mptr<int32_t>(parents), mptr<int32_t>(tokens), E ? mptr<float>(end_scores) : nullptr,
+                                 ws_ptr(ws), ws_bytes(ws), st);
+    }
+    check(rc, "ftq_beam_select");
+    Ref r0(THPVariable_Wrap(best)), r1(THPVariable_Wrap(parents)), r2(THPVariable_Wrap(tokens)),
+        r3(end_scores.defined() ? THPVariable_Wrap(end_scores) : Py_NewRef(Py_None));
+    return PyTuple_Pack(4, r0.o, r1.o, r2.o, r3.o);
+}
+
 // bind({name: address}, check, get_workspace, workspaces, host_table)
 PyObject* bind(PyObject* const* a) {
 #define X(name)                                                                     \
@@ -999,6 +1149,11 @@ PyMethodDef methods[] = {
     FTQ_ENTRY(paged_tree, 11),
     FTQ_ENTRY(tree_commit, 7),
     FTQ_ENTRY(logits_process, 16),
+    FTQ_ENTRY(pages_fork, 8),
+    FTQ_ENTRY(pages_compact, 6),
+    FTQ_ENTRY(pages_shared_lens, 3),
+    FTQ_ENTRY(copy_pages, 2),
+    FTQ_ENTRY(beam_select, 5),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", "Tensor-level host path over libftq_b200.so.",
                           -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -230,6 +230,13 @@ class PagedKVPool:
         _require_cuda(self.pool, "pool")
         return Accepted(*_lib.native().tree_commit(self, block_table, seq_lens, tokens, parents, next_tokens, tree_lens))
 
+    def copy_pages(self, copies: torch.Tensor) -> None:
+        """Block ``copies[i, 0]`` over block ``copies[i, 1]``, in all layers (copies int32 [n, 2], as ``PageTable.fork`` and
+        ``PageTable.compact`` list them; a pair with an id outside the pool is passed over).  No block may be written that
+        another pair names.  No host synchronisation."""
+        _require_cuda(self.pool, "pool")
+        _lib.native().copy_pages(self, copies)
+
 
 def synthetic_decode_batch(block_table: torch.Tensor, seq_lens: torch.Tensor, q_len: int):
     """Per-query block tables and lengths that turn a causal multi-query step into decode steps."""

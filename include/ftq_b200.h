@@ -561,6 +561,79 @@ int ftq_logits_process(const void *logits, int dtype, int64_t row_stride, int n_
                        const int32_t *tree_masks, float *out, int32_t *best, void *workspace,
                        size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------ beam search and parallel sampling */
+
+/*
+ * No counterpart in the reference.  Several candidate answers (beams, samples) of a prompt are rows
+ * of one block table that hold the prompt's blocks together.  A step: the best continuations of
+ * every request's beams (ftq_beam_select), rows that become copies of those they go on from
+ * (ftq_pages_fork, ftq_copy_pages), room for the next token (ftq_pages_extend), its keys and values
+ * stored (ftq_paged_store), attention that reads common blocks once (ftq_pages_shared_lens,
+ * ftq_shared_attn).
+ */
+
+/* Beams of a request and continuations selected for it, and tokens that end an answer, at most. */
+#define FTQ_BEAM_MAX 64
+#define FTQ_BEAM_MAX_ENDS 16
+
+/*
+ * Selection.  logits: n_requests x beams rows of `vocab` values of `dtype`, row_stride elements
+ * apart; scores [n_requests, beams]: what the beams score so far (-inf: not alive; its logits do
+ * not matter then).  total(b, v) = scores[b] + logits[b][v] - log(sum exp(logits[b])).  Written, of
+ * every request: the n_best largest totals of all beams and of all tokens but end_tokens [n_ends],
+ * in order, of equal ones the lowest beam's lowest token first: out_scores, parents (the beam, 0
+ * to beams - 1), tokens, all [n_requests, n_best]; and end_scores [n_requests, beams, n_ends], the
+ * totals of the end tokens (-inf for one outside the vocabulary).  A total of -inf is none: where
+ * fewer are left, -inf, -1, -1.  A beam whose logits are no distribution (a NaN, +inf, nothing but
+ * -inf) has none.  Totals are compared in 64 bits and rounded once.
+ */
+size_t ftq_beam_workspace_bytes(int dtype, int n_requests, int beams, int vocab, int n_best, int n_ends);
+int ftq_beam_select(const void *logits, int dtype, int64_t row_stride, int n_requests, int beams,
+                    int vocab, const float *scores, const int32_t *end_tokens, int n_ends, int n_best,
+                    float *out_scores, int32_t *parents, int32_t *tokens, float *end_scores,
+                    void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * A table (see ftq_pages_extend, which takes such a one as any other) whose rows may hold the
+ * same block: shares [num_blocks] counts the rows that hold a block besides the first one (0 for a
+ * block that one row holds, and for a free one).  A row's partly filled last block is never shared.
+ * ftq_pages_trim is for tables without common blocks.
+ *
+ * ftq_pages_fork: all rows at once, row r becomes the first keep_lens[r] (NULL: all; negative: 0)
+ * tokens of what row parents[r] was: the row r / group * group + parents[r] for parents[r] in
+ * [0, group), or (group = 0) the row parents[r]; any other parent ends the row.  Blocks that no
+ * row holds any more go back to the stack (the first of them, by row and place, on top).  Of the
+ * rows whose partly filled last block would be the same one the first keeps it, unless it is a
+ * whole block of another row; each of the others, in order, takes one from the stack instead, and
+ * (from, to) is listed in copies [n_requests, 2], behind the last of which lies -1: ftq_copy_pages
+ * copies them.  *done = 1; or 0, and nothing has changed, where the stack has too few.
+ *
+ * ftq_pages_compact: blocks in use (those that are not on the stack) beyond the first num_blocks -
+ * *n_free move into the holes before, the lowest into the lowest; copies [num_blocks / 2, 2] as
+ * above.  The stack then has the last *n_free blocks, the lowest on top.  shares may be NULL for a
+ * table without common blocks.
+ *
+ * ftq_pages_shared_lens: of every `group` successive rows, the tokens in leading blocks that are
+ * whole and the same in all of them that have tokens (0 where none has).
+ *
+ * ftq_copy_pages: block copies[i][0] over block copies[i][1], in all layers; a pair with an id
+ * outside the pool is passed over.  No block may be written that another pair names.
+ */
+size_t ftq_pages_fork_workspace_bytes(int n_requests, int max_blocks, int num_blocks);
+int ftq_pages_fork(int32_t *block_table, int32_t *seq_lens, int32_t *free_blocks, int32_t *n_free,
+                   int32_t *shares, int n_requests, int max_blocks, int num_blocks,
+                   const int32_t *parents, int group, const int32_t *keep_lens, int32_t *copies,
+                   int32_t *done, void *workspace, size_t workspace_bytes, void *stream);
+size_t ftq_pages_compact_workspace_bytes(int num_blocks);
+int ftq_pages_compact(int32_t *block_table, int32_t *seq_lens, int32_t *free_blocks, int32_t *n_free,
+                      int32_t *shares, int n_requests, int max_blocks, int num_blocks,
+                      int32_t *copies, void *workspace, size_t workspace_bytes, void *stream);
+int ftq_pages_shared_lens(const int32_t *block_table, const int32_t *seq_lens, int n_groups, int group,
+                          int max_blocks, int32_t *shared_lens, void *stream);
+int ftq_copy_pages(uint8_t *pool, int64_t num_blocks, int64_t pool_layer_stride, int n_layers, int Hkv,
+                   int head_dim, int bits_k, int bits_v, const int32_t *copies, int n_copies,
+                   void *stream);
+
 #ifdef __cplusplus
 }
 #endif
