@@ -80,6 +80,9 @@ SIGNATURES = {
     "ftq_pages_compact_workspace_bytes": (_sz, [_i]),
     "ftq_pages_compact": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _sz, _vp]),
     "ftq_pages_shared_lens": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp]),
+    "ftq_shared_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "ftq_shared_attn": (_i, [_vp, _i, _vp, _i, _vp, _i64, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _fp, _fp, _fp, _f,
+                             _vp, _sz, _vp]),
     "ftq_copy_pages": (_i, [_vp, _i64, _i64, _i, _i, _i, _i, _i, _vp, _i, _vp]),
 }
 

@@ -20,6 +20,7 @@
 #include "ftq_dense.cuh"
 #include "ftq_launch.h"
 #include "ftq_serve_launch.h"
+#include "ftq_shared_launch.h"
 #include "ftq_tree_launch.h"
 #include "ftq_tq_v1_launch.h"
 
@@ -1993,4 +1994,121 @@ extern "C" int ftq_beam_select(const void* logits, int dtype, int64_t row_stride
     p.chunks = plan.chunks; p.chunk = plan.chunk;
     const cudaError_t e = ftq::launch_select(dtype, p, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? FTQ_OK : cuda_fail(e, "ftq_beam_select launch");
+}
+
+// ------------------------------------------------------------------ attention with common leading blocks
+
+namespace {
+struct SharedLayout {   // of the workspace, behind a decode workspace of one sequence (whose status word it uses)
+    int requests;                            // of a launch
+    int units_group, units_row, rows_group, rows_row;
+    size_t plan, q, rows, end;
+    int64_t base_row;
+};
+SharedLayout shared_layout(int requests, int group, int Hq, int Hkv, int d, size_t head) {
+    SharedLayout l{};
+    const int G = Hq / Hkv, cols = 8 * ftq::shared_tiles(d), both = group * G;
+    l.requests = std::min(requests, std::max(1, ftq::kSharedMaxRows / group));
+    l.units_group = Hkv * ((both + cols - 1) / cols);
+    l.units_row = Hkv * ((G + cols - 1) / cols);
+    l.rows_group = std::min(both, cols);
+    l.rows_row = std::min(G, cols);
+    const int64_t R = l.requests, B = R * group, warps = static_cast<int64_t>(ftq::sm_count()) * ftq::kSharedWarps;
+    l.plan = round256(head);
+    l.q = l.plan + round256(static_cast<size_t>(3 * (R + B) + 2) * 4);
+    l.rows = l.q + round256(static_cast<size_t>(B) * Hq * d * 2);
+    l.base_row = (warps + R * l.units_group) * l.rows_group;
+    l.end = l.rows + static_cast<size_t>(l.base_row + (warps + B * l.units_row) * l.rows_row) * (d + 4) * sizeof(float);
+    return l;
+}
+}  // namespace
+
+extern "C" size_t ftq_shared_workspace_bytes(int n_requests, int group, int Hq, int Hkv, int head_dim, int max_seq_len) {
+    if (n_requests <= 0 || group <= 0 || group > ftq::kSharedMaxRows) return 0;
+    const size_t head = ftq_decode_workspace_bytes(1, Hq, Hkv, head_dim, max_seq_len, 1);
+    return head == 0 ? 0 : shared_layout(n_requests, group, Hq, Hkv, head_dim, head).end;
+}
+
+extern "C" int ftq_shared_attn(const void* q, int q_dtype, void* out, int out_dtype, const uint8_t* pool, int64_t num_blocks,
+                               const int32_t* block_table, int max_blocks, const int32_t* seq_lens, int max_seq_len,
+                               const int32_t* shared_lens, int n_requests, int group, int Hq, int Hkv, int head_dim, int bits_k,
+                               int bits_v, const float* levels_k_host, const float* levels_v_host, const float* signs_host,
+                               float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_attn_common(n_requests, Hq, Hkv, head_dim, bits_k, bits_v, q_dtype, out_dtype);
+    if (rc) return rc;
+    if (q_dtype == FTQ_F32) return fail(FTQ_ERR_UNSUPPORTED, "attention with shared blocks takes 16-bit queries");
+    if (group <= 0 || group > ftq::kSharedMaxRows)
+        return fail(FTQ_ERR_UNSUPPORTED, "a group has 1 to %d rows, got %d", ftq::kSharedMaxRows, group);
+    if (max_blocks <= 0 || max_seq_len < 0 || num_blocks < 0 || static_cast<int64_t>(n_requests) * group > INT32_MAX)
+        return fail(FTQ_ERR_INVALID, "bad shape groups=%d of %d max_blocks=%d max_seq_len=%d", n_requests, group, max_blocks, max_seq_len);
+    if (n_requests == 0) return FTQ_OK;
+    if (!q || !out || !pool || !block_table || !seq_lens || !shared_lens) return fail(FTQ_ERR_INVALID, "NULL tensor pointer");
+    if (static_cast<int64_t>(max_blocks) * FTQ_PAGE_TOKENS < max_seq_len)
+        return fail(FTQ_ERR_INVALID, "block_table too narrow: %d blocks < max_seq_len %d", max_blocks, max_seq_len);
+    if (!aligned(q, 16) || !aligned(out, 4) || !aligned(pool, 16))
+        return fail(FTQ_ERR_INVALID, "q and pool must be 16-byte aligned");
+    const size_t need = ftq_shared_workspace_bytes(n_requests, group, Hq, Hkv, head_dim, max_seq_len);
+    rc = check_workspace(workspace, workspace_bytes, need);
+    if (rc) return rc;
+    const size_t head = ftq_decode_workspace_bytes(1, Hq, Hkv, head_dim, max_seq_len, 1);
+    const SharedLayout l = shared_layout(n_requests, group, Hq, Hkv, head_dim, head);
+    ftq::SharedAttnParams p{};
+    rc = pack_levels(levels_k_host, bits_k, &p.lk);
+    if (rc == FTQ_OK) rc = pack_levels(levels_v_host, bits_v, &p.lv);
+    if (rc == FTQ_OK) rc = pack_signs(signs_host, head_dim, &p.signs);
+    if (rc) return rc;
+    const float ks = choose_k_scale(levels_k_host, bits_k, head_dim), vs = choose_v_scale(levels_v_host, bits_v, head_dim);
+    for (int i = 0; i < (1 << bits_k); i++) p.lk.v[i] = levels_k_host[i] * ks;
+    for (int i = 0; i < (1 << bits_v); i++) p.lv.v[i] = levels_v_host[i] * vs;
+    p.inv_v_scale = 1.0f / vs;
+    p.rsqrt_d = rsqrt_dim(head_dim);
+    p.q_scale = p.rsqrt_d * (scale / ks * ftq::kLog2e);
+    p.pool = pool; p.num_blocks = num_blocks; p.max_blocks = max_blocks; p.max_seq = max_seq_len;
+    p.K = group; p.Hq = Hq; p.Hkv = Hkv; p.q_dtype = q_dtype;
+    p.units_group = l.units_group; p.units_row = l.units_row; p.rows_group = l.rows_group; p.rows_row = l.rows_row;
+    p.cols = 8 * ftq::shared_tiles(head_dim);
+    // what a page costs: its look-ups and byte work, and a share of that for each tile of columns (see ftq_shared_attn.cuh)
+    p.cost_group = 9 + 2 * ((l.rows_group + 7) / 8);
+    p.cost_row = 9 + 2 * ((l.rows_row + 7) / 8);
+    p.least_pages = 2;
+    const int64_t pages = (static_cast<int64_t>(max_seq_len) + FTQ_PAGE_TOKENS - 1) / FTQ_PAGE_TOKENS,
+                  places = (ftq::kSharedPiece + pages * p.cost_group) * l.units_group + group * (ftq::kSharedPiece + pages * p.cost_row) * l.units_row;
+    const int requests = static_cast<int>(std::min<int64_t>(l.requests, (INT32_MAX / 2) / places));
+    if (requests < 1) return fail(FTQ_ERR_UNSUPPORTED, "too many tokens, heads and rows for one call");
+    const int grid = ftq::sm_count();
+    p.warps = grid * ftq::kSharedWarps;
+    uint8_t* const ws = static_cast<uint8_t*>(workspace);
+    const int entries = requests * (1 + group);
+    p.plan = reinterpret_cast<int*>(ws + l.plan);
+    p.plan_tokens = p.plan + entries + 2;
+    p.plan_leader = p.plan_tokens + entries;
+    p.q_rows = ws + l.q;
+    p.rows = reinterpret_cast<float*>(ws + l.rows);
+    p.base_row = l.base_row;
+    p.status = reinterpret_cast<int*>(ws + head - counter_bytes(1, Hkv, 1)) + ftq::kStatusWord;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    for (int r0 = 0; r0 < n_requests; r0 += requests) {
+        const int64_t b0 = static_cast<int64_t>(r0) * group, vec = b0 * Hq * head_dim;
+        p.R = std::min(requests, n_requests - r0);
+        p.q = static_cast<const uint8_t*>(q) + vec * dtype_size(q_dtype);
+        p.out = static_cast<uint8_t*>(out) + vec * dtype_size(out_dtype);
+        p.block_table = block_table + b0 * max_blocks;
+        p.seq_lens = seq_lens + b0;
+        p.shared_lens = shared_lens + r0;
+        p.first = r0 == 0;
+        cudaError_t e = ftq::launch_shared_prepare(head_dim, p, st);
+        if (e != cudaSuccess) return cuda_fail(e, "ftq_shared_attn prepare launch");
+        e = cudaErrorInvalidValue;
+        switch (head_dim * 10 + bits_k) {
+#define FTQ_SHARED_CASE(DD, KB) case DD * 10 + KB: e = ftq::launch_shared_attn_d##DD##_k##KB(bits_v, p, grid, st); break;
+            FTQ_SHARED_CASE(64, 2) FTQ_SHARED_CASE(64, 3) FTQ_SHARED_CASE(64, 4)
+            FTQ_SHARED_CASE(128, 2) FTQ_SHARED_CASE(128, 3) FTQ_SHARED_CASE(128, 4)
+            FTQ_SHARED_CASE(256, 2) FTQ_SHARED_CASE(256, 3) FTQ_SHARED_CASE(256, 4)
+#undef FTQ_SHARED_CASE
+        }
+        if (e != cudaSuccess) return cuda_fail(e, "ftq_shared_attn launch");
+        e = ftq::launch_shared_merge(head_dim, out_dtype, p, st);
+        if (e != cudaSuccess) return cuda_fail(e, "ftq_shared_attn merge launch");
+    }
+    return FTQ_OK;
 }

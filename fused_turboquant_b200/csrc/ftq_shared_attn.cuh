@@ -1,0 +1,655 @@
+// Paged decode attention of rows that share their leading blocks (beams, samples of a prompt): one new token of every row.
+//
+//   o_b = sum_j softmax_j(q_b . k_j scale) v_j     over the row's tokens, k_j = |k_j| levels[code] in the rotated space
+//
+// A page of common tokens is fetched and dequantised once for all rows of a group; look-ups and byte work, which bound the
+// decode kernel (ftq_attn_flow.cuh), are the same for one row as for eight, and only the products and the softmax grow.
+//
+// Units.  The common tokens of a group and one KV head, with the group's rows x heads as the columns of the products, in
+// blocks of 8 NT; and the tokens that a row has to itself, with its heads as columns.  All units lie on one line of places: so
+// many for a unit on its own, and so many more for each of its pages, by what they cost; warp w of the grid takes the places
+// [w share, (w + 1) share).  A warp works for itself: its pages come by bulk copies to a ring of its own, it keeps
+// (O, m, l) of all columns in registers and leaves them in the workspace, a piece of a unit at a time.  No barrier, no atomic.
+// shared_merge_kernel joins a row's pieces by their maxima, rotates back (core/hadamard.py:93-100) and stores.
+// shared_prepare_kernel, before both, rotates the queries and makes the prefix sums of the places.
+//
+// Tables, page layout and fragment maps are those of ftq_attn_mma.cuh with the columns as heads (NH = 2).  Weights carry the
+// values' norms into fp16: they are scaled by a power of two that goes with the largest norm so far (lazily, as the maximum).
+#pragma once
+
+#include "ftq_attn_mma.cuh"
+#include "ftq_shared_launch.h"
+
+namespace ftq {
+
+template <int D, int BK, int BV, int NT>
+struct SharedCfg : MmaCfg<D, BK, BV, 2> {
+    using M = MmaCfg<D, BK, BV, 2>;
+    static constexpr int WARPS = kSharedWarps, THREADS = 32 * WARPS, COLS = 8 * NT;
+    static constexpr bool ROT = !(BV == 3 && D <= 128);     // (see FlowCfg)
+    static constexpr int RING = D == 256 ? 2 : 4;           // pages on their way, per warp
+    static constexpr int RING_BYTES = (RING * M::PAGE_BYTES + 127) / 128 * 128;
+    static constexpr int Q_BYTES = COLS * D * 2;
+    static constexpr int PLAN_BYTES = (2 * kSharedMaxRows + 4) * 4;
+    // before and behind the 64 KB window of the tables: first-fit, as in FlowCfg; bytes needed from `base`
+    __host__ __device__ static constexpr int plan(int base) {
+        int free0 = base, free1 = (base + 65535) / 65536 * 65536;
+        const int end0 = free1;
+        free1 += 65536;
+        for (int i = 0; i < 2 * WARPS + 1; i++) {
+            const int bytes = i < WARPS ? RING_BYTES : i < 2 * WARPS ? Q_BYTES : PLAN_BYTES;
+            const int a0 = (free0 + 127) / 128 * 128;
+            if (a0 + bytes <= end0) free0 = a0 + bytes;
+            else free1 = (free1 + 127) / 128 * 128 + bytes;
+        }
+        return (free1 > free0 ? free1 : free0) - base;
+    }
+    __host__ __device__ static constexpr int need() {
+        int worst = plan(0);
+        for (int base = 16; base <= 4096; base += 128) worst = plan(base) > worst ? plan(base) : worst;
+        return worst;
+    }
+    static constexpr int SMEM_BYTES = need();
+    static_assert(SMEM_BYTES <= 226 * 1024, "shared memory of a CTA");
+};
+
+// ------------------------------------------------------------------ plan
+// Units of an entry (the common tokens of a group, or a row's own), and where their places are.
+struct SharedEntry {
+    int first, pages, unit;     // the entry's first place, pages of a unit, places of a unit
+};
+// first page of a unit's piece that starts `at` places into it
+__device__ __forceinline__ int shared_page_of(int at, int cost, int pages) {
+    const int x = at - kSharedPiece;
+    return x <= 0 ? 0 : min((x + cost - 1) / cost, pages);
+}
+__device__ __forceinline__ int shared_len(const SharedAttnParams& p, int b) { return max(0, min(p.seq_lens[b], p.max_seq)); }
+// tokens of group r that are taken as common (whole blocks, as far as its longest row goes), and that row
+__device__ __forceinline__ int shared_common(const SharedAttnParams& p, int r, int& leader) {
+    int most = 0;
+    leader = r * p.K;
+    for (int k = 0; k < p.K; k++) {
+        const int n = shared_len(p, r * p.K + k);
+        if (n > most) {
+            most = n;
+            leader = r * p.K + k;
+        }
+    }
+    return max(0, min(p.shared_lens[r], most)) / kPageTokens * kPageTokens;
+}
+
+// plan: [e] first place of entry e (groups, then rows), [entries]: the end; then per entry the leader of a group / the common
+// tokens before a row's own, and its pages
+template <int D>
+__global__ void __launch_bounds__(256) shared_prepare_kernel(const __grid_constant__ SharedAttnParams p) {
+    constexpr int E = D / kOctet;
+    __shared__ int s_sum[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    let_next_kernel_start();
+    after_previous_kernel();
+    if (blockIdx.x == 0) {
+        const int entries = p.R + p.R * p.K;
+        int base = 0;
+        for (int e0 = 0; e0 < entries; e0 += 256) {
+            const int e = e0 + tid;
+            int places = 0;
+            if (e < entries) {
+                int leader;
+                const bool group = e < p.R;
+                const int common = shared_common(p, group ? e : (e - p.R) / p.K, leader);
+                const int pages = (group ? common : max(0, shared_len(p, e - p.R) - common) + kPageTokens - 1) / kPageTokens;
+                places = pages == 0 ? 0 : (kSharedPiece + pages * (group ? p.cost_group : p.cost_row)) * (group ? p.units_group : p.units_row);
+                p.plan_tokens[e] = common;
+                p.plan_leader[e] = leader;
+            }
+            int x = places;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, d);
+                if (lane >= d) x += y;
+            }
+            __syncthreads();
+            if (lane == 31) s_sum[warp] = x;
+            __syncthreads();
+            int before = base;
+            for (int w = 0; w < 8; w++) {
+                before += w < warp ? s_sum[w] : 0;
+                base += s_sum[w];
+            }
+            if (e < entries) p.plan[e] = before + x - places;
+        }
+        if (tid == 0) {
+            p.plan[entries] = base;
+            // (a piece has some pages at least, whatever there is to do)
+            p.plan[entries + 1] = max((base + p.warps - 1) / p.warps, kSharedPiece + p.least_pages * p.cost_group);
+            if (p.first) *p.status = 0;
+        }
+        return;
+    }
+    // a row's head per octet; a row's 16-byte chunks lie in the order in which the lanes of a product take them, those of odd
+    // rows with each four exchanged
+    const int t8 = lane & 7, G = p.Hq / p.Hkv;
+    const int64_t rows = static_cast<int64_t>(p.R) * p.K * p.Hq;
+    for (int64_t i0 = (static_cast<int64_t>(blockIdx.x - 1) * 8 + warp) * 4; i0 < rows; i0 += static_cast<int64_t>(gridDim.x - 1) * 32) {
+        const int64_t i = i0 + (lane >> 3);
+        const bool live = i < rows;
+        const uint8_t* src = static_cast<const uint8_t*>(p.q) + (live ? i : 0) * (D * 2);
+        float a[E];
+#pragma unroll
+        for (int k = 0; k < E / 8; k++) {
+            float tmp[8];
+            const uint8_t* at = src + 16 * (t8 + 8 * k);
+            if (p.q_dtype == kBF16) load8<__nv_bfloat16>(reinterpret_cast<const __nv_bfloat16*>(at), tmp);
+            else load8<__half>(reinterpret_cast<const __half*>(at), tmp);
+#pragma unroll
+            for (int c = 0; c < 8; c++)
+                a[8 * k + c] = __uint_as_float(__float_as_uint(tmp[c]) ^ sign_mask(p.signs, load_coord(t8, 8 * k + c)));
+        }
+        octet_fwht<E>(a, lane);
+        if (!live) continue;
+        const int hq = static_cast<int>(i % p.Hq), h = hq / G;
+        const int64_t b = i / p.Hq, r = b / p.K;
+        const int n = static_cast<int>(b - r * p.K) * G + hq - h * G;      // row of the (group, KV head)
+        __half* dst = reinterpret_cast<__half*>(p.q_rows) + ((r * p.Hkv + h) * p.K * G + n) * D;
+#pragma unroll
+        for (int k = 0; k < E; k++) {
+            const int coord = t8 + 8 * k, tg = coord / (D / 4), chunk = coord % (D / 4) / 8;
+            dst[8 * ((4 * chunk + tg) ^ ((n & 1) * 4)) + coord % 8] = __ushort_as_half(static_cast<unsigned short>(f2h_sat(a[k] * p.q_scale)));
+        }
+    }
+}
+
+// ------------------------------------------------------------------ attention
+// (weights stay below 2^14, see below; those of infinite norms are infinite)
+__device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+struct SharedPiece {
+    int next;            // where the next piece starts
+    int row;             // row of the block table
+    int page0, n_pages;  // of the row's pages
+    int tokens;          // from page0 on
+    int cols, tiles;     // columns, and tiles of eight
+    int col0;            // first column's row in its (group, KV head)
+    int qh;              // group x Hkv + KV head
+    int hkv;
+    int limit0;          // tokens before page0
+    bool ragged;         // columns of a group with fewer tokens
+    int64_t out;         // rows in the workspace
+};
+
+template <int D, int BK, int BV, int NT>
+__global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_attn_kernel(const __grid_constant__ SharedAttnParams p) {
+    using C = SharedCfg<D, BK, BV, NT>;
+    using WK = Window<BK, false>;
+    using WV = Window<BV, false>;
+    constexpr int NKB = C::NKB, NMT = C::NMT, ROW = D + 4;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    const uint32_t sbase = static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw));
+    const uint32_t window = (sbase + 65535u) & ~65535u, end0 = window;
+    uint32_t free0 = sbase, free1 = window + 65536u;
+    auto take = [&](uint32_t bytes) {
+        uint32_t a = (free0 + 127u) & ~127u;
+        if (a + bytes <= end0) { free0 = a + bytes; return a; }
+        a = (free1 + 127u) & ~127u;
+        free1 = a + bytes;
+        return a;
+    };
+    auto gptr = [&](uint32_t saddr) { return smem_raw + (saddr - sbase); };
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tg = lane & 3;
+    uint32_t my_ring = 0, my_q = 0;
+#pragma unroll
+    for (int w = 0; w < C::WARPS; w++) { const uint32_t a = take(C::RING_BYTES); if (w == warp) my_ring = a; }
+#pragma unroll
+    for (int w = 0; w < C::WARPS; w++) { const uint32_t a = take(C::Q_BYTES); if (w == warp) my_q = a; }
+    int* const s_plan = reinterpret_cast<int*>(gptr(take(C::PLAN_BYTES)));
+    __shared__ __align__(8) unsigned long long s_bars[C::WARPS][C::RING + 1];
+    const uint32_t my_bars = static_cast<uint32_t>(__cvta_generic_to_shared(&s_bars[warp][0])), q_bar = my_bars + 8 * C::RING;
+
+    let_next_kernel_start();
+    // ---- tables: a row of 32 copies of an entry is two shuffles, a conversion and one store
+    {
+        const float lev_k = p.lk.v[lane & 15], lev_v = p.lv.v[lane & 15];
+        auto pair = [&](float lev, int lo, int hi) {
+            const __half2 h = __floats2half2_rn(__shfl_sync(0xffffffffu, lev, lo), __shfl_sync(0xffffffffu, lev, hi));
+            return *reinterpret_cast<const uint32_t*>(&h);
+        };
+        auto entry = [&](float lev, int bits, int e) {
+            if (bits == 4) return pair(lev, e & 15, e >> 4);
+            if (bits == 3) return pair(lev, e & 7, e >> 3 & 7);
+            const uint32_t x = pair(lev, e & 3, (e >> 2) & 3), y = pair(lev, (e >> 4) & 3, e >> 6);
+            return (lane & 1) ? y : x;
+        };
+        uint32_t* tb = reinterpret_cast<uint32_t*>(gptr(window));
+#pragma unroll 4
+        for (int e = warp; e < 256; e += C::WARPS) {
+            tb[e * 64 + lane] = entry(lev_k, BK, e);
+            tb[e * 64 + 32 + lane] = entry(lev_v, BV, e);
+        }
+        // (columns that a unit does not have are computed too: from zeros, or from what an earlier unit left)
+        for (int i = lane; i < C::Q_BYTES / 16; i += 32) reinterpret_cast<uint4*>(gptr(my_q))[i] = make_uint4(0, 0, 0, 0);
+    }
+    if (lane == 0) {
+#pragma unroll
+        for (int r = 0; r <= C::RING; r++) mbar_init(my_bars + 8 * r, 1);
+    }
+    mbar_fence_init();
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    after_previous_kernel();
+    const int entries = p.R + p.R * p.K;
+    for (int i = tid; i < entries + 2; i += C::THREADS) s_plan[i] = p.plan[i];
+    __syncthreads();
+
+    const int total = s_plan[entries], share = s_plan[entries + 1], G = p.Hq / p.Hkv;
+    const int64_t from = static_cast<int64_t>(blockIdx.x * C::WARPS + warp) * share;
+    if (from >= total) return;
+    const int end = static_cast<int>(min(from + share, static_cast<int64_t>(total)));
+    const int me = blockIdx.x * C::WARPS + warp;
+
+    auto locate = [&](int pos) {
+        SharedPiece it{};
+        int lo = 0, hi = entries;     // plan[lo] <= pos < plan[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (s_plan[mid] <= pos) lo = mid; else hi = mid;
+        }
+        const bool group = lo < p.R;
+        const int units = group ? p.units_group : p.units_row, cost = group ? p.cost_group : p.cost_row;
+        const int unit_places = (s_plan[lo + 1] - s_plan[lo]) / units, pages = (unit_places - kSharedPiece) / cost;
+        const int u = (pos - s_plan[lo]) / unit_places, at = pos - s_plan[lo] - u * unit_places;
+        const int to = min(unit_places, at + end - pos);
+        const int blocks = units / p.Hkv, all = group ? p.K * G : G, blk = u % blocks;
+        it.hkv = u / blocks;
+        const int r = group ? lo : (lo - p.R) / p.K, common = p.plan_tokens[lo], leader = p.plan_leader[lo];
+        it.cols = min(C::COLS, all - blk * C::COLS);
+        it.tiles = (it.cols + 7) / 8;
+        it.qh = r * p.Hkv + it.hkv;
+        it.row = group ? leader : lo - p.R;
+        it.col0 = (group ? 0 : (lo - p.R - r * p.K) * G) + blk * C::COLS;
+        const int page0 = shared_page_of(at, cost, pages);
+        it.n_pages = shared_page_of(to, cost, pages) - page0;
+        it.page0 = page0 + (group ? 0 : common / kPageTokens);
+        it.limit0 = it.page0 * kPageTokens;
+        it.tokens = min((group ? common : shared_len(p, it.row)) - it.limit0, it.n_pages * kPageTokens);
+        // rows of a group that end before the common tokens do
+        it.ragged = false;
+        if (group) {
+            bool shorter = false;
+            for (int k = lane; k < p.K; k += 32) {
+                const int n = shared_len(p, r * p.K + k);
+                shorter |= n > 0 && n < it.limit0 + it.tokens;      // (rows without tokens are left out at the end)
+            }
+            it.ragged = __any_sync(0xffffffffu, shorter);
+        }
+        const int64_t slot = me + static_cast<int64_t>(group ? lo : lo - p.R) * units + u;
+        it.out = group ? slot * p.rows_group : p.base_row + slot * p.rows_row;
+        it.next = pos + to - at;
+        return it;
+    };
+
+    const uint32_t blk_stride = static_cast<uint32_t>(p.Hkv) * C::PAGE_BYTES;
+    const uint64_t policy = l2_evict_first_policy();
+    const bool odd = g & 1;
+    const uint32_t sel_own = odd ? 0x4432u : 0x4410u;
+    const uint32_t koff = (4 * (g >> 1) + (g & 1)) * C::PDK + slice_word<C::KSB>(tg), ksh = slice_shift<C::KSB>(tg);
+    const uint32_t noff = C::OFF_KN + 8 * (g >> 1);
+    const uint32_t vsh = slice_shift<C::VSB>(g);
+    const uint32_t lk_lane = window | (BK == 2 ? (lane & 15) * 8 : lane * 4);
+    const uint32_t lv_lane = window | 128u | (BV == 2 ? (lane & 15) * 8 : lane * 4);
+    uint32_t phases = 0;      // bit r: parity that the next wait on ring buffer r expects; bit RING: the queries'
+    bool lost = false;        // a wait ran out: nothing is requested any more, and the warp's pieces are NaN
+    bool bad_any = false;
+#ifdef FTQ_TEST_WAIT_EXPIRY
+    bool test_drop = blockIdx.x == 0 && warp == 5;
+#endif
+
+    SharedPiece it{};
+    for (int pos = static_cast<int>(from); pos < end; pos = it.next) {
+        it = locate(pos);
+        if (it.n_pages == 0) continue;      // (a share that ends among a unit's places on its own)
+        const uint8_t* const base = p.pool + static_cast<int64_t>(it.hkv) * C::PAGE_BYTES;
+        bool bad = false;
+        // block ids of pages k0 .. k0 + 31 of the piece; an id outside the pool is replaced by 0 and remembered
+        auto load_ids = [&](int k0) {
+            const int k = k0 + lane;
+            int id = 0;
+            if (k < it.n_pages) {
+                id = p.block_table[static_cast<int64_t>(it.row) * p.max_blocks + it.page0 + k];
+                if (static_cast<uint32_t>(id) >= static_cast<uint64_t>(p.num_blocks)) {
+                    id = 0;
+                    bad = true;
+                }
+            }
+            return id;
+        };
+        auto request = [&](int ids, int k) {
+            const uint32_t id = __shfl_sync(0xffffffffu, ids, k & 31);
+            const int rb = k % C::RING;
+            if (lane == 0) {
+                mbar_expect_tx(my_bars + 8 * rb, C::PAGE_BYTES);
+#ifdef FTQ_TEST_WAIT_EXPIRY
+                const bool drop = test_drop;    // (see kMbarSpinLimit)
+                test_drop = false;
+                if (!drop)
+#endif
+                bulk_g2s_hint(my_ring + rb * C::PAGE_BYTES, base + static_cast<uint64_t>(id) * blk_stride, C::PAGE_BYTES, my_bars + 8 * rb, policy);
+            }
+            __syncwarp();
+        };
+        int ids = load_ids(0), ids_next = 0;
+        const bool requested = !lost;
+        if (requested) {
+            if (lane == 0) {
+                mbar_expect_tx(q_bar, it.cols * D * 2);
+                bulk_g2s_hint(my_q, p.q_rows + (static_cast<int64_t>(it.qh) * p.K * G + it.col0) * (D * 2), it.cols * D * 2, q_bar, policy);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < C::RING; k++)
+                if (k < it.n_pages) request(ids, k);
+        }
+        float oacc[NT][2 * NMT][4], m_run[NT][2], l_run[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+            for (int mt = 0; mt < 2 * NMT; mt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) oacc[nt][mt][i] = 0.f;
+            m_run[nt][0] = m_run[nt][1] = -INFINITY;
+            l_run[nt][0] = l_run[nt][1] = 0.f;
+        }
+        float vmax = 0.f, vscale = 1.f;     // the largest norm of a value so far, lazily, and the power of two that goes with it
+        const uint32_t q_lane = my_q + g * (D * 2), q_odd = ((it.col0 + g) & 1) * 64 ^ tg * 16;
+        if (!lost && !mbar_wait(q_bar, (phases >> C::RING) & 1)) lost = true;
+        phases ^= 1u << C::RING;
+        lost = __any_sync(0xffffffffu, lost);
+
+        int k = 0;
+        for (; k < it.n_pages; k++) {
+            if ((k & 31) == 0) {        // (a batch of ids ahead)
+                if (k > 0) ids = ids_next;
+                ids_next = load_ids(k + 32);
+            }
+            const int rb = k % C::RING;
+            if (!lost) {
+                if (!mbar_wait(my_bars + 8 * rb, (phases >> rb) & 1)) lost = true;
+                lost = __any_sync(0xffffffffu, lost);
+            }
+            if (lost) break;
+            phases ^= 1u << rb;
+            const uint32_t page = my_ring + rb * C::PAGE_BYTES;
+            uint32_t kw[2][C::KW], vw[4][C::VW];
+            lds_slice<C::KSB>(page + koff, ksh, kw[0]);
+            lds_slice<C::KSB>(page + koff + 2 * C::PDK, ksh, kw[1]);
+            const uint2 kn = lds64(page + noff), vn = lds64(page + noff + (C::OFF_VN - C::OFF_KN));
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int u = C::ROT ? (j + tg) & 3 : j, slice = g ^ ((u & 2) << 1);
+                lds_slice<C::VSB>(page + C::OFF_VC + (4 * tg + u) * C::PDV + slice_word<C::VSB>(slice), vsh, vw[j]);
+            }
+            // the buffer is free for the page RING further on
+            __syncwarp();
+            if (k + C::RING < it.n_pages) request((k + C::RING) >> 5 == k >> 5 ? ids : ids_next, k + C::RING);
+
+            // ---- S = K Q^T
+            float c[NT][4];
+            {
+                typename WK::template Run<C::KW> run[2];
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+#pragma unroll
+                    for (int j = 0; j < C::KW; j++) run[r].w[j] = kw[r][j];
+                    WK::shift(run[r]);
+                }
+#pragma unroll
+                for (int kb = 0; kb < NKB; kb += 2) {
+                    uint32_t a[2][4];
+#pragma unroll
+                    for (int s = 0; s < 2; s++) {
+                        WK::pairs(run[0], kb + s, lk_lane, a[s][0], a[s][2]);
+                        WK::pairs(run[1], kb + s, lk_lane, a[s][1], a[s][3]);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        if (nt >= it.tiles) continue;
+                        const uint4 q = lds128(q_lane + nt * 8 * (D * 2) + ((kb / 2 * 64) ^ q_odd));
+                        if (kb == 0) mma_16816_z(c[nt], a[0][0], a[0][1], a[0][2], a[0][3], q.x, q.y);
+                        else mma_16816(c[nt], a[0][0], a[0][1], a[0][2], a[0][3], q.x, q.y);
+                        mma_16816(c[nt], a[1][0], a[1][1], a[1][2], a[1][3], q.z, q.w);
+                    }
+                }
+            }
+            // ---- softmax (base 2), per column; lanes of a column: the eight that differ in g
+            const int tokA = 4 * (g >> 1) + (g & 1), left = it.tokens - k * kPageTokens;
+            const float kna = half_bits_to_float(__byte_perm(kn.x, 0u, sel_own)), knb = half_bits_to_float(__byte_perm(kn.y, 0u, sel_own));
+            float vna = half_bits_to_float(__byte_perm(vn.x, 0u, sel_own)), vnb = half_bits_to_float(__byte_perm(vn.y, 0u, sel_own));
+            const bool whole = left >= kPageTokens && !it.ragged;
+            bool above = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                if (nt >= it.tiles) continue;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    c[nt][h] *= kna;
+                    c[nt][2 + h] *= knb;
+                }
+            }
+            if (!whole) {
+                if (tokA >= left) vna = 0.f;
+                if (tokA + 2 >= left) vnb = 0.f;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        int mine = left;
+                        const int col = 8 * nt + 2 * tg + h;
+                        if (it.ragged && col < it.cols)
+                            mine = min(mine, shared_len(p, it.qh / p.Hkv * p.K + (it.col0 + col) / G) - it.limit0 - k * kPageTokens);
+                        if (tokA >= mine) c[nt][h] = -INFINITY;
+                        if (tokA + 2 >= mine) c[nt][2 + h] = -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                if (nt >= it.tiles) continue;
+#pragma unroll
+                for (int h = 0; h < 2; h++) above |= fmaxf(c[nt][h], c[nt][2 + h]) > m_run[nt][h] + kLazyMaxSlack;
+            }
+            above |= fmaxf(vna, vnb) > vmax * 1024.f;
+            if (__any_sync(0xffffffffu, above)) {
+                float v = fmaxf(vna, vnb);
+#pragma unroll
+                for (int d = 4; d <= 16; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+                float change = 1.f;
+                if (v > vmax * 1024.f) {        // (norms are not negative; infinite ones stay what they are)
+                    vmax = fminf(v, 65504.f);
+                    // 2^-e with vmax in [2^e, 2^(e + 1))
+                    const float now = __uint_as_float((254u << 23) - (__float_as_uint(vmax) & 0x7f800000u));
+                    change = now / vscale;
+                    vscale = now;
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float corr[2];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float m = nt < it.tiles ? fmaxf(c[nt][h], c[nt][2 + h]) : -INFINITY;
+#pragma unroll
+                        for (int d = 4; d <= 16; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+                        const float now = fmaxf(m_run[nt][h], m);
+                        corr[h] = now == -INFINITY ? 1.f : fast_exp2(m_run[nt][h] - now);
+                        l_run[nt][h] *= corr[h];
+                        m_run[nt][h] = now;
+                        corr[h] *= change;
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < 2 * NMT; mt++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) oacc[nt][mt][i] *= corr[i & 1];
+                }
+            }
+            vna *= vscale;
+            vnb *= vscale;
+            uint32_t pb[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                if (nt >= it.tiles) continue;
+                float wa[2], wb[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    // (a column without a token yet has nothing but -inf)
+                    const float ref = m_run[nt][h] == -INFINITY ? 0.f : m_run[nt][h];
+                    const float pa = fast_exp2(c[nt][h] - ref), pbv = fast_exp2(c[nt][2 + h] - ref);
+                    l_run[nt][h] += pa + pbv;
+                    wa[h] = pa * vna;
+                    wb[h] = pbv * vnb;
+                }
+                uint32_t t0 = movmatrix_trans(pack_weights(wa[0], wa[1])), t1 = movmatrix_trans(pack_weights(wb[0], wb[1]));
+                if constexpr (C::ROT) {     // by tg tokens, to match the values' registers
+                    if (tg & 2) { const uint32_t x = t0; t0 = t1; t1 = x; }
+                    const uint32_t sh = (tg & 1) * 16;
+                    const uint32_t lo = __funnelshift_r(t0, t1, sh), hi = __funnelshift_r(t1, t0, sh);
+                    t0 = lo;
+                    t1 = hi;
+                }
+                pb[nt][0] = t0;
+                pb[nt][1] = t1;
+            }
+            // ---- O^T += V^T P^T
+            {
+                typename WV::template Run<C::VW> run[4];
+                WV::merge(vw[0], vw[1], run[0], run[1]);
+                WV::merge(vw[2], vw[3], run[2], run[3]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) WV::shift(run[j]);
+#pragma unroll
+                for (int m2 = 0; m2 < NMT; m2++) {
+                    uint32_t x[4], y[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) WV::pairs(run[j], m2, lv_lane, x[j], y[j]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        if (nt >= it.tiles) continue;
+                        mma_16816(oacc[nt][2 * m2], x[0], x[1], x[2], x[3], pb[nt][0], pb[nt][1]);
+                        mma_16816(oacc[nt][2 * m2 + 1], y[0], y[1], y[2], y[3], pb[nt][0], pb[nt][1]);
+                    }
+                }
+            }
+        }
+        // (no copy of this warp's is on its way when it gives up)
+        if (lost && requested)
+            for (const int last = min(k + C::RING, it.n_pages); k < last; k++) mbar_wait(my_bars + 8 * (k % C::RING), (phases >> (k % C::RING)) & 1);
+        // ---- the piece's rows: O in coordinates (D/8) g .. + D/8 of columns 2 tg, 2 tg + 1, (m, l) behind them
+        bad = __any_sync(0xffffffffu, bad);
+        bad_any |= bad;
+        const float scale = lost || bad ? __int_as_float(0x7fc00000) : p.inv_v_scale / vscale;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            if (nt >= it.tiles) continue;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int col = 8 * nt + 2 * tg + h;
+                float l = l_run[nt][h];
+#pragma unroll
+                for (int d = 4; d <= 16; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+                if (col >= it.cols) continue;
+                float* const to = p.rows + (it.out + col) * ROW;
+#pragma unroll
+                for (int f = 0; f < NMT; f++)
+                    *reinterpret_cast<float4*>(to + (D / 8) * g + 4 * f) =
+                        make_float4(oacc[nt][2 * f][h] * scale, oacc[nt][2 * f][2 + h] * scale, oacc[nt][2 * f + 1][h] * scale, oacc[nt][2 * f + 1][2 + h] * scale);
+                if (g == 0) *reinterpret_cast<float2*>(to + D) = make_float2(lost || bad ? __int_as_float(0x7fc00000) : m_run[nt][h], l);
+            }
+        }
+        __syncwarp();       // (the next piece's queries come to where these were read)
+    }
+    if (lane == 0 && (lost || bad_any)) atomicOr(p.status, (lost ? kStatusWaitExpired : 0) | (bad_any ? kStatusBadBlock : 0));
+}
+
+// ------------------------------------------------------------------ merge
+template <int D, typename OT, int OCTETS>
+__global__ void __launch_bounds__(128) shared_merge_kernel(const __grid_constant__ SharedAttnParams p) {
+    constexpr int E = D / kOctet, ROW = D + 4;
+    const int lane = threadIdx.x & 31, t = lane & 7, o = (lane >> 3) & (OCTETS - 1);
+    let_next_kernel_start();
+    after_previous_kernel();
+    const int64_t n_rows = static_cast<int64_t>(p.R) * p.K * p.Hq;
+    const int64_t mine = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / (8 * OCTETS);
+    const int64_t v = mine < n_rows ? mine : n_rows - 1;
+    const int hq = static_cast<int>(v % p.Hq), G = p.Hq / p.Hkv, h = hq / G, b = static_cast<int>(v / p.Hq), r = b / p.K;
+    const int share = p.plan[p.R + p.R * p.K + 1];
+    struct Parts { int first, n, pos, places, cost, pages; int64_t row, step; };
+    auto parts_of = [&](bool group) {
+        const int e = group ? r : p.R + b, units = group ? p.units_group : p.units_row, blocks = units / p.Hkv;
+        const int i = (group ? (b - r * p.K) * G : 0) + hq - h * G, blk = i / p.cols, u = h * blocks + blk;
+        const int e0 = p.plan[e], places = (p.plan[e + 1] - e0) / units;
+        Parts x{0, 0, 0, places, group ? p.cost_group : p.cost_row, 0, 0, group ? p.rows_group : p.rows_row};
+        if (places == 0) return x;
+        x.pages = (places - kSharedPiece) / x.cost;
+        x.pos = e0 + u * places;
+        x.first = x.pos / share;
+        x.n = (x.pos + places - 1) / share - x.first + 1;
+        const int64_t slot = x.first + static_cast<int64_t>(group ? e : e - p.R) * units + u;
+        x.row = (group ? 0 : p.base_row) + slot * x.step + i - blk * p.cols;
+        return x;
+    };
+    const Parts a = parts_of(true), z = parts_of(false);
+    auto row_of = [&](int k) -> const float* {     // part k of both, NULL: it has no pages
+        const Parts& x = k < a.n ? a : z;
+        const int j = k < a.n ? k : k - a.n;
+        const int64_t c = static_cast<int64_t>(x.first + j) * share;
+        const int from = static_cast<int>(max(c, static_cast<int64_t>(x.pos)) - x.pos);
+        const int to = static_cast<int>(min(c + share, static_cast<int64_t>(x.pos) + x.places) - x.pos);
+        if (shared_page_of(to, x.cost, x.pages) <= shared_page_of(from, x.cost, x.pages)) return nullptr;
+        return p.rows + (x.row + j * x.step) * ROW;
+    };
+    const int n = shared_len(p, b) > 0 ? a.n + z.n : 0;
+    float M = -INFINITY;
+    for (int k = 8 * o + t; k < n; k += 8 * OCTETS) {
+        const float* row = row_of(k);
+        if (row) M = fmaxf(M, row[D]);
+    }
+#pragma unroll
+    for (int d = 1; d < 8 * OCTETS; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    float acc[E];
+#pragma unroll
+    for (int k = 0; k < E; k++) acc[k] = 0.f;
+    float L = 0.f;
+#pragma unroll 2
+    for (int k = o; k < n; k += OCTETS) {
+        const float* row = row_of(k);
+        if (!row) continue;
+        const float m = row[D];
+        if (m == -INFINITY) continue;       // (no token of this row: a group's common ones that lie behind its end)
+        const float f = exp2f(m - M);       // (not a number where the piece's rows are none)
+        L = fmaf(row[D + 1], f, L);
+#pragma unroll
+        for (int x = 0; x < E / 8; x++) {
+            float tmp[8];
+            load8<float>(row + 8 * (t + 8 * x), tmp);
+#pragma unroll
+            for (int c = 0; c < 8; c++) acc[8 * x + c] = fmaf(tmp[c], f, acc[8 * x + c]);
+        }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int d = 8; d < 8 * OCTETS; d <<= 1) {
+        L += __shfl_xor_sync(0xffffffffu, L, d);
+#pragma unroll
+        for (int k = 0; k < E; k++) acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], d);
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int k = 0; k < E; k++) acc[k] *= inv;
+    octet_fwht<E>(acc, lane);
+#pragma unroll
+    for (int k = 0; k < E; k++) {
+        if (mine >= n_rows || (k & (OCTETS - 1)) != o) continue;
+        const float x = acc[k] * p.rsqrt_d;
+        reinterpret_cast<OT*>(p.out)[v * D + t + 8 * k] = from_float<OT>(__uint_as_float(__float_as_uint(x) ^ sign_mask(p.signs, t + 8 * k)));
+    }
+}
+
+}  // namespace ftq

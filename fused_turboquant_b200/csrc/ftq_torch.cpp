@@ -38,7 +38,8 @@ namespace {
     X(ftq_tree_workspace_bytes) X(ftq_tree_attn)                                           \
     X(ftq_logits_workspace_bytes) X(ftq_logits_process)                                    \
     X(ftq_beam_workspace_bytes) X(ftq_beam_select) X(ftq_pages_fork_workspace_bytes) X(ftq_pages_fork) \
-    X(ftq_pages_compact_workspace_bytes) X(ftq_pages_compact) X(ftq_pages_shared_lens) X(ftq_copy_pages)
+    X(ftq_pages_compact_workspace_bytes) X(ftq_pages_compact) X(ftq_pages_shared_lens) X(ftq_copy_pages) \
+    X(ftq_shared_workspace_bytes) X(ftq_shared_attn)
 struct Api {
 #define X(name) decltype(&::name) name = nullptr;
     FTQ_BOUND(X)
@@ -1101,6 +1102,59 @@ PyObject* beam_select(PyObject* const* a) {
     return PyTuple_Pack(4, r0.o, r1.o, r2.o, r3.o);
 }
 
+// paged_shared(self, q, block_table, seq_lens, max_seq_len, shared_lens, scale, layer, out, workspace)
+PyObject* paged_shared(PyObject* const* a) {
+    PyObject* self = a[0];
+    at::Tensor q = cuda_tensor(a[1], "q");
+    if (!q.is_contiguous()) q = q.contiguous();
+    else if (reinterpret_cast<uintptr_t>(q.data_ptr()) % 16) q = q.clone();     // (a part of a larger tensor, at an odd place)
+    const Pool p(self);
+    if (q.dim() != 3 || q.size(2) != p.d) raise(PyExc_ValueError, "q must be [B, Hq, " + std::to_string(p.d) + "]");
+    if (dtype_code(q.scalar_type()) < 0) raise(PyExc_ValueError, "q must be fp16 or bf16");
+    const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2);
+    const double scale = a[6] == Py_None ? std::pow(static_cast<double>(D), -0.5) : as_double(a[6]);
+    const at::Device dev = q.device();
+    const at::Tensor bt = as_i32(a[2], "block_table", dev), sl = as_i32(a[3], "seq_lens", dev), sh = as_i32(a[5], "shared_lens", dev);
+    const long long max_seq = as_int(a[4]);
+    if (bt.dim() != 2 || bt.size(0) != B) raise(PyExc_ValueError, "block_table must be [B, max_blocks]");
+    if (max_seq < 0 || max_seq > INT32_MAX) raise(PyExc_ValueError, "max_seq_len must be 0 to 2^31 - 1, got " + std::to_string(max_seq));
+    want_shape(sl, {B}, "seq_lens");
+    if (sh.dim() != 1 || (B > 0 ? sh.size(0) == 0 || B % sh.size(0) != 0 : sh.size(0) != 0))
+        raise(PyExc_ValueError, "shared_lens must be [groups], of equally many of the " + std::to_string(B) + " rows each");
+    const int64_t R = sh.size(0), K = B > 0 ? B / R : 1;
+    const c10::cuda::CUDAGuard guard(dev);
+    at::Tensor out;
+    if (a[8] == Py_None) {
+        out = empty(q.sizes(), q.scalar_type(), dev);
+    } else {
+        out = cuda_tensor(a[8], "out");
+        if (!out.is_contiguous() || out.device() != dev) raise(PyExc_ValueError, "out must be contiguous and on q's device");
+        want_shape(out, q.sizes(), "out");
+    }
+    const int oc = out_dtype_code(out);
+    void* st = stream_of(dev);
+    const at::Tensor ws = maybe_workspace(a[9], dev, st, api.ftq_shared_workspace_bytes(R, K, Hq, p.hkv, p.d, max_seq));
+    uint8_t* base = p.base(a[7]);
+    Ref so(PyObject_GetAttr(self, names.signs)), ko(PyObject_GetAttr(self, names.levels_k)),
+        vo(PyObject_GetAttr(self, names.levels_v));
+    const Table signs(so.o), lk(ko.o), lv(vo.o);
+    int rc;
+    {
+        NoGil nogil;
+        rc = api.ftq_shared_attn(ptr<void>(q), dtype_code(q.scalar_type()), mptr<void>(out), oc, base, p.num_blocks, ptr<int32_t>(bt),
+                                 bt.size(1), ptr<int32_t>(sl), max_seq, ptr<int32_t>(sh), R, K, Hq, p.hkv, D, p.kb, p.vb, lk.p, lv.p,
+                                 signs.p, static_cast<float>(scale), ws_ptr(ws), ws_bytes(ws), st);
+    }
+    check(rc, "ftq_shared_attn");
+    if (ws.defined()) {     // (the status word lies where a decode call of one sequence has it)
+        Ref w(THPVariable_Wrap(ws)), d(THPDevice_New(dev));
+        Ref last(Py_BuildValue("(OLLLLO)", w.o, 1ll, static_cast<long long>(Hq), max_seq, 1ll, d.o));
+        if (PyObject_SetAttr(self, names._last_decode, last.o) < 0) throw PyError{};
+    }
+    if (a[8] != Py_None) return Py_NewRef(a[8]);
+    return THPVariable_Wrap(out);
+}
+
 // bind({name: address}, check, get_workspace, workspaces, host_table)
 PyObject* bind(PyObject* const* a) {
 #define X(name)                                                                     \
@@ -1154,6 +1208,7 @@ PyMethodDef methods[] = {
     FTQ_ENTRY(pages_shared_lens, 3),
     FTQ_ENTRY(copy_pages, 2),
     FTQ_ENTRY(beam_select, 5),
+    FTQ_ENTRY(paged_shared, 10),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", "Tensor-level host path over libftq_b200.so.",
                           -1, methods, nullptr, nullptr, nullptr, nullptr};

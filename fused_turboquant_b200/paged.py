@@ -230,6 +230,26 @@ class PagedKVPool:
         _require_cuda(self.pool, "pool")
         return Accepted(*_lib.native().tree_commit(self, block_table, seq_lens, tokens, parents, next_tokens, tree_lens))
 
+    def shared_workspace_bytes(self, groups: int, group: int, num_q_heads: int, max_seq_len: int) -> int:
+        return int(_lib.load().ftq_shared_workspace_bytes(groups, group, num_q_heads, self.num_kv_heads, self.head_dim, max_seq_len))
+
+    def shared_attention(self, q: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, max_seq_len: int,
+                         shared_lens: torch.Tensor, scale: float | None = None, layer: int = 0, out: torch.Tensor | None = None,
+                         workspace: torch.Tensor | None = None) -> torch.Tensor:
+        """One decode step of rows that share their leading blocks (beams, samples of a prompt).
+
+        q: [B, Hq, D], fp16 or bf16, not rotated; block_table [B, max_blocks], seq_lens [B]; shared_lens [groups]: B / groups
+        successive rows are a group, and the first ``shared_lens[g]`` tokens of its rows, rounded down to whole blocks, lie in the
+        same blocks (``PageTable.shared_lens`` says how many do).  They are read once for the group, through its longest
+        row.  The result is that of ``decode_attention`` on the rows; rows without tokens are zero.  Up to 1024 rows a group.
+        No host synchronisation; graph-capturable when out / workspace are passed in.  ``decode_status`` covers this call too.
+        """
+        _require_cuda(q, "q")
+        if _trace.ENABLED:
+            with _trace.nvtx("ftq.decode"):
+                return _lib.native().paged_shared(self, q, block_table, seq_lens, max_seq_len, shared_lens, scale, layer, out, workspace)
+        return _lib.native().paged_shared(self, q, block_table, seq_lens, max_seq_len, shared_lens, scale, layer, out, workspace)
+
     def copy_pages(self, copies: torch.Tensor) -> None:
         """Block ``copies[i, 0]`` over block ``copies[i, 1]``, in all layers (copies int32 [n, 2], as ``PageTable.fork`` and
         ``PageTable.compact`` list them; a pair with an id outside the pool is passed over).  No block may be written that

@@ -634,6 +634,25 @@ int ftq_copy_pages(uint8_t *pool, int64_t num_blocks, int64_t pool_layer_stride,
                    int head_dim, int bits_k, int bits_v, const int32_t *copies, int n_copies,
                    void *stream);
 
+/*
+ * Attention of one new token of every row, n_requests groups of `group` successive rows (at most
+ * 1024) whose leading blocks are the same.  q / out: [n_requests * group, Hq, head_dim], 16-bit
+ * queries; block_table, seq_lens as for ftq_paged_decode_attn, a row each.  shared_lens
+ * [n_requests]: the first so many tokens of a group's rows, rounded down to whole blocks, are
+ * common (ftq_pages_shared_lens); they are read once, through the row of the group that has the
+ * most tokens (of equal ones the first), and a row with fewer tokens attends those it has.  The
+ * result is that of ftq_paged_decode_attn on the rows.  Rows without tokens are zero.  The workspace
+ * holds at least ftq_shared_workspace_bytes(...) bytes, 16-byte aligned; the call's status is read with
+ * ftq_paged_decode_status(workspace, 1, Hq, Hkv, head_dim, max_seq_len, 1, ...).
+ */
+size_t ftq_shared_workspace_bytes(int n_requests, int group, int Hq, int Hkv, int head_dim, int max_seq_len);
+int ftq_shared_attn(const void *q, int q_dtype, void *out, int out_dtype, const uint8_t *pool,
+                    int64_t num_blocks, const int32_t *block_table, int max_blocks,
+                    const int32_t *seq_lens, int max_seq_len, const int32_t *shared_lens,
+                    int n_requests, int group, int Hq, int Hkv, int head_dim, int bits_k, int bits_v,
+                    const float *levels_k_host, const float *levels_v_host, const float *signs_host,
+                    float scale, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
