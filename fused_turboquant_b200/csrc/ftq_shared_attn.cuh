@@ -171,13 +171,21 @@ struct SharedPiece {
     int row;             // row of the block table
     int page0, n_pages;  // of the row's pages
     int tokens;          // from page0 on
-    int cols, tiles;     // columns, and tiles of eight
+    int cols;            // columns
     int col0;            // first column's row in its (group, KV head)
     int qh;              // group x Hkv + KV head
     int hkv;
     int limit0;          // tokens before page0
     bool ragged;         // columns of a group with fewer tokens
     int64_t out;         // rows in the workspace
+};
+
+// What a warp does with a piece: pages from its ring, TILES tiles of eight columns.
+template <int D, int BK, int BV, int TILES>
+struct SharedState {
+    using M = MmaCfg<D, BK, BV, 2>;
+    float o[TILES][2 * M::NMT][4], m[TILES][2], l[TILES][2];
+    float vlimit, vscale;       // the largest norm of a value that needs no other scale, and the power of two that goes with it
 };
 
 template <int D, int BK, int BV, int NT>
@@ -243,10 +251,10 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
     __syncthreads();
 
     const int total = s_plan[entries], share = s_plan[entries + 1], G = p.Hq / p.Hkv;
-    const int64_t from = static_cast<int64_t>(blockIdx.x * C::WARPS + warp) * share;
+    const int me = blockIdx.x * C::WARPS + warp;
+    const int64_t from = static_cast<int64_t>(me) * share;
     if (from >= total) return;
     const int end = static_cast<int>(min(from + share, static_cast<int64_t>(total)));
-    const int me = blockIdx.x * C::WARPS + warp;
 
     auto locate = [&](int pos) {
         SharedPiece it{};
@@ -264,7 +272,6 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
         it.hkv = u / blocks;
         const int r = group ? lo : (lo - p.R) / p.K, common = p.plan_tokens[lo], leader = p.plan_leader[lo];
         it.cols = min(C::COLS, all - blk * C::COLS);
-        it.tiles = (it.cols + 7) / 8;
         it.qh = r * p.Hkv + it.hkv;
         it.row = group ? leader : lo - p.R;
         it.col0 = (group ? 0 : (lo - p.R - r * p.K) * G) + blk * C::COLS;
@@ -291,11 +298,12 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
 
     const uint32_t blk_stride = static_cast<uint32_t>(p.Hkv) * C::PAGE_BYTES;
     const uint64_t policy = l2_evict_first_policy();
-    const bool odd = g & 1;
-    const uint32_t sel_own = odd ? 0x4432u : 0x4410u;
-    const uint32_t koff = (4 * (g >> 1) + (g & 1)) * C::PDK + slice_word<C::KSB>(tg), ksh = slice_shift<C::KSB>(tg);
-    const uint32_t noff = C::OFF_KN + 8 * (g >> 1);
-    const uint32_t vsh = slice_shift<C::VSB>(g);
+    // A lane's rows of S: the page tokens whose weights the transposition then hands to the lanes that have those tokens'
+    // values, in the order of their registers (register j of lane tg: token 4 tg + (j + tg) % 4 where ROT is set)
+    const int q4 = g >> 1, turn = C::ROT ? q4 : 0, tokA = 4 * q4 + (((g & 1) + turn) & 3), tokB = 4 * q4 + (((g & 1) + 2 + turn) & 3);
+    const uint32_t koffA = tokA * C::PDK + slice_word<C::KSB>(tg), koffB = tokB * C::PDK + slice_word<C::KSB>(tg), ksh = slice_shift<C::KSB>(tg);
+    const uint32_t noff = C::OFF_KN + 8 * q4, vsh = slice_shift<C::VSB>(g);
+    const uint32_t sel_norms = (2 * (tokA & 3)) * 0x11u + 0x10u + ((2 * (tokB & 3)) * 0x11u + 0x10u) * 0x100u;     // the two tokens' of a quad's fp16 norms
     const uint32_t lk_lane = window | (BK == 2 ? (lane & 15) * 8 : lane * 4);
     const uint32_t lv_lane = window | 128u | (BV == 2 ? (lane & 15) * 8 : lane * 4);
     uint32_t phases = 0;      // bit r: parity that the next wait on ring buffer r expects; bit RING: the queries'
@@ -305,10 +313,8 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
     bool test_drop = blockIdx.x == 0 && warp == 5;
 #endif
 
-    SharedPiece it{};
-    for (int pos = static_cast<int>(from); pos < end; pos = it.next) {
-        it = locate(pos);
-        if (it.n_pages == 0) continue;      // (a share that ends among a unit's places on its own)
+    auto walk = [&](auto tiles_tag, const SharedPiece& it) {
+        constexpr int TILES = decltype(tiles_tag)::value;
         const uint8_t* const base = p.pool + static_cast<int64_t>(it.hkv) * C::PAGE_BYTES;
         bool bad = false;
         // block ids of pages k0 .. k0 + 31 of the piece; an id outside the pool is replaced by 0 and remembered
@@ -350,18 +356,20 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
             for (int k = 0; k < C::RING; k++)
                 if (k < it.n_pages) request(ids, k);
         }
-        float oacc[NT][2 * NMT][4], m_run[NT][2], l_run[NT][2];
+        SharedState<D, BK, BV, TILES> st;
+        constexpr float NONE = -3e38f;      // the maximum of no tokens: every score is far above it
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
+        for (int nt = 0; nt < TILES; nt++) {
 #pragma unroll
             for (int mt = 0; mt < 2 * NMT; mt++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) oacc[nt][mt][i] = 0.f;
-            m_run[nt][0] = m_run[nt][1] = -INFINITY;
-            l_run[nt][0] = l_run[nt][1] = 0.f;
+                for (int i = 0; i < 4; i++) st.o[nt][mt][i] = 0.f;
+            st.m[nt][0] = st.m[nt][1] = NONE;
+            st.l[nt][0] = st.l[nt][1] = 0.f;
         }
-        float vmax = 0.f, vscale = 1.f;     // the largest norm of a value so far, lazily, and the power of two that goes with it
-        const uint32_t q_lane = my_q + g * (D * 2), q_odd = ((it.col0 + g) & 1) * 64 ^ tg * 16;
+        st.vlimit = 0.f;
+        st.vscale = 1.f;
+        const uint32_t q_lane = my_q + g * (D * 2), q_odd = (((it.col0 + g) & 1) * 64) ^ (tg * 16);
         if (!lost && !mbar_wait(q_bar, (phases >> C::RING) & 1)) lost = true;
         phases ^= 1u << C::RING;
         lost = __any_sync(0xffffffffu, lost);
@@ -381,9 +389,9 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
             phases ^= 1u << rb;
             const uint32_t page = my_ring + rb * C::PAGE_BYTES;
             uint32_t kw[2][C::KW], vw[4][C::VW];
-            lds_slice<C::KSB>(page + koff, ksh, kw[0]);
-            lds_slice<C::KSB>(page + koff + 2 * C::PDK, ksh, kw[1]);
-            const uint2 kn = lds64(page + noff), vn = lds64(page + noff + (C::OFF_VN - C::OFF_KN));
+            lds_slice<C::KSB>(page + koffA, ksh, kw[0]);
+            lds_slice<C::KSB>(page + koffB, ksh, kw[1]);
+            const uint2 kn2 = lds64(page + noff), vn2 = lds64(page + noff + (C::OFF_VN - C::OFF_KN));
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int u = C::ROT ? (j + tg) & 3 : j, slice = g ^ ((u & 2) << 1);
@@ -393,8 +401,8 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
             __syncwarp();
             if (k + C::RING < it.n_pages) request((k + C::RING) >> 5 == k >> 5 ? ids : ids_next, k + C::RING);
 
-            // ---- S = K Q^T
-            float c[NT][4];
+            // ---- S = K Q^T, two chains
+            float c[TILES][2][4];
             {
                 typename WK::template Run<C::KW> run[2];
 #pragma unroll
@@ -412,110 +420,98 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
                         WK::pairs(run[1], kb + s, lk_lane, a[s][1], a[s][3]);
                     }
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        if (nt >= it.tiles) continue;
+                    for (int nt = 0; nt < TILES; nt++) {
                         const uint4 q = lds128(q_lane + nt * 8 * (D * 2) + ((kb / 2 * 64) ^ q_odd));
-                        if (kb == 0) mma_16816_z(c[nt], a[0][0], a[0][1], a[0][2], a[0][3], q.x, q.y);
-                        else mma_16816(c[nt], a[0][0], a[0][1], a[0][2], a[0][3], q.x, q.y);
-                        mma_16816(c[nt], a[1][0], a[1][1], a[1][2], a[1][3], q.z, q.w);
+                        if (kb == 0) {
+                            mma_16816_z(c[nt][0], a[0][0], a[0][1], a[0][2], a[0][3], q.x, q.y);
+                            mma_16816_z(c[nt][1], a[1][0], a[1][1], a[1][2], a[1][3], q.z, q.w);
+                        } else {
+                            mma_16816(c[nt][0], a[0][0], a[0][1], a[0][2], a[0][3], q.x, q.y);
+                            mma_16816(c[nt][1], a[1][0], a[1][1], a[1][2], a[1][3], q.z, q.w);
+                        }
                     }
                 }
             }
             // ---- softmax (base 2), per column; lanes of a column: the eight that differ in g
-            const int tokA = 4 * (g >> 1) + (g & 1), left = it.tokens - k * kPageTokens;
-            const float kna = half_bits_to_float(__byte_perm(kn.x, 0u, sel_own)), knb = half_bits_to_float(__byte_perm(kn.y, 0u, sel_own));
-            float vna = half_bits_to_float(__byte_perm(vn.x, 0u, sel_own)), vnb = half_bits_to_float(__byte_perm(vn.y, 0u, sel_own));
+            const uint32_t knab = __byte_perm(kn2.x, kn2.y, sel_norms), vnab = __byte_perm(vn2.x, vn2.y, sel_norms);
+            const float2 kn = __half22float2(*reinterpret_cast<const __half2*>(&knab));
+            float2 vn = __half22float2(*reinterpret_cast<const __half2*>(&vnab));
+            const int left = it.tokens - k * kPageTokens;
             const bool whole = left >= kPageTokens && !it.ragged;
-            bool above = false;
+            auto masked = [&](int nt, int h, int tok) {
+                int mine = left;
+                const int col = 8 * nt + 2 * tg + h;
+                if (it.ragged && col < it.cols)
+                    mine = min(mine, shared_len(p, it.qh / p.Hkv * p.K + (it.col0 + col) / G) - it.limit0 - k * kPageTokens);
+                return tok >= mine;
+            };
+            float x[TILES][4];          // scores less the maximum
+            float most = -INFINITY;
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                if (nt >= it.tiles) continue;
+            for (int nt = 0; nt < TILES; nt++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    c[nt][h] *= kna;
-                    c[nt][2 + h] *= knb;
+                for (int i = 0; i < 4; i++) {
+                    c[nt][0][i] += c[nt][1][i];
+                    x[nt][i] = fmaf(c[nt][0][i], i < 2 ? kn.x : kn.y, -st.m[nt][i & 1]);
                 }
-            }
             if (!whole) {
-                if (tokA >= left) vna = 0.f;
-                if (tokA + 2 >= left) vnb = 0.f;
+                if (tokA >= left) vn.x = 0.f;
+                if (tokB >= left) vn.y = 0.f;
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                for (int nt = 0; nt < TILES; nt++)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        int mine = left;
-                        const int col = 8 * nt + 2 * tg + h;
-                        if (it.ragged && col < it.cols)
-                            mine = min(mine, shared_len(p, it.qh / p.Hkv * p.K + (it.col0 + col) / G) - it.limit0 - k * kPageTokens);
-                        if (tokA >= mine) c[nt][h] = -INFINITY;
-                        if (tokA + 2 >= mine) c[nt][2 + h] = -INFINITY;
-                    }
+                    for (int i = 0; i < 4; i++)
+                        if (masked(nt, i & 1, i < 2 ? tokA : tokB)) x[nt][i] = -INFINITY;
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                if (nt >= it.tiles) continue;
+            for (int nt = 0; nt < TILES; nt++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) above |= fmaxf(c[nt][h], c[nt][2 + h]) > m_run[nt][h] + kLazyMaxSlack;
-            }
-            above |= fmaxf(vna, vnb) > vmax * 1024.f;
-            if (__any_sync(0xffffffffu, above)) {
-                float v = fmaxf(vna, vnb);
+                for (int i = 0; i < 4; i++) most = fmaxf(most, x[nt][i]);
+            if (__any_sync(0xffffffffu, most > kLazyMaxSlack || fmaxf(vn.x, vn.y) > st.vlimit)) {
+                float v = fmaxf(vn.x, vn.y), change = 1.f;
 #pragma unroll
                 for (int d = 4; d <= 16; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-                float change = 1.f;
-                if (v > vmax * 1024.f) {        // (norms are not negative; infinite ones stay what they are)
-                    vmax = fminf(v, 65504.f);
-                    // 2^-e with vmax in [2^e, 2^(e + 1))
-                    const float now = __uint_as_float((254u << 23) - (__float_as_uint(vmax) & 0x7f800000u));
-                    change = now / vscale;
-                    vscale = now;
+                if (v > st.vlimit) {        // (norms are not negative; infinite ones stay what they are)
+                    // 2^-e with the norm in [2^e, 2^(e + 1))
+                    const float top = fminf(v, 65504.f), now = __uint_as_float((254u << 23) - (__float_as_uint(top) & 0x7f800000u));
+                    change = now / st.vscale;
+                    st.vscale = now;
+                    st.vlimit = top * 1024.f;
                 }
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
+                for (int nt = 0; nt < TILES; nt++) {
                     float corr[2];
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        float m = nt < it.tiles ? fmaxf(c[nt][h], c[nt][2 + h]) : -INFINITY;
+                        const float a = c[nt][0][h] * kn.x, b = c[nt][0][2 + h] * kn.y;
+                        float m = fmaxf(x[nt][h] == -INFINITY ? NONE : a, x[nt][2 + h] == -INFINITY ? NONE : b);
 #pragma unroll
                         for (int d = 4; d <= 16; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-                        const float now = fmaxf(m_run[nt][h], m);
-                        corr[h] = now == -INFINITY ? 1.f : fast_exp2(m_run[nt][h] - now);
-                        l_run[nt][h] *= corr[h];
-                        m_run[nt][h] = now;
+                        const float now = fmaxf(st.m[nt][h], m);
+                        corr[h] = fast_exp2(st.m[nt][h] - now);
+                        st.l[nt][h] *= corr[h];
                         corr[h] *= change;
+                        st.m[nt][h] = now;
+                        x[nt][h] = x[nt][h] == -INFINITY ? -INFINITY : a - now;
+                        x[nt][2 + h] = x[nt][2 + h] == -INFINITY ? -INFINITY : b - now;
                     }
 #pragma unroll
                     for (int mt = 0; mt < 2 * NMT; mt++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) oacc[nt][mt][i] *= corr[i & 1];
+                        for (int i = 0; i < 4; i++) st.o[nt][mt][i] *= corr[i & 1];
                 }
             }
-            vna *= vscale;
-            vnb *= vscale;
-            uint32_t pb[NT][2];
+            vn.x *= st.vscale;
+            vn.y *= st.vscale;
+            uint32_t pb[TILES][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                if (nt >= it.tiles) continue;
-                float wa[2], wb[2];
+            for (int nt = 0; nt < TILES; nt++) {
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    // (a column without a token yet has nothing but -inf)
-                    const float ref = m_run[nt][h] == -INFINITY ? 0.f : m_run[nt][h];
-                    const float pa = fast_exp2(c[nt][h] - ref), pbv = fast_exp2(c[nt][2 + h] - ref);
-                    l_run[nt][h] += pa + pbv;
-                    wa[h] = pa * vna;
-                    wb[h] = pbv * vnb;
-                }
-                uint32_t t0 = movmatrix_trans(pack_weights(wa[0], wa[1])), t1 = movmatrix_trans(pack_weights(wb[0], wb[1]));
-                if constexpr (C::ROT) {     // by tg tokens, to match the values' registers
-                    if (tg & 2) { const uint32_t x = t0; t0 = t1; t1 = x; }
-                    const uint32_t sh = (tg & 1) * 16;
-                    const uint32_t lo = __funnelshift_r(t0, t1, sh), hi = __funnelshift_r(t1, t0, sh);
-                    t0 = lo;
-                    t1 = hi;
-                }
-                pb[nt][0] = t0;
-                pb[nt][1] = t1;
+                for (int i = 0; i < 4; i++) x[nt][i] = fast_exp2(x[nt][i]);
+                st.l[nt][0] += x[nt][0] + x[nt][2];
+                st.l[nt][1] += x[nt][1] + x[nt][3];
+                pb[nt][0] = movmatrix_trans(pack_weights(x[nt][0] * vn.x, x[nt][1] * vn.x));
+                pb[nt][1] = movmatrix_trans(pack_weights(x[nt][2] * vn.y, x[nt][3] * vn.y));
             }
             // ---- O^T += V^T P^T
             {
@@ -526,14 +522,13 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
                 for (int j = 0; j < 4; j++) WV::shift(run[j]);
 #pragma unroll
                 for (int m2 = 0; m2 < NMT; m2++) {
-                    uint32_t x[4], y[4];
+                    uint32_t e[4], f[4];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) WV::pairs(run[j], m2, lv_lane, x[j], y[j]);
+                    for (int j = 0; j < 4; j++) WV::pairs(run[j], m2, lv_lane, e[j], f[j]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        if (nt >= it.tiles) continue;
-                        mma_16816(oacc[nt][2 * m2], x[0], x[1], x[2], x[3], pb[nt][0], pb[nt][1]);
-                        mma_16816(oacc[nt][2 * m2 + 1], y[0], y[1], y[2], y[3], pb[nt][0], pb[nt][1]);
+                    for (int nt = 0; nt < TILES; nt++) {
+                        mma_16816(st.o[nt][2 * m2], e[0], e[1], e[2], e[3], pb[nt][0], pb[nt][1]);
+                        mma_16816(st.o[nt][2 * m2 + 1], f[0], f[1], f[2], f[3], pb[nt][0], pb[nt][1]);
                     }
                 }
             }
@@ -544,14 +539,13 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
         // ---- the piece's rows: O in coordinates (D/8) g .. + D/8 of columns 2 tg, 2 tg + 1, (m, l) behind them
         bad = __any_sync(0xffffffffu, bad);
         bad_any |= bad;
-        const float scale = lost || bad ? __int_as_float(0x7fc00000) : p.inv_v_scale / vscale;
+        const float scale = lost || bad ? __int_as_float(0x7fc00000) : p.inv_v_scale / st.vscale;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            if (nt >= it.tiles) continue;
+        for (int nt = 0; nt < TILES; nt++) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int col = 8 * nt + 2 * tg + h;
-                float l = l_run[nt][h];
+                float l = st.l[nt][h];
 #pragma unroll
                 for (int d = 4; d <= 16; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
                 if (col >= it.cols) continue;
@@ -559,11 +553,21 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
 #pragma unroll
                 for (int f = 0; f < NMT; f++)
                     *reinterpret_cast<float4*>(to + (D / 8) * g + 4 * f) =
-                        make_float4(oacc[nt][2 * f][h] * scale, oacc[nt][2 * f][2 + h] * scale, oacc[nt][2 * f + 1][h] * scale, oacc[nt][2 * f + 1][2 + h] * scale);
-                if (g == 0) *reinterpret_cast<float2*>(to + D) = make_float2(lost || bad ? __int_as_float(0x7fc00000) : m_run[nt][h], l);
+                        make_float4(st.o[nt][2 * f][h] * scale, st.o[nt][2 * f][2 + h] * scale, st.o[nt][2 * f + 1][h] * scale, st.o[nt][2 * f + 1][2 + h] * scale);
+                if (g == 0)
+                    *reinterpret_cast<float2*>(to + D) =
+                        make_float2(lost || bad ? __int_as_float(0x7fc00000) : st.m[nt][h] == NONE ? -INFINITY : st.m[nt][h], l);
             }
         }
         __syncwarp();       // (the next piece's queries come to where these were read)
+    };
+
+    for (int pos = static_cast<int>(from); pos < end;) {
+        const SharedPiece it = locate(pos);
+        pos = it.next;
+        if (it.n_pages == 0) continue;      // (a share that ends among a unit's places on its own)
+        if (NT > 1 && it.cols <= 8) walk(std::integral_constant<int, 1>{}, it);
+        else walk(std::integral_constant<int, NT>{}, it);
     }
     if (lane == 0 && (lost || bad_any)) atomicOr(p.status, (lost ? kStatusWaitExpired : 0) | (bad_any ? kStatusBadBlock : 0));
 }
