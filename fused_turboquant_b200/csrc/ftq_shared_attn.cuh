@@ -160,7 +160,12 @@ __global__ void __launch_bounds__(256) shared_prepare_kernel(const __grid_consta
 }
 
 // ------------------------------------------------------------------ attention
-// (weights stay below 2^14, see below; those of infinite norms are infinite)
+// The reference maximum of a column is renewed when a score exceeds it by 2^kSharedSlack, the values' scale when a norm
+// exceeds the one that it goes with by kSharedNorms: a weight stays below 2^10 * 2 * 16 = 2^15, which fp16 holds, and one that is
+// 2^-14 of a column's largest still has all its bits.  (One for all columns of a warp: with the decode kernel's slack of 3
+// every third page of the serving batch below did it, 512 scores of which one in fifty has three times the others' size.)
+constexpr float kSharedSlack = 10.f, kSharedNorms = 16.f;
+// (those of infinite norms are infinite)
 __device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -467,7 +472,7 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
             for (int nt = 0; nt < TILES; nt++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) most = fmaxf(most, x[nt][i]);
-            if (__any_sync(0xffffffffu, most > kLazyMaxSlack || fmaxf(vn.x, vn.y) > st.vlimit)) {
+            if (__any_sync(0xffffffffu, most > kSharedSlack || fmaxf(vn.x, vn.y) > st.vlimit)) {
                 float v = fmaxf(vn.x, vn.y), change = 1.f;
 #pragma unroll
                 for (int d = 4; d <= 16; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
@@ -476,7 +481,7 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
                     const float top = fminf(v, 65504.f), now = __uint_as_float((254u << 23) - (__float_as_uint(top) & 0x7f800000u));
                     change = now / st.vscale;
                     st.vscale = now;
-                    st.vlimit = top * 1024.f;
+                    st.vlimit = top * kSharedNorms;
                 }
 #pragma unroll
                 for (int nt = 0; nt < TILES; nt++) {
