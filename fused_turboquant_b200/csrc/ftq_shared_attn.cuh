@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
     const uint32_t sel_norms = (2 * (tokA & 3)) * 0x11u + 0x10u + ((2 * (tokB & 3)) * 0x11u + 0x10u) * 0x100u;     // the two tokens' of a quad's fp16 norms
     const uint32_t lk_lane = window | (BK == 2 ? (lane & 15) * 8 : lane * 4);
     const uint32_t lv_lane = window | 128u | (BV == 2 ? (lane & 15) * 8 : lane * 4);
-    uint32_t phases = 0;      // bit r: parity that the next wait on ring buffer r expects; bit RING: the queries'
+    uint32_t taken = 0, q_parity = 0;     // pages that the warp has taken from its ring: buffer taken % RING, its parity (taken / RING) % 2
     bool lost = false;        // a wait ran out: nothing is requested any more, and the warp's pieces are NaN
     bool bad_any = false;
 #ifdef FTQ_TEST_WAIT_EXPIRY
@@ -335,21 +335,22 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
             }
             return id;
         };
-        auto request = [&](int ids, int k) {
-            const uint32_t id = __shfl_sync(0xffffffffu, ids, k & 31);
-            const int rb = k % C::RING;
-            if (lane == 0) {
+        // page k of the piece to the ring, by the lane that has its id
+        const uint32_t first_page = taken;
+        auto request = [&](int ids, uint32_t k) {
+            const uint32_t rb = (first_page + k) % C::RING;
+            if (lane == (k & 31)) {
                 mbar_expect_tx(my_bars + 8 * rb, C::PAGE_BYTES);
 #ifdef FTQ_TEST_WAIT_EXPIRY
-                const bool drop = test_drop;    // (see kMbarSpinLimit)
+                const bool drop = test_drop && k == 0;    // (see kMbarSpinLimit)
                 test_drop = false;
                 if (!drop)
 #endif
-                bulk_g2s_hint(my_ring + rb * C::PAGE_BYTES, base + static_cast<uint64_t>(id) * blk_stride, C::PAGE_BYTES, my_bars + 8 * rb, policy);
+                bulk_g2s_hint(my_ring + rb * C::PAGE_BYTES, base + static_cast<uint64_t>(static_cast<uint32_t>(ids)) * blk_stride, C::PAGE_BYTES, my_bars + 8 * rb, policy);
             }
             __syncwarp();
         };
-        int ids = load_ids(0), ids_next = 0;
+        int ids = load_ids(0), ids_next = load_ids(32);
         const bool requested = !lost;
         if (requested) {
             if (lane == 0) {
@@ -359,55 +360,38 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
             __syncwarp();
 #pragma unroll
             for (int k = 0; k < C::RING; k++)
-                if (k < it.n_pages) request(ids, k);
+                if (k < it.n_pages) request(ids, static_cast<uint32_t>(k));
         }
         SharedState<D, BK, BV, TILES> st;
-        constexpr float NONE = -3e38f;      // the maximum of no tokens: every score is far above it
 #pragma unroll
         for (int nt = 0; nt < TILES; nt++) {
 #pragma unroll
             for (int mt = 0; mt < 2 * NMT; mt++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) st.o[nt][mt][i] = 0.f;
-            st.m[nt][0] = st.m[nt][1] = NONE;
+            st.m[nt][0] = st.m[nt][1] = 0.f;
             st.l[nt][0] = st.l[nt][1] = 0.f;
         }
         st.vlimit = 0.f;
         st.vscale = 1.f;
         const uint32_t q_lane = my_q + g * (D * 2), q_odd = (((it.col0 + g) & 1) * 64) ^ (tg * 16);
-        if (!lost && !mbar_wait(q_bar, (phases >> C::RING) & 1)) lost = true;
-        phases ^= 1u << C::RING;
-        lost = __any_sync(0xffffffffu, lost);
+        if (!lost) lost = !__all_sync(0xffffffffu, mbar_wait(q_bar, q_parity));
+        q_parity ^= 1;
 
         int k = 0;
         for (; k < it.n_pages; k++) {
-            if ((k & 31) == 0) {        // (a batch of ids ahead)
-                if (k > 0) ids = ids_next;
-                ids_next = load_ids(k + 32);
-            }
-            const int rb = k % C::RING;
-            if (!lost) {
-                if (!mbar_wait(my_bars + 8 * rb, (phases >> rb) & 1)) lost = true;
-                lost = __any_sync(0xffffffffu, lost);
-            }
+            const uint32_t rb = taken % C::RING;
+            // (every lane polls; the vote makes one answer of theirs)
+            if (!lost) lost = !__all_sync(0xffffffffu, mbar_wait(my_bars + 8 * rb, taken / C::RING & 1));
             if (lost) break;
-            phases ^= 1u << rb;
+            taken++;
             const uint32_t page = my_ring + rb * C::PAGE_BYTES;
             uint32_t kw[2][C::KW], vw[4][C::VW];
             lds_slice<C::KSB>(page + koffA, ksh, kw[0]);
             lds_slice<C::KSB>(page + koffB, ksh, kw[1]);
             const uint2 kn2 = lds64(page + noff), vn2 = lds64(page + noff + (C::OFF_VN - C::OFF_KN));
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int u = C::ROT ? (j + tg) & 3 : j, slice = g ^ ((u & 2) << 1);
-                lds_slice<C::VSB>(page + C::OFF_VC + (4 * tg + u) * C::PDV + slice_word<C::VSB>(slice), vsh, vw[j]);
-            }
-            // the buffer is free for the page RING further on
-            __syncwarp();
-            if (k + C::RING < it.n_pages) request((k + C::RING) >> 5 == k >> 5 ? ids : ids_next, k + C::RING);
-
-            // ---- S = K Q^T, two chains
-            float c[TILES][2][4];
+            // ---- S = K Q^T
+            float x[TILES][4];          // scores, then less the maximum, then weights
             {
                 typename WK::template Run<C::KW> run[2];
 #pragma unroll
@@ -427,52 +411,59 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
 #pragma unroll
                     for (int nt = 0; nt < TILES; nt++) {
                         const uint4 q = lds128(q_lane + nt * 8 * (D * 2) + ((kb / 2 * 64) ^ q_odd));
-                        if (kb == 0) {
-                            mma_16816_z(c[nt][0], a[0][0], a[0][1], a[0][2], a[0][3], q.x, q.y);
-                            mma_16816_z(c[nt][1], a[1][0], a[1][1], a[1][2], a[1][3], q.z, q.w);
-                        } else {
-                            mma_16816(c[nt][0], a[0][0], a[0][1], a[0][2], a[0][3], q.x, q.y);
-                            mma_16816(c[nt][1], a[1][0], a[1][1], a[1][2], a[1][3], q.z, q.w);
-                        }
+                        if (kb == 0) mma_16816_z(x[nt], a[0][0], a[0][1], a[0][2], a[0][3], q.x, q.y);
+                        else mma_16816(x[nt], a[0][0], a[0][1], a[0][2], a[0][3], q.x, q.y);
+                        mma_16816(x[nt], a[1][0], a[1][1], a[1][2], a[1][3], q.z, q.w);
                     }
                 }
             }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int u = C::ROT ? (j + tg) & 3 : j, slice = g ^ ((u & 2) << 1);
+                lds_slice<C::VSB>(page + C::OFF_VC + (4 * tg + u) * C::PDV + slice_word<C::VSB>(slice), vsh, vw[j]);
+            }
+            // the buffer is free for the page RING further on
+            __syncwarp();
+            const int next = k + C::RING;
+            if (next < it.n_pages) {
+                if ((next & 31) == 0) {     // (a batch of ids ahead)
+                    ids = ids_next;
+                    ids_next = load_ids(next + 32);
+                }
+                request(ids, next);
+            }
+
             // ---- softmax (base 2), per column; lanes of a column: the eight that differ in g
             const uint32_t knab = __byte_perm(kn2.x, kn2.y, sel_norms), vnab = __byte_perm(vn2.x, vn2.y, sel_norms);
             const float2 kn = __half22float2(*reinterpret_cast<const __half2*>(&knab));
             float2 vn = __half22float2(*reinterpret_cast<const __half2*>(&vnab));
             const int left = it.tokens - k * kPageTokens;
             const bool whole = left >= kPageTokens && !it.ragged;
-            auto masked = [&](int nt, int h, int tok) {
-                int mine = left;
-                const int col = 8 * nt + 2 * tg + h;
-                if (it.ragged && col < it.cols)
-                    mine = min(mine, shared_len(p, it.qh / p.Hkv * p.K + (it.col0 + col) / G) - it.limit0 - k * kPageTokens);
-                return tok >= mine;
-            };
-            float x[TILES][4];          // scores less the maximum
             float most = -INFINITY;
 #pragma unroll
             for (int nt = 0; nt < TILES; nt++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    c[nt][0][i] += c[nt][1][i];
-                    x[nt][i] = fmaf(c[nt][0][i], i < 2 ? kn.x : kn.y, -st.m[nt][i & 1]);
-                }
+                for (int i = 0; i < 4; i++) x[nt][i] = fmaf(x[nt][i], i < 2 ? kn.x : kn.y, -st.m[nt][i & 1]);
             if (!whole) {
                 if (tokA >= left) vn.x = 0.f;
                 if (tokB >= left) vn.y = 0.f;
 #pragma unroll
                 for (int nt = 0; nt < TILES; nt++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (masked(nt, i & 1, i < 2 ? tokA : tokB)) x[nt][i] = -INFINITY;
+                    for (int h = 0; h < 2; h++) {
+                        int mine = left;
+                        const int col = 8 * nt + 2 * tg + h;
+                        if (it.ragged && col < it.cols)
+                            mine = min(mine, shared_len(p, it.qh / p.Hkv * p.K + (it.col0 + col) / G) - it.limit0 - k * kPageTokens);
+                        if (tokA >= mine) x[nt][h] = -INFINITY;
+                        if (tokB >= mine) x[nt][2 + h] = -INFINITY;
+                    }
             }
 #pragma unroll
             for (int nt = 0; nt < TILES; nt++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) most = fmaxf(most, x[nt][i]);
-            if (__any_sync(0xffffffffu, most > kSharedSlack || fmaxf(vn.x, vn.y) > st.vlimit)) {
+            if (__any_sync(0xffffffffu, k == 0 || most > kSharedSlack || fmaxf(vn.x, vn.y) > st.vlimit)) {
                 float v = fmaxf(vn.x, vn.y), change = 1.f;
 #pragma unroll
                 for (int d = 4; d <= 16; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
@@ -488,17 +479,17 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
                     float corr[2];
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        const float a = c[nt][0][h] * kn.x, b = c[nt][0][2 + h] * kn.y;
-                        float m = fmaxf(x[nt][h] == -INFINITY ? NONE : a, x[nt][2 + h] == -INFINITY ? NONE : b);
+                        float m = fmaxf(x[nt][h], x[nt][2 + h]);
 #pragma unroll
                         for (int d = 4; d <= 16; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-                        const float now = fmaxf(st.m[nt][h], m);
-                        corr[h] = fast_exp2(st.m[nt][h] - now);
+                        // (of a column that has no token in its first page there are none, see below)
+                        const float up = k == 0 ? (m == -INFINITY ? 0.f : m) : fmaxf(m, 0.f);
+                        corr[h] = k == 0 ? 0.f : fast_exp2(-up);
                         st.l[nt][h] *= corr[h];
                         corr[h] *= change;
-                        st.m[nt][h] = now;
-                        x[nt][h] = x[nt][h] == -INFINITY ? -INFINITY : a - now;
-                        x[nt][2 + h] = x[nt][2 + h] == -INFINITY ? -INFINITY : b - now;
+                        st.m[nt][h] += up;
+                        x[nt][h] -= up;
+                        x[nt][2 + h] -= up;
                     }
 #pragma unroll
                     for (int mt = 0; mt < 2 * NMT; mt++)
@@ -540,7 +531,7 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
         }
         // (no copy of this warp's is on its way when it gives up)
         if (lost && requested)
-            for (const int last = min(k + C::RING, it.n_pages); k < last; k++) mbar_wait(my_bars + 8 * (k % C::RING), (phases >> (k % C::RING)) & 1);
+            for (const int last = min(k + C::RING, it.n_pages); k < last; k++, taken++) mbar_wait(my_bars + 8 * (taken % C::RING), taken / C::RING & 1);
         // ---- the piece's rows: O in coordinates (D/8) g .. + D/8 of columns 2 tg, 2 tg + 1, (m, l) behind them
         bad = __any_sync(0xffffffffu, bad);
         bad_any |= bad;
@@ -561,7 +552,7 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
                         make_float4(st.o[nt][2 * f][h] * scale, st.o[nt][2 * f][2 + h] * scale, st.o[nt][2 * f + 1][h] * scale, st.o[nt][2 * f + 1][2 + h] * scale);
                 if (g == 0)
                     *reinterpret_cast<float2*>(to + D) =
-                        make_float2(lost || bad ? __int_as_float(0x7fc00000) : st.m[nt][h] == NONE ? -INFINITY : st.m[nt][h], l);
+                        make_float2(lost || bad ? __int_as_float(0x7fc00000) : l == 0.f ? -INFINITY : st.m[nt][h], l);
             }
         }
         __syncwarp();       // (the next piece's queries come to where these were read)
