@@ -10,26 +10,26 @@ namespace {
 
 template <typename T>
 cudaError_t run_select(const SelectParams& p, cudaStream_t stream) {
-    const int rows_smem = 8 * select_pow2(std::max(kSelectMaxKeep * kSelectVectors, kSelectThreads));
-    const int join_smem = 16 * select_join_size(p.K, p.chunks, p.keep, p.n);
+    // what the sorts need (the tokens that are ranked by counting are fewer)
+    const int rounds = ((p.chunk * static_cast<int>(sizeof(T)) + 15) / 16 + 1 + kSelectThreads - 1) / kSelectThreads;
+    const int rows_smem = 8 * select_pow2(std::max({kSelectRoom, p.keep * rounds, p.keep * 16 / static_cast<int>(sizeof(T))}));
+    const int join_smem = 16 * std::max(kSelectRoom, select_join_size(p.K, p.chunks, p.keep, p.n));
     cudaError_t e = allow_smem<beam_join_kernel<T>>(16 * kSelectJoin);
     if (e != cudaSuccess) return e;
-    const int rounds = ((p.chunk * static_cast<int>(sizeof(T)) + 15) / 16 + 1 + kSelectThreads - 1) / kSelectThreads;
-    const int sorted = std::max({kSelectThreads, p.keep * rounds, p.keep * 16 / static_cast<int>(sizeof(T))});
     const int64_t ctas = static_cast<int64_t>(p.R) * p.K * p.chunks;
-    e = launch_dependent(beam_rows_kernel<T>, dim3(static_cast<unsigned>(ctas)), kSelectThreads, std::min(rows_smem, 8 * select_pow2(sorted)),
-                         stream, p);
+    e = launch_dependent(beam_rows_kernel<T>, dim3(static_cast<unsigned>(ctas)), kSelectThreads, rows_smem, stream, p);
     if (e != cudaSuccess) return e;
     return launch_dependent(beam_join_kernel<T>, dim3(p.R), kSelectThreads, join_smem, stream, p);
 }
+static_assert(8 * select_pow2(kSelectMaxKeep * kSelectVectors) <= 48 * 1024, "shared memory of beam_rows_kernel");
 
 }  // namespace
 
-// A CTA's part of a row is as long as its threads' vectors can be sorted, and as short as fills the device where there are few
-// rows, but at least a vector a thread (shorter ones leave more to be joined than they save).
+// A CTA's part of a row is as long as its threads' vectors can be looked at again, and as short as fills the device where there are
+// few rows, but at least a vector a thread (shorter ones leave more to be joined than they save).
 SelectPlan select_plan(int dtype, int requests, int beams, int vocab, int keep) {
     const int n = dtype == kF32 ? 4 : 8, most = (kSelectVectors * kSelectThreads - 1) * n, least = kSelectThreads * n;
-    const int64_t rows = static_cast<int64_t>(requests) * beams, want = 2 * sm_count();
+    const int64_t rows = static_cast<int64_t>(requests) * beams, want = 12 * sm_count();
     int64_t chunks = std::max<int64_t>((static_cast<int64_t>(vocab) + most - 1) / most, rows > 0 ? (want + rows - 1) / rows : 1);
     int64_t chunk = std::max<int64_t>((vocab + chunks - 1) / chunks, std::min(least, vocab));
     chunk = std::min<int64_t>((chunk + n - 1) / n * n, most);

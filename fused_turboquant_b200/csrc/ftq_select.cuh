@@ -6,27 +6,34 @@
 // their totals returned by themselves.
 //
 // The logits are read once.  A CTA has a chunk of a row: every thread keeps the maximum and the sum of exponentials of its 16-byte
-// vectors, and which vector the maximum came from.  Any of the chunk's `keep` largest tokens lies in one of the `keep` threads,
-// and there in one of the `keep` vectors, that are first when ordered by their largest token (of equal ones the
-// first): otherwise as many threads or vectors would each hold a token that goes before it.  So a sort of the threads, one of
-// their vectors' maxima, and one of those vectors' tokens leave the exact order, whatever the logits are, and what is read again
-// is a few hundred vectors.  keep = n + the tokens that end an answer.  beam_join_kernel adds up a request's rows and sorts their
-// tokens by their totals, in 64 bits (totals of different beams may lie closer than fp32 tells apart).
+// vectors.  Any `keep` of the threads' maxima bound the chunk's keep-th largest token from below (keep = n + the tokens that end
+// an answer), so the keep-th of the warps' few largest is a threshold: threads whose maximum reaches it are few, their vectors are
+// looked at again, and the few tokens that reach it are ranked by counting (threshold, push and rank below).  Where more tokens reach it than there is
+// room for (equal logits, or large ones in a few threads' vectors only) sorts leave the exact order whatever the logits are: any of the `keep` largest tokens lies in
+// one of the `keep` threads, and there in one of the `keep` vectors, that are first by their largest token (of equal ones
+// the first), since otherwise as many threads or vectors would each hold a token that goes before it.
+// beam_join_kernel adds up a request's rows and does the same with their tokens' totals, in 64 bits (totals of different beams
+// may lie closer than fp32 tells apart).
 #pragma once
+
+#include <type_traits>
 
 #include "ftq_beam_launch.h"
 
 namespace ftq {
 
-constexpr int kSelectThreads = 512, kSelectMaxKeep = kBeamMax + kBeamMaxEnds;
-constexpr int kSelectVectors = 32;      // vectors of a thread at most, so that those of `keep` threads can be sorted
+constexpr int kSelectThreads = 256, kSelectWarps = kSelectThreads / 32, kSelectMaxKeep = kBeamMax + kBeamMaxEnds;
+constexpr int kSelectVectors = 32;      // vectors of a thread at most: a lane each when a thread's are looked at again
+constexpr int kSelectBatch = 4;         // of which a thread loads so many at a time
+constexpr int kSelectRoom = 1024;       // tokens that are ranked by counting
+constexpr int kSelectTop = 16;          // a warp's largest keys that a threshold is made of, at most
 
 __host__ __device__ constexpr int select_pow2(int n) {
     int x = 1;
     while (x < n) x *= 2;
     return x;
 }
-// tokens that beam_join_kernel sorts at a time
+// tokens that beam_join_kernel sorts at a time, where it has to
 constexpr int kSelectJoin = 4096;
 __host__ __device__ constexpr int select_join_size(int beams, int chunks, int keep, int n) {
     const int64_t all = static_cast<int64_t>(beams) * chunks * keep + n;
@@ -41,6 +48,28 @@ __device__ __forceinline__ uint32_t select_order(float x) {
 __device__ __forceinline__ float select_value(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o); }
 __device__ __forceinline__ unsigned long long select_key(float x, uint32_t place) {     // (lower places are larger)
     return static_cast<unsigned long long>(select_order(x)) << 32 | static_cast<uint32_t>(~place);
+}
+
+// A key that at least `keep` of the CTA's threads' keys reach, 0 where fewer are above 0; by the whole CTA.  `s` has room for
+// kSelectTop keys of each warp and one more.
+__device__ __forceinline__ uint32_t select_threshold(uint32_t key, int keep, uint32_t* s) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // (two more of each warp than an even spread needs)
+    const int top = min(kSelectTop, (keep + kSelectWarps - 1) / kSelectWarps + 2), all = top * kSelectWarps;
+    for (int i = 0; i < top; i++) {
+        const uint32_t m = __reduce_max_sync(0xffffffffu, key);
+        if (lane == 0) s[warp * top + i] = m;
+        if (lane == __ffs(__ballot_sync(0xffffffffu, key == m)) - 1) key = 0;
+    }
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < all) {
+        const uint32_t mine = s[threadIdx.x];
+        int rank = 0;
+        for (int i = 0; i < all; i++) rank += s[i] > mine || (s[i] == mine && i < static_cast<int>(threadIdx.x));
+        if (rank == keep - 1) s[kSelectTop * kSelectWarps] = mine;
+    }
+    __syncthreads();
+    return s[kSelectTop * kSelectWarps];
 }
 
 // Sorts n = 2^k keys in shared memory, the largest first; by the whole CTA.
@@ -64,19 +93,7 @@ __device__ __forceinline__ void select_sort(unsigned long long* s, int n) {
 template <typename T>
 struct SelectVec {
     static constexpr int N = 16 / sizeof(T);
-    float v[N];
-    // vector i of the row part [begin, end) of x, where vectors lie on 16-byte boundaries and the first one `head` tokens before
-    // begin: what does not belong to it is -inf
-    __device__ __forceinline__ void load(const T* x, int head, int len, int i) {
-        const int at = i * N - head;
-        if (at >= 0 && at + N <= len) {
-            unpack(*reinterpret_cast<const uint4*>(x + at));
-        } else {
-#pragma unroll
-            for (int k = 0; k < N; k++) v[k] = at + k >= 0 && at + k < len ? to_float<T>(x[at + k]) : -INFINITY;
-        }
-    }
-    __device__ __forceinline__ void unpack(uint4 u) {
+    static __device__ __forceinline__ void unpack(uint4 u, float (&v)[N]) {
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -92,7 +109,18 @@ struct SelectVec {
             }
         }
     }
-    __device__ __forceinline__ float largest() const {
+    // vector i of the row part [x, x + len), where vectors lie on 16-byte boundaries and the first one begins `head` tokens before
+    // x: what does not belong to it is -inf
+    static __device__ __forceinline__ void load(const T* x, int head, int len, int i, float (&v)[N]) {
+        const int at = i * N - head;
+        if (at >= 0 && at + N <= len) {
+            unpack(*reinterpret_cast<const uint4*>(x + at), v);
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; k++) v[k] = at + k >= 0 && at + k < len ? to_float<T>(x[at + k]) : -INFINITY;
+        }
+    }
+    static __device__ __forceinline__ float largest(const float (&v)[N]) {
         float m = v[0];
 #pragma unroll
         for (int k = 1; k < N; k++) m = fmaxf(m, v[k]);
@@ -100,97 +128,166 @@ struct SelectVec {
     }
 };
 
+// a thread's maximum, and the sum of exp(x - maximum)
+struct SelectSum {
+    float m = -INFINITY, sum = 0.f;
+    // (x - m first: logits far from zero lose nothing that way.  Packed: half the instructions)
+    template <int N, int B>
+    __device__ __forceinline__ void add(const float (&v)[B][N]) {
+        constexpr float kLog2 = 1.4426950408889634f;
+        float top[B];
+#pragma unroll
+        for (int k = 0; k < B; k++) top[k] = SelectVec<std::conditional_t<N == 4, float, __half>>::largest(v[k]);
+        const float before = m;
+#pragma unroll
+        for (int k = 0; k < B; k++) m = fmaxf(m, top[k]);
+        const float ref = m == -INFINITY ? 0.f : m;
+        if (m > before) sum *= fast_exp2((before - ref) * kLog2);
+        const u64 ref2 = pk2(ref, ref), log2 = pk2(kLog2, kLog2);
+        u64 part[B];
+#pragma unroll
+        for (int k = 0; k < B; k++) {
+            part[k] = 0;
+#pragma unroll
+            for (int c = 0; c < N; c += 2) {
+                float a, b;
+                upk2(mul2(sub2(pk2(v[k][c], v[k][c + 1]), ref2), log2), a, b);
+                part[k] = add2(part[k], pk2(fast_exp2(a), fast_exp2(b)));
+            }
+        }
+#pragma unroll
+        for (int k = 1; k < B; k++) part[0] = add2(part[0], part[k]);
+        float a, b;
+        upk2(part[0], a, b);
+        sum += a + b;
+    }
+};
+
 template <typename T>
-__global__ void __launch_bounds__(kSelectThreads) beam_rows_kernel(const SelectParams p) {
-    constexpr int N = SelectVec<T>::N;
+__global__ void __launch_bounds__(kSelectThreads, 4) beam_rows_kernel(const SelectParams p) {
+    using V = SelectVec<T>;
+    constexpr int N = V::N, B = kSelectBatch;
     extern __shared__ unsigned long long s_keys[];
-    __shared__ float s_max[kSelectThreads / 32], s_sum[kSelectThreads / 32];
-    const int tid = threadIdx.x, lane = tid & 31, row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
+    __shared__ float s_max[kSelectWarps], s_sum[kSelectWarps];
+    __shared__ uint32_t s_top[kSelectTop * kSelectWarps + 1];
+    __shared__ int s_first[kSelectThreads], s_n[2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
     after_previous_kernel();
     let_next_kernel_start();
     if (!(p.scores[row] > -INFINITY)) return;     // (a beam that is not alive; beam_join_kernel asks the same)
     const int begin = chunk * p.chunk, len = min(p.chunk, p.V - begin);
     const T* const x = static_cast<const T*>(p.logits) + row * p.row_stride + begin;
     const int head = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)), n_vec = (head + len + N - 1) / N;
-    float m = -INFINITY, sum = 0.f;
-    int where = tid;        // the vector that the maximum came from
+    if (tid < 2) s_n[tid] = 0;
     constexpr float kLog2 = 1.4426950408889634f;
-    for (int i0 = tid; i0 < n_vec; i0 += 4 * kSelectThreads) {
-        SelectVec<T> v[4];
-        float top[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int i = i0 + k * kSelectThreads;
-            if (i < n_vec) {
-                v[k].load(x, head, len, i);
-            } else {
-#pragma unroll
-                for (int c = 0; c < N; c++) v[k].v[c] = -INFINITY;
-            }
+    SelectSum own;
+    {
+        // vectors that are whole; at most one before them and one behind is not
+        const int lo = head > 0 ? 1 : 0, hi = (head + len) / N;
+        int i = tid;
+        if (i < lo) {
+            float v[1][N];
+            V::load(x, head, len, i, v[0]);
+            own.add(v);
+            i += kSelectThreads;
         }
-        const float before = m;
+        const uint4* const from = reinterpret_cast<const uint4*>(x - head);
+        for (; i + (B - 1) * kSelectThreads < hi; i += B * kSelectThreads) {
+            uint4 u[B];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            top[k] = v[k].largest();
-            where = top[k] > m ? i0 + k * kSelectThreads : where;
-            m = fmaxf(m, top[k]);
+            for (int k = 0; k < B; k++) u[k] = from[i + k * kSelectThreads];
+            float v[B][N];
+#pragma unroll
+            for (int k = 0; k < B; k++) V::unpack(u[k], v[k]);
+            own.add(v);
         }
-        const float ref = m == -INFINITY ? 0.f : m;
-        if (m > before) sum *= fast_exp2((before - ref) * kLog2);
-        // (x - m first: logits far from zero lose nothing that way.  Packed: half the instructions)
-        const u64 ref2 = pk2(ref, ref), log2 = pk2(kLog2, kLog2);
-        u64 part[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            part[k] = 0;
-#pragma unroll
-            for (int c = 0; c < N; c += 2) {
-                float a, b;
-                upk2(mul2(sub2(pk2(v[k].v[c], v[k].v[c + 1]), ref2), log2), a, b);
-                part[k] = add2(part[k], pk2(fast_exp2(a), fast_exp2(b)));
-            }
+        for (; i < n_vec; i += kSelectThreads) {
+            float v[1][N];
+            V::load(x, head, len, i, v[0]);
+            own.add(v);
         }
-        float a, b;
-        upk2(add2(add2(part[0], part[1]), add2(part[2], part[3])), a, b);
-        sum += a + b;
     }
     // ---- the chunk's maximum and sum, in an order of their own
     {
-        float mw = m;
+        float mw = own.m;
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, d));
-        float s = m == -INFINITY ? sum : sum * fast_exp2((m - mw) * kLog2);     // (not a number stays so)
+        float s = own.m == -INFINITY ? own.sum : own.sum * fast_exp2((own.m - mw) * kLog2);     // (not a number stays so)
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
         if (lane == 0) {
-            s_max[tid / 32] = mw;
-            s_sum[tid / 32] = s;
+            s_max[warp] = mw;
+            s_sum[warp] = s;
         }
     }
-    s_keys[tid] = tid < n_vec ? select_key(m, where) : 0;
-    __syncthreads();
+    const uint32_t mine = tid < n_vec ? select_order(own.m) : 0;
+    const uint32_t least = select_threshold(mine, p.keep, s_top);
     if (tid == 0) {
         float mc = s_max[0];
-        for (int w = 1; w < kSelectThreads / 32; w++) mc = fmaxf(mc, s_max[w]);
+        for (int w = 1; w < kSelectWarps; w++) mc = fmaxf(mc, s_max[w]);
         float s = 0.f;
-        for (int w = 0; w < kSelectThreads / 32; w++) s += s_max[w] == -INFINITY ? s_sum[w] : s_sum[w] * fast_exp2((s_max[w] - mc) * kLog2);
+        for (int w = 0; w < kSelectWarps; w++) s += s_max[w] == -INFINITY ? s_sum[w] : s_sum[w] * fast_exp2((s_max[w] - mc) * kLog2);
         p.sums[blockIdx.x] = make_float2(mc, s);
     }
-    // ---- the first `keep` threads by their largest token
+    // ---- the threads whose maximum reaches it, a warp each, a lane to a vector: their tokens that do
+    if (mine > 0 && mine >= least) s_first[atomicAdd(&s_n[0], 1)] = tid;
+    __syncthreads();
+    const int rounds = (n_vec + kSelectThreads - 1) / kSelectThreads;
+    for (int c = warp; c < s_n[0]; c += kSelectWarps) {
+        const int i = s_first[c] + lane * kSelectThreads;
+        if (lane >= rounds || i >= n_vec || s_n[1] > kSelectRoom) continue;
+        float v[N];
+        V::load(x, head, len, i, v);
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const int t = i * N - head + k;
+            if (select_order(v[k]) >= least && t >= 0 && t < len) {
+                const int at = atomicAdd(&s_n[1], 1);
+                if (at < kSelectRoom) s_keys[at] = select_key(v[k], begin + t);
+            }
+        }
+    }
+    __syncthreads();
+    unsigned long long* const to = p.keys + static_cast<int64_t>(blockIdx.x) * p.keep;
+    if (s_n[1] <= kSelectRoom) {
+        const int n = s_n[1];
+        for (int e = tid; e < n; e += kSelectThreads) {
+            const unsigned long long key = s_keys[e];
+            int rank = 0;
+#pragma unroll 8
+            for (int i = 0; i < n; i++) rank += s_keys[i] > key;
+            if (rank < p.keep) to[rank] = key;
+        }
+        for (int e = n + tid; e < p.keep; e += kSelectThreads) to[e] = 0;
+        return;
+    }
+    // ---- too many of them.  The first `keep` threads by their largest token (and the vector that it lies in)
+    {
+        float best = -INFINITY;
+        int where = tid;
+        for (int i = tid; i < n_vec; i += kSelectThreads) {
+            float v[N];
+            V::load(x, head, len, i, v);
+            const float t = V::largest(v);
+            where = t > best ? i : where;
+            best = fmaxf(best, t);
+        }
+        __syncthreads();
+        s_keys[tid] = tid < n_vec ? select_key(best, where) : 0;
+    }
     select_sort(s_keys, kSelectThreads);
-    const int threads = min(p.keep, min(n_vec, kSelectThreads)), rounds = (n_vec + kSelectThreads - 1) / kSelectThreads;
-    __shared__ int s_first[kSelectMaxKeep];
+    const int threads = min(p.keep, min(n_vec, kSelectThreads));
     if (tid < threads) s_first[tid] = static_cast<int>(~static_cast<uint32_t>(s_keys[tid])) % kSelectThreads;
     __syncthreads();
-    // ---- of their vectors the first `keep`
+    // of their vectors the first `keep`
     int n = select_pow2(threads * rounds);
     for (int e = tid; e < n; e += kSelectThreads) {
         const int i = e < threads * rounds ? s_first[e / rounds] + e % rounds * kSelectThreads : n_vec;
         unsigned long long key = 0;
         if (i < n_vec) {
-            SelectVec<T> v;
-            v.load(x, head, len, i);
-            key = select_key(v.largest(), i);
+            float v[N];
+            V::load(x, head, len, i, v);
+            key = select_key(V::largest(v), i);
         }
         s_keys[e] = key;
     }
@@ -198,7 +295,7 @@ __global__ void __launch_bounds__(kSelectThreads) beam_rows_kernel(const SelectP
     const int vectors = min(p.keep, min(n, n_vec));
     if (tid < vectors) s_first[tid] = static_cast<int>(~static_cast<uint32_t>(s_keys[tid]));
     __syncthreads();
-    // ---- of their tokens the first `keep`
+    // of their tokens the first `keep`
     n = select_pow2(max(vectors * N, p.keep));
     for (int e = tid; e < n; e += kSelectThreads) {
         unsigned long long key = 0;
@@ -209,7 +306,7 @@ __global__ void __launch_bounds__(kSelectThreads) beam_rows_kernel(const SelectP
         s_keys[e] = key;
     }
     select_sort(s_keys, n);
-    for (int e = tid; e < p.keep; e += kSelectThreads) p.keys[static_cast<int64_t>(blockIdx.x) * p.keep + e] = s_keys[e];
+    for (int e = tid; e < p.keep; e += kSelectThreads) to[e] = s_keys[e];
 }
 
 // Orders as the value does.
@@ -227,10 +324,14 @@ __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectP
     extern __shared__ unsigned long long s_keys[];
     // a beam's score (-inf: it has no continuation), its row's maximum, and the logarithm of the sum of exponentials less that
     __shared__ double s_score[kBeamMax], s_max[kBeamMax], s_log[kBeamMax];
+    __shared__ uint32_t s_top[kSelectTop * kSelectWarps + 1];
+    __shared__ int s_end[kBeamMaxEnds], s_n;
     const int tid = threadIdx.x, r = blockIdx.x;
     after_previous_kernel();
     let_next_kernel_start();
-    for (int b = tid / 32; b < p.K; b += kSelectThreads / 32) {
+    if (tid == 0) s_n = 0;
+    if (tid < p.n_ends) s_end[tid] = p.ends[tid];
+    for (int b = tid / 32; b < p.K; b += kSelectWarps) {
         const int64_t row = static_cast<int64_t>(r) * p.K + b;
         const float score = p.scores[row];
         double s = 0.0;
@@ -257,35 +358,78 @@ __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectP
     auto total_of = [&](int b, float x) { return (x - s_max[b]) - s_log[b] + s_score[b]; };
     __syncthreads();
     for (int e = tid; e < p.K * p.n_ends; e += kSelectThreads) {
-        const int b = e / p.n_ends, id = p.ends[e - b * p.n_ends];
+        const int b = e / p.n_ends, id = s_end[e - b * p.n_ends];
         double total = -INFINITY;
         if (s_score[b] > -INFINITY && id >= 0 && id < p.V)
             total = total_of(b, to_float<T>(static_cast<const T*>(p.logits)[(static_cast<int64_t>(r) * p.K + b) * p.row_stride + id]));
         p.end_scores[static_cast<int64_t>(r) * p.K * p.n_ends + e] = static_cast<float>(total);
     }
-    // ---- the n best so far and as many others as there is room for, until there are no others
-    const int per_row = p.chunks * p.keep, all = p.K * per_row, n = select_join_size(p.K, p.chunks, p.keep, p.n);
+    const int per_row = p.chunks * p.keep, all = p.K * per_row;
+    // token i of those that the request's rows kept: (order of its total, place); 0: none
+    auto token_of = [&](int i, unsigned long long& place) -> unsigned long long {
+        const int b = i / per_row;
+        if (!(s_score[b] > -INFINITY)) return 0;
+        const unsigned long long k = __ldcg(p.keys + static_cast<int64_t>(r) * all + i);
+        const uint32_t token = ~static_cast<uint32_t>(k);
+        bool end = k == 0;
+        for (int c = 0; c < p.n_ends; c++) end |= static_cast<uint32_t>(s_end[c]) == token;
+        const double total = total_of(b, select_value(static_cast<uint32_t>(k >> 32)));
+        place = static_cast<unsigned long long>(b) << 32 | token;
+        return !end && total > -INFINITY ? select_order64(total) : 0;
+    };
+    auto store = [&](int e, unsigned long long key, unsigned long long place) {
+        const int64_t at = static_cast<int64_t>(r) * p.n + e;
+        p.out_scores[at] = key ? static_cast<float>(select_value64(key)) : -INFINITY;
+        p.parents[at] = key ? static_cast<int>(place >> 32) : -1;
+        p.tokens[at] = key ? static_cast<int>(place & 0xffffffffu) : -1;
+    };
+    // ---- those that reach a threshold, by counting
+    {
+        uint32_t most = 0;
+        unsigned long long place;
+        for (int i = tid; i < all; i += kSelectThreads) most = max(most, static_cast<uint32_t>(token_of(i, place) >> 32));
+        const uint32_t least = select_threshold(most, p.n, s_top);
+        if (most > 0 && most >= least)
+            for (int i = tid; i < all; i += kSelectThreads) {
+                const unsigned long long key = token_of(i, place);
+                if (key == 0 || static_cast<uint32_t>(key >> 32) < least) continue;
+                const int at = atomicAdd(&s_n, 1);
+                if (at < kSelectRoom) {
+                    s_keys[2 * at] = key;
+                    s_keys[2 * at + 1] = place;
+                }
+            }
+        __syncthreads();
+    }
+    if (s_n <= kSelectRoom) {
+        const int n = s_n;
+        const ulonglong2* const s = reinterpret_cast<const ulonglong2*>(s_keys);
+        for (int e = tid; e < n; e += kSelectThreads) {
+            const ulonglong2 mine = s[e];
+            int rank = 0;
+#pragma unroll 4
+            for (int i = 0; i < n; i++) {
+                const ulonglong2 x = s[i];
+                rank += x.x > mine.x || (x.x == mine.x && x.y < mine.y);
+            }
+            if (rank < p.n) store(rank, mine.x, mine.y);
+        }
+        for (int e = n + tid; e < p.n; e += kSelectThreads) store(e, 0, 0);
+        return;
+    }
+    // ---- too many of them: the n best so far and as many others as there is room for, until there are no others
+    const int n = select_join_size(p.K, p.chunks, p.keep, p.n);
     unsigned long long* const s_place = s_keys + n;
+    __syncthreads();
     for (int e = tid; e < p.n; e += kSelectThreads) {
         s_keys[e] = 0;
         s_place[e] = ~0ull;
     }
     for (int done = 0; done < all; done += n - p.n) {
         for (int e = p.n + tid; e < n; e += kSelectThreads) {
-            unsigned long long key = 0, place = ~0ull;
-            const int i = done + e - p.n, b = i / per_row;
-            if (i < all && s_score[b] > -INFINITY) {
-                const unsigned long long k = __ldcg(p.keys + static_cast<int64_t>(r) * all + i);
-                const uint32_t token = ~static_cast<uint32_t>(k);
-                const double total = total_of(b, select_value(static_cast<uint32_t>(k >> 32)));
-                bool end = k == 0;
-                for (int c = 0; c < p.n_ends; c++) end |= static_cast<uint32_t>(p.ends[c]) == token;
-                if (!end && total > -INFINITY) {
-                    key = select_order64(total);
-                    place = static_cast<unsigned long long>(b) << 32 | token;
-                }
-            }
-            s_keys[e] = key;
+            unsigned long long place = ~0ull;
+            const int i = done + e - p.n;
+            s_keys[e] = i < all ? token_of(i, place) : 0;
             s_place[e] = place;
         }
         for (int k = 2; k <= n; k <<= 1)
@@ -303,13 +447,7 @@ __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectP
             }
         __syncthreads();
     }
-    for (int e = tid; e < p.n; e += kSelectThreads) {
-        const unsigned long long key = s_keys[e], place = s_place[e];
-        const int64_t at = static_cast<int64_t>(r) * p.n + e;
-        p.out_scores[at] = key ? static_cast<float>(select_value64(key)) : -INFINITY;
-        p.parents[at] = key ? static_cast<int>(place >> 32) : -1;
-        p.tokens[at] = key ? static_cast<int>(place & 0xffffffffu) : -1;
-    }
+    for (int e = tid; e < p.n; e += kSelectThreads) store(e, s_keys[e], s_place[e]);
 }
 
 }  // namespace ftq
