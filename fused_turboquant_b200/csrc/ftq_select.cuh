@@ -128,6 +128,12 @@ struct SelectVec {
     }
 };
 
+// Asks for bytes that will be read (16-byte aligned, a multiple of 16): a CTA's whole chunk is on its way to L2 while its first
+// vectors are waited for, and while other CTAs look for their largest tokens.
+__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(p), "r"(bytes) : "memory");
+}
+
 // a thread's maximum, and the sum of exp(x - maximum)
 struct SelectSum {
     float m = -INFINITY, sum = 0.f;
@@ -137,7 +143,11 @@ struct SelectSum {
         constexpr float kLog2 = 1.4426950408889634f;
         float top[B];
 #pragma unroll
-        for (int k = 0; k < B; k++) top[k] = SelectVec<std::conditional_t<N == 4, float, __half>>::largest(v[k]);
+        for (int k = 0; k < B; k++) {
+            top[k] = v[k][0];
+#pragma unroll
+            for (int c = 1; c < N; c++) top[k] = fmaxf(top[k], v[k][c]);
+        }
         const float before = m;
 #pragma unroll
         for (int k = 0; k < B; k++) m = fmaxf(m, top[k]);
@@ -192,6 +202,7 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_rows_kernel(const Sele
             i += kSelectThreads;
         }
         const uint4* const from = reinterpret_cast<const uint4*>(x - head);
+        if (tid == 0 && hi > lo) prefetch_l2(from + lo, 16 * (hi - lo));
         for (; i + (B - 1) * kSelectThreads < hi; i += B * kSelectThreads) {
             uint4 u[B];
 #pragma unroll
@@ -331,26 +342,32 @@ __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectP
     let_next_kernel_start();
     if (tid == 0) s_n = 0;
     if (tid < p.n_ends) s_end[tid] = p.ends[tid];
+    const int per_row = p.chunks * p.keep, all = p.K * per_row;
+    // (the thread's first tokens are on their way while the sums are made)
+    constexpr int FEW = 4;
+    unsigned long long kept[FEW];
+#pragma unroll
+    for (int j = 0; j < FEW; j++) {
+        const int i = tid + j * kSelectThreads;
+        kept[j] = i < all ? __ldcg(p.keys + static_cast<int64_t>(r) * all + i) : 0;     // (of a row that is not alive: anything)
+    }
     for (int b = tid / 32; b < p.K; b += kSelectWarps) {
         const int64_t row = static_cast<int64_t>(r) * p.K + b;
+        const float2* const at = p.sums + row * p.chunks;
         const float score = p.scores[row];
-        double s = 0.0;
-        float m = -INFINITY;
-        if (score > -INFINITY) {
-            const float2* at = p.sums + row * p.chunks;
-            for (int c = tid & 31; c < p.chunks; c += 32) m = fmaxf(m, __ldcg(at + c).x);
+        const float2 first = (tid & 31) < p.chunks ? __ldcg(at + (tid & 31)) : make_float2(-INFINITY, 0.f);
+        float m = first.x;
+        for (int c = 32 + (tid & 31); c < p.chunks; c += 32) m = fmaxf(m, __ldcg(at + c).x);
 #pragma unroll
-            for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-            for (int c = tid & 31; c < p.chunks; c += 32) {
-                const float2 x = __ldcg(at + c);
-                // (a sum that is not a number says so whatever its maximum is)
-                s += x.x == -INFINITY ? static_cast<double>(x.y) : x.y * exp(static_cast<double>(x.x) - m);
-            }
+        for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        // (a sum that is not a number says so whatever its maximum is)
+        auto part = [&](float2 x) { return x.x == -INFINITY ? static_cast<double>(x.y) : x.y * exp(static_cast<double>(x.x) - m); };
+        double s = part(first);
+        for (int c = 32 + (tid & 31); c < p.chunks; c += 32) s += part(__ldcg(at + c));
 #pragma unroll
-            for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        }
+        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
         if ((tid & 31) == 0) {
-            s_score[b] = s > 0.0 && m > -INFINITY && m < INFINITY ? score : -INFINITY;
+            s_score[b] = score > -INFINITY && s > 0.0 && m > -INFINITY && m < INFINITY ? score : -INFINITY;
             s_max[b] = m;
             s_log[b] = log(s);
         }
@@ -364,12 +381,10 @@ __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectP
             total = total_of(b, to_float<T>(static_cast<const T*>(p.logits)[(static_cast<int64_t>(r) * p.K + b) * p.row_stride + id]));
         p.end_scores[static_cast<int64_t>(r) * p.K * p.n_ends + e] = static_cast<float>(total);
     }
-    const int per_row = p.chunks * p.keep, all = p.K * per_row;
-    // token i of those that the request's rows kept: (order of its total, place); 0: none
-    auto token_of = [&](int i, unsigned long long& place) -> unsigned long long {
+    // token i of those that the request's rows kept, of the key k: (order of its total, place); 0: none
+    auto total_key = [&](int i, unsigned long long k, unsigned long long& place) -> unsigned long long {
         const int b = i / per_row;
         if (!(s_score[b] > -INFINITY)) return 0;
-        const unsigned long long k = __ldcg(p.keys + static_cast<int64_t>(r) * all + i);
         const uint32_t token = ~static_cast<uint32_t>(k);
         bool end = k == 0;
         for (int c = 0; c < p.n_ends; c++) end |= static_cast<uint32_t>(s_end[c]) == token;
@@ -377,6 +392,7 @@ __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectP
         place = static_cast<unsigned long long>(b) << 32 | token;
         return !end && total > -INFINITY ? select_order64(total) : 0;
     };
+    auto token_of = [&](int i, unsigned long long& place) { return total_key(i, __ldcg(p.keys + static_cast<int64_t>(r) * all + i), place); };
     auto store = [&](int e, unsigned long long key, unsigned long long place) {
         const int64_t at = static_cast<int64_t>(r) * p.n + e;
         p.out_scores[at] = key ? static_cast<float>(select_value64(key)) : -INFINITY;
@@ -386,19 +402,31 @@ __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectP
     // ---- those that reach a threshold, by counting
     {
         uint32_t most = 0;
-        unsigned long long place;
-        for (int i = tid; i < all; i += kSelectThreads) most = max(most, static_cast<uint32_t>(token_of(i, place) >> 32));
+        unsigned long long place[FEW], other;
+#pragma unroll
+        for (int j = 0; j < FEW; j++) {
+            const int i = tid + j * kSelectThreads;
+            kept[j] = i < all ? total_key(i, kept[j], place[j]) : 0;
+            most = max(most, static_cast<uint32_t>(kept[j] >> 32));
+        }
+        for (int i = tid + FEW * kSelectThreads; i < all; i += kSelectThreads) most = max(most, static_cast<uint32_t>(token_of(i, other) >> 32));
         const uint32_t least = select_threshold(most, p.n, s_top);
-        if (most > 0 && most >= least)
-            for (int i = tid; i < all; i += kSelectThreads) {
-                const unsigned long long key = token_of(i, place);
-                if (key == 0 || static_cast<uint32_t>(key >> 32) < least) continue;
-                const int at = atomicAdd(&s_n, 1);
-                if (at < kSelectRoom) {
-                    s_keys[2 * at] = key;
-                    s_keys[2 * at + 1] = place;
-                }
+        auto push = [&](unsigned long long key, unsigned long long at) {
+            if (key == 0 || static_cast<uint32_t>(key >> 32) < least) return;
+            const int n = atomicAdd(&s_n, 1);
+            if (n < kSelectRoom) {
+                s_keys[2 * n] = key;
+                s_keys[2 * n + 1] = at;
             }
+        };
+        if (most >= least) {
+#pragma unroll
+            for (int j = 0; j < FEW; j++) push(kept[j], place[j]);
+            for (int i = tid + FEW * kSelectThreads; i < all; i += kSelectThreads) {
+                const unsigned long long key = token_of(i, other);
+                push(key, other);
+            }
+        }
         __syncthreads();
     }
     if (s_n <= kSelectRoom) {
