@@ -23,8 +23,8 @@
 namespace ftq {
 
 constexpr int kSelectThreads = 256, kSelectWarps = kSelectThreads / 32, kSelectMaxKeep = kBeamMax + kBeamMaxEnds;
-constexpr int kSelectVectors = 32;      // vectors of a thread at most: a lane each when a thread's are looked at again
-constexpr int kSelectBatch = 4;         // of which a thread loads so many at a time
+constexpr int kSelectVectors = 32;      // vectors of a thread at most, so that those of `keep` threads can be sorted
+constexpr int kSelectBatch = 2;         // of which a thread loads so many at a time
 constexpr int kSelectRoom = 1024;       // tokens that are ranked by counting
 constexpr int kSelectTop = 16;          // a warp's largest keys that a threshold is made of, at most
 
@@ -65,6 +65,7 @@ __device__ __forceinline__ uint32_t select_threshold(uint32_t key, int keep, uin
     if (static_cast<int>(threadIdx.x) < all) {
         const uint32_t mine = s[threadIdx.x];
         int rank = 0;
+#pragma unroll 8
         for (int i = 0; i < all; i++) rank += s[i] > mine || (s[i] == mine && i < static_cast<int>(threadIdx.x));
         if (rank == keep - 1) s[kSelectTop * kSelectWarps] = mine;
     }
@@ -174,7 +175,7 @@ struct SelectSum {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kSelectThreads, 4) beam_rows_kernel(const SelectParams p) {
+__global__ void __launch_bounds__(kSelectThreads, 5) beam_rows_kernel(const SelectParams p) {
     using V = SelectVec<T>;
     constexpr int N = V::N, B = kSelectBatch;
     extern __shared__ unsigned long long s_keys[];
@@ -203,10 +204,21 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_rows_kernel(const Sele
         }
         const uint4* const from = reinterpret_cast<const uint4*>(x - head);
         if (tid == 0 && hi > lo) prefetch_l2(from + lo, 16 * (hi - lo));
-        for (; i + (B - 1) * kSelectThreads < hi; i += B * kSelectThreads) {
+        // (the next batch is on its way while this one is added up)
+        uint4 next[B];
+        auto fetch = [&]() {
+#pragma unroll
+            for (int k = 0; k < B; k++) next[k] = from[i + k * kSelectThreads];
+        };
+        bool more = i + (B - 1) * kSelectThreads < hi;
+        if (more) fetch();
+        while (more) {
             uint4 u[B];
 #pragma unroll
-            for (int k = 0; k < B; k++) u[k] = from[i + k * kSelectThreads];
+            for (int k = 0; k < B; k++) u[k] = next[k];
+            i += B * kSelectThreads;
+            more = i + (B - 1) * kSelectThreads < hi;
+            if (more) fetch();
             float v[B][N];
 #pragma unroll
             for (int k = 0; k < B; k++) V::unpack(u[k], v[k]);
@@ -240,13 +252,13 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_rows_kernel(const Sele
         for (int w = 0; w < kSelectWarps; w++) s += s_max[w] == -INFINITY ? s_sum[w] : s_sum[w] * fast_exp2((s_max[w] - mc) * kLog2);
         p.sums[blockIdx.x] = make_float2(mc, s);
     }
-    // ---- the threads whose maximum reaches it, a warp each, a lane to a vector: their tokens that do
+    // ---- the vectors of the threads whose maximum reaches it: their tokens that do
     if (mine > 0 && mine >= least) s_first[atomicAdd(&s_n[0], 1)] = tid;
     __syncthreads();
     const int rounds = (n_vec + kSelectThreads - 1) / kSelectThreads;
-    for (int c = warp; c < s_n[0]; c += kSelectWarps) {
-        const int i = s_first[c] + lane * kSelectThreads;
-        if (lane >= rounds || i >= n_vec || s_n[1] > kSelectRoom) continue;
+    for (int e = tid; e < s_n[0] * rounds; e += kSelectThreads) {
+        const int c = e / rounds, i = s_first[c] + (e - c * rounds) * kSelectThreads;
+        if (i >= n_vec || s_n[1] > kSelectRoom) continue;
         float v[N];
         V::load(x, head, len, i, v);
 #pragma unroll
