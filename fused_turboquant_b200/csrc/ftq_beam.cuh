@@ -36,11 +36,14 @@ __device__ __forceinline__ int fork_scan(int v, int* warp_sums, int& total) {
     return before + x - v;
 }
 
-// (what one CTA wrote before it, the others read after it: past L1, by __ldcg)
+// of the cluster, or of the only CTA (what one CTA wrote before it, the others read after it: past L1, by __ldcg)
 __device__ __forceinline__ void fork_barrier() {
-    __threadfence();
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    if (gridDim.x > 1) {
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    } else {
+        __syncthreads();
+    }
 }
 
 __device__ __forceinline__ int fork_pages(int tokens) { return (tokens + kPageTokens - 1) / kPageTokens; }
@@ -55,11 +58,24 @@ __device__ __forceinline__ int fork_pages(int tokens) { return (tokens + kPageTo
 //
 // or, where the stack has too few, nothing does.  The new table is made beside the old one.  Only entries that differ change a
 // count (beams differ in their last few blocks).  A block that nobody holds any more is claimed by its first entry in the old
-// table: an atomic minimum on its count, which is below zero then.  Six phases between the barriers of a cluster of 8 CTAs;
-// a warp has a contiguous part of the entries, so that the sums of the warps' counts give the order.
-__global__ void __cluster_dims__(kForkCtas) __launch_bounds__(kForkThreads) pages_fork_kernel(const ForkParams p) {
+// table: an atomic minimum on its count, which is below zero then.
+//
+// One cluster of 8 CTAs, or one CTA where there is little; four barriers.  A warp has a contiguous part of the entries, so that the
+// sums of the warps' counts give the order, and keeps its first ones in shared memory from phase to phase; CTA 0 has the
+// rows' last blocks besides.  Bound by the chain parents -> lengths -> entries -> counts -> claims -> stack, each a round trip to L2.
+constexpr int kForkKept = 2;        // spans of entries that a warp keeps
+struct ForkSpan { int n, pages; int64_t at; };      // entries (old or new ones), new ones of them, the first one's place
+constexpr int fork_smem(int R) { return kForkThreads / 32 * kForkKept * (kForkSpan * 8 + static_cast<int>(sizeof(ForkSpan))) + 8 * R; }
+
+__global__ void __launch_bounds__(kForkThreads) pages_fork_kernel(const ForkParams p) {
+    extern __shared__ __align__(16) uint8_t s_raw[];
     __shared__ int warp_sums[kForkThreads / 32];
-    const int tid = threadIdx.x, lane = tid & 31, cta = blockIdx.x, warp = cta * (kForkThreads / 32) + (tid >> 5);
+    constexpr int WARPS = kForkThreads / 32, PER = kForkSpan / 32;
+    const int tid = threadIdx.x, lane = tid & 31, cta = blockIdx.x, warp = cta * WARPS + (tid >> 5), warps = gridDim.x * WARPS;
+    int2* const s_entry = reinterpret_cast<int2*>(s_raw) + (tid >> 5) * kForkKept * kForkSpan;        // the warp's: (old, new)
+    ForkSpan* const s_span = reinterpret_cast<ForkSpan*>(s_raw + WARPS * kForkKept * kForkSpan * 8) + (tid >> 5) * kForkKept;
+    int* const s_last = reinterpret_cast<int*>(s_raw + fork_smem(0));     // CTA 0: rows' partly filled last blocks, -1: none
+    int* const s_len = s_last + p.R;                                      // ... and lengths
     after_previous_kernel();
     let_next_kernel_start();
     const int room = kPageTokens * p.max_blocks;
@@ -73,94 +89,113 @@ __global__ void __cluster_dims__(kForkCtas) __launch_bounds__(kForkThreads) page
         return row;
     };
     auto valid = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(p.num_blocks); };
-    // the partly filled last block of row r, before anybody takes one; -1: it has none
-    auto last_of = [&](const Row& row) {
-        if (row.len % kPageTokens == 0) return -1;
-        const int id = p.table[static_cast<int64_t>(row.parent) * p.max_blocks + fork_pages(row.len) - 1];
-        return valid(id) ? id : -1;
-    };
-    // the warp's entries, by spans of a row: f(index of the entry in the table, old block, new block)
+    // the warp's entries, by spans of a row: f(place in the table, it is one, old block, new block, it stays)
     const int spans = (p.max_blocks + kForkSpan - 1) / kForkSpan;
-    const int64_t items = static_cast<int64_t>(p.R) * spans, per = (items + kForkWarps - 1) / kForkWarps;
+    const int64_t items = static_cast<int64_t>(p.R) * spans, per = (items + warps - 1) / warps, item0 = warp * per, item1 = min(items, (warp + 1) * per);
     auto each_entry = [&](bool made, auto&& f) {
-        const int64_t end = min(items, (warp + 1) * per);
-        for (int64_t it = warp * per; it < end; it++) {
-            const int r = static_cast<int>(it / spans), j0 = static_cast<int>(it - static_cast<int64_t>(r) * spans) * kForkSpan;
-            const Row row = row_of(r);
-            const int old_pages = fork_pages(row.old), new_pages = fork_pages(row.len), n = min(max(old_pages, new_pages) - j0, kForkSpan);
-            if (n <= 0) continue;
-            const int64_t at = static_cast<int64_t>(r) * p.max_blocks + j0;
-            const int32_t* from = p.table + static_cast<int64_t>(max(row.parent, 0)) * p.max_blocks + j0;
-            int x[kForkSpan / 32], y[kForkSpan / 32];
+        for (int64_t it = item0; it < item1; it++) {
+            const int kept = it - item0 < kForkKept ? static_cast<int>(it - item0) : -1;
+            ForkSpan span;
+            int x[PER], y[PER];
+            if (made && kept >= 0) {
+                span = s_span[kept];
 #pragma unroll
-            for (int k = 0; k < kForkSpan / 32; k++) {
-                const int j = 32 * k + lane;
-                x[k] = j0 + j < old_pages && j < n ? p.table[at + j] : -1;
-                y[k] = j0 + j >= new_pages || j >= n ? -1 : made ? __ldcg(p.next + at + j) : from[j];
+                for (int k = 0; k < PER; k++) {
+                    const int2 e = s_entry[kept * kForkSpan + 32 * k + lane];
+                    x[k] = e.x;
+                    y[k] = e.y;
+                }
+            } else {
+                const int r = static_cast<int>(it / spans), j0 = static_cast<int>(it - static_cast<int64_t>(r) * spans) * kForkSpan;
+                const Row row = row_of(r);
+                const int old_pages = fork_pages(row.old), new_pages = fork_pages(row.len);
+                span.n = min(max(old_pages, new_pages) - j0, kForkSpan);
+                span.pages = min(max(new_pages - j0, 0), kForkSpan);
+                span.at = static_cast<int64_t>(r) * p.max_blocks + j0;
+                const int32_t* from = p.table + static_cast<int64_t>(max(row.parent, 0)) * p.max_blocks + j0;
+#pragma unroll
+                for (int k = 0; k < PER; k++) {
+                    const int j = 32 * k + lane;
+                    x[k] = j0 + j < old_pages && j < span.n ? p.table[span.at + j] : -1;
+                    y[k] = j >= span.pages ? -1 : made ? __ldcg(p.next + span.at + j) : from[j];
+                }
+                if (kept >= 0) {
+                    if (lane == 0) s_span[kept] = span;
+#pragma unroll
+                    for (int k = 0; k < PER; k++) s_entry[kept * kForkSpan + 32 * k + lane] = make_int2(x[k], y[k]);
+                }
             }
 #pragma unroll
-            for (int k = 0; k < kForkSpan / 32; k++)
-                if (32 * k < n) f(at + 32 * k + lane, 32 * k + lane < n, x[k], y[k]);
+            for (int k = 0; k < PER; k++)
+                if (32 * k < span.n) f(span.at + 32 * k + lane, 32 * k + lane < span.n, x[k], y[k], kept >= 0);
+            __syncwarp();
         }
     };
-    // ---- the new table; counts of what differs
-    for (int r = cta * kForkThreads + tid; r < p.R; r += kForkCtas * kForkThreads) {
-        const int b = last_of(row_of(r));
-        if (b >= 0) {
-            __stcg(p.part_count + b, 0);
-            __stcg(p.part_first + b, INT32_MAX);
-        }
-    }
-    for (int i = cta * kForkThreads + tid; i < 2 * p.R; i += kForkCtas * kForkThreads) p.copies[i] = -1;
-    each_entry(false, [&](int64_t at, bool live, int x, int y) {
+    // ---- the new table; counts of what differs; who has which partly filled last block
+    each_entry(false, [&](int64_t at, bool live, int x, int y, bool kept) {
         if (!live) return;
-        __stcg(p.next + at, y);
+        if (!kept) __stcg(p.next + at, y);
         if (x == y) return;
         if (valid(y)) atomicAdd(p.shares + y, 1);
         if (valid(x)) atomicAdd(p.shares + x, -1);
     });
-    fork_barrier();
-    // ---- who claims the blocks that nobody holds, and who has a partly filled last block
-    each_entry(true, [&](int64_t at, bool live, int x, int y) {
-        if (live && x != y && valid(x) && __ldcg(p.shares + x) < 0) atomicMin(p.shares + x, INT32_MIN + static_cast<int>(at));
-    });
-    for (int r = cta * kForkThreads + tid; r < p.R; r += kForkCtas * kForkThreads) {
-        const int b = last_of(row_of(r));
-        if (b >= 0) {
+    for (int i = cta * kForkThreads + tid; i < 2 * p.R; i += gridDim.x * kForkThreads) p.copies[i] = -1;
+    if (cta == 0) {
+        for (int r = tid; r < p.R; r += kForkThreads) {
+            const Row row = row_of(r);
+            int b = -1;
+            if (row.len % kPageTokens != 0) b = p.table[static_cast<int64_t>(row.parent) * p.max_blocks + fork_pages(row.len) - 1];
+            if (!valid(b)) b = -1;
+            s_len[r] = row.len;
+            s_last[r] = b;
+            if (b >= 0) {
+                __stcg(p.part_count + b, 0);
+                __stcg(p.part_first + b, INT32_MAX);
+            }
+        }
+        __syncthreads();
+        for (int r = tid; r < p.R; r += kForkThreads) {
+            const int b = s_last[r];
+            if (b < 0) continue;
             atomicAdd(p.part_count + b, 1);
             atomicMin(p.part_first + b, r);
         }
     }
     fork_barrier();
-    // ---- how many there are of both
+    // ---- who claims the blocks that nobody holds
+    each_entry(true, [&](int64_t at, bool live, int x, int y, bool) {
+        if (live && x != y && valid(x) && __ldcg(p.shares + x) < 0) atomicMin(p.shares + x, INT32_MIN + static_cast<int>(at));
+    });
+    fork_barrier();
+    // ---- how many there are, and how many rows need a block
     auto claims = [&](int64_t at, bool live, int x, int y) {
         return live && x != y && valid(x) && __ldcg(p.shares + x) == INT32_MIN + static_cast<int>(at);
     };
     {
         int mine = 0;
-        each_entry(true, [&](int64_t at, bool live, int x, int y) { mine += __popc(__ballot_sync(0xffffffffu, claims(at, live, x, y))); });
+        each_entry(true, [&](int64_t at, bool live, int x, int y, bool) { mine += __popc(__ballot_sync(0xffffffffu, claims(at, live, x, y))); });
         if (lane == 0) __stcg(p.counts + warp, mine);
     }
     if (cta == 0) {
         int base = 0;
         for (int r0 = 0; r0 < p.R; r0 += kForkThreads) {
-            const int r = r0 + tid, b = r < p.R ? last_of(row_of(r)) : -1;
+            const int r = r0 + tid, b = r < p.R ? s_last[r] : -1;
             const int held = b >= 0 ? __ldcg(p.shares + b) + 1 : 0;
             const int need = held > 1 && !(held == __ldcg(p.part_count + b) && __ldcg(p.part_first + b) == r);
             int total;
             const int rank = base + fork_scan(need, warp_sums, total);
-            if (r < p.R) p.ranks[r] = need ? rank : -1;     // (read by this CTA's same thread only)
+            if (r < p.R) p.ranks[r] = need ? rank : -1;     // (read by the same thread only)
             base += total;
         }
         if (tid == 0) __stcg(p.counts + kForkWarps, base);
     }
     fork_barrier();
-    // ---- give back, or take all of it back
+    // ---- give back and write the table, or take all of it back
     int freed = 0, before = 0;
     {
         int c[kForkWarps / 32];
 #pragma unroll
-        for (int k = 0; k < kForkWarps / 32; k++) c[k] = __ldcg(p.counts + 32 * k + lane);
+        for (int k = 0; k < kForkWarps / 32; k++) c[k] = 32 * k + lane < warps ? __ldcg(p.counts + 32 * k + lane) : 0;
 #pragma unroll
         for (int k = 0; k < kForkWarps / 32; k++) {
             freed += __reduce_add_sync(0xffffffffu, c[k]);
@@ -169,22 +204,22 @@ __global__ void __cluster_dims__(kForkCtas) __launch_bounds__(kForkThreads) page
     }
     const int wanted = __ldcg(p.counts + kForkWarps), top = min(avail + freed, p.num_blocks);
     const bool ok = wanted <= top;
-    each_entry(true, [&](int64_t at, bool live, int x, int y) {
+    each_entry(true, [&](int64_t at, bool live, int x, int y, bool) {
+        // (a claim that somebody else has cleared by now was not this entry's)
         const bool mine = claims(at, live, x, y);
         const uint32_t all = __ballot_sync(0xffffffffu, mine);
         if (mine) {
             const int to = avail + freed - 1 - (before + __popc(all & ((1u << lane) - 1)));
             if (ok && to < p.num_blocks) __stcg(p.free_blocks + to, x);
+            atomicExch(p.shares + x, ok ? 0 : -1);
         }
         before += __popc(all);
+        // (what others need of the old table is in the new one, and its lengths stay until they are done)
+        if (ok && live && x != y) p.table[at] = y;
     });
-    fork_barrier();     // (the claims have been read)
-    each_entry(true, [&](int64_t at, bool live, int x, int y) {
-        if (claims(at, live, x, y)) atomicExch(p.shares + x, ok ? 0 : -1);
-    });
+    fork_barrier();
     if (!ok) {
-        fork_barrier();
-        each_entry(true, [&](int64_t, bool live, int x, int y) {
+        each_entry(true, [&](int64_t, bool live, int x, int y, bool) {
             if (!live || x == y) return;
             if (valid(y)) atomicAdd(p.shares + y, -1);
             if (valid(x)) atomicAdd(p.shares + x, 1);
@@ -192,47 +227,18 @@ __global__ void __cluster_dims__(kForkCtas) __launch_bounds__(kForkThreads) page
         if (cta == 0 && tid == 0) *p.done = 0;
         return;
     }
-    // ---- take: the rows' own last blocks, then the table
+    // ---- take: the rows' own last blocks, and the lengths
     if (cta == 0) {
-        for (int r0 = 0; r0 < p.R; r0 += kForkThreads) {
-            const int r = r0 + tid, rank = r < p.R ? p.ranks[r] : -1;
-            if (rank < 0) continue;
-            const Row row = row_of(r);
-            const int b = last_of(row), to = __ldcg(p.free_blocks + top - 1 - rank);
-            p.copies[2 * rank] = b;
-            p.copies[2 * rank + 1] = to;
-            atomicAdd(p.shares + b, -1);
-            __stcg(p.next + static_cast<int64_t>(r) * p.max_blocks + fork_pages(row.len) - 1, to);
-        }
-    }
-    fork_barrier();
-    // (the old table goes row by row; what others still need of it is in the new one, but for the lengths)
-    const int64_t end = min(items, (warp + 1) * per);
-    for (int64_t it = warp * per; it < end; it++) {
-        const int r = static_cast<int>(it / spans), j0 = static_cast<int>(it - static_cast<int64_t>(r) * spans) * kForkSpan;
-        const Row row = row_of(r);
-        const int old_pages = fork_pages(row.old), new_pages = fork_pages(row.len), n = min(max(old_pages, new_pages), j0 + kForkSpan);
-        for (int j = j0 + lane; j < n; j += 32) {
-            const int64_t at = static_cast<int64_t>(r) * p.max_blocks + j;
-            p.table[at] = j < new_pages ? __ldcg(p.next + at) : -1;
-        }
-    }
-    // (a length is somebody else's parent's until everybody is done with it)
-    constexpr int MOST = 8192 / kForkThreads;
-    int len[MOST];
-    if (cta == 0) {
-#pragma unroll
-        for (int k = 0; k < MOST; k++) {
-            const int r = k * kForkThreads + tid;
-            len[k] = r < p.R ? row_of(r).len : 0;
-        }
-    }
-    fork_barrier();
-    if (cta == 0) {
-#pragma unroll
-        for (int k = 0; k < MOST; k++) {
-            const int r = k * kForkThreads + tid;
-            if (r < p.R) p.lens[r] = len[k];
+        for (int r = tid; r < p.R; r += kForkThreads) {
+            const int rank = p.ranks[r], len = s_len[r];
+            if (rank >= 0) {
+                const int b = s_last[r], to = __ldcg(p.free_blocks + top - 1 - rank);
+                p.copies[2 * rank] = b;
+                p.copies[2 * rank + 1] = to;
+                atomicAdd(p.shares + b, -1);
+                p.table[static_cast<int64_t>(r) * p.max_blocks + fork_pages(len) - 1] = to;
+            }
+            p.lens[r] = len;
         }
         if (tid == 0) {
             *p.n_free = top - wanted;
@@ -245,10 +251,10 @@ __global__ void __cluster_dims__(kForkCtas) __launch_bounds__(kForkThreads) page
 // Of num_blocks - n blocks in use those beyond the first num_blocks - n places move down: the k-th of them, by its id, into
 // the k-th hole.  Every other block stays where it is, so that this is the least that has to move, and no block that is
 // written is read.  The free ones are then the last n, the lowest of them on top of the stack.
-__global__ void __cluster_dims__(kForkCtas) __launch_bounds__(kForkThreads) pages_compact_kernel(const CompactParams p) {
+__global__ void __launch_bounds__(kForkThreads) pages_compact_kernel(const CompactParams p) {
     __shared__ int warp_sums[kForkThreads / 32];
     const int tid = threadIdx.x, cta = blockIdx.x, first = cta * kForkThreads + tid;
-    constexpr int ALL = kForkCtas * kForkThreads;
+    const int ctas = gridDim.x, ALL = ctas * kForkThreads;
     after_previous_kernel();
     let_next_kernel_start();
     const int nb = p.num_blocks, n = min(max(*p.n_free, 0), nb), used = nb - n;
@@ -262,7 +268,7 @@ __global__ void __cluster_dims__(kForkCtas) __launch_bounds__(kForkThreads) page
     }
     fork_barrier();
     // ---- holes below `used` and blocks beyond it, counted and then numbered by id
-    const int per = (nb + kForkCtas - 1) / kForkCtas, from = min(nb, cta * per), to = min(nb, from + per);
+    const int per = (nb + ctas - 1) / ctas, from = min(nb, cta * per), to = min(nb, from + per);
     int holes = 0, movers = 0;
     for (int i0 = from; i0 < to; i0 += kForkThreads) {
         const int i = i0 + tid;
@@ -276,7 +282,7 @@ __global__ void __cluster_dims__(kForkCtas) __launch_bounds__(kForkThreads) page
     }
     fork_barrier();
     int at_hole = 0, at_mover = 0, all_holes = 0, all_movers = 0;
-    for (int c = 0; c < kForkCtas; c++) {
+    for (int c = 0; c < ctas; c++) {
         const int h = __ldcg(p.counts + c), m = __ldcg(p.counts + kForkCtas + c);
         at_hole += c < cta ? h : 0;
         at_mover += c < cta ? m : 0;
@@ -348,18 +354,16 @@ __global__ void __launch_bounds__(256) shared_lens_kernel(const SharedLensParams
     const int whole = s_first == INT32_MAX ? 0 : s_whole, first = s_first;
     if (tid == 0) s_cut = whole;
     __syncthreads();
-    for (int j0 = 0; j0 < whole; j0 += blockDim.x) {
-        const int j = j0 + tid;
-        if (j < whole) {
-            const int id = p.table[(row0 + first) * p.max_blocks + j];
-            bool same = true;
-#pragma unroll 4
-            for (int k = 0; k < p.group; k++)
-                if (k > first && p.lens[row0 + k] > 0) same &= p.table[(row0 + k) * p.max_blocks + j] == id;
-            if (!same) atomicMin(&s_cut, j);
+    // a part of the columns at a time, a (row, column) a thread: an entry of a row that has tokens against the first such row's
+    constexpr int COLUMNS = 1024;
+    for (int j0 = 0; j0 < whole; j0 += COLUMNS) {
+        const int n = min(COLUMNS, whole - j0);
+        for (int i = tid; i < (p.group - first - 1) * n; i += blockDim.x) {
+            const int k = first + 1 + i / n, j = j0 + i % n;
+            if (p.table[(row0 + k) * p.max_blocks + j] != p.table[(row0 + first) * p.max_blocks + j] && p.lens[row0 + k] > 0) atomicMin(&s_cut, j);
         }
         __syncthreads();
-        if (s_cut < j0 + static_cast<int>(blockDim.x)) break;
+        if (s_cut < j0 + n) break;
     }
     if (tid == 0) p.out[blockIdx.x] = kPageTokens * s_cut;
 }

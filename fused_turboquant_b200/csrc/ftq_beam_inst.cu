@@ -3,6 +3,7 @@
 
 #include "ftq_beam.cuh"
 #include "ftq_launch.h"
+#include "ftq_serve_launch.h"
 #include "ftq_select.cuh"
 
 namespace ftq {
@@ -41,11 +42,38 @@ cudaError_t launch_select(int dtype, const SelectParams& p, cudaStream_t stream)
     return dtype == kF32 ? run_select<float>(p, stream) : dtype == kF16 ? run_select<__half>(p, stream) : run_select<__nv_bfloat16>(p, stream);
 }
 
+namespace {
+// a cluster of all CTAs, or a single one
+template <auto kern, typename P>
+cudaError_t run_fork(const P& p, bool little, int smem, int most_smem, cudaStream_t stream) {
+    if (most_smem > 48 * 1024) {
+        const cudaError_t e = allow_smem<kern>(most_smem);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(little ? 1 : kForkCtas);
+    cfg.blockDim = dim3(kForkThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attrs[2]{};
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = kForkCtas;
+    attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = little ? 1 : 2;
+    return cudaLaunchKernelEx(&cfg, kern, p);
+}
+}  // namespace
+
+// One CTA where its warps keep all entries in shared memory; a few thousand blocks.
 cudaError_t launch_pages_fork(const ForkParams& p, cudaStream_t stream) {
-    return launch_dependent(pages_fork_kernel, dim3(kForkCtas), kForkThreads, 0, stream, p);
+    const int64_t items = static_cast<int64_t>(p.R) * ((p.max_blocks + kForkSpan - 1) / kForkSpan);
+    return run_fork<pages_fork_kernel>(p, items <= kForkThreads / 32 * kForkKept, fork_smem(p.R), fork_smem(kPagesMaxRequests), stream);
 }
 cudaError_t launch_pages_compact(const CompactParams& p, cudaStream_t stream) {
-    return launch_dependent(pages_compact_kernel, dim3(kForkCtas), kForkThreads, 0, stream, p);
+    return run_fork<pages_compact_kernel>(p, p.num_blocks <= 4 * kForkThreads && static_cast<int64_t>(p.R) * p.max_blocks <= 16 * kForkThreads, 0, 0, stream);
 }
 cudaError_t launch_shared_lens(const SharedLensParams& p, cudaStream_t stream) {
     return launch_dependent(shared_lens_kernel, dim3(p.groups), 256, 0, stream, p);
