@@ -2001,19 +2001,31 @@ extern "C" int ftq_beam_select(const void* logits, int dtype, int64_t row_stride
 namespace {
 struct SharedLayout {   // of the workspace, behind a decode workspace of one sequence (whose status word it uses)
     int requests;                            // of a launch
+    int tiles;                               // of columns, of a warp
     int units_group, units_row, rows_group, rows_row;
     size_t plan, q, rows, end;
     int64_t base_row;
 };
 SharedLayout shared_layout(int requests, int group, int Hq, int Hkv, int d, size_t head) {
     SharedLayout l{};
-    const int G = Hq / Hkv, cols = 8 * ftq::shared_tiles(d), both = group * G;
+    const int G = Hq / Hkv, both = group * G;
+    // The tiles of columns that a page's look-ups serve: a page costs about as much as five tiles besides them, and the wider
+    // kernels, with fewer warps, take a third longer for the same instructions.
+    double least = 0.0;
+    for (int t = ftq::shared_least_tiles(d); t <= ftq::shared_most_tiles(d); t *= 2) {
+        const double cost = ((both + 8 * t - 1) / (8 * t)) * (5.0 + t) * (t * d / 4 > 64 ? 1.33 : 1.0);
+        if (l.tiles == 0 || cost < least) {
+            least = cost;
+            l.tiles = t;
+        }
+    }
+    const int cols = 8 * l.tiles;
     l.requests = std::min(requests, std::max(1, ftq::kSharedMaxRows / group));
     l.units_group = Hkv * ((both + cols - 1) / cols);
     l.units_row = Hkv * ((G + cols - 1) / cols);
     l.rows_group = std::min(both, cols);
     l.rows_row = std::min(G, cols);
-    const int64_t R = l.requests, B = R * group, warps = static_cast<int64_t>(ftq::sm_count()) * ftq::kSharedWarps;
+    const int64_t R = l.requests, B = R * group, warps = static_cast<int64_t>(ftq::sm_count()) * ftq::kSharedMaxWarps;
     l.plan = round256(head);
     l.q = l.plan + round256(static_cast<size_t>(3 * (R + B) + 2) * 4);
     l.rows = l.q + round256(static_cast<size_t>(B) * Hq * d * 2);
@@ -2066,17 +2078,16 @@ extern "C" int ftq_shared_attn(const void* q, int q_dtype, void* out, int out_dt
     p.pool = pool; p.num_blocks = num_blocks; p.max_blocks = max_blocks; p.max_seq = max_seq_len;
     p.K = group; p.Hq = Hq; p.Hkv = Hkv; p.q_dtype = q_dtype;
     p.units_group = l.units_group; p.units_row = l.units_row; p.rows_group = l.rows_group; p.rows_row = l.rows_row;
-    p.cols = 8 * ftq::shared_tiles(head_dim);
+    p.cols = 8 * l.tiles;
     // what a page costs: its look-ups and byte work, and a share of that for each tile of columns (see ftq_shared_attn.cuh)
     p.cost_group = 9 + 2 * ((l.rows_group + 7) / 8);
     p.cost_row = 9 + 2 * ((l.rows_row + 7) / 8);
-    p.least_pages = 2;
     const int64_t pages = (static_cast<int64_t>(max_seq_len) + FTQ_PAGE_TOKENS - 1) / FTQ_PAGE_TOKENS,
                   places = (ftq::kSharedPiece + pages * p.cost_group) * l.units_group + group * (ftq::kSharedPiece + pages * p.cost_row) * l.units_row;
     const int requests = static_cast<int>(std::min<int64_t>(l.requests, (INT32_MAX / 2) / places));
     if (requests < 1) return fail(FTQ_ERR_UNSUPPORTED, "too many tokens, heads and rows for one call");
     const int grid = ftq::sm_count();
-    p.warps = grid * ftq::kSharedWarps;
+    p.warps = grid * ftq::shared_shape(head_dim, static_cast<int>(ftq_page_bytes(head_dim, bits_k, bits_v)), l.tiles).warps;
     uint8_t* const ws = static_cast<uint8_t*>(workspace);
     const int entries = requests * (1 + group);
     p.plan = reinterpret_cast<int*>(ws + l.plan);
@@ -2100,7 +2111,7 @@ extern "C" int ftq_shared_attn(const void* q, int q_dtype, void* out, int out_dt
         if (e != cudaSuccess) return cuda_fail(e, "ftq_shared_attn prepare launch");
         e = cudaErrorInvalidValue;
         switch (head_dim * 10 + bits_k) {
-#define FTQ_SHARED_CASE(DD, KB) case DD * 10 + KB: e = ftq::launch_shared_attn_d##DD##_k##KB(bits_v, p, grid, st); break;
+#define FTQ_SHARED_CASE(DD, KB) case DD * 10 + KB: e = ftq::launch_shared_attn_d##DD##_k##KB(bits_v, l.tiles, p, grid, st); break;
             FTQ_SHARED_CASE(64, 2) FTQ_SHARED_CASE(64, 3) FTQ_SHARED_CASE(64, 4)
             FTQ_SHARED_CASE(128, 2) FTQ_SHARED_CASE(128, 3) FTQ_SHARED_CASE(128, 4)
             FTQ_SHARED_CASE(256, 2) FTQ_SHARED_CASE(256, 3) FTQ_SHARED_CASE(256, 4)

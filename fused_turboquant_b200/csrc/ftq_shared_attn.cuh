@@ -25,32 +25,11 @@ namespace ftq {
 template <int D, int BK, int BV, int NT>
 struct SharedCfg : MmaCfg<D, BK, BV, 2> {
     using M = MmaCfg<D, BK, BV, 2>;
-    static constexpr int WARPS = kSharedWarps, THREADS = 32 * WARPS, COLS = 8 * NT;
+    static constexpr SharedShape SHAPE = shared_shape(D, M::PAGE_BYTES, NT);
+    static constexpr int WARPS = SHAPE.warps, THREADS = 32 * WARPS, COLS = 8 * NT;
+    static constexpr int RING = SHAPE.ring, RING_BYTES = shared_ring_bytes(M::PAGE_BYTES, RING);     // pages on their way, per warp
+    static constexpr int Q_BYTES = COLS * D * 2, PLAN_BYTES = kSharedPlanBytes, SMEM_BYTES = SHAPE.smem;
     static constexpr bool ROT = !(BV == 3 && D <= 128);     // (see FlowCfg)
-    static constexpr int RING = D == 256 ? 2 : 4;           // pages on their way, per warp
-    static constexpr int RING_BYTES = (RING * M::PAGE_BYTES + 127) / 128 * 128;
-    static constexpr int Q_BYTES = COLS * D * 2;
-    static constexpr int PLAN_BYTES = (2 * kSharedMaxRows + 4) * 4;
-    // before and behind the 64 KB window of the tables: first-fit, as in FlowCfg; bytes needed from `base`
-    __host__ __device__ static constexpr int plan(int base) {
-        int free0 = base, free1 = (base + 65535) / 65536 * 65536;
-        const int end0 = free1;
-        free1 += 65536;
-        for (int i = 0; i < 2 * WARPS + 1; i++) {
-            const int bytes = i < WARPS ? RING_BYTES : i < 2 * WARPS ? Q_BYTES : PLAN_BYTES;
-            const int a0 = (free0 + 127) / 128 * 128;
-            if (a0 + bytes <= end0) free0 = a0 + bytes;
-            else free1 = (free1 + 127) / 128 * 128 + bytes;
-        }
-        return (free1 > free0 ? free1 : free0) - base;
-    }
-    __host__ __device__ static constexpr int need() {
-        int worst = plan(0);
-        for (int base = 16; base <= 4096; base += 128) worst = plan(base) > worst ? plan(base) : worst;
-        return worst;
-    }
-    static constexpr int SMEM_BYTES = need();
-    static_assert(SMEM_BYTES <= 226 * 1024, "shared memory of a CTA");
 };
 
 // ------------------------------------------------------------------ plan
@@ -89,7 +68,7 @@ __global__ void __launch_bounds__(256) shared_prepare_kernel(const __grid_consta
     after_previous_kernel();
     if (blockIdx.x == 0) {
         const int entries = p.R + p.R * p.K;
-        int base = 0;
+        int base = 0, longest = 0;
         for (int e0 = 0; e0 < entries; e0 += 256) {
             const int e = e0 + tid;
             int places = 0;
@@ -99,6 +78,7 @@ __global__ void __launch_bounds__(256) shared_prepare_kernel(const __grid_consta
                 const int common = shared_common(p, group ? e : (e - p.R) / p.K, leader);
                 const int pages = (group ? common : max(0, shared_len(p, e - p.R) - common) + kPageTokens - 1) / kPageTokens;
                 places = pages == 0 ? 0 : (kSharedPiece + pages * (group ? p.cost_group : p.cost_row)) * (group ? p.units_group : p.units_row);
+                longest = max(longest, pages);
                 p.plan_tokens[e] = common;
                 p.plan_leader[e] = leader;
             }
@@ -118,10 +98,16 @@ __global__ void __launch_bounds__(256) shared_prepare_kernel(const __grid_consta
             }
             if (e < entries) p.plan[e] = before + x - places;
         }
+        // A unit's pieces are walked side by side but joined one after the other: the longest one has at most so many that the two balance.
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        __syncthreads();
+        if (lane == 0) s_sum[warp] = longest;
+        __syncthreads();
         if (tid == 0) {
+            for (int w = 0; w < 8; w++) longest = max(longest, s_sum[w]);
+            const int least = max(2, static_cast<int>(0.8f * sqrtf(static_cast<float>(longest))));
             p.plan[entries] = base;
-            // (a piece has some pages at least, whatever there is to do)
-            p.plan[entries + 1] = max((base + p.warps - 1) / p.warps, kSharedPiece + p.least_pages * p.cost_group);
+            p.plan[entries + 1] = max((base + p.warps - 1) / p.warps, kSharedPiece + least * p.cost_group);
             if (p.first) *p.status = 0;
         }
         return;
@@ -256,7 +242,8 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
     __syncthreads();
 
     const int total = s_plan[entries], share = s_plan[entries + 1], G = p.Hq / p.Hkv;
-    const int me = blockIdx.x * C::WARPS + warp;
+    // (neighbours on the line are on different SMs, so that a short line has them all)
+    const int me = warp * gridDim.x + blockIdx.x;
     const int64_t from = static_cast<int64_t>(me) * share;
     if (from >= total) return;
     const int end = static_cast<int>(min(from + share, static_cast<int64_t>(total)));
@@ -580,36 +567,31 @@ __global__ void __launch_bounds__(128) shared_merge_kernel(const __grid_constant
     const int64_t v = mine < n_rows ? mine : n_rows - 1;
     const int hq = static_cast<int>(v % p.Hq), G = p.Hq / p.Hkv, h = hq / G, b = static_cast<int>(v / p.Hq), r = b / p.K;
     const int share = p.plan[p.R + p.R * p.K + 1];
-    struct Parts { int first, n, pos, places, cost, pages; int64_t row, step; };
+    // the row's pieces of its group's unit, and of its own: rows `step` floats apart
+    struct Parts { const float* first; int n, step; };
     auto parts_of = [&](bool group) {
         const int e = group ? r : p.R + b, units = group ? p.units_group : p.units_row, blocks = units / p.Hkv;
         const int i = (group ? (b - r * p.K) * G : 0) + hq - h * G, blk = i / p.cols, u = h * blocks + blk;
-        const int e0 = p.plan[e], places = (p.plan[e + 1] - e0) / units;
-        Parts x{0, 0, 0, places, group ? p.cost_group : p.cost_row, 0, 0, group ? p.rows_group : p.rows_row};
+        const int e0 = p.plan[e], places = (p.plan[e + 1] - e0) / units, cost = group ? p.cost_group : p.cost_row;
+        Parts x{nullptr, 0, (group ? p.rows_group : p.rows_row) * ROW};
         if (places == 0) return x;
-        x.pages = (places - kSharedPiece) / x.cost;
-        x.pos = e0 + u * places;
-        x.first = x.pos / share;
-        x.n = (x.pos + places - 1) / share - x.first + 1;
-        const int64_t slot = x.first + static_cast<int64_t>(group ? e : e - p.R) * units + u;
-        x.row = (group ? 0 : p.base_row) + slot * x.step + i - blk * p.cols;
+        const int pages = (places - kSharedPiece) / cost, pos = e0 + u * places;
+        int c0 = pos / share, c1 = (pos + places - 1) / share;
+        // (a share that ends among the unit's places on its own has none of its pages, nor has one that begins behind its last page's first place)
+        if (shared_page_of(static_cast<int>(min(static_cast<int64_t>(c0 + 1) * share - pos, static_cast<int64_t>(places))), cost, pages) == 0) c0++;
+        if (c1 > c0 && shared_page_of(c1 * share - pos, cost, pages) == pages) c1--;
+        x.n = c1 - c0 + 1;
+        const int64_t slot = c0 + static_cast<int64_t>(group ? e : e - p.R) * units + u;
+        x.first = p.rows + ((group ? 0 : p.base_row) * ROW + slot * x.step + static_cast<int64_t>(i - blk * p.cols) * ROW);
         return x;
     };
+    const bool any = shared_len(p, b) > 0;
     const Parts a = parts_of(true), z = parts_of(false);
-    auto row_of = [&](int k) -> const float* {     // part k of both, NULL: it has no pages
-        const Parts& x = k < a.n ? a : z;
-        const int j = k < a.n ? k : k - a.n;
-        const int64_t c = static_cast<int64_t>(x.first + j) * share;
-        const int from = static_cast<int>(max(c, static_cast<int64_t>(x.pos)) - x.pos);
-        const int to = static_cast<int>(min(c + share, static_cast<int64_t>(x.pos) + x.places) - x.pos);
-        if (shared_page_of(to, x.cost, x.pages) <= shared_page_of(from, x.cost, x.pages)) return nullptr;
-        return p.rows + (x.row + j * x.step) * ROW;
-    };
-    const int n = shared_len(p, b) > 0 ? a.n + z.n : 0;
+    auto row_of = [&](int k) { return k < a.n ? a.first + static_cast<int64_t>(k) * a.step : z.first + static_cast<int64_t>(k - a.n) * z.step; };
+    const int n = any ? a.n + z.n : 0;
     float M = -INFINITY;
     for (int k = 8 * o + t; k < n; k += 8 * OCTETS) {
-        const float* row = row_of(k);
-        if (row) M = fmaxf(M, row[D]);
+        M = fmaxf(M, row_of(k)[D]);
     }
 #pragma unroll
     for (int d = 1; d < 8 * OCTETS; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
@@ -617,21 +599,21 @@ __global__ void __launch_bounds__(128) shared_merge_kernel(const __grid_constant
 #pragma unroll
     for (int k = 0; k < E; k++) acc[k] = 0.f;
     float L = 0.f;
-#pragma unroll 2
+#pragma unroll 4
     for (int k = o; k < n; k += OCTETS) {
-        const float* row = row_of(k);
-        if (!row) continue;
-        const float m = row[D];
-        if (m == -INFINITY) continue;       // (no token of this row: a group's common ones that lie behind its end)
+        const float* const row = row_of(k);
+        const float m = row[D], l = row[D + 1];
+        float tmp[E / 8][8];
+#pragma unroll
+        for (int x = 0; x < E / 8; x++) load8<float>(row + 8 * (t + 8 * x), tmp[x]);
+        // (no token of this row: a group's common ones that lie behind its end)
+        const bool live = m != -INFINITY;
         const float f = exp2f(m - M);       // (not a number where the piece's rows are none)
-        L = fmaf(row[D + 1], f, L);
+        L = live ? fmaf(l, f, L) : L;
 #pragma unroll
-        for (int x = 0; x < E / 8; x++) {
-            float tmp[8];
-            load8<float>(row + 8 * (t + 8 * x), tmp);
+        for (int x = 0; x < E / 8; x++)
 #pragma unroll
-            for (int c = 0; c < 8; c++) acc[8 * x + c] = fmaf(tmp[c], f, acc[8 * x + c]);
-        }
+            for (int c = 0; c < 8; c++) acc[8 * x + c] = live ? fmaf(tmp[x][c], f, acc[8 * x + c]) : acc[8 * x + c];
     }
     __syncwarp();
 #pragma unroll
