@@ -2027,7 +2027,7 @@ SharedLayout shared_layout(int requests, int group, int Hq, int Hkv, int d, size
     l.rows_row = std::min(G, cols);
     const int64_t R = l.requests, B = R * group, warps = static_cast<int64_t>(ftq::sm_count()) * ftq::kSharedMaxWarps;
     l.plan = round256(head);
-    l.q = l.plan + round256(static_cast<size_t>(3 * (R + B) + 2) * 4);
+    l.q = l.plan + round256(static_cast<size_t>(4 * (R + B) + 4) * 4);
     l.rows = l.q + round256(static_cast<size_t>(B) * Hq * d * 2);
     l.base_row = (warps + R * l.units_group) * l.rows_group;
     l.end = l.rows + static_cast<size_t>(l.base_row + (warps + B * l.units_row) * l.rows_row) * (d + 4) * sizeof(float);
@@ -2051,7 +2051,7 @@ extern "C" int ftq_shared_attn(const void* q, int q_dtype, void* out, int out_dt
     if (q_dtype == FTQ_F32) return fail(FTQ_ERR_UNSUPPORTED, "attention with shared blocks takes 16-bit queries");
     if (group <= 0 || group > ftq::kSharedMaxRows)
         return fail(FTQ_ERR_UNSUPPORTED, "a group has 1 to %d rows, got %d", ftq::kSharedMaxRows, group);
-    if (max_blocks <= 0 || max_seq_len < 0 || num_blocks < 0 || static_cast<int64_t>(n_requests) * group > INT32_MAX)
+    if (max_blocks <= 0 || max_seq_len < 0 || num_blocks < 0 || static_cast<int64_t>(n_requests) * group > INT32_MAX || Hq > 65535)
         return fail(FTQ_ERR_INVALID, "bad shape groups=%d of %d max_blocks=%d max_seq_len=%d", n_requests, group, max_blocks, max_seq_len);
     if (n_requests == 0) return FTQ_OK;
     if (!q || !out || !pool || !block_table || !seq_lens || !shared_lens) return fail(FTQ_ERR_INVALID, "NULL tensor pointer");
@@ -2079,9 +2079,12 @@ extern "C" int ftq_shared_attn(const void* q, int q_dtype, void* out, int out_dt
     p.K = group; p.Hq = Hq; p.Hkv = Hkv; p.q_dtype = q_dtype;
     p.units_group = l.units_group; p.units_row = l.units_row; p.rows_group = l.rows_group; p.rows_row = l.rows_row;
     p.cols = 8 * l.tiles;
+    p.blocks_group = l.units_group / Hkv; p.blocks_row = l.units_row / Hkv;
     // what a page costs: its look-ups and byte work, and a share of that for each tile of columns (see ftq_shared_attn.cuh)
     p.cost_group = 9 + 2 * ((l.rows_group + 7) / 8);
     p.cost_row = 9 + 2 * ((l.rows_row + 7) / 8);
+    p.by_hq = ftq::make_fastdiv(Hq); p.by_group = ftq::make_fastdiv(Hq / Hkv); p.by_rows = ftq::make_fastdiv(group);
+    p.by_cols = ftq::make_fastdiv(p.cols); p.by_cost_group = ftq::make_fastdiv(p.cost_group); p.by_cost_row = ftq::make_fastdiv(p.cost_row);
     const int64_t pages = (static_cast<int64_t>(max_seq_len) + FTQ_PAGE_TOKENS - 1) / FTQ_PAGE_TOKENS,
                   places = (ftq::kSharedPiece + pages * p.cost_group) * l.units_group + group * (ftq::kSharedPiece + pages * p.cost_row) * l.units_row;
     const int requests = static_cast<int>(std::min<int64_t>(l.requests, (INT32_MAX / 2) / places));
@@ -2091,7 +2094,8 @@ extern "C" int ftq_shared_attn(const void* q, int q_dtype, void* out, int out_dt
     uint8_t* const ws = static_cast<uint8_t*>(workspace);
     const int entries = requests * (1 + group);
     p.plan = reinterpret_cast<int*>(ws + l.plan);
-    p.plan_tokens = p.plan + entries + 2;
+    p.plan_unit = p.plan + entries + 4;
+    p.plan_tokens = p.plan_unit + entries;
     p.plan_leader = p.plan_tokens + entries;
     p.q_rows = ws + l.q;
     p.rows = reinterpret_cast<float*>(ws + l.rows);

@@ -33,14 +33,10 @@ struct SharedCfg : MmaCfg<D, BK, BV, 2> {
 };
 
 // ------------------------------------------------------------------ plan
-// Units of an entry (the common tokens of a group, or a row's own), and where their places are.
-struct SharedEntry {
-    int first, pages, unit;     // the entry's first place, pages of a unit, places of a unit
-};
 // first page of a unit's piece that starts `at` places into it
-__device__ __forceinline__ int shared_page_of(int at, int cost, int pages) {
+__device__ __forceinline__ int shared_page_of(int at, const FastDiv& cost, int pages) {
     const int x = at - kSharedPiece;
-    return x <= 0 ? 0 : min((x + cost - 1) / cost, pages);
+    return x <= 0 ? 0 : min(static_cast<int>(fast_div(x + cost.d - 1, cost)), pages);
 }
 __device__ __forceinline__ int shared_len(const SharedAttnParams& p, int b) { return max(0, min(p.seq_lens[b], p.max_seq)); }
 // tokens of group r that are taken as common (whole blocks, as far as its longest row goes), and that row
@@ -57,8 +53,8 @@ __device__ __forceinline__ int shared_common(const SharedAttnParams& p, int r, i
     return max(0, min(p.shared_lens[r], most)) / kPageTokens * kPageTokens;
 }
 
-// plan: [e] first place of entry e (groups, then rows), [entries]: the end; then per entry the leader of a group / the common
-// tokens before a row's own, and its pages
+// plan: [e] first place of entry e (groups, then rows), [entries] the end, then the share of a warp as a divisor; plan_unit: places
+// of a unit of an entry (0: it has no pages); plan_tokens, plan_leader: the common tokens, and the row that they are read through.
 template <int D>
 __global__ void __launch_bounds__(256) shared_prepare_kernel(const __grid_constant__ SharedAttnParams p) {
     constexpr int E = D / kOctet;
@@ -77,7 +73,9 @@ __global__ void __launch_bounds__(256) shared_prepare_kernel(const __grid_consta
                 const bool group = e < p.R;
                 const int common = shared_common(p, group ? e : (e - p.R) / p.K, leader);
                 const int pages = (group ? common : max(0, shared_len(p, e - p.R) - common) + kPageTokens - 1) / kPageTokens;
-                places = pages == 0 ? 0 : (kSharedPiece + pages * (group ? p.cost_group : p.cost_row)) * (group ? p.units_group : p.units_row);
+                const int unit = pages == 0 ? 0 : kSharedPiece + pages * (group ? p.cost_group : p.cost_row);
+                places = unit * (group ? p.units_group : p.units_row);
+                p.plan_unit[e] = unit;
                 longest = max(longest, pages);
                 p.plan_tokens[e] = common;
                 p.plan_leader[e] = leader;
@@ -105,9 +103,12 @@ __global__ void __launch_bounds__(256) shared_prepare_kernel(const __grid_consta
         __syncthreads();
         if (tid == 0) {
             for (int w = 0; w < 8; w++) longest = max(longest, s_sum[w]);
-            const int least = max(2, static_cast<int>(0.8f * sqrtf(static_cast<float>(longest))));
+            const int least = max(2, static_cast<int>(0.4f * sqrtf(static_cast<float>(longest))));
             p.plan[entries] = base;
-            p.plan[entries + 1] = max((base + p.warps - 1) / p.warps, kSharedPiece + least * p.cost_group);
+            const uint32_t share = max((base + p.warps - 1) / p.warps, kSharedPiece + least * p.cost_group), bits = 32 - __clz(share - 1);
+            p.plan[entries + 1] = share;        // (make_fastdiv)
+            p.plan[entries + 2] = static_cast<int>(static_cast<uint32_t>(((1ull << (31 + bits)) + share - 1) / share));
+            p.plan[entries + 3] = 31 + bits;
             if (p.first) *p.status = 0;
         }
         return;
@@ -256,13 +257,14 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
             if (s_plan[mid] <= pos) lo = mid; else hi = mid;
         }
         const bool group = lo < p.R;
-        const int units = group ? p.units_group : p.units_row, cost = group ? p.cost_group : p.cost_row;
-        const int unit_places = (s_plan[lo + 1] - s_plan[lo]) / units, pages = (unit_places - kSharedPiece) / cost;
+        const int units = group ? p.units_group : p.units_row, unit_places = p.plan_unit[lo];
+        const FastDiv cost = group ? p.by_cost_group : p.by_cost_row;
+        const int pages = fast_div(unit_places - kSharedPiece, cost);
         const int u = (pos - s_plan[lo]) / unit_places, at = pos - s_plan[lo] - u * unit_places;
         const int to = min(unit_places, at + end - pos);
         const int blocks = units / p.Hkv, all = group ? p.K * G : G, blk = u % blocks;
         it.hkv = u / blocks;
-        const int r = group ? lo : (lo - p.R) / p.K, common = p.plan_tokens[lo], leader = p.plan_leader[lo];
+        const int r = group ? lo : static_cast<int>(fast_div(lo - p.R, p.by_rows)), common = p.plan_tokens[lo], leader = p.plan_leader[lo];
         it.cols = min(C::COLS, all - blk * C::COLS);
         it.qh = r * p.Hkv + it.hkv;
         it.row = group ? leader : lo - p.R;
@@ -556,30 +558,36 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
 }
 
 // ------------------------------------------------------------------ merge
+// OCTETS octets per row: 1 (many rows, which have few pieces each), or 16, a CTA (their pieces are a chain of loads otherwise: 1536
+// rows of heads of 256 with up to 36 pieces took a warp each 37 us, as long as the attention).
 template <int D, typename OT, int OCTETS>
 __global__ void __launch_bounds__(128) shared_merge_kernel(const __grid_constant__ SharedAttnParams p) {
     constexpr int E = D / kOctet, ROW = D + 4;
-    const int lane = threadIdx.x & 31, t = lane & 7, o = (lane >> 3) & (OCTETS - 1);
+    __shared__ float s_max[4], s_sum[4];
+    __shared__ __align__(16) float s_acc[OCTETS > 1 ? 4 * D : 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 7, o = (threadIdx.x >> 3) & (OCTETS - 1);
     let_next_kernel_start();
     after_previous_kernel();
     const int64_t n_rows = static_cast<int64_t>(p.R) * p.K * p.Hq;
     const int64_t mine = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / (8 * OCTETS);
     const int64_t v = mine < n_rows ? mine : n_rows - 1;
-    const int hq = static_cast<int>(v % p.Hq), G = p.Hq / p.Hkv, h = hq / G, b = static_cast<int>(v / p.Hq), r = b / p.K;
-    const int share = p.plan[p.R + p.R * p.K + 1];
+    const int b = fast_div(static_cast<uint32_t>(v), p.by_hq), hq = static_cast<int>(v) - b * p.Hq, G = p.by_group.d, h = fast_div(hq, p.by_group), r = fast_div(b, p.by_rows);
+    const int* const tail = p.plan + p.R + p.R * p.K;
+    const FastDiv share{static_cast<uint32_t>(tail[1]), static_cast<uint32_t>(tail[2]), static_cast<uint32_t>(tail[3])};
     // the row's pieces of its group's unit, and of its own: rows `step` floats apart
     struct Parts { const float* first; int n, step; };
     auto parts_of = [&](bool group) {
-        const int e = group ? r : p.R + b, units = group ? p.units_group : p.units_row, blocks = units / p.Hkv;
-        const int i = (group ? (b - r * p.K) * G : 0) + hq - h * G, blk = i / p.cols, u = h * blocks + blk;
-        const int e0 = p.plan[e], places = (p.plan[e + 1] - e0) / units, cost = group ? p.cost_group : p.cost_row;
+        const int e = group ? r : p.R + b, units = group ? p.units_group : p.units_row;
+        const int i = (group ? (b - r * p.K) * G : 0) + hq - h * G, blk = fast_div(i, p.by_cols), u = h * (group ? p.blocks_group : p.blocks_row) + blk;
+        const int e0 = p.plan[e], places = p.plan_unit[e];
+        const FastDiv cost = group ? p.by_cost_group : p.by_cost_row;
         Parts x{nullptr, 0, (group ? p.rows_group : p.rows_row) * ROW};
         if (places == 0) return x;
-        const int pages = (places - kSharedPiece) / cost, pos = e0 + u * places;
-        int c0 = pos / share, c1 = (pos + places - 1) / share;
+        const int pages = fast_div(places - kSharedPiece, cost), pos = e0 + u * places;
+        int c0 = fast_div(pos, share), c1 = fast_div(pos + places - 1, share);
         // (a share that ends among the unit's places on its own has none of its pages, nor has one that begins behind its last page's first place)
-        if (shared_page_of(static_cast<int>(min(static_cast<int64_t>(c0 + 1) * share - pos, static_cast<int64_t>(places))), cost, pages) == 0) c0++;
-        if (c1 > c0 && shared_page_of(c1 * share - pos, cost, pages) == pages) c1--;
+        if (shared_page_of(static_cast<int>(min(static_cast<int64_t>(c0 + 1) * share.d - pos, static_cast<int64_t>(places))), cost, pages) == 0) c0++;
+        if (c1 > c0 && shared_page_of(static_cast<int>(c1 * share.d) - pos, cost, pages) == pages) c1--;
         x.n = c1 - c0 + 1;
         const int64_t slot = c0 + static_cast<int64_t>(group ? e : e - p.R) * units + u;
         x.first = p.rows + ((group ? 0 : p.base_row) * ROW + slot * x.step + static_cast<int64_t>(i - blk * p.cols) * ROW);
@@ -594,12 +602,17 @@ __global__ void __launch_bounds__(128) shared_merge_kernel(const __grid_constant
         M = fmaxf(M, row_of(k)[D]);
     }
 #pragma unroll
-    for (int d = 1; d < 8 * OCTETS; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    for (int d = 1; d < 8 * (OCTETS > 1 ? 4 : 1); d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    if constexpr (OCTETS > 1) {
+        if (lane == 0) s_max[warp] = M;
+        __syncthreads();
+        M = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    }
     float acc[E];
 #pragma unroll
     for (int k = 0; k < E; k++) acc[k] = 0.f;
     float L = 0.f;
-#pragma unroll 4
+#pragma unroll (OCTETS > 1 ? 2 : 4)
     for (int k = o; k < n; k += OCTETS) {
         const float* const row = row_of(k);
         const float m = row[D], l = row[D + 1];
@@ -616,11 +629,24 @@ __global__ void __launch_bounds__(128) shared_merge_kernel(const __grid_constant
             for (int c = 0; c < 8; c++) acc[8 * x + c] = live ? fmaf(tmp[x][c], f, acc[8 * x + c]) : acc[8 * x + c];
     }
     __syncwarp();
+    if constexpr (OCTETS > 1) {
 #pragma unroll
-    for (int d = 8; d < 8 * OCTETS; d <<= 1) {
-        L += __shfl_xor_sync(0xffffffffu, L, d);
+        for (int d = 8; d < 32; d <<= 1) {
+            L += __shfl_xor_sync(0xffffffffu, L, d);
 #pragma unroll
-        for (int k = 0; k < E; k++) acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], d);
+            for (int k = 0; k < E; k++) acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], d);
+        }
+        // each warp's sums, then the first warp's of all
+        if (lane == 0) s_sum[warp] = L;
+        if (lane < 8) {
+#pragma unroll
+            for (int k = 0; k < E; k++) s_acc[warp * D + k * 8 + t] = acc[k];
+        }
+        __syncthreads();
+        if (warp > 0) return;
+        L = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+#pragma unroll
+        for (int k = 0; k < E; k++) acc[k] = (s_acc[k * 8 + t] + s_acc[D + k * 8 + t]) + (s_acc[2 * D + k * 8 + t] + s_acc[3 * D + k * 8 + t]);
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
@@ -628,7 +654,7 @@ __global__ void __launch_bounds__(128) shared_merge_kernel(const __grid_constant
     octet_fwht<E>(acc, lane);
 #pragma unroll
     for (int k = 0; k < E; k++) {
-        if (mine >= n_rows || (k & (OCTETS - 1)) != o) continue;
+        if (mine >= n_rows || (OCTETS > 1 && (k & 3) != (lane >> 3))) continue;
         const float x = acc[k] * p.rsqrt_d;
         reinterpret_cast<OT*>(p.out)[v * D + t + 8 * k] = from_float<OT>(__uint_as_float(__float_as_uint(x) ^ sign_mask(p.signs, t + 8 * k)));
     }

@@ -59,9 +59,8 @@ cudaError_t launch_shared_prepare(int head_dim, const SharedAttnParams& p, cudaS
 template <int D, typename OT>
 static cudaError_t run_merge(const SharedAttnParams& p, cudaStream_t stream) {
     const int64_t rows = static_cast<int64_t>(p.R) * p.K * p.Hq;
-    // (a warp per row, an octet where there are many, which have few pieces each: 2800 rows of contexts of up to 4096 tokens 41 -> 19 us)
     if (rows <= 2 * static_cast<int64_t>(kWideMerge) * sm_count())
-        return launch_dependent(shared_merge_kernel<D, OT, 4>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream, p);
+        return launch_dependent(shared_merge_kernel<D, OT, 16>, dim3(static_cast<unsigned>(rows)), 128, 0, stream, p);
     return launch_dependent(shared_merge_kernel<D, OT, 1>, dim3(static_cast<unsigned>((rows + 15) / 16)), 128, 0, stream, p);
 }
 template <int D>

@@ -15,7 +15,7 @@ constexpr int shared_least_tiles(int head_dim) { return head_dim == 64 ? 2 : 1; 
 
 // Shared memory of a CTA from `base` on: the 64 KB window of the tables on a boundary of its size; before and behind it, first-fit,
 // the warps' rings and queries, then the plan.
-constexpr int kSharedPlanBytes = (2 * kSharedMaxRows + 4) * 4, kSharedSmemLimit = 226 * 1024;
+constexpr int kSharedPlanBytes = (2 * kSharedMaxRows + 8) * 4, kSharedSmemLimit = 226 * 1024;
 constexpr int shared_ring_bytes(int page_bytes, int ring) { return (ring * page_bytes + 127) / 128 * 128; }
 constexpr int shared_smem_from(int base, int warps, int ring_bytes, int q_bytes) {
     int free0 = base, free1 = (base + 65535) / 65536 * 65536;
@@ -56,10 +56,11 @@ struct SharedAttnParams {
     const int32_t *block_table, *seq_lens, *shared_lens;   // [R * K, max_blocks], [R * K], [R]
     int max_blocks, max_seq, R, K, Hq, Hkv, q_dtype;
     void* out;
-    // units of a KV head and head block, their columns' rows in the workspace, places of a page
-    int units_group, units_row, rows_group, rows_row, cost_group, cost_row, cols;
+    // units of an entry, of a KV head; their columns' rows in the workspace; places of a page; columns of a unit
+    int units_group, units_row, blocks_group, blocks_row, rows_group, rows_row, cost_group, cost_row, cols;
     int warps;                   // of the grid
-    int *plan, *plan_tokens, *plan_leader;
+    int *plan, *plan_unit, *plan_tokens, *plan_leader;
+    FastDiv by_hq, by_group, by_rows, by_cols, by_cost_group, by_cost_row;      // Hq, Hq / Hkv, K, cols, places of a page
     uint8_t* q_rows;             // fp16 [R, Hkv, K * G, D]
     float* rows;                 // (O, m, l) [D + 4]: the groups' pieces, from base_row on those of single rows
     int64_t base_row;
