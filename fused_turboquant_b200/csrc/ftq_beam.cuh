@@ -358,8 +358,8 @@ __global__ void __launch_bounds__(256) shared_lens_kernel(const SharedLensParams
     constexpr int COLUMNS = 1024;
     for (int j0 = 0; j0 < whole; j0 += COLUMNS) {
         const int n = min(COLUMNS, whole - j0);
-        for (int i = tid; i < (p.group - first - 1) * n; i += blockDim.x) {
-            const int k = first + 1 + i / n, j = j0 + i % n;
+        for (int64_t i = tid; i < static_cast<int64_t>(p.group - first - 1) * n; i += blockDim.x) {
+            const int k = first + 1 + static_cast<int>(i / n), j = j0 + static_cast<int>(i % n);
             if (p.table[(row0 + k) * p.max_blocks + j] != p.table[(row0 + first) * p.max_blocks + j] && p.lens[row0 + k] > 0) atomicMin(&s_cut, j);
         }
         __syncthreads();

@@ -178,7 +178,7 @@ template <typename T>
 __global__ void __launch_bounds__(kSelectThreads, 5) beam_rows_kernel(const SelectParams p) {
     using V = SelectVec<T>;
     constexpr int N = V::N, B = kSelectBatch;
-    extern __shared__ unsigned long long s_keys[];
+    extern __shared__ __align__(16) unsigned long long s_keys[];
     __shared__ float s_max[kSelectWarps], s_sum[kSelectWarps];
     __shared__ uint32_t s_top[kSelectTop * kSelectWarps + 1];
     __shared__ int s_first[kSelectThreads], s_n[2];
@@ -344,7 +344,7 @@ __device__ __forceinline__ double select_value64(unsigned long long o) {
 // A CTA has a request: its rows' sums, the ends' totals, and the order of the tokens that the rows kept.
 template <typename T>
 __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectParams p) {
-    extern __shared__ unsigned long long s_keys[];
+    extern __shared__ __align__(16) unsigned long long s_keys[];
     // a beam's score (-inf: it has no continuation), its row's maximum, and the logarithm of the sum of exponentials less that
     __shared__ double s_score[kBeamMax], s_max[kBeamMax], s_log[kBeamMax];
     __shared__ uint32_t s_top[kSelectTop * kSelectWarps + 1];

@@ -558,19 +558,20 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
 }
 
 // ------------------------------------------------------------------ merge
-// An octet per row where rows are many, which have few pieces each; else (CTA) a CTA, its warps a piece at a time each, a lane D / 32
-// coordinates of it: pieces are a chain of loads otherwise (1536 rows of heads of 256 with up to 50 pieces took a warp each 40 us, as
-// long as the attention).
-template <int D, typename OT, bool CTA>
+// A warp per row, or WARPS = 4 where rows are few: each takes a piece at a time, a lane D / 32 coordinates of it, so that the loads of
+// several pieces are on their way together (1536 rows of heads of 256 with up to 50 pieces: an octet a piece, a warp a row 40 us, as long as the
+// attention; 15 now.  8192 rows of a few pieces: an octet a row 15 us).
+template <int D, typename OT, int WARPS>
 __global__ void __launch_bounds__(128) shared_merge_kernel(const __grid_constant__ SharedAttnParams p) {
     constexpr int E = D / kOctet, ROW = D + 4, PL = D / 32;
     __shared__ float s_max[4], s_sum[4];
-    __shared__ __align__(16) float s_acc[CTA ? 4 * D : 1];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 7;
+    __shared__ __align__(16) float s_all[4 * D];
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % WARPS, t = lane & 7;
+    float* const s_acc = s_all + (threadIdx.x >> 5) / WARPS * WARPS * D;      // the row's warps'
     let_next_kernel_start();
     after_previous_kernel();
     const int64_t n_rows = static_cast<int64_t>(p.R) * p.K * p.Hq;
-    const int64_t mine = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / (CTA ? 128 : 8);
+    const int64_t mine = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / (32 * WARPS);
     const int64_t v = mine < n_rows ? mine : n_rows - 1;
     const int b = fast_div(static_cast<uint32_t>(v), p.by_hq), hq = static_cast<int>(v) - b * p.Hq, G = p.by_group.d, h = fast_div(hq, p.by_group), r = fast_div(b, p.by_rows);
     const int* const tail = p.plan + p.R + p.R * p.K;
@@ -602,76 +603,58 @@ __global__ void __launch_bounds__(128) shared_merge_kernel(const __grid_constant
     // (0 of a piece without a token of this row, a group's common ones that lie behind its end; not a number where the piece's
     // rows are none)
     auto weight = [&](float m) { return m == -INFINITY ? 0.f : fast_exp2(m - M); };
-    if constexpr (CTA) {
-        for (int k = threadIdx.x; k < n; k += 128) M = fmaxf(M, row_of(k)[D]);
+    for (int k = 32 * warp + lane; k < n; k += 32 * WARPS) M = fmaxf(M, row_of(k)[D]);
+    __syncwarp();
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    for (int d = 1; d < 32; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    if constexpr (WARPS > 1) {
         if (lane == 0) s_max[warp] = M;
         __syncthreads();
         M = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-        float mine_acc[PL];
+    }
+    float mine_acc[PL];
 #pragma unroll
-        for (int i = 0; i < PL; i++) mine_acc[i] = 0.f;
+    for (int i = 0; i < PL; i++) mine_acc[i] = 0.f;
 #pragma unroll 4
-        for (int k = warp; k < n; k += 4) {
-            const float* const row = row_of(k);
-            const float m = row[D], l = row[D + 1];
-            float x[PL];
-            if constexpr (PL == 2) {
-                *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(row + 2 * lane);
-            } else {
+    for (int k = warp; k < n; k += WARPS) {
+        const float* const row = row_of(k);
+        const float m = row[D], l = row[D + 1];
+        float x[PL];
+        if constexpr (PL == 2) {
+            *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(row + 2 * lane);
+        } else {
 #pragma unroll
-                for (int i = 0; i < PL; i += 4) *reinterpret_cast<float4*>(x + i) = *reinterpret_cast<const float4*>(row + PL * lane + i);
-            }
-            const float f = weight(m);
-            L = fmaf(l, f, L);
-#pragma unroll
-            for (int i = 0; i < PL; i++) mine_acc[i] = fmaf(x[i], f, mine_acc[i]);
+            for (int i = 0; i < PL; i += 4) *reinterpret_cast<float4*>(x + i) = *reinterpret_cast<const float4*>(row + PL * lane + i);
         }
-        // each warp's sums, then the first warp's of all
+        const float f = weight(m);
+        L = fmaf(l, f, L);
 #pragma unroll
-        for (int i = 0; i < PL; i++) s_acc[warp * D + PL * lane + i] = mine_acc[i];
+        for (int i = 0; i < PL; i++) mine_acc[i] = fmaf(x[i], f, mine_acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < PL; i++) s_acc[warp * D + PL * lane + i] = mine_acc[i];
+    if constexpr (WARPS > 1) {      // each warp's sums, then the first warp's of all
         if (lane == 0) s_sum[warp] = L;
         __syncthreads();
         if (warp > 0) return;
         L = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-#pragma unroll
-        for (int x = 0; x < E / 8; x++)
-#pragma unroll
-            for (int c = 0; c < 8; c++) {
-                const float* const at = s_acc + 8 * (t + 8 * x) + c;
-                acc[8 * x + c] = (at[0] + at[D]) + (at[2 * D] + at[3 * D]);
-            }
     } else {
-        for (int k = t; k < n; k += 8) M = fmaxf(M, row_of(k)[D]);
-        __syncwarp();
-#pragma unroll
-        for (int d = 1; d < 8; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-#pragma unroll
-        for (int k = 0; k < E; k++) acc[k] = 0.f;
-#pragma unroll 4
-        for (int k = 0; k < n; k++) {
-            const float* const row = row_of(k);
-            const float m = row[D], l = row[D + 1];
-            float x[E / 8][8];
-#pragma unroll
-            for (int i = 0; i < E / 8; i++) load8<float>(row + 8 * (t + 8 * i), x[i]);
-            const float f = weight(m);
-            L = fmaf(l, f, L);
-#pragma unroll
-            for (int i = 0; i < E / 8; i++)
-#pragma unroll
-                for (int c = 0; c < 8; c++) acc[8 * i + c] = fmaf(x[i][c], f, acc[8 * i + c]);
-        }
         __syncwarp();
     }
+#pragma unroll
+    for (int x = 0; x < E / 8; x++)
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            const float* const at = s_acc + 8 * (t + 8 * x) + c;
+            acc[8 * x + c] = WARPS > 1 ? (at[0] + at[D]) + (at[2 * D] + at[3 * D]) : at[0];
+        }
     const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
     for (int k = 0; k < E; k++) acc[k] *= inv;
     octet_fwht<E>(acc, lane);
 #pragma unroll
     for (int k = 0; k < E; k++) {
-        if (mine >= n_rows || (CTA && (k & 3) != (lane >> 3))) continue;
+        if (mine >= n_rows || (k & 3) != (lane >> 3)) continue;
         const float x = acc[k] * p.rsqrt_d;
         reinterpret_cast<OT*>(p.out)[v * D + t + 8 * k] = from_float<OT>(__uint_as_float(__float_as_uint(x) ^ sign_mask(p.signs, t + 8 * k)));
     }

@@ -60,8 +60,8 @@ template <int D, typename OT>
 static cudaError_t run_merge(const SharedAttnParams& p, cudaStream_t stream) {
     const int64_t rows = static_cast<int64_t>(p.R) * p.K * p.Hq;
     if (rows <= 2 * static_cast<int64_t>(kWideMerge) * sm_count())
-        return launch_dependent(shared_merge_kernel<D, OT, true>, dim3(static_cast<unsigned>(rows)), 128, 0, stream, p);
-    return launch_dependent(shared_merge_kernel<D, OT, false>, dim3(static_cast<unsigned>((rows + 15) / 16)), 128, 0, stream, p);
+        return launch_dependent(shared_merge_kernel<D, OT, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, stream, p);
+    return launch_dependent(shared_merge_kernel<D, OT, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream, p);
 }
 template <int D>
 static cudaError_t merge_by_type(int out_dtype, const SharedAttnParams& p, cudaStream_t stream) {
