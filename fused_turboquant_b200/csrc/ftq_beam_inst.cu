@@ -26,16 +26,26 @@ static_assert(8 * select_pow2(kSelectMaxKeep * kSelectVectors) <= 48 * 1024, "sh
 
 }  // namespace
 
-// A CTA's part of a row is as long as its threads' vectors can be looked at again, and as short as fills the device where there are
-// few rows, but at least a vector a thread (shorter ones leave more to be joined than they save).
+// A CTA's part of a row is as long as its threads' vectors can be sorted, at most, and a vector a thread at least (shorter ones leave more
+// to be joined than they save).  In between, the number of parts that gives the shortest schedule: rounds of five CTAs an SM, of which
+// each costs its vectors and, for the threshold and the tokens that reach it, as much as 1024 more; and the request's CTA of
+// beam_join_kernel about one for each token that it gets.  (Eight beams of 131072 bf16 logits, in a graph: 2, 8, 16 and 64 requests 49,
+// 35, 29 and 42 us in parts that fill 12 CTAs an SM; 14, 20, 18 and 42 so.)
 SelectPlan select_plan(int dtype, int requests, int beams, int vocab, int keep) {
-    const int n = dtype == kF32 ? 4 : 8, most = (kSelectVectors * kSelectThreads - 1) * n, least = kSelectThreads * n;
-    const int64_t rows = static_cast<int64_t>(requests) * beams, want = 12 * sm_count();
-    int64_t chunks = std::max<int64_t>((static_cast<int64_t>(vocab) + most - 1) / most, rows > 0 ? (want + rows - 1) / rows : 1);
-    int64_t chunk = std::max<int64_t>((vocab + chunks - 1) / chunks, std::min(least, vocab));
-    chunk = std::min<int64_t>((chunk + n - 1) / n * n, most);
-    chunks = (vocab + chunk - 1) / chunk;
-    return {static_cast<int>(chunks), static_cast<int>(chunk)};
+    const int n = dtype == kF32 ? 4 : 8;
+    const int64_t most = (kSelectVectors * kSelectThreads - 1) * n, least = std::min<int64_t>(kSelectThreads * n, vocab);
+    const int64_t rows = std::max<int64_t>(1, static_cast<int64_t>(requests) * beams), slots = 5 * sm_count();
+    auto chunk_of = [&](int64_t chunks) { return std::min(most, (std::max((vocab + chunks - 1) / chunks, least) + n - 1) / n * n); };
+    int64_t chunk = 0, cost = 0;
+    const int64_t lo = (vocab + most - 1) / most, hi = std::max<int64_t>(lo, (vocab + least - 1) / least);
+    for (int64_t chunks = lo; chunks <= std::min(hi, lo + 64); chunks++) {
+        const int64_t c = chunk_of(chunks), all = rows * ((vocab + c - 1) / c), t = (all + slots - 1) / slots * (c / n + 1024) + beams * ((vocab + c - 1) / c) * keep;
+        if (chunk == 0 || t < cost) {
+            cost = t;
+            chunk = c;
+        }
+    }
+    return {static_cast<int>((vocab + chunk - 1) / chunk), static_cast<int>(chunk)};
 }
 
 cudaError_t launch_select(int dtype, const SelectParams& p, cudaStream_t stream) {
