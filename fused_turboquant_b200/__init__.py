@@ -6,7 +6,7 @@ Public names follow the reference package (src/fused_turboquant/__init__.py):
 ``fused_turboquant_b200.kernels``; ``PagedKVPool`` is the paged cache the vLLM
 attention impl drives, ``hf_cache.CompressedKVCache`` the HF-style cache on top of it and
 ``tq_v1`` the vLLM-v1 slot-format store / decode.  ``PageTable``, ``tree`` and ``logits`` are what a serving
-step with drafted token trees needs beside the pool.
+step with drafted token trees needs beside the pool, ``beam`` and a ``PageTable`` with ``sharing`` what one with beams does.
 """
 from .quantizer import CompressedTensor, TurboQuantMSE  # noqa: F401
 from .paged import PagedKVPool  # noqa: F401

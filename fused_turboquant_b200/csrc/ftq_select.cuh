@@ -14,6 +14,11 @@
 // the first), since otherwise as many threads or vectors would each hold a token that goes before it.
 // beam_join_kernel adds up a request's rows and does the same with their tokens' totals, in 64 bits (totals of different beams
 // may lie closer than fp32 tells apart).
+//
+// 64 requests of 8 beams, 131072 bf16 logits: 42 us, 36 of them the rows (134 MB: 20.5 us of HBM).  A logit takes 7 instructions (its
+// exponential one of 16 a cycle and SM: 15 us), threshold and ranks a quarter of all; issue is busy half of the time, and what
+// keeps the rest is loads and the few barriers of CTAs of 32768 tokens.  With three bitonic sorts a CTA 133 us; thresholds 54; the
+// chunk prefetched and the join's loads side by side 47; the next batch on its way, vectors looked at again one a thread 44.
 #pragma once
 
 #include <type_traits>

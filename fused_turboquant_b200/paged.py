@@ -231,7 +231,31 @@ class PagedKVPool:
         return Accepted(*_lib.native().tree_commit(self, block_table, seq_lens, tokens, parents, next_tokens, tree_lens))
 
     def shared_workspace_bytes(self, groups: int, group: int, num_q_heads: int, max_seq_len: int) -> int:
-        return int(_lib.load().ftq_shared_workspace_bytes(groups, group, num_q_heads, self.num_kv_heads, self.head_dim, max_seq_len))
+        both = int(_lib.load().ftq_shared_workspace_bytes(groups, group, num_q_heads, self.num_kv_heads, self.head_dim, max_seq_len))
+        return max(both, self.workspace_bytes(groups * group, num_q_heads, max_seq_len)) if both else 0
+
+    def _takes_shared_kernel(self, q, block_table, seq_lens, max_seq_len, shared_lens, out, workspace) -> bool:
+        """Whether a call goes to the kernels that read common blocks once; the decode kernel takes the rows as they are.
+
+        A page for a group costs those about 0.7 + 0.5 for each eight columns (rows x heads of a KV head) of what it costs
+        the decode kernel for a row, and they are three launches, 10 us more than its one: 4 samples of 900 tokens, 32 / 8 heads of 128, 17 us
+        against 10; 40 x 5 of up to 4096, 14 / 2 heads of 64, 29 against 19; 32 x 8 of 8192, 32 / 8 heads, 168 against 423.  Lengths
+        are on the device: about half of the most that they may be is taken for granted.  GQA groups above 8 always go
+        there (the decode kernel for them is the fp32 one), and so do arguments that are to be refused.
+        """
+        B, D = q.shape[0], q.shape[-1]
+        n = shared_lens.shape[0] if shared_lens.dim() == 1 else 0
+        if not (q.is_cuda and q.dim() == 3 and q.dtype in (torch.float16, torch.bfloat16) and D == self.head_dim and n > 0 and B > 0 and
+                B % n == 0 and block_table.dim() == 2 and block_table.shape[0] == B and seq_lens.shape == (B,) and
+                0 < max_seq_len <= PAGE_TOKENS * block_table.shape[1] and q.shape[1] > 0 and q.shape[1] % self.num_kv_heads == 0 and
+                B // n <= 1024 and (out is None or (out.is_cuda and out.shape == q.shape and out.is_contiguous() and out.dtype in _DT))):
+            return True
+        group, heads = B // n, q.shape[1] // self.num_kv_heads
+        if heads > 8 or (workspace is not None and
+                         workspace.numel() * workspace.element_size() < self.shared_workspace_bytes(n, group, q.shape[1], max_seq_len)):
+            return True
+        saved = 1 - (0.7 + 0.52 * -(-group * heads // 8)) / group
+        return saved * B * self.num_kv_heads * -(-max_seq_len // PAGE_TOKENS) * D >= 55000 * 128
 
     def shared_attention(self, q: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, max_seq_len: int,
                          shared_lens: torch.Tensor, scale: float | None = None, layer: int = 0, out: torch.Tensor | None = None,
@@ -241,10 +265,13 @@ class PagedKVPool:
         q: [B, Hq, D], fp16 or bf16, not rotated; block_table [B, max_blocks], seq_lens [B]; shared_lens [groups]: B / groups
         successive rows are a group, and the first ``shared_lens[g]`` tokens of its rows, rounded down to whole blocks, lie in the
         same blocks (``PageTable.shared_lens`` says how many do).  They are read once for the group, through its longest
-        row.  The result is that of ``decode_attention`` on the rows; rows without tokens are zero.  Up to 1024 rows a group.
-        No host synchronisation; graph-capturable when out / workspace are passed in.  ``decode_status`` covers this call too.
+        row, where that pays (see _takes_shared_kernel).  The result is that of ``decode_attention`` on the rows; rows without tokens are
+        zero.  Up to 1024 rows a group.  No host synchronisation; graph-capturable when out / workspace are passed in.
+        ``decode_status`` covers this call too.
         """
         _require_cuda(q, "q")
+        if not self._takes_shared_kernel(q, block_table, seq_lens, max_seq_len, shared_lens, out, workspace):
+            return self.decode_attention(q, block_table, seq_lens, max_seq_len, scale, layer, out, workspace)
         if _trace.ENABLED:
             with _trace.nvtx("ftq.decode"):
                 return _lib.native().paged_shared(self, q, block_table, seq_lens, max_seq_len, shared_lens, scale, layer, out, workspace)

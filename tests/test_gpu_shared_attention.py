@@ -17,6 +17,14 @@ pytestmark = pytest.mark.gpu
 E = 2.0 ** -11 / math.sqrt(3)
 
 
+@pytest.fixture(autouse=True)
+def kernels_that_read_common_blocks_once(request, monkeypatch):
+    """Small calls go to the decode kernel otherwise, which has tests of its own."""
+    if "as_a_user_calls_it" not in request.node.name:
+        from fused_turboquant_b200 import PagedKVPool
+        monkeypatch.setattr(PagedKVPool, "_takes_shared_kernel", lambda *a: True)
+
+
 class Case:
     """Groups of rows: ctx[r] common tokens, lens[r][k] tokens of row k (0: none; else at least the whole blocks of ctx[r])."""
 
@@ -316,3 +324,22 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="1024 rows"):
         call(q[:1].expand(1025, -1, -1), table[:1].expand(1025, -1), lens[:1].expand(1025), top, shared[:1])
     assert call(q[:0], table[:0], lens[:0], top, shared[:0]).shape == (0, 8, 64)
+
+
+@pytest.mark.parametrize("hkv,g,k,ctx,groups,both", [(8, 4, 4, 900, 1, False), (2, 7, 5, 1000, 9, False), (8, 4, 8, 4096, 12, True), (2, 16, 2, 100, 3, True),
+                                                     (8, 4, 1, 3000, 40, False)])
+def test_as_a_user_calls_it(hkv, g, k, ctx, groups, both):
+    """Calls that go to either kernel say the same, with memory of their own too; so do refusals (above: test_refusals)."""
+    import torch
+    c = Case(23 + k, 128 if g != 7 else 64, 4, 4, hkv, g, [ctx] * groups, beams([ctx] * groups, range(5, 5 + groups), k))
+    args = c.args()
+    assert c.pool._takes_shared_kernel(*args, None, None) == both
+    rows = [0, k - 1, groups * k - 1]
+    check32(c, rows=rows)
+    ws = torch.empty(c.pool.shared_workspace_bytes(groups, k, hkv * g, args[3]), dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(c.q)
+    assert torch.equal(c.run(out=out, workspace=ws), c.run())
+
+
+def test_refusals_as_a_user_calls_it():
+    test_refusals()
