@@ -243,9 +243,11 @@ class PagedKVPool:
         are on the device: about half of the most that they may be is taken for granted.  GQA groups above 8 always go
         there (the decode kernel for them is the fp32 one), and so do arguments that are to be refused.
         """
-        B, D = q.shape[0], q.shape[-1]
-        n = shared_lens.shape[0] if shared_lens.dim() == 1 else 0
-        if not (q.is_cuda and q.dim() == 3 and q.dtype in (torch.float16, torch.bfloat16) and D == self.head_dim and n > 0 and B > 0 and
+        if (not all(isinstance(x, torch.Tensor) for x in (block_table, seq_lens, shared_lens)) or q.dim() != 3 or shared_lens.dim() != 1 or
+                (q.is_contiguous() and q.data_ptr() % 16 != 0)):     # (a part of a larger tensor, at an odd place)
+            return True
+        B, D, n = q.shape[0], q.shape[2], shared_lens.shape[0]
+        if not (q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and D == self.head_dim and n > 0 and B > 0 and
                 B % n == 0 and block_table.dim() == 2 and block_table.shape[0] == B and seq_lens.shape == (B,) and
                 0 < max_seq_len <= PAGE_TOKENS * block_table.shape[1] and q.shape[1] > 0 and q.shape[1] % self.num_kv_heads == 0 and
                 B // n <= 1024 and (out is None or (out.is_cuda and out.shape == q.shape and out.is_contiguous() and out.dtype in _DT))):

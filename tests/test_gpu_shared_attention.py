@@ -343,3 +343,7 @@ def test_as_a_user_calls_it(hkv, g, k, ctx, groups, both):
 
 def test_refusals_as_a_user_calls_it():
     test_refusals()
+
+
+def test_queries_anywhere_as_a_user_calls_it():
+    test_queries_anywhere()
