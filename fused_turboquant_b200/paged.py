@@ -243,8 +243,7 @@ class PagedKVPool:
         are on the device: about half of the most that they may be is taken for granted.  GQA groups above 8 always go
         there (the decode kernel for them is the fp32 one), and so do arguments that are to be refused.
         """
-        if (not all(isinstance(x, torch.Tensor) for x in (block_table, seq_lens, shared_lens)) or q.dim() != 3 or shared_lens.dim() != 1 or
-                (q.is_contiguous() and q.data_ptr() % 16 != 0)):     # (a part of a larger tensor, at an odd place)
+        if not all(isinstance(x, torch.Tensor) for x in (block_table, seq_lens, shared_lens)) or q.dim() != 3 or shared_lens.dim() != 1:
             return True
         B, D, n = q.shape[0], q.shape[2], shared_lens.shape[0]
         if not (q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and D == self.head_dim and n > 0 and B > 0 and
@@ -273,6 +272,8 @@ class PagedKVPool:
         """
         _require_cuda(q, "q")
         if not self._takes_shared_kernel(q, block_table, seq_lens, max_seq_len, shared_lens, out, workspace):
+            if q.is_contiguous() and q.data_ptr() % 16 != 0:        # (a part of a larger tensor, at an odd place)
+                q = q.clone()
             return self.decode_attention(q, block_table, seq_lens, max_seq_len, scale, layer, out, workspace)
         if _trace.ENABLED:
             with _trace.nvtx("ftq.decode"):
