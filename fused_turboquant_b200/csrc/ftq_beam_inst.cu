@@ -15,12 +15,15 @@ cudaError_t run_select(const SelectParams& p, cudaStream_t stream) {
     const int rounds = ((p.chunk * static_cast<int>(sizeof(T)) + 15) / 16 + 1 + kSelectThreads - 1) / kSelectThreads;
     const int rows_smem = 8 * select_pow2(std::max({kSelectRoom, p.keep * rounds, p.keep * 16 / static_cast<int>(sizeof(T))}));
     const int join_smem = 16 * std::max(kSelectRoom, select_join_size(p.K, p.chunks, p.keep, p.n));
-    cudaError_t e = allow_smem<beam_join_kernel<T>>(16 * kSelectJoin);
+    cudaError_t e = allow_smem<beam_join_kernel<T, 512>>(16 * kSelectJoin);
     if (e != cudaSuccess) return e;
     const int64_t ctas = static_cast<int64_t>(p.R) * p.K * p.chunks;
     e = launch_dependent(beam_rows_kernel<T>, dim3(static_cast<unsigned>(ctas)), kSelectThreads, rows_smem, stream, p);
     if (e != cudaSuccess) return e;
-    return launch_dependent(beam_join_kernel<T>, dim3(p.R), kSelectThreads, join_smem, stream, p);
+    // (8 requests of eight beams, 2300 tokens each: 20 us with 256 threads, 15 with 512; 64 requests of 576 42 and 44)
+    if (static_cast<int64_t>(p.K) * p.chunks * p.keep > kJoinFew)
+        return launch_dependent(beam_join_kernel<T, 512>, dim3(p.R), 512, join_smem, stream, p);
+    return launch_dependent(beam_join_kernel<T, 256>, dim3(p.R), 256, join_smem, stream, p);
 }
 static_assert(8 * select_pow2(kSelectMaxKeep * kSelectVectors) <= 48 * 1024, "shared memory of beam_rows_kernel");
 
@@ -30,7 +33,7 @@ static_assert(8 * select_pow2(kSelectMaxKeep * kSelectVectors) <= 48 * 1024, "sh
 // to be joined than they save).  In between, the number of parts that gives the shortest schedule: rounds of five CTAs an SM, of which
 // each costs its vectors and, for the threshold and the tokens that reach it, as much as 1024 more; and the request's CTA of
 // beam_join_kernel about one for each token that it gets.  (Eight beams of 131072 bf16 logits, in a graph: 2, 8, 16 and 64 requests 49,
-// 35, 29 and 42 us in parts that fill 12 CTAs an SM; 14, 20, 18 and 42 so.)
+// 35, 29 and 42 us in parts that fill 12 CTAs an SM; 12, 15, 18 and 42 now.)
 SelectPlan select_plan(int dtype, int requests, int beams, int vocab, int keep) {
     const int n = dtype == kF32 ? 4 : 8;
     const int64_t most = (kSelectVectors * kSelectThreads - 1) * n, least = std::min<int64_t>(kSelectThreads * n, vocab);

@@ -27,7 +27,9 @@
 
 namespace ftq {
 
-constexpr int kSelectThreads = 256, kSelectWarps = kSelectThreads / 32, kSelectMaxKeep = kBeamMax + kBeamMaxEnds;
+constexpr int kSelectThreads = 256, kSelectWarps = kSelectThreads / 32;     // of beam_rows_kernel
+constexpr int kJoinFew = 1024;          // tokens of a request that 256 threads of beam_join_kernel take as they come; more take 512
+constexpr int kSelectMaxKeep = kBeamMax + kBeamMaxEnds;
 constexpr int kSelectVectors = 32;      // vectors of a thread at most, so that those of `keep` threads can be sorted
 constexpr int kSelectBatch = 2;         // of which a thread loads so many at a time
 constexpr int kSelectRoom = 1024;       // tokens that are ranked by counting
@@ -57,10 +59,11 @@ __device__ __forceinline__ unsigned long long select_key(float x, uint32_t place
 
 // A key that at least `keep` of the CTA's threads' keys reach, 0 where fewer are above 0; by the whole CTA.  `s` has room for
 // kSelectTop keys of each warp and one more.
+template <int WARPS>
 __device__ __forceinline__ uint32_t select_threshold(uint32_t key, int keep, uint32_t* s) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // (two more of each warp than an even spread needs)
-    const int top = min(kSelectTop, (keep + kSelectWarps - 1) / kSelectWarps + 2), all = top * kSelectWarps;
+    const int top = min(kSelectTop, (keep + WARPS - 1) / WARPS + 2), all = top * WARPS;
     for (int i = 0; i < top; i++) {
         const uint32_t m = __reduce_max_sync(0xffffffffu, key);
         if (lane == 0) s[warp * top + i] = m;
@@ -72,10 +75,10 @@ __device__ __forceinline__ uint32_t select_threshold(uint32_t key, int keep, uin
         int rank = 0;
 #pragma unroll 8
         for (int i = 0; i < all; i++) rank += s[i] > mine || (s[i] == mine && i < static_cast<int>(threadIdx.x));
-        if (rank == keep - 1) s[kSelectTop * kSelectWarps] = mine;
+        if (rank == keep - 1) s[kSelectTop * WARPS] = mine;
     }
     __syncthreads();
-    return s[kSelectTop * kSelectWarps];
+    return s[kSelectTop * WARPS];
 }
 
 // Sorts n = 2^k keys in shared memory, the largest first; by the whole CTA.
@@ -249,7 +252,7 @@ __global__ void __launch_bounds__(kSelectThreads, 5) beam_rows_kernel(const Sele
         }
     }
     const uint32_t mine = tid < n_vec ? select_order(own.m) : 0;
-    const uint32_t least = select_threshold(mine, p.keep, s_top);
+    const uint32_t least = select_threshold<kSelectWarps>(mine, p.keep, s_top);
     if (tid == 0) {
         float mc = s_max[0];
         for (int w = 1; w < kSelectWarps; w++) mc = fmaxf(mc, s_max[w]);
@@ -347,12 +350,12 @@ __device__ __forceinline__ double select_value64(unsigned long long o) {
 }
 
 // A CTA has a request: its rows' sums, the ends' totals, and the order of the tokens that the rows kept.
-template <typename T>
-__global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectParams p) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) beam_join_kernel(const SelectParams p) {
     extern __shared__ __align__(16) unsigned long long s_keys[];
     // a beam's score (-inf: it has no continuation), its row's maximum, and the logarithm of the sum of exponentials less that
     __shared__ double s_score[kBeamMax], s_max[kBeamMax], s_log[kBeamMax];
-    __shared__ uint32_t s_top[kSelectTop * kSelectWarps + 1];
+    __shared__ uint32_t s_top[kSelectTop * THREADS / 32 + 1];
     __shared__ int s_end[kBeamMaxEnds], s_n;
     const int tid = threadIdx.x, r = blockIdx.x;
     after_previous_kernel();
@@ -361,14 +364,14 @@ __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectP
     if (tid < p.n_ends) s_end[tid] = p.ends[tid];
     const int per_row = p.chunks * p.keep, all = p.K * per_row;
     // (the thread's first tokens are on their way while the sums are made)
-    constexpr int FEW = 4;
+    constexpr int FEW = kJoinFew / THREADS;
     unsigned long long kept[FEW];
 #pragma unroll
     for (int j = 0; j < FEW; j++) {
-        const int i = tid + j * kSelectThreads;
+        const int i = tid + j * THREADS;
         kept[j] = i < all ? __ldcg(p.keys + static_cast<int64_t>(r) * all + i) : 0;     // (of a row that is not alive: anything)
     }
-    for (int b = tid / 32; b < p.K; b += kSelectWarps) {
+    for (int b = tid / 32; b < p.K; b += THREADS / 32) {
         const int64_t row = static_cast<int64_t>(r) * p.K + b;
         const float2* const at = p.sums + row * p.chunks;
         const float score = p.scores[row];
@@ -391,7 +394,7 @@ __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectP
     }
     auto total_of = [&](int b, float x) { return (x - s_max[b]) - s_log[b] + s_score[b]; };
     __syncthreads();
-    for (int e = tid; e < p.K * p.n_ends; e += kSelectThreads) {
+    for (int e = tid; e < p.K * p.n_ends; e += THREADS) {
         const int b = e / p.n_ends, id = s_end[e - b * p.n_ends];
         double total = -INFINITY;
         if (s_score[b] > -INFINITY && id >= 0 && id < p.V)
@@ -422,12 +425,12 @@ __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectP
         unsigned long long place[FEW], other;
 #pragma unroll
         for (int j = 0; j < FEW; j++) {
-            const int i = tid + j * kSelectThreads;
+            const int i = tid + j * THREADS;
             kept[j] = i < all ? total_key(i, kept[j], place[j]) : 0;
             most = max(most, static_cast<uint32_t>(kept[j] >> 32));
         }
-        for (int i = tid + FEW * kSelectThreads; i < all; i += kSelectThreads) most = max(most, static_cast<uint32_t>(token_of(i, other) >> 32));
-        const uint32_t least = select_threshold(most, p.n, s_top);
+        for (int i = tid + FEW * THREADS; i < all; i += THREADS) most = max(most, static_cast<uint32_t>(token_of(i, other) >> 32));
+        const uint32_t least = select_threshold<THREADS / 32>(most, p.n, s_top);
         auto push = [&](unsigned long long key, unsigned long long at) {
             if (key == 0 || static_cast<uint32_t>(key >> 32) < least) return;
             const int n = atomicAdd(&s_n, 1);
@@ -439,7 +442,7 @@ __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectP
         if (most >= least) {
 #pragma unroll
             for (int j = 0; j < FEW; j++) push(kept[j], place[j]);
-            for (int i = tid + FEW * kSelectThreads; i < all; i += kSelectThreads) {
+            for (int i = tid + FEW * THREADS; i < all; i += THREADS) {
                 const unsigned long long key = token_of(i, other);
                 push(key, other);
             }
@@ -449,7 +452,7 @@ __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectP
     if (s_n <= kSelectRoom) {
         const int n = s_n;
         const ulonglong2* const s = reinterpret_cast<const ulonglong2*>(s_keys);
-        for (int e = tid; e < n; e += kSelectThreads) {
+        for (int e = tid; e < n; e += THREADS) {
             const ulonglong2 mine = s[e];
             int rank = 0;
 #pragma unroll 4
@@ -459,19 +462,19 @@ __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectP
             }
             if (rank < p.n) store(rank, mine.x, mine.y);
         }
-        for (int e = n + tid; e < p.n; e += kSelectThreads) store(e, 0, 0);
+        for (int e = n + tid; e < p.n; e += THREADS) store(e, 0, 0);
         return;
     }
     // ---- too many of them: the n best so far and as many others as there is room for, until there are no others
     const int n = select_join_size(p.K, p.chunks, p.keep, p.n);
     unsigned long long* const s_place = s_keys + n;
     __syncthreads();
-    for (int e = tid; e < p.n; e += kSelectThreads) {
+    for (int e = tid; e < p.n; e += THREADS) {
         s_keys[e] = 0;
         s_place[e] = ~0ull;
     }
     for (int done = 0; done < all; done += n - p.n) {
-        for (int e = p.n + tid; e < n; e += kSelectThreads) {
+        for (int e = p.n + tid; e < n; e += THREADS) {
             unsigned long long place = ~0ull;
             const int i = done + e - p.n;
             s_keys[e] = i < all ? token_of(i, place) : 0;
@@ -480,7 +483,7 @@ __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectP
         for (int k = 2; k <= n; k <<= 1)
             for (int j = k >> 1; j > 0; j >>= 1) {
                 __syncthreads();
-                for (int i = tid; i < n / 2; i += kSelectThreads) {
+                for (int i = tid; i < n / 2; i += THREADS) {
                     const int a = 2 * i - (i & (j - 1)), b = a + j;
                     const unsigned long long x = s_keys[a], y = s_keys[b], px = s_place[a], py = s_place[b];
                     const bool less = x < y || (x == y && px > py);
@@ -492,7 +495,7 @@ __global__ void __launch_bounds__(kSelectThreads) beam_join_kernel(const SelectP
             }
         __syncthreads();
     }
-    for (int e = tid; e < p.n; e += kSelectThreads) store(e, s_keys[e], s_place[e]);
+    for (int e = tid; e < p.n; e += THREADS) store(e, s_keys[e], s_place[e]);
 }
 
 }  // namespace ftq
