@@ -38,7 +38,9 @@ def select(logits: torch.Tensor, scores: torch.Tensor, n_best: int, *, end_token
 
     logits: [R, K, V], fp32 / fp16 / bf16; scores: [R, K], the beams' log-probabilities so far, -inf for a beam that is not
     alive (of which at the first step of a request all but one are: they would all say the same).  Token v after beam b scores
-    ``scores[b] + log_softmax(logits[b])[v]``, compared in 64 bits; of equal ones the lowest beam's lowest token comes first.
+    ``scores[b] + log_softmax(logits[b])[v]``; of equal ones the lowest beam's lowest token comes first.  Totals are compared in 64
+    bits, but the sums of exponentials in them are fp32's: totals of different beams that lie within some 1e-7 may come in either
+    order, those of beams with the same logits and scores are equal.
     ``end_tokens`` [n] end an answer: they are not selected, and ``end_scores`` says what each beam would score with each of them.
     A beam whose logits hold a NaN or +inf, or nothing but -inf, has no continuation.
 

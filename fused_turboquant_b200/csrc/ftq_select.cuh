@@ -8,7 +8,8 @@
 // The logits are read once.  A CTA has a chunk of a row: every thread keeps the maximum and the sum of exponentials of its 16-byte
 // vectors.  Any `keep` of the threads' maxima bound the chunk's keep-th largest token from below (keep = n + the tokens that end
 // an answer), so the keep-th of the warps' few largest is a threshold: threads whose maximum reaches it are few, their vectors are
-// looked at again, and the few tokens that reach it are ranked by counting (threshold, push and rank below).  Where more tokens reach it than there is
+// looked at again, and the few tokens that reach it are ranked by counting (threshold, push and rank below).  Masked tokens (-inf) never do: a chunk
+// whose mask leaves fewer than `keep` threads a token has all of its others looked at.  Where more tokens reach it than there is
 // room for (equal logits, or large ones in a few threads' vectors only) sorts leave the exact order whatever the logits are: any of the `keep` largest tokens lies in
 // one of the `keep` threads, and there in one of the `keep` vectors, that are first by their largest token (of equal ones
 // the first), since otherwise as many threads or vectors would each hold a token that goes before it.
@@ -18,7 +19,8 @@
 // 64 requests of 8 beams, 131072 bf16 logits: 42 us, 36 of them the rows (134 MB: 20.5 us of HBM).  A logit takes 7 instructions (its
 // exponential one of 16 a cycle and SM: 15 us), threshold and ranks a quarter of all; issue is busy half of the time, and what
 // keeps the rest is loads and the few barriers of CTAs of 32768 tokens.  With three bitonic sorts a CTA 133 us; thresholds 54; the
-// chunk prefetched and the join's loads side by side 47; the next batch on its way, vectors looked at again one a thread 44.
+// chunk prefetched and the join's loads side by side 47; the next batch on its way, vectors looked at again one a thread 44.  With a
+// mask that leaves 50 tokens a row 39 us (120 with masked tokens as candidates, which went to the sorts).
 #pragma once
 
 #include <type_traits>
@@ -34,6 +36,7 @@ constexpr int kSelectVectors = 32;      // vectors of a thread at most, so that 
 constexpr int kSelectBatch = 2;         // of which a thread loads so many at a time
 constexpr int kSelectRoom = 1024;       // tokens that are ranked by counting
 constexpr int kSelectTop = 16;          // a warp's largest keys that a threshold is made of, at most
+constexpr uint32_t kSelectLeast = 0x00800000u;      // select_order of the least finite value: what is masked (-inf) is no candidate
 
 __host__ __device__ constexpr int select_pow2(int n) {
     int x = 1;
@@ -251,8 +254,8 @@ __global__ void __launch_bounds__(kSelectThreads, 5) beam_rows_kernel(const Sele
             s_sum[warp] = s;
         }
     }
-    const uint32_t mine = tid < n_vec ? select_order(own.m) : 0;
-    const uint32_t least = select_threshold<kSelectWarps>(mine, p.keep, s_top);
+    const uint32_t mine = own.m > -INFINITY ? select_order(own.m) : 0;
+    const uint32_t least = max(select_threshold<kSelectWarps>(mine, p.keep, s_top), kSelectLeast);
     if (tid == 0) {
         float mc = s_max[0];
         for (int w = 1; w < kSelectWarps; w++) mc = fmaxf(mc, s_max[w]);
@@ -261,7 +264,7 @@ __global__ void __launch_bounds__(kSelectThreads, 5) beam_rows_kernel(const Sele
         p.sums[blockIdx.x] = make_float2(mc, s);
     }
     // ---- the vectors of the threads whose maximum reaches it: their tokens that do
-    if (mine > 0 && mine >= least) s_first[atomicAdd(&s_n[0], 1)] = tid;
+    if (mine >= least) s_first[atomicAdd(&s_n[0], 1)] = tid;
     __syncthreads();
     const int rounds = (n_vec + kSelectThreads - 1) / kSelectThreads;
     for (int e = tid; e < s_n[0] * rounds; e += kSelectThreads) {
