@@ -12,7 +12,7 @@ namespace {
 template <typename T>
 cudaError_t run_select(const SelectParams& p, cudaStream_t stream) {
     // what the sorts need (the tokens that are ranked by counting are fewer)
-    const int rounds = ((p.chunk * static_cast<int>(sizeof(T)) + 15) / 16 + 1 + kSelectThreads - 1) / kSelectThreads;
+    const int rounds = ((p.chunk * static_cast<int>(sizeof(T)) + 15) / 16 + kSelectThreads - 1) / kSelectThreads;
     const int rows_smem = 8 * select_pow2(std::max({kSelectRoom, p.keep * rounds, p.keep * 16 / static_cast<int>(sizeof(T))}));
     const int join_smem = 16 * std::max(kSelectRoom, select_join_size(p.K, p.chunks, p.keep, p.n));
     cudaError_t e = allow_smem<beam_join_kernel<T, 512>>(16 * kSelectJoin);

@@ -14,13 +14,15 @@
 // one of the `keep` threads, and there in one of the `keep` vectors, that are first by their largest token (of equal ones
 // the first), since otherwise as many threads or vectors would each hold a token that goes before it.
 // beam_join_kernel adds up a request's rows and does the same with their tokens' totals, in 64 bits (totals of different beams
-// may lie closer than fp32 tells apart).
+// may lie closer than fp32 tells apart).  A chunk's sum is fp32's: the logarithm of a row's is good to some 1e-7, and beams whose totals
+// lie closer come in either order.  Those with the same logits and scores have the same totals.
 //
-// 64 requests of 8 beams, 131072 bf16 logits: 42 us, 36 of them the rows (134 MB: 20.5 us of HBM).  A logit takes 7 instructions (its
+// 64 requests of 8 beams, 131072 bf16 logits: 41 us, 35 of them the rows (134 MB: 20.5 us of HBM).  A logit takes 7 instructions (its
 // exponential one of 16 a cycle and SM: 15 us), threshold and ranks a quarter of all; issue is busy half of the time, and what
 // keeps the rest is loads and the few barriers of CTAs of 32768 tokens.  With three bitonic sorts a CTA 133 us; thresholds 54; the
-// chunk prefetched and the join's loads side by side 47; the next batch on its way, vectors looked at again one a thread 44.  With a
-// mask that leaves 50 tokens a row 39 us (120 with masked tokens as candidates, which went to the sorts).
+// chunk prefetched and the join's loads side by side 47; vectors looked at again one a thread 44; no batch of vectors on its way while the
+// one before is added up, which only took registers, 42 -> 41.  With a
+// mask that leaves 50 tokens a row 38 us (120 with masked tokens as candidates, which went to the sorts).
 #pragma once
 
 #include <type_traits>
@@ -121,16 +123,41 @@ struct SelectVec {
             }
         }
     }
-    // vector i of the row part [x, x + len), where vectors lie on 16-byte boundaries and the first one begins `head` tokens before
-    // x: what does not belong to it is -inf
+    // the N values that begin `head` values into two neighbouring vectors; HEAD: known to the compiler, or -1
+    template <int HEAD>
+    static __device__ __forceinline__ uint4 shifted(uint4 a, uint4 b, int head) {
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        const int bytes = (HEAD < 0 ? head : HEAD) * static_cast<int>(sizeof(T));
+        uint32_t t[6], u[5], out[4];
+#pragma unroll
+        for (int k = 0; k < 6; k++) t[k] = (bytes & 8) ? w[k + 2] : w[k];
+#pragma unroll
+        for (int k = 0; k < 5; k++) u[k] = (bytes & 4) ? t[k + 1] : t[k];
+#pragma unroll
+        for (int k = 0; k < 4; k++) out[k] = sizeof(T) == 4 ? u[k] : __funnelshift_r(u[k], u[k + 1], 8 * (bytes & 3));
+        return make_uint4(out[0], out[1], out[2], out[3]);
+    }
+    // whether the two are nothing but tokens of the row part [x, x + len), which begins `head` tokens behind a 16-byte boundary
+    static __device__ __forceinline__ bool inside(int head, int len, int i) { return i * N >= head && i * N - head + 2 * N <= len; }
+    // vector i of it, tokens i N .. i N + N - 1: what does not belong to it is -inf
     static __device__ __forceinline__ void load(const T* x, int head, int len, int i, float (&v)[N]) {
-        const int at = i * N - head;
-        if (at >= 0 && at + N <= len) {
-            unpack(*reinterpret_cast<const uint4*>(x + at), v);
+        const uint4* const from = reinterpret_cast<const uint4*>(x - head) + i;
+        if (head == 0 && i * N + N <= len) {
+            unpack(*from, v);
+        } else if (head > 0 && inside(head, len, i)) {
+            unpack(shifted<-1>(from[0], from[1], head), v);
         } else {
 #pragma unroll
-            for (int k = 0; k < N; k++) v[k] = at + k >= 0 && at + k < len ? to_float<T>(x[at + k]) : -INFINITY;
+            for (int k = 0; k < N; k++) v[k] = i * N + k < len ? to_float<T>(x[i * N + k]) : -INFINITY;
         }
+    }
+    // f(std::integral_constant<int, head>), 0 <= head < N
+    template <int HEAD = 0, typename F>
+    static __device__ __forceinline__ void with_head(int head, F&& f) {
+        if constexpr (HEAD + 1 < N) {
+            if (head != HEAD) return with_head<HEAD + 1>(head, f);
+        }
+        f(std::integral_constant<int, HEAD>{});
     }
     static __device__ __forceinline__ float largest(const float (&v)[N]) {
         float m = v[0];
@@ -185,6 +212,10 @@ struct SelectSum {
     }
 };
 
+// Which tokens a thread adds up, and in which order, is the same for all rows, wherever they begin in memory: beams that say the same
+// have the same sums.  A vector of a row that begins between 16-byte boundaries is made of two that lie on them, by shifts that
+// the compiler knows (64 requests of 8 beams, 131071 bf16 logits 49 us, 50257 fp32 ones 33, where vectors that lie on boundaries, so that
+// sums differed by row, took 45 and 32; shifts that it does not know 52 and 35, tokens loaded one by one, 32 apart, 56 and 33).
 template <typename T>
 __global__ void __launch_bounds__(kSelectThreads, 5) beam_rows_kernel(const SelectParams p) {
     using V = SelectVec<T>;
@@ -199,47 +230,42 @@ __global__ void __launch_bounds__(kSelectThreads, 5) beam_rows_kernel(const Sele
     if (!(p.scores[row] > -INFINITY)) return;     // (a beam that is not alive; beam_join_kernel asks the same)
     const int begin = chunk * p.chunk, len = min(p.chunk, p.V - begin);
     const T* const x = static_cast<const T*>(p.logits) + row * p.row_stride + begin;
-    const int head = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)), n_vec = (head + len + N - 1) / N;
+    const int head = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)), n_vec = (len + N - 1) / N;
     if (tid < 2) s_n[tid] = 0;
     constexpr float kLog2 = 1.4426950408889634f;
     SelectSum own;
     {
-        // vectors that are whole; at most one before them and one behind is not
-        const int lo = head > 0 ? 1 : 0, hi = (head + len) / N;
-        int i = tid;
-        if (i < lo) {
-            float v[1][N];
-            V::load(x, head, len, i, v[0]);
-            own.add(v);
-            i += kSelectThreads;
-        }
         const uint4* const from = reinterpret_cast<const uint4*>(x - head);
+        const int lo = head > 0 ? 1 : 0, hi = (head + len) / N, whole = len / N;     // vectors between boundaries; tokens' whole ones
         if (tid == 0 && hi > lo) prefetch_l2(from + lo, 16 * (hi - lo));
-        // (the next batch is on its way while this one is added up)
-        uint4 next[B];
-        auto fetch = [&]() {
+        V::with_head(head, [&](auto head_tag) {
+            constexpr int HEAD = decltype(head_tag)::value, S = HEAD > 0 ? 2 : 1;
+            int i = tid;
+            for (; i + (B - 1) * kSelectThreads < whole; i += B * kSelectThreads) {
+                uint4 u[B][S];
+                float v[B][N];
 #pragma unroll
-            for (int k = 0; k < B; k++) next[k] = from[i + k * kSelectThreads];
-        };
-        bool more = i + (B - 1) * kSelectThreads < hi;
-        if (more) fetch();
-        while (more) {
-            uint4 u[B];
+                for (int k = 0; k < B; k++) {
+                    const int j = i + k * kSelectThreads;
+                    if (HEAD > 0 && !V::inside(HEAD, len, j)) continue;
 #pragma unroll
-            for (int k = 0; k < B; k++) u[k] = next[k];
-            i += B * kSelectThreads;
-            more = i + (B - 1) * kSelectThreads < hi;
-            if (more) fetch();
-            float v[B][N];
+                    for (int c = 0; c < S; c++) u[k][c] = from[j + c];
+                }
 #pragma unroll
-            for (int k = 0; k < B; k++) V::unpack(u[k], v[k]);
-            own.add(v);
-        }
-        for (; i < n_vec; i += kSelectThreads) {
-            float v[1][N];
-            V::load(x, head, len, i, v[0]);
-            own.add(v);
-        }
+                for (int k = 0; k < B; k++) {
+                    const int j = i + k * kSelectThreads;
+                    if (HEAD == 0) V::unpack(u[k][0], v[k]);
+                    else if (V::inside(HEAD, len, j)) V::unpack(V::template shifted<HEAD>(u[k][0], u[k][S - 1], HEAD), v[k]);
+                    else V::load(x, HEAD, len, j, v[k]);
+                }
+                own.add(v);
+            }
+            for (; i < n_vec; i += kSelectThreads) {
+                float v[1][N];
+                V::load(x, HEAD, len, i, v[0]);
+                own.add(v);
+            }
+        });
     }
     // ---- the chunk's maximum and sum, in an order of their own
     {
@@ -274,8 +300,8 @@ __global__ void __launch_bounds__(kSelectThreads, 5) beam_rows_kernel(const Sele
         V::load(x, head, len, i, v);
 #pragma unroll
         for (int k = 0; k < N; k++) {
-            const int t = i * N - head + k;
-            if (select_order(v[k]) >= least && t >= 0 && t < len) {
+            const int t = i * N + k;
+            if (select_order(v[k]) >= least && t < len) {
                 const int at = atomicAdd(&s_n[1], 1);
                 if (at < kSelectRoom) s_keys[at] = select_key(v[k], begin + t);
             }
@@ -334,8 +360,8 @@ __global__ void __launch_bounds__(kSelectThreads, 5) beam_rows_kernel(const Sele
     for (int e = tid; e < n; e += kSelectThreads) {
         unsigned long long key = 0;
         if (e < vectors * N && s_first[e / N] < n_vec) {
-            const int t = s_first[e / N] * N - head + e % N;
-            if (t >= 0 && t < len) key = select_key(to_float<T>(x[t]), begin + t);
+            const int t = s_first[e / N] * N + e % N;
+            if (t < len) key = select_key(to_float<T>(x[t]), begin + t);
         }
         s_keys[e] = key;
     }

@@ -585,7 +585,9 @@ int ftq_logits_process(const void *logits, int dtype, int64_t row_stride, int n_
  * to beams - 1), tokens, all [n_requests, n_best]; and end_scores [n_requests, beams, n_ends], the
  * totals of the end tokens (-inf for one outside the vocabulary).  A total of -inf is none: where
  * fewer are left, -inf, -1, -1.  A beam whose logits are no distribution (a NaN, +inf, nothing but
- * -inf) has none.  Totals are compared in 64 bits and rounded once.
+ * -inf) has none.  Totals are compared in 64 bits and rounded once; the sums of exponentials in them
+ * are fp32's, in an order that goes by token: beams with the same logits and scores have equal
+ * totals, those of different beams that lie within some 1e-7 may come in either order.
  */
 size_t ftq_beam_workspace_bytes(int dtype, int n_requests, int beams, int vocab, int n_best, int n_ends);
 int ftq_beam_select(const void *logits, int dtype, int64_t row_stride, int n_requests, int beams,
