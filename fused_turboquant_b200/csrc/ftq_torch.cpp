@@ -46,7 +46,7 @@ struct Api {
 #undef X
 } api;
 PyObject* g_check = nullptr;        // _lib.check(rc, name): raises what the status stands for
-PyObject* g_get_workspace = nullptr;  // kernels.get_workspace(device, nbytes)
+PyObject* g_get_workspace = nullptr;  // kernels.get_workspace(device, nbytes, status)
 PyObject* g_workspaces = nullptr;     // kernels._workspaces
 PyObject* g_host_table = nullptr;     // kernels._host_table: fp32 copy of an array of any type and strides
 
@@ -218,16 +218,17 @@ struct Table {
     }
 };
 
-// Scratch of the current (device, stream), shared with the Python callers (kernels.get_workspace).
-at::Tensor workspace(PyObject* given, const at::Device& dev, void* stream, size_t need) {
+// Scratch of the current (device, stream), shared with the Python callers (kernels.get_workspace).  A pool's attention calls, whose
+// status word is read after other calls may have run, have theirs to themselves.
+at::Tensor workspace(PyObject* given, const at::Device& dev, void* stream, size_t need, bool status = false) {
     if (given != Py_None) {
         const at::Tensor& t = tensor(given, "workspace");
         if (t.device() != dev || !t.is_contiguous())
             raise(PyExc_ValueError, "workspace must be a contiguous tensor on the call's device");
         return t;
     }
-    PyObject* key = Py_BuildValue("(iK)", static_cast<int>(dev.index()),
-                                  static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(stream)));
+    PyObject* key = Py_BuildValue("(iKO)", static_cast<int>(dev.index()),
+                                  static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(stream)), status ? Py_True : Py_False);
     if (!key) throw PyError{};
     PyObject* hit = PyDict_GetItemWithError(g_workspaces, key);
     Py_DECREF(key);
@@ -236,7 +237,7 @@ at::Tensor workspace(PyObject* given, const at::Device& dev, void* stream, size_
         return THPVariable_Unpack(hit);
     if (PyErr_Occurred()) throw PyError{};
     PyObject* d = THPDevice_New(dev);
-    PyObject* r = PyObject_CallFunction(g_get_workspace, "OK", d, static_cast<unsigned long long>(need));
+    PyObject* r = PyObject_CallFunction(g_get_workspace, "OKO", d, static_cast<unsigned long long>(need), status ? Py_True : Py_False);
     Py_DECREF(d);
     if (!r) throw PyError{};
     at::Tensor t = THPVariable_Unpack(r);
@@ -343,7 +344,7 @@ PyObject* paged_decode(PyObject* const* a) {
     const int oc = out_dtype_code(out);
     void* st = stream_of(dev);
     const at::Tensor ws = workspace(a[8], dev, st,
-                                    api.ftq_decode_workspace_bytes(B, Hq, p.hkv, p.d, max_seq, L));
+                                    api.ftq_decode_workspace_bytes(B, Hq, p.hkv, p.d, max_seq, L), true);
     uint8_t* base = p.base(a[6]);
     Ref so(PyObject_GetAttr(self, names.signs)), ko(PyObject_GetAttr(self, names.levels_k)),
         vo(PyObject_GetAttr(self, names.levels_v));
@@ -381,7 +382,7 @@ PyObject* paged_chunk(PyObject* const* a) {
     const at::Tensor out = empty(q.sizes(), q.scalar_type(), dev);
     void* st = stream_of(dev);
     const at::Tensor ws = workspace(Py_None, dev, st, api.ftq_paged_chunk_workspace_bytes(
-                                                          B, q_len, Hq, p.hkv, p.d, max_seq));
+                                                          B, q_len, Hq, p.hkv, p.d, max_seq), true);
     uint8_t* base = p.base(a[6]);
     Ref so(PyObject_GetAttr(self, names.signs)), ko(PyObject_GetAttr(self, names.levels_k)),
         vo(PyObject_GetAttr(self, names.levels_v));
@@ -835,7 +836,7 @@ PyObject* paged_tree(PyObject* const* a) {
     const int oc = out_dtype_code(out);
     void* st = stream_of(dev);
     const int nodes = T > INT32_MAX ? INT32_MAX : static_cast<int>(T);
-    const at::Tensor ws = workspace(a[10], dev, st, api.ftq_tree_workspace_bytes(B, nodes, Hq, p.hkv, p.d, max_seq));
+    const at::Tensor ws = workspace(a[10], dev, st, api.ftq_tree_workspace_bytes(B, nodes, Hq, p.hkv, p.d, max_seq), true);
     uint8_t* base = p.base(a[8]);
     Ref so(PyObject_GetAttr(self, names.signs)), ko(PyObject_GetAttr(self, names.levels_k)),
         vo(PyObject_GetAttr(self, names.levels_v));
@@ -956,8 +957,8 @@ PyObject* logits_process(PyObject* const* a) {
 
 // ------------------------------------------------------------------ beam search and parallel sampling
 // Scratch that a call without any is not asked for.
-at::Tensor maybe_workspace(PyObject* given, const at::Device& dev, void* stream, size_t need) {
-    return need || given != Py_None ? workspace(given, dev, stream, need) : at::Tensor();
+at::Tensor maybe_workspace(PyObject* given, const at::Device& dev, void* stream, size_t need, bool status = false) {
+    return need || given != Py_None ? workspace(given, dev, stream, need, status) : at::Tensor();
 }
 void* ws_ptr(const at::Tensor& ws) { return ws.defined() ? mptr<void>(ws) : nullptr; }
 size_t ws_bytes(const at::Tensor& ws) { return ws.defined() ? ws.nbytes() : 0; }
@@ -1133,7 +1134,7 @@ PyObject* paged_shared(PyObject* const* a) {
     }
     const int oc = out_dtype_code(out);
     void* st = stream_of(dev);
-    const at::Tensor ws = maybe_workspace(a[9], dev, st, api.ftq_shared_workspace_bytes(R, K, Hq, p.hkv, p.d, max_seq));
+    const at::Tensor ws = maybe_workspace(a[9], dev, st, api.ftq_shared_workspace_bytes(R, K, Hq, p.hkv, p.d, max_seq), true);
     uint8_t* base = p.base(a[7]);
     Ref so(PyObject_GetAttr(self, names.signs)), ko(PyObject_GetAttr(self, names.levels_k)),
         vo(PyObject_GetAttr(self, names.levels_v));

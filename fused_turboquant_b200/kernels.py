@@ -31,7 +31,7 @@ _DT = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF
 # id(tensor) -> (weak reference, tensor version, host copy).  Keyed by identity: tensors compare
 # element-wise, which rules them out as dictionary keys.
 _table_cache: dict[int, tuple[weakref.ref, int, np.ndarray]] = {}
-_workspaces: dict[tuple[int, int], torch.Tensor] = {}
+_workspaces: dict[tuple[int, int, bool], torch.Tensor] = {}
 
 
 def is_available() -> bool:
@@ -84,10 +84,14 @@ def sm_count(device: torch.device) -> int:
     return torch.cuda.get_device_properties(device).multi_processor_count
 
 
-def get_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    """Per (device, stream) scratch buffer, grown on demand and reused across calls."""
+def get_workspace(device: torch.device, nbytes: int, status: bool = False) -> torch.Tensor:
+    """Per (device, stream) scratch buffer, grown on demand and reused across calls.
+
+    ``status``: that of a pool's attention calls, which leave a status word in it that the host may ask for after
+    other calls (``PagedKVPool.decode_status``).
+    """
     key = (device.index if device.index is not None else torch.cuda.current_device(),
-           _stream(device))
+           _stream(device), status)
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)

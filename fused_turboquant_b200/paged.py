@@ -106,7 +106,8 @@ class PagedKVPool:
         """Status bits of this pool's last ``decode_attention`` call (0: nothing to report;
         1: a block id outside the pool was met, 2: a bounded wait inside a kernel ran out -- the
         rows concerned are NaN either way).  Copies one word back and synchronises the current
-        stream; the kernels themselves never trap on such input."""
+        stream; the kernels themselves never trap on such input.  The word lies in the call's workspace: ask before that
+        is used again, by this or another pool's attention on the same stream, or, where it was passed in, by any call."""
         last = getattr(self, "_last_decode", None)
         if last is None:
             return 0
