@@ -500,15 +500,26 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
             vn.x *= st.vscale;
             vn.y *= st.vscale;
             uint32_t pb[TILES][2];
+            auto weights = [&](auto masked) {
 #pragma unroll
-            for (int nt = 0; nt < TILES; nt++) {
+                for (int nt = 0; nt < TILES; nt++) {
+                    float w[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[nt][i] = fast_exp2(x[nt][i]);
-                st.l[nt][0] += x[nt][0] + x[nt][2];
-                st.l[nt][1] += x[nt][1] + x[nt][3];
-                pb[nt][0] = movmatrix_trans(pack_weights(x[nt][0] * vn.x, x[nt][1] * vn.x));
-                pb[nt][1] = movmatrix_trans(pack_weights(x[nt][2] * vn.y, x[nt][3] * vn.y));
-            }
+                    for (int i = 0; i < 4; i++) {
+                        const float s = x[nt][i];
+                        x[nt][i] = fast_exp2(s);
+                        w[i] = x[nt][i] * (i < 2 ? vn.x : vn.y);
+                        if constexpr (decltype(masked)::value) w[i] = s == -INFINITY ? 0.f : w[i];
+                    }
+                    st.l[nt][0] += x[nt][0] + x[nt][2];
+                    st.l[nt][1] += x[nt][1] + x[nt][3];
+                    pb[nt][0] = movmatrix_trans(pack_weights(w[0], w[1]));
+                    pb[nt][1] = movmatrix_trans(pack_weights(w[2], w[3]));
+                }
+            };
+            // (a token behind a column's end takes no part, whatever its norm is: an infinite one of a longer row's too)
+            if (whole) weights(std::false_type{});
+            else weights(std::true_type{});
             // ---- O^T += V^T P^T
             {
                 typename WV::template Run<C::VW> run[4];

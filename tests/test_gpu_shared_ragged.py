@@ -1,0 +1,34 @@
+"""Shared attention of rows of different length: what lies behind a row's end is nothing to it."""
+import numpy as np
+import pytest
+
+from helpers import PAGE, page_offsets
+from test_gpu_shared_attention import Case, check32
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def kernels_that_read_common_blocks_once(monkeypatch):
+    from fused_turboquant_b200 import PagedKVPool
+    monkeypatch.setattr(PagedKVPool, "_takes_shared_kernel", lambda *a: True)
+
+
+def set_norm(case, which, row, token, value):
+    """The norm of a row's token, of all KV heads, keys' or values'."""
+    import torch
+    kn, vc, vn, end = page_offsets(case.d, case.bk, case.bv)
+    at = (kn if which == "k" else vn) + 2 * (token % PAGE)
+    page = case.pool.pool[0, int(case.table[row, token // PAGE])]
+    page[:, at:at + 2] = torch.tensor([value], dtype=torch.float16, device="cuda").view(torch.uint8)
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("d,g", [(64, 1), (64, 6), (128, 2), (128, 6), (256, 1), (256, 4)])        # (one tile of columns and more)
+def test_norms_that_are_no_numbers_behind_a_rows_end(d, g, which, value):
+    """In the page in which a row ends, of tokens that are common to longer rows, and in those behind it."""
+    case = Case(d + g, d, 4, 4, 2, g, [320], [[100, 321, 251, 0, 16, 1]])
+    for token, fine in ((300, [0, 2, 4, 5]), (255, [0, 2, 4, 5]), (101, [0, 4, 5]), (16, [4, 5]), (1, [5])):
+        set_norm(case, which, 1, token, value)
+        check32(case, rows=fine)
