@@ -464,15 +464,15 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
 #pragma unroll
                 for (int i = 0; i < 4; i++) most = fmaxf(most, x[nt][i]);
             if (__any_sync(0xffffffffu, k == 0 || most > kSharedSlack || fmaxf(vn.x, vn.y) > st.vlimit)) {
-                float v = fmaxf(vn.x, vn.y), change = 1.f;
+                float v = fmaxf(vn.x < INFINITY ? vn.x : 0.f, vn.y < INFINITY ? vn.y : 0.f), change = 1.f;
 #pragma unroll
                 for (int d = 4; d <= 16; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-                if (v > st.vlimit) {        // (norms are not negative; infinite ones stay what they are)
+                if (v > st.vlimit) {        // (norms are not negative; infinite ones stay that at any scale, and are none of all rows')
                     // 2^-e with the norm in [2^e, 2^(e + 1))
-                    const float top = fminf(v, 65504.f), now = __uint_as_float((254u << 23) - (__float_as_uint(top) & 0x7f800000u));
+                    const float now = __uint_as_float((254u << 23) - (__float_as_uint(v) & 0x7f800000u));
                     change = now / st.vscale;
                     st.vscale = now;
-                    st.vlimit = top * kSharedNorms;
+                    st.vlimit = v * kSharedNorms;
                 }
 #pragma unroll
                 for (int nt = 0; nt < TILES; nt++) {

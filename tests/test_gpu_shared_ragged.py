@@ -32,3 +32,11 @@ def test_norms_that_are_no_numbers_behind_a_rows_end(d, g, which, value):
     for token, fine in ((300, [0, 2, 4, 5]), (255, [0, 2, 4, 5]), (101, [0, 4, 5]), (16, [4, 5]), (1, [5])):
         set_norm(case, which, 1, token, value)
         check32(case, rows=fine)
+
+
+@pytest.mark.parametrize("d,g", [(64, 6), (128, 2)])
+def test_infinite_norms_take_nothing_from_small_values(d, g):
+    """Values of 2^-12 keep their bits where a longer row has an infinite one in the same page."""
+    case = Case(5 + d, d, 4, 4, 2, g, [320], [[100, 321, 251]], norm=(0.4, 2.0 ** -12))
+    set_norm(case, "v", 1, 101, float("inf"))
+    check32(case, rows=[0])
