@@ -179,7 +179,7 @@ struct SharedPiece {
     int qh;              // group x Hkv + KV head
     int hkv;
     int limit0;          // tokens before page0
-    bool ragged;         // columns of a group with fewer tokens
+    bool group, ragged;  // common tokens; columns of a group with fewer of them
     int64_t out;         // rows in the workspace
 };
 
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
             const int mid = (lo + hi) >> 1;
             if (s_plan[mid] <= pos) lo = mid; else hi = mid;
         }
-        const bool group = lo < p.R;
+        const bool group = it.group = lo < p.R;
         const int units = group ? p.units_group : p.units_row, unit_places = p.plan_unit[lo];
         const FastDiv cost = group ? p.by_cost_group : p.by_cost_row;
         const int pages = fast_div(unit_places - kSharedPiece, cost);
@@ -321,8 +321,8 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
     auto walk = [&](auto tiles_tag, const SharedPiece& it) {
         constexpr int TILES = decltype(tiles_tag)::value;
         const uint8_t* const base = p.pool + static_cast<int64_t>(it.hkv) * C::PAGE_BYTES;
-        bool bad = false;
-        // block ids of pages k0 .. k0 + 31 of the piece; an id outside the pool is replaced by 0 and remembered
+        int bad = INT32_MAX;
+        // block ids of pages k0 .. k0 + 31 of the piece; an id outside the pool is replaced by 0, and the first such page remembered
         auto load_ids = [&](int k0) {
             const int k = k0 + lane;
             int id = 0;
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
                 id = p.block_table[static_cast<int64_t>(it.row) * p.max_blocks + it.page0 + k];
                 if (static_cast<uint32_t>(id) >= static_cast<uint64_t>(p.num_blocks)) {
                     id = 0;
-                    bad = true;
+                    bad = min(bad, k);
                 }
             }
             return id;
@@ -544,9 +544,12 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
         if (lost && requested)
             for (const int last = min(k + C::RING, it.n_pages); k < last; k++, taken++) mbar_wait(my_bars + 8 * (taken % C::RING), taken / C::RING & 1);
         // ---- the piece's rows: O in coordinates (D/8) g .. + D/8 of columns 2 tg, 2 tg + 1, (m, l) behind them
-        bad = __any_sync(0xffffffffu, bad);
-        bad_any |= bad;
-        const float scale = lost || bad ? __int_as_float(0x7fc00000) : p.inv_v_scale / st.vscale;
+        bad = __reduce_min_sync(0xffffffffu, bad);
+        bad_any |= bad != INT32_MAX;
+        // (rows that end before the piece, or the first bad page of it, have lost nothing)
+        const bool spoilt = lost || bad != INT32_MAX;
+        const int sound = it.limit0 + (lost || !spoilt ? 0 : bad * kPageTokens);
+        auto row_len = [&](int col) { return shared_len(p, it.group ? it.qh / p.Hkv * p.K + (it.col0 + col) / G : it.row); };
 #pragma unroll
         for (int nt = 0; nt < TILES; nt++) {
 #pragma unroll
@@ -556,6 +559,8 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
 #pragma unroll
                 for (int d = 4; d <= 16; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
                 if (col >= it.cols) continue;
+                const bool none = spoilt && row_len(col) > sound;
+                const float scale = none ? __int_as_float(0x7fc00000) : p.inv_v_scale / st.vscale;
                 float* const to = p.rows + (it.out + col) * ROW;
 #pragma unroll
                 for (int f = 0; f < NMT; f++)
@@ -563,7 +568,7 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
                         make_float4(st.o[nt][2 * f][h] * scale, st.o[nt][2 * f][2 + h] * scale, st.o[nt][2 * f + 1][h] * scale, st.o[nt][2 * f + 1][2 + h] * scale);
                 if (g == 0)
                     *reinterpret_cast<float2*>(to + D) =
-                        make_float2(lost || bad ? __int_as_float(0x7fc00000) : l == 0.f ? -INFINITY : st.m[nt][h], l);
+                        make_float2(none ? __int_as_float(0x7fc00000) : l == 0.f ? -INFINITY : st.m[nt][h], l);
             }
         }
         __syncwarp();       // (the next piece's queries come to where these were read)

@@ -40,3 +40,19 @@ def test_infinite_norms_take_nothing_from_small_values(d, g):
     case = Case(5 + d, d, 4, 4, 2, g, [320], [[100, 321, 251]], norm=(0.4, 2.0 ** -12))
     set_norm(case, "v", 1, 101, float("inf"))
     check32(case, rows=[0])
+
+
+def test_block_ids_outside_the_pool_behind_a_rows_end():
+    """A bad block makes no number of the rows that have tokens in it; the others' bits stay what they were."""
+    import torch
+    lens = [320, 16, 17, 100, 112, 113, 250, 304]
+    case = Case(31, 128, 4, 4, 2, 2, [320], [lens])
+    good, table = case.run(), case.table.copy()
+    assert good.isfinite().all()
+    for page in range(20):
+        case.table = table.copy()
+        case.table[:, page] = 10 ** 6
+        out = case.run()
+        hit = torch.tensor([n > PAGE * page for n in lens], device="cuda")
+        assert out[hit].isnan().all() and torch.equal(out[~hit], good[~hit]), page
+        assert case.pool.decode_status() == 1
