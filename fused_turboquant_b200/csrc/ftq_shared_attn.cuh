@@ -315,7 +315,8 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
     bool lost = false;        // a wait ran out: nothing is requested any more, and the warp's pieces are NaN
     bool bad_any = false;
 #ifdef FTQ_TEST_WAIT_EXPIRY
-    bool test_drop = blockIdx.x == 0 && warp == 5;
+    // a page, or where a group has five rows the queries
+    bool test_drop = blockIdx.x == 0 && warp == 5 && p.K != 5, test_drop_q = blockIdx.x == 0 && warp == 5 && p.K == 5;
 #endif
 
     auto walk = [&](auto tiles_tag, const SharedPiece& it) {
@@ -355,6 +356,11 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
         if (requested) {
             if (lane == 0) {
                 mbar_expect_tx(q_bar, it.cols * D * 2);
+#ifdef FTQ_TEST_WAIT_EXPIRY
+                const bool drop = test_drop_q;
+                test_drop_q = false;
+                if (!drop)
+#endif
                 bulk_g2s_hint(my_q, p.q_rows + (static_cast<int64_t>(it.qh) * p.K * G + it.col0) * (D * 2), it.cols * D * 2, q_bar, policy);
             }
             __syncwarp();
@@ -376,6 +382,7 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
         st.vscale = 1.f;
         const uint32_t q_lane = my_q + g * (D * 2), q_odd = (((it.col0 + g) & 1) * 64) ^ (tg * 16);
         if (!lost) lost = !__all_sync(0xffffffffu, mbar_wait(q_bar, q_parity));
+        const bool no_queries = lost;
         q_parity ^= 1;
 
         int k = 0;
@@ -540,9 +547,12 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
                 }
             }
         }
-        // (no copy of this warp's is on its way when it gives up)
-        if (lost && requested)
+        // (a warp that gives up waits once more for each copy that is on its way, so that none comes after the CTA has left; as long as
+        // a wait may take)
+        if (lost && requested) {
+            if (no_queries) mbar_wait(q_bar, q_parity ^ 1);
             for (const int last = min(k + C::RING, it.n_pages); k < last; k++, taken++) mbar_wait(my_bars + 8 * (taken % C::RING), taken / C::RING & 1);
+        }
         // ---- the piece's rows: O in coordinates (D/8) g .. + D/8 of columns 2 tg, 2 tg + 1, (m, l) behind them
         bad = __reduce_min_sync(0xffffffffu, bad);
         bad_any |= bad != INT32_MAX;
