@@ -22,9 +22,9 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 OBJ_DIR = os.path.join(PKG_DIR, "build")
 LIB_PATH = os.path.join(PKG_DIR, "libftq_b200.so")
 # A second library for ONE test (tests/test_gpu_wait_expiry.py): the same objects, except that the
-# head_dim-128 decode, chunk attention, tree and shared attention (4-bit) and slot-format decode units are compiled with FTQ_TEST_WAIT_EXPIRY (one page copy, or copy of queries, of
-# one warp is never issued, one tile of one warp never reported, and the poll limits are small), so that
-# a bounded wait runs out and the give-up path (NaN rows, status word, the context stays usable)
+# head_dim-128 decode, chunk attention, tree and shared attention (4-bit) and slot-format decode units are compiled with
+# FTQ_TEST_WAIT_EXPIRY (one page copy, or copy of queries, of one warp is never issued, one tile of one warp never reported, and the
+# poll limits are small), so that a bounded wait runs out and the give-up path (NaN rows, status word, the context stays usable)
 # executes.  Never loaded by the package.
 TEST_LIB_PATH = os.path.join(PKG_DIR, "libftq_b200_waittest.so")
 # The tensor-level host path (csrc/ftq_torch.cpp): a CPython module compiled with the host compiler

@@ -2083,12 +2083,16 @@ extern "C" int ftq_shared_attn(const void* q, int q_dtype, void* out, int out_dt
     // what a page costs: its look-ups and byte work, and a share of that for each tile of columns (see ftq_shared_attn.cuh)
     p.cost_group = 9 + 2 * ((l.rows_group + 7) / 8);
     p.cost_row = 9 + 2 * ((l.rows_row + 7) / 8);
+    // 2^30 places are a launch's most.  A group that could have more (1024 rows of 150 000 tokens, 8 KV heads) has a page cost one place
+    const int64_t pages = (static_cast<int64_t>(max_seq_len) + FTQ_PAGE_TOKENS - 1) / FTQ_PAGE_TOKENS;
+    auto places = [&] {
+        return (ftq::kSharedPiece + pages * p.cost_group) * l.units_group + group * (ftq::kSharedPiece + pages * p.cost_row) * l.units_row;
+    };
+    if (places() > INT32_MAX / 2) p.cost_group = p.cost_row = 1;
+    const int requests = static_cast<int>(std::min<int64_t>(l.requests, (INT32_MAX / 2) / places()));
+    if (requests < 1) return fail(FTQ_ERR_UNSUPPORTED, "too many tokens, heads and rows for one call");
     p.by_hq = ftq::make_fastdiv(Hq); p.by_group = ftq::make_fastdiv(Hq / Hkv); p.by_rows = ftq::make_fastdiv(group);
     p.by_cols = ftq::make_fastdiv(p.cols); p.by_cost_group = ftq::make_fastdiv(p.cost_group); p.by_cost_row = ftq::make_fastdiv(p.cost_row);
-    const int64_t pages = (static_cast<int64_t>(max_seq_len) + FTQ_PAGE_TOKENS - 1) / FTQ_PAGE_TOKENS,
-                  places = (ftq::kSharedPiece + pages * p.cost_group) * l.units_group + group * (ftq::kSharedPiece + pages * p.cost_row) * l.units_row;
-    const int requests = static_cast<int>(std::min<int64_t>(l.requests, (INT32_MAX / 2) / places));
-    if (requests < 1) return fail(FTQ_ERR_UNSUPPORTED, "too many tokens, heads and rows for one call");
     const int grid = ftq::sm_count();
     p.warps = grid * ftq::shared_shape(head_dim, static_cast<int>(ftq_page_bytes(head_dim, bits_k, bits_v)), l.tiles).warps;
     uint8_t* const ws = static_cast<uint8_t*>(workspace);

@@ -268,8 +268,8 @@ class PagedKVPool:
         successive rows are a group, and the first ``shared_lens[g]`` tokens of its rows, rounded down to whole blocks, lie in the
         same blocks (``PageTable.shared_lens`` says how many do).  They are read once for the group, through its longest
         row, where that pays (see _takes_shared_kernel).  The result is that of ``decode_attention`` on the rows; rows without tokens are
-        zero.  Up to 1024 rows a group.  No host synchronisation; graph-capturable when out / workspace are passed in.
-        ``decode_status`` covers this call too.
+        zero.  Up to 1024 rows a group, with rows x KV heads x max_seq_len up to some 10^10.  No host synchronisation;
+        graph-capturable when out / workspace are passed in.  ``decode_status`` covers this call too.
         """
         _require_cuda(q, "q")
         if not self._takes_shared_kernel(q, block_table, seq_lens, max_seq_len, shared_lens, out, workspace):

@@ -56,3 +56,19 @@ def test_block_ids_outside_the_pool_behind_a_rows_end():
         hit = torch.tensor([n > PAGE * page for n in lens], device="cuda")
         assert out[hit].isnan().all() and torch.equal(out[~hit], good[~hit]), page
         assert case.pool.decode_status() == 1
+
+
+def test_a_group_of_many_rows_over_a_long_table():
+    """The most that a group may have, under a bound of lengths far beyond what there is."""
+    import torch
+    case = Case(41, 128, 4, 4, 8, 1, [40], [[41 + i % 5 for i in range(1024)]])
+    q, table, lens, top, shared = case.args()
+    want = case.pool.shared_attention(q, table, lens, top, shared)
+    wide = torch.full((1024, 1 << 14), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    for bound in (16 << 13, 16 << 14):
+        got = case.pool.shared_attention(q, wide, lens, bound, shared)
+        full, far = case.expect(rows=range(0, 1024, 100))
+        keep = list(range(0, 1024, 100))
+        assert ((got.double() - full).norm(dim=-1) <= far + 2.0 ** -8 * full.norm(dim=-1))[keep].all()
+        assert (got.float() - want.float()).abs().max() <= 2.0 ** -6 * want.float().abs().max()
