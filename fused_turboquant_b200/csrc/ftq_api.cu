@@ -2055,6 +2055,8 @@ extern "C" int ftq_shared_attn(const void* q, int q_dtype, void* out, int out_dt
         return fail(FTQ_ERR_INVALID, "bad shape groups=%d of %d max_blocks=%d max_seq_len=%d", n_requests, group, max_blocks, max_seq_len);
     if (n_requests == 0) return FTQ_OK;
     if (!q || !out || !pool || !block_table || !seq_lens || !shared_lens) return fail(FTQ_ERR_INVALID, "NULL tensor pointer");
+    // (block 0 stands in for an id outside the pool)
+    if (num_blocks == 0) return fail(FTQ_ERR_INVALID, "the pool has no blocks");
     if (static_cast<int64_t>(max_blocks) * FTQ_PAGE_TOKENS < max_seq_len)
         return fail(FTQ_ERR_INVALID, "block_table too narrow: %d blocks < max_seq_len %d", max_blocks, max_seq_len);
     if (!aligned(q, 16) || !aligned(out, 4) || !aligned(pool, 16))

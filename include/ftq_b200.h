@@ -645,7 +645,8 @@ int ftq_copy_pages(uint8_t *pool, int64_t num_blocks, int64_t pool_layer_stride,
  * most tokens (of equal ones the first), and a row with fewer tokens attends those it has.  The
  * result is that of ftq_paged_decode_attn on the rows.  Rows without tokens are zero.  A group that
  * could have 2^30 pages (its blocks of up to 32 rows x heads, and its rows' KV heads, each by the
- * pages of max_seq_len tokens) is refused (FTQ_ERR_UNSUPPORTED).  The workspace
+ * pages of max_seq_len tokens) is refused (FTQ_ERR_UNSUPPORTED), and so is a pool without blocks
+ * (FTQ_ERR_INVALID).  The workspace
  * holds at least ftq_shared_workspace_bytes(...) bytes, 16-byte aligned; the call's status is read with
  * ftq_paged_decode_status(workspace, 1, Hq, Hkv, head_dim, max_seq_len, 1, ...).
  */

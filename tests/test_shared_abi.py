@@ -6,6 +6,7 @@ A = 0x10000        # an address that nothing follows
 
 
 @pytest.mark.parametrize("change,rc,text", [
+    (dict(num_blocks=0), -1, "no blocks"),
     (dict(max_seq_len=1 << 30, max_blocks=1 << 26, n_requests=1, group=1024), -2, "too many tokens"),
 ])
 def test_refusals(change, rc, text):
