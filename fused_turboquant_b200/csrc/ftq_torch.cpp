@@ -1044,7 +1044,7 @@ PyObject* pages_shared_lens(PyObject* const* a) {
 PyObject* copy_pages(PyObject* const* a) {
     const Pool p(a[0]);
     const at::Device dev = p.pool.device();
-    const at::Tensor c = as_i32(a[1], "copies", dev);
+    const at::Tensor c = counts_i32(a[1], "copies", dev);     // (an id that 32 bits do not hold is outside the pool)
     if (c.dim() != 2 || c.size(1) != 2) raise(PyExc_ValueError, "copies must be [n, 2]");
     if (c.size(0) > INT32_MAX) raise(PyExc_ValueError, "too many copies");
     const c10::cuda::CUDAGuard guard(dev);
