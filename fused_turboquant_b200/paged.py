@@ -250,7 +250,7 @@ class PagedKVPool:
         if not (q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and D == self.head_dim and n > 0 and B > 0 and
                 B % n == 0 and block_table.dim() == 2 and block_table.shape[0] == B and seq_lens.shape == (B,) and
                 0 < max_seq_len <= PAGE_TOKENS * block_table.shape[1] and q.shape[1] > 0 and q.shape[1] % self.num_kv_heads == 0 and
-                B // n <= 1024 and (out is None or (out.is_cuda and out.shape == q.shape and out.is_contiguous() and out.dtype in _DT))):
+                B // n <= 1024 and (out is None or (out.device == q.device and out.shape == q.shape and out.is_contiguous() and out.dtype in _DT))):
             return True
         group, heads = B // n, q.shape[1] // self.num_kv_heads
         if heads > 8 or (workspace is not None and
