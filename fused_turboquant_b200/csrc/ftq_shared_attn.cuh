@@ -163,7 +163,6 @@ __global__ void __launch_bounds__(256) shared_prepare_kernel(const __grid_consta
 // 2^-14 of a column's largest still has all its bits.  (One for all columns of a warp: with the decode kernel's slack of 3
 // every third page of the serving batch below did it, 512 scores of which one in fifty has three times the others' size.)
 constexpr float kSharedSlack = 10.f, kSharedNorms = 16.f;
-// (those of infinite norms are infinite)
 __device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -385,6 +384,12 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
         const bool no_queries = lost;
         q_parity ^= 1;
 
+        auto row_len = [&](int col) { return shared_len(p, it.group ? it.qh / p.Hkv * p.K + (it.col0 + col) / G : it.row); };
+        // tokens of a column from page k on
+        auto tokens_of = [&](int col, int k) {
+            const int left = it.tokens - k * kPageTokens;
+            return it.ragged && col < it.cols ? min(left, row_len(col) - it.limit0 - k * kPageTokens) : left;
+        };
         int k = 0;
         for (; k < it.n_pages; k++) {
             const uint32_t rb = taken % C::RING;
@@ -442,8 +447,12 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
 
             // ---- softmax (base 2), per column; lanes of a column: the eight that differ in g
             const uint32_t knab = __byte_perm(kn2.x, kn2.y, sel_norms), vnab = __byte_perm(vn2.x, vn2.y, sel_norms);
-            const float2 kn = __half22float2(*reinterpret_cast<const __half2*>(&knab));
-            float2 vn = __half22float2(*reinterpret_cast<const __half2*>(&vnab));
+            // A value whose norm is infinite, or none, makes no number of the columns that attend it: by its score, so that it is nothing
+            // to those that it is masked for (0 times it would be no number either), nor to the scale of the others
+            const __half2 vn_half = *reinterpret_cast<const __half2*>(&vnab), none = __hsub2(vn_half, vn_half);
+            const uint32_t vn_fine = vnab & __hlt2_mask(vn_half, __half2half2(__ushort_as_half(0x7c00)));
+            const float2 kn = __half22float2(__hadd2(*reinterpret_cast<const __half2*>(&knab), none));
+            float2 vn = __half22float2(*reinterpret_cast<const __half2*>(&vn_fine));
             const int left = it.tokens - k * kPageTokens;
             const bool whole = left >= kPageTokens && !it.ragged;
             float most = -INFINITY;
@@ -458,10 +467,7 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
                 for (int nt = 0; nt < TILES; nt++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        int mine = left;
-                        const int col = 8 * nt + 2 * tg + h;
-                        if (it.ragged && col < it.cols)
-                            mine = min(mine, shared_len(p, it.qh / p.Hkv * p.K + (it.col0 + col) / G) - it.limit0 - k * kPageTokens);
+                        const int mine = tokens_of(8 * nt + 2 * tg + h, k);
                         if (tokA >= mine) x[nt][h] = -INFINITY;
                         if (tokB >= mine) x[nt][2 + h] = -INFINITY;
                     }
@@ -471,10 +477,10 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
 #pragma unroll
                 for (int i = 0; i < 4; i++) most = fmaxf(most, x[nt][i]);
             if (__any_sync(0xffffffffu, k == 0 || most > kSharedSlack || fmaxf(vn.x, vn.y) > st.vlimit)) {
-                float v = fmaxf(vn.x < INFINITY ? vn.x : 0.f, vn.y < INFINITY ? vn.y : 0.f), change = 1.f;
+                float v = fmaxf(vn.x, vn.y), change = 1.f;
 #pragma unroll
                 for (int d = 4; d <= 16; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-                if (v > st.vlimit) {        // (norms are not negative; infinite ones stay that at any scale, and are none of all rows')
+                if (v > st.vlimit) {        // (norms are not negative, nor infinite here)
                     // 2^-e with the norm in [2^e, 2^(e + 1))
                     const float now = __uint_as_float((254u << 23) - (__float_as_uint(v) & 0x7f800000u));
                     change = now / st.vscale;
@@ -507,26 +513,15 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
             vn.x *= st.vscale;
             vn.y *= st.vscale;
             uint32_t pb[TILES][2];
-            auto weights = [&](auto masked) {
 #pragma unroll
-                for (int nt = 0; nt < TILES; nt++) {
-                    float w[4];
+            for (int nt = 0; nt < TILES; nt++) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float s = x[nt][i];
-                        x[nt][i] = fast_exp2(s);
-                        w[i] = x[nt][i] * (i < 2 ? vn.x : vn.y);
-                        if constexpr (decltype(masked)::value) w[i] = s == -INFINITY ? 0.f : w[i];
-                    }
-                    st.l[nt][0] += x[nt][0] + x[nt][2];
-                    st.l[nt][1] += x[nt][1] + x[nt][3];
-                    pb[nt][0] = movmatrix_trans(pack_weights(w[0], w[1]));
-                    pb[nt][1] = movmatrix_trans(pack_weights(w[2], w[3]));
-                }
-            };
-            // (a token behind a column's end takes no part, whatever its norm is: an infinite one of a longer row's too)
-            if (whole) weights(std::false_type{});
-            else weights(std::true_type{});
+                for (int i = 0; i < 4; i++) x[nt][i] = fast_exp2(x[nt][i]);
+                st.l[nt][0] += x[nt][0] + x[nt][2];
+                st.l[nt][1] += x[nt][1] + x[nt][3];
+                pb[nt][0] = movmatrix_trans(pack_weights(x[nt][0] * vn.x, x[nt][1] * vn.x));
+                pb[nt][1] = movmatrix_trans(pack_weights(x[nt][2] * vn.y, x[nt][3] * vn.y));
+            }
             // ---- O^T += V^T P^T
             {
                 typename WV::template Run<C::VW> run[4];
@@ -559,7 +554,6 @@ __global__ void __launch_bounds__(SharedCfg<D, BK, BV, NT>::THREADS, 1) shared_a
         // (rows that end before the piece, or the first bad page of it, have lost nothing)
         const bool spoilt = lost || bad != INT32_MAX;
         const int sound = it.limit0 + (lost || !spoilt ? 0 : bad * kPageTokens);
-        auto row_len = [&](int col) { return shared_len(p, it.group ? it.qh / p.Hkv * p.K + (it.col0 + col) / G : it.row); };
 #pragma unroll
         for (int nt = 0; nt < TILES; nt++) {
 #pragma unroll
