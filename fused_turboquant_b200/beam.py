@@ -36,8 +36,8 @@ def select(logits: torch.Tensor, scores: torch.Tensor, n_best: int, *, end_token
            workspace: torch.Tensor | None = None) -> Selection:
     """The ``n_best`` best continuations of every request.
 
-    logits: [R, K, V], fp32 / fp16 / bf16; scores: [R, K], the beams' log-probabilities so far, -inf for a beam that is not
-    alive (of which at the first step of a request all but one are: they would all say the same).  Token v after beam b scores
+    logits: [R, K, V], fp32 / fp16 / bf16, up to 65535 requests; scores: [R, K], the beams' log-probabilities so far, -inf for a
+    beam that is not alive (of which at the first step of a request all but one are: they would all say the same).  Token v after beam b scores
     ``scores[b] + log_softmax(logits[b])[v]``; of equal ones the lowest beam's lowest token comes first.  Totals are compared in 64
     bits, but the sums of exponentials in them are fp32's: totals of different beams that lie within some 1e-7 may come in either
     order, those of beams with the same logits and scores are equal.

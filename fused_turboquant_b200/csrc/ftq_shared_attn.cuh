@@ -24,6 +24,8 @@
 // registers 175.  Without gain: the next page's scores beside this one's values (188), two pages a stage with the queries read once for
 // both (178; 190), queries in registers and 16 columns a warp, two warps to a page (223), the queries' loads free to be moved (187).
 //
+// Rounded to fp16, which the products take: queries in the rotated space, centroids, weights times norms (all else is fp32; error against 64
+// bits 3.9e-4 of the output's size with fp16 outputs, of which the output's own rounding is 2.1e-4).
 // Tables, page layout and fragment maps are those of ftq_attn_mma.cuh with the columns as heads (NH = 2).  Weights carry the
 // values' norms into fp16: they are scaled by a power of two that goes with the largest norm so far (lazily, as the maximum).
 #pragma once

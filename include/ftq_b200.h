@@ -577,8 +577,8 @@ int ftq_logits_process(const void *logits, int dtype, int64_t row_stride, int n_
 #define FTQ_BEAM_MAX_ENDS 16
 
 /*
- * Selection.  logits: n_requests x beams rows of `vocab` values of `dtype`, row_stride elements
- * apart; scores [n_requests, beams]: what the beams score so far (-inf: not alive; its logits do
+ * Selection.  logits: n_requests (at most 65535) x beams rows of `vocab` values of `dtype`,
+ * row_stride elements apart; scores [n_requests, beams]: what the beams score so far (-inf: not alive; its logits do
  * not matter then).  total(b, v) = scores[b] + logits[b][v] - log(sum exp(logits[b])).  Written, of
  * every request: the n_best largest totals of all beams and of all tokens but end_tokens [n_ends],
  * in order, of equal ones the lowest beam's lowest token first: out_scores, parents (the beam, 0
